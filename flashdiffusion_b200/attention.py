@@ -1,0 +1,286 @@
+"""Softmax attention over key spans: the learned-model form of the Q != K kernel.
+
+``FlashDiffusion`` sums values with the weights exp(-beta ||q_i - k_j||^2) and
+leaves normalisation to given row scales.  ``attend`` is the row-stochastic
+operator with exp(score) in their place, for batches of 16- or 32-bit heads and
+with gradients:
+
+  s_ij = scale q_i.k_j, or cap tanh(scale q_i.k_j / cap), minus slope_h |pos_i - j|
+  o_i  = sum_j softmax_j(s_ij) v_j       over the span first_i <= j < end_i
+
+Every mask offered is a span of keys for each row: causal, sliding window,
+documents packed into one row (``document_spans``), prefixes seen by all rows
+(``prefix_spans``), or any spans of the caller's own (``Spans``).  Rows with an
+empty span give zeros and no gradient; keys outside a row's span never reach it,
+whatever their memory holds.
+
+``attend_cached`` is the form for the newest tokens of each sequence against a
+key/value cache of which ``lengths`` rows are in use.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import native
+
+__all__ = ["attend", "attend_cached", "Spans", "document_spans", "prefix_spans"]
+
+_DTYPES = {torch.float32: native.DTYPE_F32, torch.float16: native.DTYPE_F16, torch.bfloat16: native.DTYPE_BF16}
+MAX_DIM = 256
+
+
+class Spans:
+    """Keys first[.., i] <= j < end[.., i] seen by query row i: int32 device tensors (q_len,) or (batch, q_len).
+
+    Values are clamped to the keys that exist; end <= first is a row that sees nothing.
+    """
+
+    def __init__(self, first: torch.Tensor, end: torch.Tensor):
+        for t in (first, end):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+                raise TypeError("first and end must be int32 tensors")
+        if first.shape != end.shape or first.dim() not in (1, 2) or first.device != end.device:
+            raise ValueError("first and end must be (q_len,) or (batch, q_len) tensors of one shape and device")
+        first, end = (t[None] if t.dim() == 1 else t for t in (first, end))
+        self.first, self.end = first.contiguous(), end.contiguous()
+
+    @property
+    def batch(self) -> int:
+        return self.first.shape[0]
+
+    @property
+    def q_len(self) -> int:
+        return self.first.shape[1]
+
+
+def _int32(name: str, t: torch.Tensor) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1:
+        raise TypeError(f"{name} must be a one-dimensional int32 tensor")
+    native.require_device(t.device)
+    return t.contiguous()
+
+
+def document_spans(offsets: torch.Tensor, rows: int, *, causal: bool = True, window: int | None = None,
+                   prefix: torch.Tensor | None = None) -> Spans:
+    """Spans of a packed batch: document d holds rows offsets[d] .. offsets[d + 1] of ``rows``.
+
+    A row sees its own document up to itself (all of it with causal=False), at most ``window`` rows back,
+    or also the first prefix[d] rows of the document (``prefix``: one length per document, without a
+    window).  Rows outside all documents (padding behind the last one) see nothing.
+    """
+    offsets = _int32("offsets", offsets)
+    if offsets.numel() < 1:
+        raise ValueError("offsets needs at least one entry")
+    rows, window = int(rows), _window(window, causal)
+    if rows < 0:
+        raise ValueError(f"rows must not be negative (got {rows})")
+    if prefix is not None:
+        prefix = _int32("prefix", prefix)
+        if prefix.numel() != offsets.numel() - 1 or prefix.device != offsets.device:
+            raise ValueError(f"prefix needs one length for each of the {offsets.numel() - 1} documents")
+        if window or not causal:
+            raise ValueError("a prefix needs causal=True and no window")
+    first = torch.empty((1, rows), dtype=torch.int32, device=offsets.device)
+    end = torch.empty_like(first)
+    with torch.cuda.device(offsets.device):
+        native.check(native.load().fd_attention_document_spans(
+            native._ptr(offsets), offsets.numel() - 1, native._ptr(prefix), rows, int(causal), window,
+            native._ptr(first), native._ptr(end), native._stream(offsets.device)))
+    return Spans(first, end)
+
+
+def prefix_spans(prefix: torch.Tensor, q_len: int, k_len: int | None = None) -> Spans:
+    """Spans of rows that see the first prefix[b] keys of sequence b and all keys up to their own position."""
+    prefix = _int32("prefix", prefix)
+    q_len = int(q_len)
+    k_len = q_len if k_len is None else int(k_len)
+    first = torch.empty((prefix.numel(), q_len), dtype=torch.int32, device=prefix.device)
+    end = torch.empty_like(first)
+    with torch.cuda.device(prefix.device):
+        native.check(native.load().fd_attention_prefix_spans(native._ptr(prefix), prefix.numel(), q_len, k_len,
+                                                             native._ptr(first), native._ptr(end),
+                                                             native._stream(prefix.device)))
+    return Spans(first, end)
+
+
+def _window(window, causal) -> int:
+    if window is None:
+        return 0
+    if int(window) < 1:
+        raise ValueError(f"window must be at least 1 (got {window})")
+    if not causal:
+        raise ValueError("a window needs causal=True")
+    return min(int(window), 2**31 - 1)
+
+
+def _strides(t: torch.Tensor):
+    # 0 where the extent is 1: a stride that is never taken may be anything
+    return native._L3(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+
+
+def _coordinates_together(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _arguments(q, k, v, o, lse, how) -> native.AttentionArgs:
+    spans, causal, window, lengths, slopes, scale, cap = how
+    a = native.AttentionArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=_strides(q),
+                             k_stride=_strides(k), v_stride=_strides(v), o=o.data_ptr(), o_stride=_strides(o),
+                             scale=scale, cap=cap, dtype=_DTYPES[q.dtype], causal=int(causal), window=window,
+                             batch=q.shape[0], q_len=q.shape[1], k_len=k.shape[1], heads=q.shape[2],
+                             kv_heads=k.shape[2], dim=q.shape[3])
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    if spans is not None:
+        a.first, a.end = spans.first.data_ptr(), spans.end.data_ptr()
+        a.span_stride = spans.q_len if spans.batch > 1 else 0
+    if lengths is not None:
+        a.lengths = lengths.data_ptr()
+    if slopes is not None:
+        a.slopes = slopes.data_ptr()
+    return a
+
+
+def _call(fn, a, backward, device):
+    lib = native.load()
+    # the caching allocator's own buffer per call: streams and captured graphs never share it
+    nbytes = int(lib.fd_attention_workspace_bytes(ctypes.byref(a), backward))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    with torch.cuda.device(device):
+        native.check(fn(ctypes.byref(a), native._ptr(ws), nbytes, native._stream(device)))
+
+
+def _forward(q, k, v, how, want_lse):
+    q, k, v = (_coordinates_together(t) for t in (q, k, v))
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if want_lse else None
+    _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, how), 0, q.device)
+    return o, lse
+
+
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, how):
+        q, k, v = (_coordinates_together(t) for t in (q, k, v))
+        o, lse = _forward(q, k, v, how, True)
+        spans, _, _, _, slopes, _, _ = how
+        masks = () if spans is None else (spans.first, spans.end)
+        ctx.save_for_backward(q, k, v, o, lse, *masks, *(() if slopes is None else (slopes,)))
+        ctx.how = how
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, _):
+        q, k, v, o, lse = ctx.saved_tensors[:5]
+        do = _coordinates_together(do)
+        a = _arguments(q, k, v, o, lse, ctx.how)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        a.d_o, a.do_stride = do.data_ptr(), _strides(do)
+        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        a.dq_stride, a.dk_stride, a.dv_stride = _strides(dq), _strides(dk), _strides(dv)
+        _call(native.load().fd_attention_backward, a, 1, q.device)
+        return dq, dk, dv, None
+
+
+def _check(q, k, v, slopes, scale, cap, names):
+    for name, t in zip(names, (q, k, v)):
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
+            raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{names[0]}, {names[1]} and {names[2]} must have one type and device")
+        if t.dim() != q.dim() or t.dim() not in (3, 4):
+            raise ValueError(f"{name} {tuple(t.shape)} must be (S, H, D) or (B, S, H, D), as {names[0]} is")
+    if k.shape != v.shape:
+        raise ValueError(f"{names[1]} {tuple(k.shape)} and {names[2]} {tuple(v.shape)} must have one shape")
+    if q.shape[-1] != k.shape[-1] or q.shape[:-3] != k.shape[:-3]:
+        raise ValueError(f"{names[0]} {tuple(q.shape)} and {names[1]} {tuple(k.shape)} differ in batch or head size")
+    if not 1 <= q.shape[-1] <= MAX_DIM:
+        raise ValueError(f"heads of 1 to {MAX_DIM} coordinates (got {q.shape[-1]})")
+    h, hk = q.shape[-2], k.shape[-2]
+    if hk < 1 or h < 1 or h % hk:
+        raise ValueError(f"{h} query heads are no multiple of {hk} key heads")
+    if slopes is not None:
+        if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or tuple(slopes.shape) != (h,):
+            raise ValueError(f"slopes must be a float32 tensor of {h} values")
+        if slopes.device != q.device:
+            raise ValueError("slopes must be on the device of the heads")
+        if slopes.requires_grad:
+            raise ValueError("there is no gradient for slopes: detach them")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    cap = 0.0 if cap is None else float(cap)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite (got {scale})")
+    if not (math.isfinite(cap) and cap >= 0) or (cap and cap < 1e-3):
+        raise ValueError(f"cap must be None or at least 1e-3 (got {cap})")
+    native.require_device(q.device)
+    return scale, cap
+
+
+def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None, causal: bool = False,
+           window: int | None = None, cap: float | None = None, slopes: torch.Tensor | None = None,
+           spans: Spans | None = None, return_lse: bool = False):
+    """softmax(scores) v over each row's span of keys; differentiable in q, k and v.
+
+    q (B, Sq, H, D), k and v (B, Sk, Hk, D) with H a multiple of Hk (query head h reads key head h // (H/Hk)),
+    or all three without the batch axis; float16, bfloat16 or float32, D <= 256, any strides with contiguous
+    coordinates.  Query row i stands at position Sk - Sq + i.
+
+    scale    of the products, D^-1/2 by default
+    causal   keys up to the row's own position; ``window``: at most that many of them
+    spans    a ``Spans`` in the place of causal and window
+    cap      scores become cap tanh(score / cap)
+    slopes   (H,) float32: slope times the distance |position - j| is subtracted from the scores
+    Returns the output (as q), or (output, lse): lse (B, H, Sq) float32 is the natural log of the sum of
+    exp(scores), -inf for rows that see nothing; it carries no gradient.
+    """
+    scale, cap = _check(q, k, v, slopes, scale, cap, ("q", "k", "v"))
+    flat = q.dim() == 3
+    if flat:
+        q, k, v = q[None], k[None], v[None]
+    if spans is not None:
+        if not isinstance(spans, Spans):
+            raise TypeError("spans must be a Spans")
+        if causal or window is not None:
+            raise ValueError("spans replace causal and window")
+        if spans.batch not in (1, q.shape[0]) or spans.q_len != q.shape[1] or spans.first.device != q.device:
+            raise ValueError(f"spans ({spans.batch}, {spans.q_len}) on {spans.first.device} do not fit "
+                             f"q {tuple(q.shape)} on {q.device}")
+    slopes = None if slopes is None else slopes.contiguous()
+    how = (spans, bool(causal), _window(window, causal), None, slopes, scale, cap)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        o, lse = _Attend.apply(q, k, v, how)
+    else:
+        o, lse = _forward(q, k, v, how, return_lse)
+    if flat:
+        o, lse = o[0], None if lse is None else lse[0]
+    return (o, lse) if return_lse else o
+
+
+def attend_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, *,
+                  scale: float | None = None, window: int | None = None, cap: float | None = None,
+                  slopes: torch.Tensor | None = None, return_lse: bool = False):
+    """Causal attention of the newest tokens of each sequence against a cache; no gradients.
+
+    q (B, N, H, D): the last N tokens of each sequence, which stand at positions lengths[b] - N .. lengths[b] - 1;
+    k_cache, v_cache (B, capacity, Hk, D) with the first lengths[b] rows in use (the new tokens' among them),
+    lengths (B,) int32 on the device (clamped to the capacity; a row at a negative position sees nothing).
+    Rows of the cache behind lengths[b] are never looked at.  scale, window, cap, slopes and return_lse as in
+    ``attend``.
+    """
+    scale, cap = _check(q, k_cache, v_cache, slopes, scale, cap, ("q", "k_cache", "v_cache"))
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, N, H, D) (got {tuple(q.shape)})")
+    lengths = _int32("lengths", lengths)
+    if tuple(lengths.shape) != (q.shape[0],) or lengths.device != q.device:
+        raise ValueError(f"lengths must hold {q.shape[0]} values on {q.device}")
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise ValueError("attend_cached has no gradient: detach its inputs, or use attend")
+    slopes = None if slopes is None else slopes.contiguous()
+    o, lse = _forward(q, k_cache, v_cache, (None, True, _window(window, True), lengths, slopes, scale, cap), return_lse)
+    return (o, lse) if return_lse else o

@@ -1,0 +1,167 @@
+// Entry points of softmax attention over key spans (declared in
+// include/fd_sm100.h): argument checks and the choice of kernels.
+#include "fd_attn.cuh"
+
+namespace fd {
+namespace attn {
+
+// Spans of a packed batch: each row finds its document by bisection.
+__global__ void document_spans_kernel(const int32_t* __restrict__ offsets, int n, const int32_t* __restrict__ prefix,
+                                      int64_t rows, int causal, int window, int32_t* __restrict__ first,
+                                      int32_t* __restrict__ end) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= rows) return;
+    int lo = 0, hi = n;   // the number of documents that end at or before row i
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (offsets[mid + 1] <= i) lo = mid + 1;
+        else hi = mid;
+    }
+    int f = 0, e = 0;
+    if (lo < n && offsets[lo] <= i) {
+        const int64_t a = offsets[lo], z = offsets[lo + 1];
+        int64_t ff = a, ee = causal ? i + 1 : z;
+        if (window > 0 && i - window + 1 > ff) ff = i - window + 1;
+        if (prefix) {
+            const int64_t pe = a + max(prefix[lo], 0);
+            if (pe > ee) ee = pe;
+        }
+        if (ee > z) ee = z;
+        if (ff < 0) ff = 0;
+        if (ee > rows) ee = rows;
+        f = (int)ff;
+        e = (int)ee;
+    }
+    first[i] = f;
+    end[i] = e;
+}
+
+__global__ void prefix_spans_kernel(const int32_t* __restrict__ prefix, int q_len, int k_len, int32_t* __restrict__ first,
+                                    int32_t* __restrict__ end) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x, b = blockIdx.y;
+    if (i >= q_len) return;
+    const int e = max(k_len - q_len + i + 1, prefix[b]);
+    first[(int64_t)b * q_len + i] = 0;
+    end[(int64_t)b * q_len + i] = min(max(e, 0), k_len);
+}
+
+static View view(const void* p, const int64_t* s) { return {const_cast<void*>(p), s[0], s[1], s[2]}; }
+
+static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
+    FD_CHECK_ARG(r, "fd_attention: null arguments");
+    FD_CHECK_ARG(r->dtype == FD_DTYPE_F32 || r->dtype == FD_DTYPE_F16 || r->dtype == FD_DTYPE_BF16,
+                 "fd_attention: dtype %d", r->dtype);
+    FD_CHECK_ARG(r->batch >= 0 && r->q_len >= 0 && r->k_len >= 0, "fd_attention: negative size");
+    FD_CHECK_ARG(r->q_len <= (1 << 30) && r->k_len <= (1 << 30), "fd_attention: more than 2^30 rows");
+    FD_CHECK_ARG(r->dim >= 1 && r->dim <= 256, "fd_attention: dim=%d not in 1..256", r->dim);
+    FD_CHECK_ARG(r->heads >= 1 && r->kv_heads >= 1 && r->heads % r->kv_heads == 0,
+                 "fd_attention: heads=%d must be a multiple of kv_heads=%d", r->heads, r->kv_heads);
+    FD_CHECK_ARG((int64_t)r->batch * r->heads <= 65535, "fd_attention: batch * heads = %lld above 65535",
+                 (long long)r->batch * r->heads);
+    FD_CHECK_ARG(r->scale == r->scale && r->cap >= 0.0, "fd_attention: scale and cap must be numbers, cap >= 0");
+    FD_CHECK_ARG((r->first == nullptr) == (r->end == nullptr), "fd_attention: first and end come together");
+    FD_CHECK_ARG(r->window >= 0, "fd_attention: window=%d", r->window);
+    FD_CHECK_ARG(!r->first || (!r->causal && !r->window), "fd_attention: spans replace causal and window");
+    FD_CHECK_ARG(r->window == 0 || r->causal, "fd_attention: a window needs causal");
+    Prob a{};
+    a.q = view(r->q, r->q_stride);
+    a.k = view(r->k, r->k_stride);
+    a.v = view(r->v, r->v_stride);
+    a.o = view(r->o, r->o_stride);
+    a.d_o = view(r->d_o, r->do_stride);
+    a.dq = view(r->dq, r->dq_stride);
+    a.dk = view(r->dk, r->dk_stride);
+    a.dv = view(r->dv, r->dv_stride);
+    a.lse = r->lse;
+    a.first = r->first;
+    a.end = r->end;
+    a.span_stride = r->span_stride;
+    a.lengths = r->lengths;
+    a.slopes = r->slopes;
+    a.scale = (float)r->scale;
+    a.cap = (float)r->cap;
+    a.causal = r->causal != 0;
+    // a window that reaches every key is none; this also keeps pos - window inside 32 bits
+    a.window = r->window >= (int64_t)r->q_len + r->k_len ? 0 : r->window;
+    a.batch = r->batch;
+    a.q_len = r->q_len;
+    a.k_len = r->k_len;
+    a.heads = r->heads;
+    a.kv_heads = r->kv_heads;
+    a.dim = r->dim;
+    a.group = r->heads / r->kv_heads;
+    *out = a;
+    if (a.batch == 0) return FD_OK;
+    FD_CHECK_ARG(a.q_len == 0 || (a.q.p && a.o.p), "fd_attention: null q or o");
+    FD_CHECK_ARG(a.k_len == 0 || (a.k.p && a.v.p), "fd_attention: null k or v");
+    if (backward) {
+        FD_CHECK_ARG(a.q_len == 0 || (a.d_o.p && a.dq.p && a.lse), "fd_attention_backward: null d_o, dq or lse");
+        FD_CHECK_ARG(a.k_len == 0 || (a.dk.p && a.dv.p), "fd_attention_backward: null dk or dv");
+    }
+    return FD_OK;
+}
+
+static size_t delta_bytes(const fd_attention_args* r) {
+    return align256(sizeof(float) * (size_t)r->batch * r->heads * r->q_len);
+}
+
+}  // namespace attn
+}  // namespace fd
+
+using namespace fd;
+
+extern "C" {
+
+size_t fd_attention_workspace_bytes(const fd_attention_args* r, int backward) {
+    if (!r || r->batch < 0 || r->q_len < 0 || r->k_len < 0 || r->heads < 1) return 0;
+    return backward ? attn::delta_bytes(r) : 0;
+}
+
+int fd_attention_forward(const fd_attention_args* r, void* workspace, size_t workspace_bytes, void* stream) {
+    attn::Prob a;
+    FD_TRY(attn::to_prob(r, false, &a));
+    (void)workspace;
+    (void)workspace_bytes;
+    if (a.batch == 0 || a.q_len == 0) return FD_OK;
+    return attn::simt_forward(a, r->dtype, (cudaStream_t)stream);
+}
+
+int fd_attention_backward(const fd_attention_args* r, void* workspace, size_t workspace_bytes, void* stream) {
+    attn::Prob a;
+    FD_TRY(attn::to_prob(r, true, &a));
+    if (a.batch == 0) return FD_OK;
+    const size_t need = fd_attention_workspace_bytes(r, 1);
+    if (workspace_bytes < need)
+        return set_error(FD_ERR_WORKSPACE, "fd_attention_backward: workspace %zu bytes, %zu needed", workspace_bytes, need);
+    FD_CHECK_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0),
+                 "fd_attention_backward: workspace must be 256-byte aligned");
+    return attn::simt_backward(a, r->dtype, (float*)workspace, (cudaStream_t)stream);
+}
+
+int fd_attention_document_spans(const int32_t* offsets, int n_documents, const int32_t* prefix, int64_t rows,
+                                int causal, int window, int32_t* first, int32_t* end, void* stream) {
+    FD_CHECK_ARG(n_documents >= 0 && rows >= 0 && rows <= (1 << 30), "fd_attention_document_spans: documents=%d rows=%lld",
+                 n_documents, (long long)rows);
+    FD_CHECK_ARG(window >= 0 && (window == 0 || causal), "fd_attention_document_spans: a window needs causal");
+    FD_CHECK_ARG(!prefix || (causal && !window), "fd_attention_document_spans: a prefix needs causal and no window");
+    if (rows == 0) return FD_OK;
+    FD_CHECK_ARG(offsets && first && end, "fd_attention_document_spans: null pointer");
+    attn::document_spans_kernel<<<(unsigned)cdiv(rows, 256), 256, 0, (cudaStream_t)stream>>>(
+        offsets, n_documents, prefix, rows, causal, window, first, end);
+    FD_CUDA_TRY(cudaGetLastError());
+    return FD_OK;
+}
+
+int fd_attention_prefix_spans(const int32_t* prefix, int batch, int q_len, int k_len, int32_t* first, int32_t* end,
+                              void* stream) {
+    FD_CHECK_ARG(batch >= 0 && batch <= 65535 && q_len >= 0 && k_len >= 0 && q_len <= (1 << 30) && k_len <= (1 << 30),
+                 "fd_attention_prefix_spans: batch=%d q_len=%d k_len=%d", batch, q_len, k_len);
+    if (batch == 0 || q_len == 0) return FD_OK;
+    FD_CHECK_ARG(prefix && first && end, "fd_attention_prefix_spans: null pointer");
+    attn::prefix_spans_kernel<<<dim3((unsigned)cdiv(q_len, 256), (unsigned)batch), 256, 0, (cudaStream_t)stream>>>(
+        prefix, q_len, k_len, first, end);
+    FD_CUDA_TRY(cudaGetLastError());
+    return FD_OK;
+}
+
+}  // extern "C"

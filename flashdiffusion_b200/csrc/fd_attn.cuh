@@ -1,0 +1,54 @@
+// Softmax attention over key spans: what the kernels of fd_attn_*.cu share.
+#pragma once
+#include "fd_common.cuh"
+
+namespace fd {
+namespace attn {
+
+struct View {
+    void* p;
+    int64_t sb, ss, sh;   // batch, token, head strides in elements
+};
+
+struct Prob {
+    View q, k, v, o, d_o, dq, dk, dv;
+    float* lse;
+    const int32_t *first, *end;
+    int64_t span_stride;
+    const int32_t* lengths;
+    const float* slopes;
+    float scale, cap;
+    int causal, window;
+    int batch, q_len, k_len, heads, kv_heads, dim, group;
+};
+
+// Keys in use by batch entry b.
+__device__ __forceinline__ int keys_of(const Prob& a, int b) {
+    if (!a.lengths) return a.k_len;
+    return min(max(a.lengths[b], 0), a.k_len);
+}
+
+// Span [x, y) of keys that row i of batch entry b (n keys in use) sees; empty spans come out as x = y.
+__device__ __forceinline__ int2 row_span(const Prob& a, int b, int i, int n) {
+    int lo, hi;
+    if (a.first) {
+        const int64_t at = b * a.span_stride + i;
+        lo = max(a.first[at], 0);
+        hi = min(a.end[at], n);
+    } else {
+        const int pos = n - a.q_len + i;
+        hi = a.causal ? min(pos + 1, n) : n;
+        lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    }
+    hi = max(hi, 0);
+    return make_int2(min(lo, hi), hi);
+}
+
+// Launchers (fd_attn_simt.cu).
+int simt_forward(const Prob& a, int dtype, cudaStream_t s);
+int simt_backward(const Prob& a, int dtype, float* delta, cudaStream_t s);
+// delta[b, h, i] = sum_c d_o o  (batch, heads, q_len)
+int launch_delta(const Prob& a, int dtype, float* delta, cudaStream_t s);
+
+}  // namespace attn
+}  // namespace fd

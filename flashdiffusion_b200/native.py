@@ -18,7 +18,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libfd_sm100.so")
 
 FD_OK, FD_ERR_ARG, FD_ERR_CUDA, FD_ERR_UNSUPPORTED, FD_ERR_TIMEOUT, FD_ERR_WORKSPACE, FD_ERR_RANGE = range(7)
-DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_F64 = range(4)
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_F64, DTYPE_I32, DTYPE_I64 = range(6)
 TILE_BF16, TILE_F32, TILE_F16, TILE_F16X3 = 0, 1, 2, 3
 SIDE_QUERY, SIDE_KEY = 0, 1
 
@@ -62,9 +62,40 @@ SIGNATURES = {
     "fd_pairwise_sqdist": (_I, [_P, _L, _I, _P, _P]),
     "fd_knn_tc_workspace_bytes": (_S, [_L, _L, _I, _I]),
     "fd_knn_sqdist_tc": (_I, [_P, _L, _P, _L, _I, _I, _P, _P, _S, _P]),
+    "fd_rotary": (_I, [_P, _P]),
+    "fd_attention_workspace_bytes": (_S, [_P, _I]),
+    "fd_attention_forward": (_I, [_P, _P, _S, _P]),
+    "fd_attention_backward": (_I, [_P, _P, _S, _P]),
+    "fd_attention_document_spans": (_I, [_P, _I, _P, _L, _I, _I, _P, _P, _P]),
+    "fd_attention_prefix_spans": (_I, [_P, _I, _I, _I, _P, _P, _P]),
     "fd_rope_windows": (_I, [_P, _L, _L, _P, _L, _L, _L, _I, _I, _I, _I, ctypes.c_double, _P, _I, _P, _P, _P,
                              _P]),
 }
+
+_L2, _L3 = _L * 2, _L * 3
+
+
+class RotaryArgs(ctypes.Structure):
+    """fd_rotary_args."""
+
+    _fields_ = [("q", _P), ("k", _P), ("qo", _P), ("ko", _P), ("q_stride", _L3), ("k_stride", _L3),
+                ("qo_stride", _L3), ("ko_stride", _L3), ("positions", _P), ("position_stride", _L2), ("freqs", _P),
+                ("magnitude", ctypes.c_double), ("dtype", _I), ("position_dtype", _I), ("layout", _I),
+                ("inverse", _I), ("batch", _L), ("tokens", _L), ("heads", _I), ("kv_heads", _I), ("dim", _I),
+                ("rot", _I)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """fd_attention_args."""
+
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_stride", _L3), ("k_stride", _L3), ("v_stride", _L3),
+                ("o", _P), ("o_stride", _L3), ("lse", _P), ("first", _P), ("end", _P), ("span_stride", _L),
+                ("lengths", _P), ("slopes", _P), ("scale", ctypes.c_double), ("cap", ctypes.c_double),
+                ("dtype", _I), ("causal", _I), ("window", _I), ("batch", _I), ("q_len", _I), ("k_len", _I),
+                ("heads", _I), ("kv_heads", _I), ("dim", _I),
+                ("d_o", _P), ("do_stride", _L3), ("dq", _P), ("dk", _P), ("dv", _P), ("dq_stride", _L3),
+                ("dk_stride", _L3), ("dv_stride", _L3)]
+
 
 _lib = None
 _lock = threading.Lock()

@@ -17,9 +17,16 @@ everything after it is the existing never-materialised operator:
 None here; every other learned attribute keeps its name and meaning.  The
 +1e-18 guards of the reference are kept where they change a result (row sums
 of far query windows).
+
+``apply_rotary`` is the same rotation for the query and key heads of a learned
+model: 16- or 32-bit tensors, adjacent or split pairs, part of the head,
+frequencies scaled for long contexts (``rotary_frequencies``), with gradients.
 """
 
 from __future__ import annotations
+
+import ctypes
+import math
 
 import numpy as np
 import torch
@@ -28,7 +35,8 @@ from . import native
 from .dmap import DiffusionMap
 from .kernel import GaussianOperator
 
-__all__ = ["ROPE", "make_hankel_windows", "make_window_positions"]
+__all__ = ["ROPE", "make_hankel_windows", "make_window_positions", "apply_rotary", "rotary_frequencies",
+           "rotary_magnitude"]
 
 _WINDOW_POSITION = {"start": 0, "center": 1, "end": 2}
 
@@ -314,3 +322,155 @@ class ROPE:
 
     def fit_transform(self) -> np.ndarray:
         return self.psi_
+
+
+# ---- rotary positions of query and key heads --------------------------------------
+
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_ROTARY_DTYPES = {torch.float32: native.DTYPE_F32, torch.float16: native.DTYPE_F16, torch.bfloat16: native.DTYPE_BF16}
+_POSITION_DTYPES = {torch.int32: native.DTYPE_I32, torch.int64: native.DTYPE_I64, torch.float32: native.DTYPE_F32,
+                    torch.float64: native.DTYPE_F64}
+
+
+def rotary_frequencies(rot: int, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
+                       trained: int | None = None, slow: float = 1.0, fast: float = 32.0,
+                       device=None) -> torch.Tensor:
+    """(rot/2,) float64 radians per position of each pair: base^(-2p/rot), scaled for contexts ``factor`` times longer.
+
+    scaling None      unscaled (``factor`` must be 1)
+            "linear"  every frequency divided by ``factor``
+            "base"    base raised to base * factor^(rot/(rot-2)): the fastest pair keeps its frequency, the
+                      slowest is divided by ``factor``
+            "parts"   pairs that make at most ``slow`` turns within the ``trained`` length are divided by
+                      ``factor``, those with at least ``fast`` turns are kept, linear in the turns between
+    """
+    rot = int(rot)
+    if rot < 2 or rot % 2:
+        raise ValueError(f"rot must be even and at least 2 (got {rot})")
+    if not base > 0 or not factor >= 1 or not math.isfinite(base) or not math.isfinite(factor):
+        raise ValueError(f"base must be positive and factor at least 1 (got {base}, {factor})")
+    if scaling not in (None, "linear", "base", "parts"):
+        raise ValueError(f"scaling must be None, 'linear', 'base' or 'parts' (got {scaling!r})")
+    if scaling is None and factor != 1:
+        raise ValueError("factor needs a scaling")
+    if scaling == "base":
+        if rot < 4:
+            raise ValueError("scaling='base' needs rot >= 4")
+        base = base * factor ** (rot / (rot - 2))
+    f = base ** (-2.0 * np.arange(rot // 2, dtype=np.float64) / rot)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        if trained is None or trained <= 0 or not 0 <= slow < fast:
+            raise ValueError("scaling='parts' needs the trained length and 0 <= slow < fast")
+        keep = np.clip((trained * f / (2 * math.pi) - slow) / (fast - slow), 0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+    return torch.as_tensor(f, device=native.require_device(device))
+
+
+def rotary_magnitude(factor: float) -> float:
+    """Factor on the rotated coordinates that goes with scaling="parts": 0.1 ln(factor) + 1."""
+    if not factor >= 1:
+        raise ValueError(f"factor must be at least 1 (got {factor})")
+    return 0.1 * math.log(factor) + 1.0
+
+
+def _strides3(t: torch.Tensor):
+    """Batch, token and head strides; 0 where the extent is 1, so that nothing hangs on a stride that is never taken."""
+    return native._L3(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+
+
+def _rotate_heads(xs, positions, freqs, layout, magnitude, inverse, inplace):
+    """fd_rotary on one or two (B, S, H, D) tensors; returns the rotated tensors."""
+    xs = [x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous() for x in xs]
+    outs = xs if inplace else [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    q, qo = xs[0], outs[0]
+    k, ko = (xs[1], outs[1]) if len(xs) > 1 else (None, None)
+    a = native.RotaryArgs(q=q.data_ptr(), qo=qo.data_ptr(), q_stride=_strides3(q), qo_stride=_strides3(qo),
+                          positions=positions.data_ptr(),
+                          position_stride=native._L2(*(positions.stride(i) if positions.shape[i] > 1 else 0
+                                                       for i in range(2))),
+                          freqs=freqs.data_ptr(), magnitude=magnitude, dtype=_ROTARY_DTYPES[q.dtype],
+                          position_dtype=_POSITION_DTYPES[positions.dtype], layout=layout, inverse=int(inverse),
+                          batch=q.shape[0], tokens=q.shape[1], heads=q.shape[2], dim=q.shape[3],
+                          rot=2 * freqs.numel())
+    if k is not None:
+        a.k, a.ko, a.k_stride, a.ko_stride, a.kv_heads = (k.data_ptr(), ko.data_ptr(), _strides3(k), _strides3(ko),
+                                                          k.shape[2])
+    with torch.cuda.device(q.device):
+        native.check(native.load().fd_rotary(ctypes.byref(a), native._stream(q.device)))
+    return outs
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, positions, freqs, layout, magnitude, inverse, *xs):
+        ctx.save_for_backward(positions, freqs)
+        ctx.how = (layout, magnitude, inverse)
+        return tuple(_rotate_heads(xs, positions, freqs, layout, magnitude, inverse, False))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        positions, freqs = ctx.saved_tensors
+        layout, magnitude, inverse = ctx.how
+        return (None,) * 5 + tuple(_rotate_heads(grads, positions, freqs, layout, magnitude, not inverse, False))
+
+
+def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: torch.Tensor, freqs: torch.Tensor,
+                 layout: str = "half", magnitude: float = 1.0, inverse: bool = False, inplace: bool = False):
+    """Rotate the heads of ``q`` (and ``k``) by their tokens' positions, in one launch.
+
+    q (B, S, H, D) or (S, H, D), k the same with its own number of heads; float32, float16 or bfloat16,
+    any strides with contiguous coordinates.  ``positions`` (S,) or (B, S), integer or floating (fractional
+    positions are exact to fp64).  ``freqs``: (R/2,) float64 radians per position, R <= D
+    (``rotary_frequencies``); pair p turns by positions * freqs[p] and coordinates R.. are copied.
+
+    layout "half" pairs coordinate p with p + R/2, "interleaved" 2p with 2p + 1 (as ROPE does).  ``magnitude``
+    scales the rotated coordinates, ``inverse`` turns the other way.  ``inplace`` overwrites q and k (no
+    gradients).  Returns the rotated q, or (q, k).
+    """
+    xs = [q] if k is None else [q, k]
+    for name, x in zip("qk", xs):
+        if not isinstance(x, torch.Tensor) or x.dtype not in _ROTARY_DTYPES:
+            raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
+        if x.dim() not in (3, 4) or x.dim() != q.dim() or x.dtype != q.dtype or x.device != q.device:
+            raise ValueError("q and k must be (S, H, D) or (B, S, H, D) tensors of one type on one device")
+        if x.shape[:-2] != q.shape[:-2] or x.shape[-1] != q.shape[-1]:
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(x.shape)} may differ in their heads only")
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be 'half' or 'interleaved' (got {layout!r})")
+    if not isinstance(freqs, torch.Tensor) or freqs.dtype != torch.float64 or freqs.dim() != 1:
+        raise TypeError("freqs must be a one-dimensional float64 tensor")
+    if not 1 <= freqs.numel() <= q.shape[-1] // 2:
+        raise ValueError(f"freqs has {freqs.numel()} pairs, a head of {q.shape[-1]} coordinates takes 1 to "
+                         f"{q.shape[-1] // 2}")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_DTYPES:
+        raise TypeError("positions must be an int32, int64, float32 or float64 tensor")
+    if not math.isfinite(magnitude):
+        raise ValueError(f"magnitude must be finite (got {magnitude})")
+    lead = tuple(q.shape[:-2])
+    if tuple(positions.shape) not in (lead, lead[-1:]):
+        raise ValueError(f"positions {tuple(positions.shape)} must be {lead} or {lead[-1:]}")
+    if positions.device != q.device or freqs.device != q.device:
+        raise ValueError("q, positions and freqs must be on one device")
+    if positions.requires_grad or freqs.requires_grad:
+        raise ValueError("apply_rotary has no gradient for positions and freqs: detach them")
+    native.require_device(q.device)
+    grad = torch.is_grad_enabled() and any(x.requires_grad for x in xs)
+    if inplace and grad:
+        raise ValueError("inplace=True has no gradient: detach q and k, or rotate out of place")
+    flat = q.dim() == 3
+    x4 = [x[None] if flat else x for x in xs]
+    pos = positions if positions.dim() == 2 else positions[None].expand(x4[0].shape[0], -1)
+    freqs = freqs.contiguous()
+    if inplace:
+        if any(x.stride(-1) != 1 and x.shape[-1] > 1 for x in x4):
+            raise ValueError("inplace=True needs contiguous coordinates")
+        for x in x4:
+            if any(x.stride(i) == 0 and x.shape[i] > 1 for i in range(3)):
+                raise ValueError("inplace=True cannot write to an expanded tensor")
+    args = (pos, freqs, _LAYOUTS[layout], float(magnitude), bool(inverse))
+    out = _Rotary.apply(*args, *x4) if grad else _rotate_heads(x4, *args, inplace)
+    out = [o[0] for o in out] if flat else list(out)
+    return out[0] if k is None else (out[0], out[1])

@@ -274,6 +274,104 @@ int fd_rope_windows(const double* F, int64_t sT, int64_t sC, const double* pos, 
                     int D, int L, int window_mode, int c_w, double pos_scale, const double* freqs, int n_freqs,
                     const double* mu, const double* sigma, float* Y, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions of query and key heads (the learned-model form of the
+ * rotation that fd_rope_windows applies to time-series windows).
+ * ------------------------------------------------------------------------- */
+
+/* Position element types (in addition to FD_DTYPE_F32 and FD_DTYPE_F64). */
+#define FD_DTYPE_I32 4
+#define FD_DTYPE_I64 5
+
+#define FD_ROTARY_HALF 0         /* pairs (p, p + rot/2)  */
+#define FD_ROTARY_INTERLEAVED 1  /* pairs (2p, 2p + 1)    */
+
+/* q[b, s, h, :] and k[b, s, h, :] (strides in elements, innermost stride 1;
+ * k and ko may be NULL with kv_heads = 0).  Pair p < rot/2 of every head turns
+ * by the angle positions[b, s] * freqs[p] (negated when inverse != 0):
+ *     a' = magnitude (a cos - b sin),  b' = magnitude (a sin + b cos);
+ * coordinates rot..dim are copied.  The angle is reduced in fp64, the rotation
+ * runs in fp32 and is rounded once.  qo may equal q (in place, same strides).
+ * dtype: FD_DTYPE_F32, F16 or BF16.  freqs: rot/2 fp64 values on the device. */
+typedef struct fd_rotary_args {
+    const void *q, *k;
+    void *qo, *ko;
+    int64_t q_stride[3], k_stride[3], qo_stride[3], ko_stride[3]; /* batch, token, head */
+    const void* positions;
+    int64_t position_stride[2]; /* batch, token */
+    const double* freqs;
+    double magnitude;
+    int dtype, position_dtype, layout, inverse;
+    int64_t batch, tokens;
+    int heads, kv_heads, dim, rot;
+} fd_rotary_args;
+int fd_rotary(const fd_rotary_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Softmax attention over key spans: the row-stochastic kernel of dot products
+ * (FlashDiffusion's Q != K operator with exp(score) in the place of
+ * exp(-beta d^2) and every row normalised), its gradients, and its form for
+ * the newest tokens against a cache.
+ *
+ *     s_ij = scale q_i.k_j                        (cap = 0)
+ *          = cap tanh(scale q_i.k_j / cap)        (cap > 0)
+ *     s_ij -= slopes[h] |pos_i - j|               (slopes != NULL)
+ *     o_i  = sum_j softmax_j(s_ij) v_j            over first_i <= j < end_i
+ *
+ * pos_i = n - q_len + i, n = k_len (or lengths[b] when lengths != NULL, clamped
+ * to [0, k_len]).  The span of row i is first[b, i] .. end[b, i] when both
+ * arrays are given (clamped to [0, n)); otherwise end_i = pos_i + 1 when causal
+ * != 0, else n, and first_i = pos_i - window + 1 when window > 0 (causal only),
+ * else 0.  A row with an empty span gives zeros and lse = -inf and no gradient.
+ * Keys outside a row's span never reach it, whatever their memory holds (NaN
+ * and infinities included).
+ * ------------------------------------------------------------------------- */
+
+typedef struct fd_attention_args {
+    const void *q, *k, *v;     /* q[b, s, h, :], k/v[b, s, kv_head, :], innermost stride 1 */
+    int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, token, head, in elements */
+    void* o;
+    int64_t o_stride[3];
+    float* lse;                /* (batch, heads, q_len) contiguous, natural log; may be NULL (forward) */
+    const int32_t *first, *end; /* (batch, q_len) spans, or both NULL */
+    int64_t span_stride;       /* elements between batches (0 = the same spans for all) */
+    const int32_t* lengths;    /* (batch) keys in use, or NULL */
+    const float* slopes;       /* (heads), or NULL */
+    double scale, cap;
+    int dtype;                 /* FD_DTYPE_F32, F16 or BF16: q, k, v, o, gradients */
+    int causal, window;
+    int batch, q_len, k_len, heads, kv_heads, dim;
+    /* backward only: o and lse are inputs */
+    const void* d_o;
+    int64_t do_stride[3];
+    void *dq, *dk, *dv;        /* same shapes as q, k, v */
+    int64_t dq_stride[3], dk_stride[3], dv_stride[3];
+} fd_attention_args;
+
+/* Workspace of the calls below for these arguments (pointers are not read). */
+size_t fd_attention_workspace_bytes(const fd_attention_args* args, int backward);
+
+/* o (and lse).  1 <= dim <= 256, heads a multiple of kv_heads. */
+int fd_attention_forward(const fd_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dq, dk, dv from d_o, with o and lse of the forward call.  Fixed-order sums:
+ * repeated calls give the same bits. */
+int fd_attention_backward(const fd_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal spans of a packed batch: document d holds rows offsets[d] ..
+ * offsets[d + 1] (n_documents + 1 device values, non-decreasing); rows outside
+ * all documents get empty spans.  A row sees its own document up to itself
+ * (the whole document when causal = 0), at most `window` keys back (window > 0,
+ * causal only) or, with prefix != NULL (causal, no window), also the first
+ * prefix[d] rows of the document whatever their order. */
+int fd_attention_document_spans(const int32_t* offsets, int n_documents, const int32_t* prefix, int64_t rows,
+                                int causal, int window, int32_t* first, int32_t* end, void* stream);
+
+/* Spans (batch, q_len) of rows that see the first prefix[b] keys of their
+ * sequence and every key up to their own position k_len - q_len + i. */
+int fd_attention_prefix_spans(const int32_t* prefix, int batch, int q_len, int k_len, int32_t* first, int32_t* end,
+                              void* stream);
+
 /* Failure-path self-test (no counterpart in the reference): launches one bounded
  * device wait on a barrier that nothing arrives at, with a limit of limit_ns
  * (1e6..2e9).  The wait gives up and records FD_ERR_TIMEOUT in the status word

@@ -1,0 +1,411 @@
+"""attend and attend_cached against their definition in 64 bits (tests/attention_reference.py, where the bounds come from)."""
+import pytest
+import torch
+
+from tests.attention_reference import check, reference, spans_of
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, SF = torch.bfloat16, torch.float16, torch.float32
+# fp16 holds nothing finer than 2^-25 absolute: outputs that small, and the ds values they are summed from
+FLOOR = {BF: 0.0, HF: 2.0 ** -25, SF: 0.0}
+
+
+def _inputs(b, sq, sk, h, hk, d, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    mk = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dtype)  # noqa: E731
+    return mk(b, sq, h, d), mk(b, sk, hk, d), mk(b, sk, hk, d), mk(b, sq, h, d)
+
+
+def _run(q, k, v, do, grad=True, **kw):
+    from flashdiffusion_b200.attention import attend
+    q, k, v = (t.detach().requires_grad_(grad) for t in (q, k, v))
+    o, lse = attend(q, k, v, return_lse=True, **kw)
+    out = {"o": o, "lse": lse}
+    if grad:
+        out["dq"], out["dk"], out["dv"] = torch.autograd.grad(o, (q, k, v), do)
+    return out
+
+
+def _compare(out, ref, dtype):
+    for name in out:
+        check(name, out[name], ref, 0.0 if name == "lse" else FLOOR[dtype])
+
+
+SHAPES = [
+    (1, 1, 1, 1, 1, 64), (2, 77, 77, 4, 4, 64), (1, 128, 128, 2, 1, 128), (1, 129, 257, 6, 2, 128), (2, 300, 300, 4, 2, 96),
+    (1, 5, 640, 8, 2, 128), (1, 260, 40, 2, 2, 64), (3, 31, 513, 3, 1, 72),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_values_and_gradients(shape, causal, dtype):
+    b, sq, sk, h, hk, d = shape
+    q, k, v, do = _inputs(*shape, dtype, seed=sq + sk)
+    lo, hi, pos = spans_of(sq, sk, b, causal=causal)
+    _compare(_run(q, k, v, do, causal=causal), reference(q, k, v, lo, hi, pos, do=do), dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(SF, 64), (SF, 20), (SF, 256), (BF, 7), (HF, 160), (BF, 200)], ids=str)
+def test_general_path_types_and_head_sizes(dtype, d):
+    q, k, v, do = _inputs(2, 45, 70, 4, 2, d, dtype, seed=d)
+    slopes = torch.tensor([0.5, 0.1, 0.0, -0.02], device="cuda")
+    lo, hi, pos = spans_of(45, 70, 2, causal=True, window=33)
+    out = _run(q, k, v, do, causal=True, window=33, cap=15.0, slopes=slopes)
+    _compare(out, reference(q, k, v, lo, hi, pos, cap=15.0, slopes=slopes, do=do), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kw", [
+    dict(cap=5.0), dict(cap=30.0, causal=True), dict(slopes=True), dict(slopes=True, causal=True),
+    dict(cap=8.0, slopes=True, causal=True, window=50), dict(causal=True, window=1), dict(causal=True, window=130),
+    dict(causal=True, window=2 ** 31 - 1), dict(scale=0.7), dict(scale=-0.3, causal=True), dict(scale=0.0),
+], ids=str)
+def test_scores(kw, d, dtype):
+    kw = dict(kw)
+    q, k, v, do = _inputs(2, 200, 333, 4, 2, d, dtype, seed=7)
+    if kw.pop("slopes", False):
+        kw["slopes"] = torch.tensor([0.3, 0.05, 0.004, 0.0], device="cuda")
+    lo, hi, pos = spans_of(200, 333, 2, causal=kw.get("causal", False), window=kw.get("window"))
+    out = _run(q, k, v, do, **kw)
+    ref = reference(q, k, v, lo, hi, pos, scale=kw.get("scale"), cap=kw.get("cap", 0.0), slopes=kw.get("slopes"), do=do)
+    _compare(out, ref, dtype)
+
+
+def test_large_scores_and_cap_at_its_ends():
+    """Scores of hundreds: without a cap one key takes all, with one the tanh is flat at both ends."""
+    q, k, v, do = _inputs(1, 150, 150, 2, 2, 64, BF, seed=3)
+    q = q * 20
+    for cap in (0.0, 3.0, 50.0):
+        lo, hi, pos = spans_of(150, 150, 1, causal=True)
+        out = _run(q, k, v, do, causal=True, cap=cap or None)
+        _compare(out, reference(q, k, v, lo, hi, pos, cap=cap, do=do), BF)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, BF), (128, HF), (40, SF)], ids=str)
+@pytest.mark.parametrize("causal,window,prefix", [(True, None, False), (False, None, False), (True, 20, False),
+                                                  (True, None, True)])
+def test_documents(causal, window, prefix, d, dtype):
+    from flashdiffusion_b200.attention import document_spans
+    offsets = [3, 4, 4, 140, 141, 290, 401]          # rows 0..2 and 401.. are padding; one document is empty
+    rows = 430
+    q, k, v, do = _inputs(1, rows, rows, 3, 1, d, dtype, seed=11)
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    pre = torch.tensor([1, 9, 40, 0, 500, 16], dtype=torch.int32, device="cuda") if prefix else None
+    spans = document_spans(off, rows, causal=causal, window=window, prefix=pre)
+    first, end = torch.zeros(1, rows, dtype=torch.long), torch.zeros(1, rows, dtype=torch.long)
+    for n, (a, z) in enumerate(zip(offsets[:-1], offsets[1:])):
+        for i in range(a, z):
+            first[0, i] = max(a, i - window + 1) if window else a
+            end[0, i] = i + 1 if causal else z
+            if prefix:
+                end[0, i] = min(z, max(i + 1, a + int(pre[n])))
+    empty = end[0] <= first[0]
+    assert torch.equal((spans.end <= spans.first)[0].cpu(), empty)
+    assert torch.equal(spans.first[0].cpu()[~empty], first[0][~empty].int())
+    assert torch.equal(spans.end[0].cpu()[~empty], end[0][~empty].int())
+    lo, hi, pos = spans_of(rows, rows, 1, first=first, end=end)
+    out = _run(q, k, v, do, spans=spans)
+    _compare(out, reference(q, k, v, lo, hi, pos, do=do), dtype)
+    assert (out["o"][0, empty.cuda()] == 0).all() and (out["lse"][0][:, empty.cuda()] == float("-inf")).all()
+    assert (out["dq"][0, empty.cuda()] == 0).all()
+    assert (out["dk"][0, 401:] == 0).all() and (out["dv"][0, :3] == 0).all()
+
+
+@pytest.mark.parametrize("sq,sk", [(200, 200), (130, 333)])
+def test_prefix(sq, sk):
+    from flashdiffusion_b200.attention import prefix_spans
+    q, k, v, do = _inputs(4, sq, sk, 4, 2, 128, BF, seed=5)
+    pre = torch.tensor([0, 1, 150, 10 ** 6], dtype=torch.int32, device="cuda")
+    i = torch.arange(sq)[None] + sk - sq
+    end = torch.maximum(i + 1, pre.cpu().long()[:, None])
+    lo, hi, pos = spans_of(sq, sk, 4, first=torch.zeros_like(end), end=end)
+    slopes = torch.tensor([0.2, 0.1, 0.05, 0.025], device="cuda")
+    out = _run(q, k, v, do, spans=prefix_spans(pre, sq, sk), slopes=slopes)
+    _compare(out, reference(q, k, v, lo, hi, pos, slopes=slopes, do=do), BF)
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, HF), (24, SF)], ids=str)
+def test_any_spans(d, dtype):
+    """Spans in no order, out of range, crossed and empty."""
+    from flashdiffusion_b200.attention import Spans
+    sq, sk = 270, 401
+    q, k, v, do = _inputs(2, sq, sk, 2, 1, d, dtype, seed=13)
+    g = torch.Generator().manual_seed(1)
+    first = torch.randint(-50, sk + 50, (2, sq), generator=g, dtype=torch.int32)
+    end = first + torch.randint(-20, 300, (2, sq), generator=g, dtype=torch.int32)
+    end[0, 5], first[0, 6], end[0, 6] = -(2 ** 31), -(2 ** 31), 2 ** 31 - 1
+    lo, hi, pos = spans_of(sq, sk, 2, first=first, end=end)
+    out = _run(q, k, v, do, spans=Spans(first.cuda(), end.cuda()))
+    _compare(out, reference(q, k, v, lo, hi, pos, do=do), dtype)
+    one = Spans(first[0].cuda(), end[0].cuda())          # the same spans for every batch entry
+    lo, hi, pos = spans_of(sq, sk, 2, first=first[:1], end=end[:1])
+    _compare(_run(q, k, v, do, spans=one), reference(q, k, v, lo, hi, pos, do=do), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF], ids=str)
+def test_layouts_and_strides(dtype):
+    """Packed qkv, head-major tensors, odd offsets, expanded keys, tensors without a batch axis: the same bits as contiguous ones."""
+    from flashdiffusion_b200.attention import attend
+    b, s, h, d = 2, 150, 4, 64
+    q, k, v, do = _inputs(b, s, s, h, h, d, dtype, seed=17)
+    want = _run(q, k, v, do, causal=True)
+    qkv = torch.stack([q, k, v], 2)
+    views = {
+        "packed": qkv.unbind(2),
+        "head-major": [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)],
+        "padded": [torch.nn.functional.pad(t, (0, 8))[..., :d] for t in (q, k, v)],
+        "last-major": [t.transpose(1, 3).contiguous().transpose(1, 3) for t in (q, k, v)],
+    }
+    for name, (a, b_, c) in views.items():
+        got = _run(a, b_, c, do.transpose(1, 2).contiguous().transpose(1, 2), causal=True)
+        for n in got:
+            assert torch.equal(got[n], want[n]), (name, n)
+    # odd element offsets take other kernels: compared by value
+    odd = [torch.nn.functional.pad(t, (1, 1))[..., 1:d + 1] for t in (q, k, v)]
+    lo, hi, pos = spans_of(s, s, b, causal=True)
+    _compare(_run(*odd, do, causal=True), reference(q, k, v, lo, hi, pos, do=do), dtype)
+    flat = attend(q[0], k[0], v[0], causal=True)
+    assert torch.equal(flat, attend(q[:1], k[:1], v[:1], causal=True)[0])
+    # one key sequence shared by the batch: its gradient is the sum over the batch
+    ke = k[:1].expand(b, s, h, d)
+    got = _run(q, ke, v, do, causal=True)
+    _compare(got, reference(q, ke, v, lo, hi, pos, do=do), dtype)
+    leaf = k[:1].clone().requires_grad_(True)
+    o = attend(q, leaf.expand(b, s, h, d), v, causal=True)
+    shared = torch.autograd.grad(o, leaf, do)[0]
+    u = torch.finfo(dtype).eps / 2
+    assert ((shared - got["dk"].float().sum(0, keepdim=True)).abs() <= 3 * u * got["dk"].float().abs().sum(0) + 1e-6).all()
+    # an expanded gradient, as the sum of the output gives
+    leaf = q.clone().requires_grad_(True)
+    dq = torch.autograd.grad(attend(leaf, k, v, causal=True).sum(), leaf)[0]
+    ref = reference(q, k, v, lo, hi, pos, do=torch.ones_like(do))
+    check("dq", dq, ref, FLOOR[dtype])
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (SF, 48)], ids=str)
+def test_masked_places_hold_anything(dtype, d):
+    """NaN and infinities behind the last document, and in its padding rows of q and do, change nothing."""
+    from flashdiffusion_b200.attention import document_spans
+    rows, used = 300, 210
+    q, k, v, do = _inputs(1, rows, rows, 2, 2, d, dtype, seed=19)
+    off = torch.tensor([0, 100, used], dtype=torch.int32, device="cuda")
+    spans = document_spans(off, rows)
+    want = _run(q, k, v, do, spans=spans)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        q2, k2, v2, do2 = (t.clone() for t in (q, k, v, do))
+        for t in (q2, k2, v2, do2):
+            t[:, used:] = bad
+        got = _run(q2, k2, v2, do2, spans=spans)
+        for n in got:
+            assert torch.equal(got[n], want[n]), (n, bad)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (SF, 48)], ids=str)
+def test_causal_future_holds_anything(dtype, d):
+    """A NaN or infinity in a key or value reaches the rows that see it and no other."""
+    s, at = 300, 170
+    q, k, v, do = _inputs(1, s, s, 2, 2, d, dtype, seed=23)
+    want = _run(q, k, v, do, causal=True, grad=False)
+    for bad in (float("nan"), float("inf")):
+        v2 = v.clone()
+        v2[:, at, :, 3] = bad
+        got = _run(q, k, v2, do, causal=True, grad=False)
+        assert torch.equal(got["o"][:, :at], want["o"][:, :at])
+        assert not torch.isfinite(got["o"][:, at:, :, 3]).any()
+        assert torch.equal(got["o"][:, at:, :, 4:], want["o"][:, at:, :, 4:])
+        k2 = k.clone()
+        k2[:, at] = bad
+        got = _run(q, k2, v, do, causal=True, grad=False)
+        assert torch.equal(got["o"][:, :at], want["o"][:, :at])
+        assert not torch.isfinite(got["o"][:, at + 1:]).all(-1).any()
+    want = _run(q, k, v, do, causal=True)
+    # gradients: a row's NaN stays out of the keys that the row does not see
+    for which in ("q", "do"):
+        q2, do2 = q.clone(), do.clone()
+        (q2 if which == "q" else do2)[:, at] = float("nan")
+        got = _run(q2, k, v, do2, causal=True)
+        for n in ("dk", "dv"):
+            assert torch.equal(got[n][:, at + 1:], want[n][:, at + 1:]), (which, n)
+        assert not torch.isfinite(got["dk"][:, :at + 1]).any()
+        assert torch.equal(got["dq"][:, :at], want["dq"][:, :at]) and torch.equal(got["dq"][:, at + 1:], want["dq"][:, at + 1:])
+    k2 = k.clone()
+    k2[:, at] = float("nan")
+    got = _run(q, k2, v, do, causal=True)
+    assert torch.equal(got["dq"][:, :at], want["dq"][:, :at])
+
+
+def test_empty_sizes():
+    from flashdiffusion_b200.attention import attend, attend_cached
+    q, k, v, do = _inputs(2, 5, 0, 2, 1, 64, BF)
+    out = _run(q, k, v, do)
+    assert (out["o"] == 0).all() and (out["lse"] == float("-inf")).all() and (out["dq"] == 0).all()
+    q, k, v, do = _inputs(2, 0, 9, 2, 1, 64, BF)
+    out = _run(q, k, v, do)
+    assert out["o"].shape == (2, 0, 2, 64) and (out["dk"] == 0).all() and (out["dv"] == 0).all()
+    assert attend(*(torch.empty(0, 4, 2, 64, device="cuda", dtype=BF) for _ in range(3))).shape == (0, 4, 2, 64)
+    q, k, v, _ = _inputs(3, 1, 16, 2, 1, 64, BF)
+    o = attend_cached(q, k, v, torch.tensor([0, 1, -7], dtype=torch.int32, device="cuda"))
+    assert (o[0] == 0).all() and (o[2] == 0).all() and torch.equal(o[1, 0], v[1, 0].expand(2, 64))
+
+
+def test_same_bits_again():
+    q, k, v, do = _inputs(2, 513, 513, 6, 2, 128, BF, seed=29)
+    a = _run(q, k, v, do, causal=True, cap=20.0)
+    for _ in range(3):
+        b = _run(q, k, v, do, causal=True, cap=20.0)
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_gradient_against_differences():
+    """fp32 heads: the derivative along a random direction against central differences of the loss in 64 bits."""
+    q, k, v, do = _inputs(1, 40, 55, 2, 1, 32, SF, seed=31)
+    slopes = torch.tensor([0.1, 0.01], device="cuda")
+    out = _run(q, k, v, do, causal=True, cap=4.0, slopes=slopes)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    lo, hi, pos = spans_of(40, 55, 1, causal=True)
+    for n, t in (("dq", q), ("dk", k), ("dv", v)):
+        e = torch.randn(t.shape, device="cuda", generator=g)
+        ends = []
+        for sign in (1, -1):
+            moved = {"dq": q, "dk": k, "dv": v} | {n: (t.double() + sign * 1e-4 * e.double())}
+            o = _exact_output(moved["dq"].double(), moved["dk"].double(), moved["dv"].double(), lo, hi, pos, 4.0, slopes)
+            ends.append(float((o * do.cpu().double()).sum()))
+        want = (ends[0] - ends[1]) / 2e-4
+        got = float((out[n].double() * e.double()).sum())
+        # differences: third derivatives of order 1 times 1e-8 per direction of 1760 coordinates; kernel: fp32 rounding
+        assert abs(got - want) <= 1e-4 * (1 + float((out[n].double() * e.double()).abs().sum())), (n, got, want)
+
+
+def _exact_output(q, k, v, lo, hi, pos, cap, slopes):
+    return reference(q, k, v, lo, hi, pos, cap=cap, slopes=slopes)["o"]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF], ids=str)
+@pytest.mark.parametrize("new,h,hk,d,cap,window", [
+    (1, 8, 2, 128, None, None), (1, 8, 8, 64, 30.0, None), (4, 8, 2, 128, None, 100), (2, 5, 1, 64, 10.0, None),
+    (1, 32, 1, 128, None, None), (3, 24, 2, 96, None, 1), (1, 7, 7, 40, None, None), (17, 4, 2, 128, None, None),
+])
+def test_cached(new, h, hk, d, cap, window, dtype):
+    from flashdiffusion_b200.attention import attend_cached
+    capacity = 1100
+    lengths = [1, 2, 63, 64, 65, 300, 1000, capacity, capacity + 5, 0]
+    q, k, v, _ = _inputs(len(lengths), new, capacity, h, hk, d, dtype, seed=new + h)
+    n = torch.tensor(lengths, dtype=torch.int32)
+    for b, m in enumerate(lengths):            # the cache behind the length was never written
+        k[b, m:] = float("nan")
+        v[b, m:] = float("inf")
+    slopes = torch.linspace(0.5, 0.001, h, device="cuda")
+    lo, hi, pos = spans_of(new, capacity, len(lengths), causal=True, window=window, lengths=n)
+    o, lse = attend_cached(q, k, v, n.cuda(), cap=cap, window=window, slopes=slopes, return_lse=True)
+    ref = reference(q, k, v, lo, hi, pos, cap=cap or 0.0, slopes=slopes)
+    check("o", o, ref, FLOOR[dtype])
+    check("lse", lse, ref)
+
+
+def test_cached_long_and_strided():
+    """A cache longer than one split, in head-major memory, and a view of a larger cache."""
+    from flashdiffusion_b200.attention import attend_cached
+    q, k, v, _ = _inputs(2, 1, 20000, 8, 2, 128, BF, seed=41)
+    n = torch.tensor([20000, 12345], dtype=torch.int32)
+    lo, hi, pos = spans_of(1, 20000, 2, causal=True, lengths=n)
+    ref = reference(q, k, v, lo, hi, pos)
+    a = attend_cached(q, k, v, n.cuda())
+    check("o", a, ref)
+    kt, vt = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (k, v))
+    assert torch.equal(attend_cached(q, kt, vt, n.cuda()), a)
+    big = torch.randn(2, 20000, 4, 256, device="cuda").to(BF)
+    big[:, :, 1:3, 64:192] = k
+    assert torch.equal(attend_cached(q, big[:, :, 1:3, 64:192], v, n.cuda()), a)
+
+
+def test_refuses_on_the_device():
+    from flashdiffusion_b200.attention import Spans, attend, attend_cached
+    q, k, v, _ = _inputs(2, 8, 8, 4, 2, 64, BF)
+    with pytest.raises(ValueError):
+        attend_cached(q.requires_grad_(True), k, v, torch.tensor([8, 8], dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError):
+        attend_cached(q.detach(), k, v, torch.tensor([8], dtype=torch.int32, device="cuda"))
+    with pytest.raises(TypeError):
+        attend_cached(q.detach(), k, v, torch.tensor([8, 8], device="cuda"))
+    s = torch.zeros(7, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        attend(q, k, v, spans=Spans(s, s))
+    with pytest.raises(ValueError):
+        attend(q, k, v, spans=Spans(s.cpu(), s.cpu()))
+
+
+def test_other_stream_and_captured_graph():
+    """Forward and backward on a side stream, and captured and replayed on new inputs, give the eager bits."""
+    from flashdiffusion_b200.attention import attend, attend_cached
+    from flashdiffusion_b200.rope import apply_rotary, rotary_frequencies
+    q, k, v, do = _inputs(1, 200, 200, 4, 2, 128, BF, seed=43)
+    q2, k2, v2, do2 = _inputs(1, 200, 200, 4, 2, 128, BF, seed=44)
+    f, pos = rotary_frequencies(128), torch.arange(200, device="cuda")
+    n = torch.tensor([150], dtype=torch.int32, device="cuda")
+
+    def step(q, k, v, do):
+        a, b, c = (t.detach().requires_grad_(True) for t in (q, k, v))
+        o = attend(*apply_rotary(a, b, positions=pos, freqs=f), c, causal=True, cap=20.0)
+        with torch.no_grad():
+            last = attend_cached(q[:, -1:], k, v, n)
+        return (o.detach(), last, *torch.autograd.grad(o, (a, b, c), do))
+
+    want = [step(q, k, v, do), step(q2, k2, v2, do2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(q, k, v, do)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(got, want[0]))
+    ins = [t.clone() for t in (q, k, v, do)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*ins)
+    for new, w in (((q2, k2, v2, do2), want[1]), ((q, k, v, do), want[0])):
+        for t, x in zip(ins, new):
+            t.copy_(x)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(outs, w))
+
+
+def test_a_prompt_its_training_step_and_its_answers():
+    """The operators together: rotate, attend over a packed prompt, gradients to the unrotated heads; then token by
+    token against the cache, where each answer equals the prompt's row within both calls' rounding."""
+    from flashdiffusion_b200.attention import attend, attend_cached
+    from flashdiffusion_b200.rope import apply_rotary, rotary_frequencies, rotary_magnitude
+    s, h, hk, d = 190, 8, 2, 128
+    q, k, v, do = _inputs(1, s, s, h, hk, d, BF, seed=47)
+    f = rotary_frequencies(d, scaling="parts", factor=4.0, trained=64, device="cuda")
+    mag = rotary_magnitude(4.0)
+    pos = torch.arange(s, device="cuda")
+    a, b, c = (t.clone().requires_grad_(True) for t in (q, k, v))
+    rq, rk = apply_rotary(a, b, positions=pos, freqs=f, magnitude=mag)
+    o = attend(rq, rk, c, causal=True, cap=25.0)
+    da, db, dc = torch.autograd.grad(o, (a, b, c), do)
+    lo, hi, p = spans_of(s, s, 1, causal=True)
+    ref = reference(rq, rk, v, lo, hi, p, cap=25.0, do=do)
+    check("o", o, ref)
+    check("dv", dc, ref)
+    # the rotation's gradient: the reference's dq turned back, in fp32 on the same formula
+    back = apply_rotary(ref["dq"].float().cuda(), positions=pos, freqs=f, magnitude=mag, inverse=True)
+    room = apply_rotary(ref["dq_tol"].float().cuda(), positions=torch.zeros_like(pos), freqs=f, magnitude=mag)
+    pair = room + room.roll(d // 2, -1)      # |cos| a + |sin| b of a pair, at most their sum
+    size = ref["dq"].abs().float().cuda()
+    u = 2.0 ** -8
+    assert ((da.float() - back).abs() <= (pair + u * mag * (size + size.roll(d // 2, -1))) * 1.01 + 1e-6).all()
+    kc = torch.full((1, 256, hk, d), float("nan"), device="cuda", dtype=BF)
+    vc = torch.full_like(kc, float("nan"))
+    n = torch.zeros(1, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        for t in range(s):
+            tq, tk = apply_rotary(q[:, t:t + 1], k[:, t:t + 1], positions=pos[t:t + 1], freqs=f, magnitude=mag)
+            kc[:, t:t + 1], vc[:, t:t + 1] = tk, v[:, t:t + 1]
+            n += 1
+            if t in (0, 1, 63, 64, 127, 128, s - 1):
+                got = attend_cached(tq, kc, vc, n, cap=25.0)
+                one = {"o": ref["o"][:, t:t + 1], "o_tol": ref["o_tol"][:, t:t + 1]}
+                check("o", got, one)
