@@ -1,6 +1,6 @@
 // Entry points of softmax attention over key spans (declared in
 // include/fd_sm100.h): argument checks and the choice of kernels.
-#include "fd_attn.cuh"
+#include "fd_attn_tc.cuh"
 
 namespace fd {
 namespace attn {
@@ -123,6 +123,7 @@ int fd_attention_forward(const fd_attention_args* r, void* workspace, size_t wor
     (void)workspace;
     (void)workspace_bytes;
     if (a.batch == 0 || a.q_len == 0) return FD_OK;
+    if (attn::tc_applies(a, r->dtype, false)) return attn::tc_forward(a, r->dtype, (cudaStream_t)stream);
     return attn::simt_forward(a, r->dtype, (cudaStream_t)stream);
 }
 

@@ -1,0 +1,487 @@
+// Forward softmax attention on the tensor cores.
+//
+//   S = Q K^T           tcgen05.mma, both operands from shared memory, fp32 in TMEM
+//   P = 2^(x - m)       x the base-2 score, m a running bound of the row (below)
+//   O += P V            P 16-bit in TMEM over S's columns, V as it lies (MN-major)
+//   o = O / l, lse = ln2 (m + log2 l),   l the fp32 sum of the unrounded P
+//
+// One pass over the keys.  m is raised only when a row's new maximum exceeds it
+// by more than 8 (a factor 256): P then stays below 2^8, exact in fp32 and far
+// inside fp16's range, and the O columns of a row are rescaled a few times per
+// row instead of at every tile, by the softmax threads themselves.
+//
+// CTA = 256 query rows of one head (two subtiles of 128) against a stream of
+// 128-key tiles; both subtiles use a K/V tile while it is in shared memory, and
+// the tensor core works on one subtile's products while the other's
+// exponentials are made.  Three warpgroups: two for the softmax (one row per
+// thread), one with a TMA producer, an MMA issuer and a guard that looks at the
+// V tiles of which some row sees only a part (see `guard`).
+#include "fd_attn_tc.cuh"
+
+namespace fd {
+namespace attn {
+namespace fwd {
+
+constexpr int TMA_WARP = 8, MMA_WARP = 9, GUARD_WARP = 10;
+constexpr int NTHREADS = 12 * 32;
+// Registers: 168 a thread at launch (64512 in all); the softmax warpgroups hold a row of 128 scores each and
+// take 208, the third gives up what it does not use: 256 * 208 + 128 * 80 = 63488.
+constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;
+constexpr uint32_t TMEM_COLS = 512;
+
+template <int DP>
+struct Cfg {
+    static constexpr int BOXES = DP / 64;
+    static constexpr uint32_t TILE = BOXES * BOX_BYTES;
+    static constexpr uint32_t Q_BYTES = 2 * TILE;
+    static constexpr int SLOTS = DP == 128 ? 5 : 8;
+    static constexpr uint32_t BAR_OFF = Q_BYTES + SLOTS * TILE;
+    // qfull, full[SLOTS], empty[SLOTS], sfull[2], pfull[2], ofull[2], toguard, guarded
+    static constexpr int NBARS = 1 + 2 * SLOTS + 6 + 2;
+    static constexpr uint32_t MISC_OFF = BAR_OFF + NBARS * 8;
+    static constexpr uint32_t SMEM = MISC_OFF + 64 + 1024;
+    static constexpr uint32_t O_COL = 256;
+    static_assert(SMEM <= 227 * 1024, "shared memory budget");
+    static_assert(O_COL + 2 * DP <= TMEM_COLS, "TMEM budget");
+};
+
+struct Misc {
+    uint32_t tmem;
+    int abort;
+    int poison;          // a partly visible V tile held a NaN or an infinity
+    int lo[2], hi[2];    // keys seen by any row of the subtile: [lo, hi)
+    int flo[2], fhi[2];  // keys seen by every row: [flo, fhi)
+};
+
+template <int DP, bool F16, bool GEN>
+__global__ void __launch_bounds__(NTHREADS, 1)
+forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+               const __grid_constant__ CUtensorMap tmv, const __grid_constant__ Prob a, int n_qt,
+               int* __restrict__ status) {
+    using C = Cfg<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* sQ = base;
+    uint8_t* ring = base + C::Q_BYTES;
+    uint64_t* qfull = (uint64_t*)(base + C::BAR_OFF);
+    uint64_t* full = qfull + 1;
+    uint64_t* empty = full + C::SLOTS;
+    uint64_t* sfull = empty + C::SLOTS;
+    uint64_t* pfull = sfull + 2;
+    uint64_t* ofull = pfull + 2;
+    uint64_t* toguard = ofull + 2;
+    uint64_t* guarded = toguard + 1;
+    Misc& ms = *(Misc*)(base + C::MISC_OFF);
+    volatile int* abort = &ms.abort;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // later query tiles see more keys under a causal mask: they start first
+    const int nh = a.heads * a.batch;
+    const int qt = n_qt - 1 - blockIdx.x / nh;
+    const int bh = blockIdx.x % nh;
+    const int b = bh / a.heads, h = bh - b * a.heads, hk = h / a.group;
+    const int q0 = qt * 2 * T;
+    const int n = keys_of(a, b);
+
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(qfull, 1);
+        for (int i = 0; i < C::SLOTS; ++i) {
+            ptx::mbar_init(&full[i], 1);
+            ptx::mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&sfull[i], 1);
+            ptx::mbar_init(&pfull[i], 4);
+            ptx::mbar_init(&ofull[i], 1);
+            ms.lo[i] = 0x7fffffff;
+            ms.hi[i] = 0;
+            ms.flo[i] = 0;
+            ms.fhi[i] = 0x7fffffff;
+        }
+        ptx::mbar_init(toguard, 1);
+        ptx::mbar_init(guarded, 1);
+        ms.abort = 0;
+        ms.poison = 0;
+        ptx::fence_mbar_init();
+    }
+    if (warp == MMA_WARP) {
+        ptx::tmem_alloc(&ms.tmem, TMEM_COLS);
+        ptx::tmem_relinquish();
+    }
+    if (warp == TMA_WARP && lane == 0) {
+        ptx::prefetch_tmap(&tmq);
+        ptx::prefetch_tmap(&tmk);
+        ptx::prefetch_tmap(&tmv);
+    }
+    __syncthreads();
+
+    const int sub = warp >> 2;                   // softmax warpgroup = query subtile
+    const int row = q0 + threadIdx.x;            // softmax threads: their query row
+    int2 span = make_int2(0, 0);
+    if (sub < 2) {
+        const bool real = row < a.q_len;
+        if (real) span = row_span(a, b, row, n);
+        const bool some = span.y > span.x;
+        const int lo = warp_min(some ? span.x : 0x7fffffff), hi = warp_max(some ? span.y : 0);
+        // rows behind the last query are never stored: they need no mask
+        const int flo = warp_max(!real ? 0 : some ? span.x : 0x7fffffff);
+        const int fhi = warp_min(!real ? 0x7fffffff : some ? span.y : 0);
+        if (!real) span = make_int2(0, 0x7fffffff);
+        if (lane == 0) {
+            atomicMin(&ms.lo[sub], lo);
+            atomicMax(&ms.hi[sub], hi);
+            atomicMax(&ms.flo[sub], flo);
+            atomicMin(&ms.fhi[sub], fhi);
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = ms.tmem;
+    int ta[2], tb[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const bool some = ms.hi[s] > ms.lo[s];
+        ta[s] = some ? ms.lo[s] / T : 0;
+        tb[s] = some ? (ms.hi[s] + T - 1) / T : 0;
+    }
+    // tiles of either subtile; an empty subtile takes no part
+    const int t0 = tb[0] == 0 ? ta[1] : tb[1] == 0 ? ta[0] : min(ta[0], ta[1]);
+    const int t1 = max(tb[0], tb[1]);
+    auto active = [&](int s, int j) { return j >= ta[s] && j < tb[s]; };
+    // some row of an active subtile sees only a part of tile j
+    auto partial = [&](int j) {
+        bool p = false;
+        for (int s = 0; s < 2; ++s) p = p || (active(s, j) && (j * T < ms.flo[s] || (j + 1) * T > ms.fhi[s]));
+        return p;
+    };
+
+    if (sub == 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    if (warp == TMA_WARP) {
+        if (lane == 0 && t1 > t0) {
+            ptx::mbar_expect_tx(qfull, C::Q_BYTES);
+            for (int s = 0; s < 2; ++s)
+                for (int c = 0; c < C::BOXES; ++c)
+                    ptx::tma_load_4d(sQ + s * C::TILE + c * BOX_BYTES, &tmq, qfull, c * 64, q0 + s * T, h, b);
+            const int items = 2 * (t1 - t0);
+            int i = 0;
+            for (; i < items; ++i) {
+                const int slot = i % C::SLOTS, round = i / C::SLOTS;
+                if (!ptx::wait_bounded(&empty[slot], (round & 1) ^ 1, abort, status, WAIT_NS)) break;
+                ptx::mbar_expect_tx(&full[slot], C::TILE);
+                for (int c = 0; c < C::BOXES; ++c)
+                    ptx::tma_load_4d(ring + slot * C::TILE + c * BOX_BYTES, (i & 1) ? &tmv : &tmk, &full[slot], c * 64,
+                                     (t0 + i / 2) * T, hk, b);
+            }
+            if (i < items) {   // gave up: the copies in flight still write into this block's memory
+                wait_landed(qfull, 0);
+                for (int z = max(0, i - C::SLOTS); z < i; ++z) wait_landed(&full[z % C::SLOTS], (z / C::SLOTS) & 1);
+            }
+        }
+    } else if (warp == MMA_WARP) {
+        if (lane == 0 && t1 > t0) {
+            const int ks_qk = (a.dim + 15) / 16;
+            const uint32_t id_qk = ptx::idesc_f32acc(T, T, F16);
+            const uint32_t id_pv = ptx::idesc_f32acc(T, ks_qk * 16, F16) | ptx::IDESC_B_MN;
+            const uint32_t q_base = ptx::smem_u32(sQ), r_base = ptx::smem_u32(ring);
+            auto slot_of = [&](int item) { return item % C::SLOTS; };
+            auto wait_full = [&](int item) {
+                return ptx::wait_bounded(&full[slot_of(item)], (item / C::SLOTS) & 1, abort, status, WAIT_NS);
+            };
+            auto issue_qk = [&](int s, int item) {
+                ptx::tc_fence_after();
+                const uint32_t kb = r_base + slot_of(item) * C::TILE, qb = q_base + s * C::TILE;
+                for (int ks = 0; ks < ks_qk; ++ks)
+                    ptx::umma_ss(tmem + s * T, kmajor(qb, ks), kmajor(kb, ks), id_qk, ks > 0);
+                ptx::umma_commit(&sfull[s]);
+            };
+            bool ok = ptx::wait_bounded(qfull, 0, abort, status, WAIT_NS) && wait_full(0);
+            if (ok) {
+                for (int s = 0; s < 2; ++s)
+                    if (active(s, t0)) issue_qk(s, 0);
+                ptx::umma_commit(&empty[0]);
+            }
+            uint32_t np[2] = {0, 0}, ng = 0;
+            for (int j = t0; j < t1 && ok; ++j) {
+                const int iv = 2 * (j - t0) + 1, ik = iv + 1;
+                ok = wait_full(iv) && (j + 1 == t1 || wait_full(ik));
+                bool look = ok && partial(j);
+                if (look) ptx::mbar_arrive(toguard);
+                for (int s = 0; s < 2 && ok; ++s) {
+                    if (active(s, j)) {
+                        ok = ptx::wait_bounded(&pfull[s], np[s] & 1, abort, status, WAIT_NS);
+                        if (!ok) break;
+                        ++np[s];
+                        if (look) {
+                            ok = ptx::wait_bounded(guarded, ng & 1, abort, status, WAIT_NS);
+                            if (!ok) break;
+                            ++ng;
+                            look = false;
+                        }
+                        ptx::tc_fence_after();
+                        const uint32_t vb = r_base + slot_of(iv) * C::TILE;
+#pragma unroll
+                        for (int ks = 0; ks < T / 16; ++ks)
+                            ptx::umma_ts(tmem + C::O_COL + s * DP, tmem + s * T + ks * 8, mnmajor(vb, ks), id_pv,
+                                         j > ta[s] || ks > 0);
+                        if (j + 1 == tb[s]) ptx::umma_commit(&ofull[s]);
+                    }
+                    if (j + 1 < t1 && active(s, j + 1)) issue_qk(s, ik);
+                }
+                ptx::umma_commit(&empty[slot_of(iv)]);
+                if (j + 1 < t1) ptx::umma_commit(&empty[slot_of(ik)]);
+            }
+        }
+    } else if (warp == GUARD_WARP) {
+        // ---- guard: where some row sees only a part of a tile, its P is zero in
+        //      the masked places, and 0 times a NaN or an infinity in V would reach
+        //      the row all the same.  Such elements become zeros in shared memory
+        //      before the product; the rows that do see them get them back at the
+        //      end (`poison`).  Partly visible tiles are the few at the ends of the
+        //      rows' spans, and the scan runs while their scores are made.
+        uint32_t ng = 0;
+        for (int j = t0; j < t1; ++j) {
+            if (!partial(j)) continue;
+            const int item = 2 * (j - t0) + 1, slot = item % C::SLOTS;
+            // the issuer says when the tile is there (and holds it until the guard answers): waiting for
+            // `full` alone, rounds ahead of the ring, would match an older phase of the same parity
+            if (!ptx::wait_bounded(toguard, ng & 1, abort, status, WAIT_NS)) break;
+            ++ng;
+            if (!ptx::wait_bounded(&full[slot], (item / C::SLOTS) & 1, abort, status, WAIT_NS)) break;
+            uint4* v = (uint4*)(ring + slot * C::TILE);
+            constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+            bool bad = false;
+#pragma unroll 8
+            for (int i = lane; i < (int)C::TILE / 16; i += 32) {
+                const uint4 x = v[i];
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    bad = bad || (w[e] & EXP) == EXP || ((w[e] >> 16) & EXP) == EXP;
+            }
+            if (__any_sync(~0u, bad)) {
+                for (int i = lane; i < (int)C::TILE / 4; i += 32) {
+                    uint32_t x = ((uint32_t*)v)[i];
+                    if ((x & EXP) == EXP) x &= 0xffff0000u;
+                    if (((x >> 16) & EXP) == EXP) x &= 0xffffu;
+                    ((uint32_t*)v)[i] = x;
+                }
+                ptx::fence_async_shared();
+                if (lane == 0) ms.poison = 1;
+                __syncwarp();
+            }
+            if (lane == 0) ptx::mbar_arrive(guarded);
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+        // ---- softmax: one query row per thread
+        const uint32_t s_addr = tmem + ((uint32_t)(warp & 3) << 21) + sub * T;
+        const uint32_t o_addr = tmem + ((uint32_t)(warp & 3) << 21) + C::O_COL + sub * DP;
+        Score sc;
+        sc.cap2 = a.cap * LOG2E;
+        sc.c = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E;
+        sc.slope2 = GEN && a.slopes ? a.slopes[h] * LOG2E : 0.f;
+        // plain scores stay raw until the exponential's own multiply-add
+        const float c = GEN ? 1.f : sc.c;
+        const float room = GEN ? 8.f : 8.f / sc.c;
+        const int pos = n - a.q_len + row;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        int it = 0;
+        for (int j = ta[sub]; j < tb[sub]; ++j, ++it) {
+            if (!ptx::wait_bounded(&sfull[sub], it & 1, abort, status, WAIT_NS)) { ok = false; break; }
+            ptx::tc_fence_after();
+            uint32_t x[4][32];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) ptx::tmem_ld32(s_addr + g * 32, x[g]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) ptx::tmem_wait_ld(x[g]);
+            float(&v)[4][32] = reinterpret_cast<float(&)[4][32]>(x);
+            if (GEN) {
+                const float at = (float)(pos - j * T);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[g][i] *= sc.c;
+                    if (sc.cap2 > 0.f) {
+                        tanh_n(v[g]);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[g][i] *= sc.cap2;
+                    }
+                    if (sc.slope2 != 0.f) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[g][i] = fmaf(-sc.slope2, fabsf(at - (float)(g * 32 + i)), v[g][i]);
+                    }
+                }
+            }
+            const int lo = span.x - j * T, len = span.y - span.x;
+            if (!__all_sync(~0u, lo <= 0 && (int64_t)lo + len >= T)) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if ((uint32_t)(g * 32 + i - lo) >= (uint32_t)len) v[g][i] = -INFINITY;
+            }
+            float top[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                top[g] = v[g][0];
+#pragma unroll
+                for (int i = 1; i < 32; ++i) top[g] = fmaxf(top[g], v[g][i]);
+            }
+            const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const bool raise = mt > m + room;
+            if (__any_sync(~0u, raise)) {
+                const float mn = raise ? mt : m;
+                const float fix = m == -INFINITY ? 0.f : ptx::ex2_mufu((m - mn) * c);
+                m = mn;
+                l *= fix;
+                if (it > 0) {
+                    // S's commit also covered the previous P V, so O is at rest
+#pragma unroll 1
+                    for (int g = 0; g < DP; g += 16) {
+                        uint32_t o[16];
+                        ptx::tmem_ld16(o_addr + g, o);
+                        ptx::tmem_wait_ld16(o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+                        ptx::tmem_st16(o_addr + g, o);
+                    }
+                }
+            }
+            const float off = m == -INFINITY ? 0.f : -m * c;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e0 = ptx::ex2_mufu(fmaf(v[g][2 * i], c, off));
+                    const float e1 = ptx::ex2_mufu(fmaf(v[g][2 * i + 1], c, off));
+                    part[g] += e0 + e1;
+                    p[i] = ptx::pack16<F16>(e0, e1);
+                }
+                ptx::tmem_st16(s_addr + g * 16, p);
+            }
+            l += (part[0] + part[1]) + (part[2] + part[3]);
+            ptx::tmem_wait_st();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&pfull[sub]);
+        }
+        if (it > 0 && ok) ok = ptx::wait_bounded(&ofull[sub], 0, abort, status, WAIT_NS);
+        ptx::tc_fence_after();
+        const bool real = row < a.q_len;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint8_t* out = (uint8_t*)a.o.p + 2 * (b * a.o.sb + (int64_t)row * a.o.ss + h * a.o.sh);
+        const bool poison = it > 0 && *(volatile int*)&ms.poison;
+#pragma unroll 1
+        for (int g = 0; g < DP; g += 32) {
+            uint32_t o[32];
+            if (it > 0 && ok) {
+                ptx::tmem_ld32(o_addr + g, o);
+                ptx::tmem_wait_ld(o);
+            }
+            float(&f)[32] = reinterpret_cast<float(&)[32]>(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = l == 0.f ? 0.f : f[i] * inv;
+            if (poison && real && l != 0.f) {
+                // put back what the guard took out, for the keys that this row sees
+                for (int j = ta[sub]; j < tb[sub]; ++j) {
+                    if (!partial(j)) continue;
+                    for (int k = max(span.x, j * T); k < min(span.y, (j + 1) * T); ++k) {
+                        const uint16_t* vr = (const uint16_t*)a.v.p + b * a.v.sb + (int64_t)k * a.v.ss + hk * a.v.sh + g;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (g + i >= a.dim) continue;
+                            const uint16_t w = vr[i];
+                            constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
+                            if ((w & EXP) == EXP) f[i] += F16 ? __half2float(__ushort_as_half(w))
+                                                              : __bfloat162float(__ushort_as_bfloat16(w));
+                        }
+                    }
+                }
+            }
+            if (real) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (g + i * 8 >= a.dim) continue;
+                    uint4 w;
+                    w.x = ptx::pack16<F16>(f[8 * i], f[8 * i + 1]);
+                    w.y = ptx::pack16<F16>(f[8 * i + 2], f[8 * i + 3]);
+                    w.z = ptx::pack16<F16>(f[8 * i + 4], f[8 * i + 5]);
+                    w.w = ptx::pack16<F16>(f[8 * i + 6], f[8 * i + 7]);
+                    *(uint4*)(out + 2 * (g + i * 8)) = w;
+                }
+            }
+        }
+        if (real && a.lse)
+            a.lse[((int64_t)b * a.heads + h) * a.q_len + row] = l == 0.f ? -INFINITY : (m * c + log2f(l)) * LN2;
+        ptx::tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == MMA_WARP) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+template <int DP, bool F16, bool GEN>
+int launch(const Prob& a, cudaStream_t s) {
+    CUtensorMap q, k, v;
+    FD_TRY(make_head_map(&q, a.q, a.q_len, a.heads, a.batch, a.dim, F16));
+    FD_TRY(make_head_map(&k, a.k, a.k_len, a.kv_heads, a.batch, a.dim, F16));
+    FD_TRY(make_head_map(&v, a.v, a.k_len, a.kv_heads, a.batch, a.dim, F16));
+    int* status = nullptr;
+    FD_TRY(status_word(&status));
+    auto fn = forward_kernel<DP, F16, GEN>;
+    FD_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM));
+    const int n_qt = (int)cdiv(a.q_len, 2 * T);
+    const int64_t blocks = (int64_t)n_qt * a.heads * a.batch;
+    FD_CHECK_ARG(blocks <= 0x7fffffff, "fd_attention: too many query tiles");
+    fn<<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, a, n_qt, status);
+    FD_CUDA_TRY(cudaGetLastError());
+    return FD_OK;
+}
+
+template <int DP>
+int by_type(const Prob& a, int dtype, cudaStream_t s) {
+    // the plain kernel keeps raw scores and needs them to grow with the products
+    const bool gen = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
+    if (dtype == FD_DTYPE_F16) return gen ? launch<DP, true, true>(a, s) : launch<DP, true, false>(a, s);
+    return gen ? launch<DP, false, true>(a, s) : launch<DP, false, false>(a, s);
+}
+
+}  // namespace fwd
+
+int make_head_map(CUtensorMap* map, const View& v, int64_t rows, int heads, int batch, int dim, bool f16) {
+    EncodeTiledFn enc;
+    FD_TRY(get_encode(&enc));
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
+    // an extent of 1 never takes its stride; the map still wants a multiple of 16 bytes
+    auto bytes = [&](int64_t stride, int64_t extent) { return (cuuint64_t)(extent > 1 ? stride * 2 : 16 * cdiv(dim, 8)); };
+    const cuuint64_t strides[3] = {bytes(v.ss, rows), bytes(v.sh, heads), bytes(v.sb, batch)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)T, 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.p, dims,
+                           strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(FD_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return FD_OK;
+}
+
+bool tc_applies(const Prob& a, int dtype, bool backward) {
+    if (dtype != FD_DTYPE_F16 && dtype != FD_DTYPE_BF16) return false;
+    if (a.dim % 8 || a.dim > 128 || a.q_len == 0 || a.k_len == 0) return false;
+    const int64_t qe[3] = {a.batch, a.q_len, a.heads}, ke[3] = {a.batch, a.k_len, a.kv_heads};
+    if (!tma_view(a.q, qe) || !tma_view(a.k, ke) || !tma_view(a.v, ke) || !tma_view(a.o, qe)) return false;
+    return !backward;
+}
+
+int tc_forward(const Prob& a, int dtype, cudaStream_t s) {
+    return a.dim <= 64 ? fwd::by_type<64>(a, dtype, s) : fwd::by_type<128>(a, dtype, s);
+}
+
+}  // namespace attn
+}  // namespace fd

@@ -72,9 +72,13 @@ const char* fd_last_error(void) { return g_err; }
 int fd_version(void) { return 100; }
 
 int fd_device_supported(int device) {
-    cudaDeviceProp prop;
-    if (cudaGetDeviceProperties(&prop, device) != cudaSuccess) return 0;
-    return prop.major == 10 ? 1 : 0;
+    // one attribute: cudaGetDeviceProperties takes milliseconds, and Python asks at every call
+    int major = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return major == 10 ? 1 : 0;
 }
 
 int fd_check_status(void* stream) {

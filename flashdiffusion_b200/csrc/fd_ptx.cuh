@@ -95,6 +95,14 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
         ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_u32(bar))
         : "memory");
 }
+// Box at (x, y, z, w) of a 4-D tensor map.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
 // 1-D bulk copy global -> shared (no multicast); both addresses 16-byte aligned,
 // size a multiple of 16.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -171,6 +179,17 @@ __device__ __forceinline__ uint64_t sw64_kmajor_desc(uint32_t saddr) {
            ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
 }
 
+// MN-major operand (the contracted index runs over rows of 128 bytes): 64
+// contiguous 16-bit elements of the kept index per row, 128-byte swizzle, groups
+// of 8 rows 1024 B apart; `block` bytes between blocks of 64 kept elements.
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr, uint32_t block) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Instruction descriptor bit: the B operand is MN-major.
+constexpr uint32_t IDESC_B_MN = 1u << 16;
+
 // Instruction descriptor, kind::f16: A and B of the same 16-bit type (fp16
 // when f16, else bf16), both K-major, fp32 D, shape MxN.
 __host__ __device__ constexpr uint32_t idesc_f32acc(int M, int N, bool f16) {
@@ -239,11 +258,31 @@ __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// Order generic-proxy writes to shared memory before later async-proxy reads (tensor core, TMA).
+__device__ __forceinline__ void fence_async_shared() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ float rcp_mufu(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // MUFU base-2 exponential (approximate, flush-to-zero).
 __device__ __forceinline__ float ex2_mufu(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two fp32 -> packed 16-bit pair (lo in the low half), rounded to nearest.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    uint32_t r;
+    if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
 // ---- packed fp32 pairs (sm_100 f32x2 arithmetic) ---------------------------

@@ -622,12 +622,7 @@ __global__ void tcw_fixup_kernel(const double* __restrict__ part, Sched sc, int6
 
 // ---- host side -----------------------------------------------------------------
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-
-static int get_encode(EncodeTiledFn* fn) {
+int get_encode(EncodeTiledFn* fn) {
     static EncodeTiledFn cached = nullptr;
     if (!cached) {
         cudaDriverEntryPointQueryResult q;

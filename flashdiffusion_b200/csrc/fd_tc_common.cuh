@@ -219,6 +219,11 @@ __device__ __forceinline__ uint64_t exp2_poly2(uint32_t a, uint32_t b) {
 }  // namespace tc
 
 // Host helpers defined in fd_tc.cu.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                  CUtensorMapFloatOOBfill);
+int get_encode(EncodeTiledFn* fn);
 // 2-D map over a [rows][cols] 16-bit row-major matrix, box_cols x box_rows boxes
 // with the swizzle that matches box_cols (64 -> 128 B, 32 -> 64 B, 16 -> 32 B).
 int make_tile_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int box_rows, bool f16,
