@@ -122,8 +122,16 @@ def _strides(t: torch.Tensor):
     return native._L3(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
 
 
-def _coordinates_together(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _loadable(t: torch.Tensor) -> torch.Tensor:
+    """t as the kernels take it: contiguous coordinates, and 16-bit heads that the tensor-core kernels could take
+    at 16-byte steps in memory.  A copy is made of what is not: it costs one pass over t."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        return t.contiguous()
+    if t.dtype == torch.float32 or t.shape[-1] % 8 or t.shape[-1] > 128:
+        return t
+    if t.data_ptr() % 16 or any(t.shape[i] > 1 and (t.stride(i) == 0 or t.stride(i) % 8) for i in range(3)):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def _arguments(q, k, v, o, lse, how) -> native.AttentionArgs:
@@ -155,7 +163,7 @@ def _call(fn, a, backward, device):
 
 
 def _forward(q, k, v, how, want_lse):
-    q, k, v = (_coordinates_together(t) for t in (q, k, v))
+    q, k, v = (_loadable(t) for t in (q, k, v))
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if want_lse else None
     _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, how), 0, q.device)
@@ -165,7 +173,7 @@ def _forward(q, k, v, how, want_lse):
 class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, how):
-        q, k, v = (_coordinates_together(t) for t in (q, k, v))
+        q, k, v = (_loadable(t) for t in (q, k, v))
         o, lse = _forward(q, k, v, how, True)
         spans, _, _, _, slopes, _, _ = how
         masks = () if spans is None else (spans.first, spans.end)
@@ -178,7 +186,7 @@ class _Attend(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, do, _):
         q, k, v, o, lse = ctx.saved_tensors[:5]
-        do = _coordinates_together(do)
+        do = _loadable(do)
         a = _arguments(q, k, v, o, lse, ctx.how)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         a.d_o, a.do_stride = do.data_ptr(), _strides(do)

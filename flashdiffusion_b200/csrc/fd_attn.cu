@@ -1,5 +1,7 @@
 // Entry points of softmax attention over key spans (declared in
 // include/fd_sm100.h): argument checks and the choice of kernels.
+#include <algorithm>
+
 #include "fd_attn_tc.cuh"
 
 namespace fd {
@@ -114,7 +116,7 @@ extern "C" {
 
 size_t fd_attention_workspace_bytes(const fd_attention_args* r, int backward) {
     if (!r || r->batch < 0 || r->q_len < 0 || r->k_len < 0 || r->heads < 1) return 0;
-    return backward ? attn::delta_bytes(r) : 0;
+    return backward ? std::max(attn::delta_bytes(r), attn::tc_backward_bytes(r->batch, r->heads, r->q_len)) : 0;
 }
 
 int fd_attention_forward(const fd_attention_args* r, void* workspace, size_t workspace_bytes, void* stream) {
@@ -136,6 +138,7 @@ int fd_attention_backward(const fd_attention_args* r, void* workspace, size_t wo
         return set_error(FD_ERR_WORKSPACE, "fd_attention_backward: workspace %zu bytes, %zu needed", workspace_bytes, need);
     FD_CHECK_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0),
                  "fd_attention_backward: workspace must be 256-byte aligned");
+    if (attn::tc_applies(a, r->dtype, true)) return attn::tc_backward(a, r->dtype, workspace, (cudaStream_t)stream);
     return attn::simt_backward(a, r->dtype, (float*)workspace, (cudaStream_t)stream);
 }
 

@@ -6,8 +6,8 @@
 //   o = O / l, lse = ln2 (m + log2 l),   l the fp32 sum of the unrounded P
 //
 // One pass over the keys.  m is raised only when a row's new maximum exceeds it
-// by more than 8 (a factor 256): P then stays below 2^8, exact in fp32 and far
-// inside fp16's range, and the O columns of a row are rescaled a few times per
+// by more than 8 (a factor 256): P then stays below 2^8 (fp16: times 2^7, so that
+// weights down to 2^-21 of the largest stay normal and the largest fit), and the O columns of a row are rescaled a few times per
 // row instead of at every tile, by the softmax threads themselves.
 //
 // CTA = 256 query rows of one head (two subtiles of 128) against a stream of
@@ -59,6 +59,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                const __grid_constant__ CUtensorMap tmv, const __grid_constant__ Prob a, int n_qt,
                int* __restrict__ status) {
     using C = Cfg<DP>;
+    constexpr float P_SHIFT = F16 ? 7.f : 0.f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = base;
@@ -351,7 +352,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                     }
                 }
             }
-            const float off = m == -INFINITY ? 0.f : -m * c;
+            const float off = m == -INFINITY ? 0.f : fmaf(-m, c, P_SHIFT);
             float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -418,7 +419,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             }
         }
         if (real && a.lse)
-            a.lse[((int64_t)b * a.heads + h) * a.q_len + row] = l == 0.f ? -INFINITY : (m * c + log2f(l)) * LN2;
+            a.lse[((int64_t)b * a.heads + h) * a.q_len + row] = l == 0.f ? -INFINITY : (m * c + (log2f(l) - P_SHIFT)) * LN2;
         ptx::tc_fence_before();
     }
     __syncthreads();
@@ -476,7 +477,8 @@ bool tc_applies(const Prob& a, int dtype, bool backward) {
     if (a.dim % 8 || a.dim > 128 || a.q_len == 0 || a.k_len == 0) return false;
     const int64_t qe[3] = {a.batch, a.q_len, a.heads}, ke[3] = {a.batch, a.k_len, a.kv_heads};
     if (!tma_view(a.q, qe) || !tma_view(a.k, ke) || !tma_view(a.v, ke) || !tma_view(a.o, qe)) return false;
-    return !backward;
+    if (!backward) return true;
+    return tma_view(a.d_o, qe) && tma_view(a.dq, qe) && tma_view(a.dk, ke) && tma_view(a.dv, ke);
 }
 
 int tc_forward(const Prob& a, int dtype, cudaStream_t s) {

@@ -93,6 +93,8 @@ __device__ __forceinline__ int warp_max(int x) { return __reduce_max_sync(~0u, x
 // Launchers of the tensor-core kernels.
 bool tc_applies(const Prob& a, int dtype, bool backward);
 int tc_forward(const Prob& a, int dtype, cudaStream_t s);
+size_t tc_backward_bytes(int64_t batch, int64_t heads, int64_t q_len);
+int tc_backward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
 
 }  // namespace attn
 }  // namespace fd
