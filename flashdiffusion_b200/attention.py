@@ -156,9 +156,9 @@ def _arguments(q, k, v, o, lse, how) -> native.AttentionArgs:
 def _call(fn, a, backward, device):
     lib = native.load()
     # the caching allocator's own buffer per call: streams and captured graphs never share it
-    nbytes = int(lib.fd_attention_workspace_bytes(ctypes.byref(a), backward))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     with torch.cuda.device(device):
+        nbytes = int(lib.fd_attention_workspace_bytes(ctypes.byref(a), backward))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         native.check(fn(ctypes.byref(a), native._ptr(ws), nbytes, native._stream(device)))
 
 

@@ -116,16 +116,23 @@ extern "C" {
 
 size_t fd_attention_workspace_bytes(const fd_attention_args* r, int backward) {
     if (!r || r->batch < 0 || r->q_len < 0 || r->k_len < 0 || r->heads < 1) return 0;
-    return backward ? std::max(attn::delta_bytes(r), attn::tc_backward_bytes(r->batch, r->heads, r->q_len)) : 0;
+    if (backward) return std::max(attn::delta_bytes(r), attn::tc_backward_bytes(r->batch, r->heads, r->q_len));
+    const bool few = r->kv_heads > 0 && (int64_t)(r->heads / r->kv_heads) * r->q_len <= attn::MAX_ROWS;
+    return few && r->dtype != FD_DTYPE_F32 && r->dim <= 128 ? align256(attn::rows_bytes(r->dim)) : 0;
 }
 
 int fd_attention_forward(const fd_attention_args* r, void* workspace, size_t workspace_bytes, void* stream) {
     attn::Prob a;
     FD_TRY(attn::to_prob(r, false, &a));
-    (void)workspace;
-    (void)workspace_bytes;
     if (a.batch == 0 || a.q_len == 0) return FD_OK;
-    if (attn::tc_applies(a, r->dtype, false)) return attn::tc_forward(a, r->dtype, (cudaStream_t)stream);
+    const size_t need = fd_attention_workspace_bytes(r, 0);
+    if (workspace_bytes < need)
+        return set_error(FD_ERR_WORKSPACE, "fd_attention_forward: workspace %zu bytes, %zu needed", workspace_bytes, need);
+    FD_CHECK_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0),
+                 "fd_attention_forward: workspace must be 256-byte aligned");
+    const bool tc = attn::tc_applies(a, r->dtype, false);
+    if (tc && attn::rows_applies(a)) return attn::rows_forward(a, r->dtype, workspace, (cudaStream_t)stream);
+    if (tc) return attn::tc_forward(a, r->dtype, (cudaStream_t)stream);
     return attn::simt_forward(a, r->dtype, (cudaStream_t)stream);
 }
 

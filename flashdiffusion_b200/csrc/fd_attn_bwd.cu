@@ -250,7 +250,7 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
     // ring B: dO or V
     uint64_t *opfull = bars, *afull = bars + 1, *aempty = afull + C::STAGES, *bfull = aempty + C::STAGES,
              *bempty = bfull + C::STAGES, *sfull = bempty + C::STAGES, *sread = sfull + 1, *pfull = sread + 1,
-             *dpfull = pfull + 1, *dsfull = dpfull + 2, *accfull = dsfull + 1, *toguard = accfull + 1,
+             *dpfull = pfull + 1, *dsfull = dpfull + 2, *accfull = dsfull + 2, *toguard = accfull + 1,
              *guarded = toguard + 1;
     Misc& ms = *(Misc*)(base + C::MISC_OFF);
     volatile int* abort = &ms.abort;
@@ -289,7 +289,8 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         ptx::mbar_init(pfull, 8);
         ptx::mbar_init(&dpfull[0], 1);
         ptx::mbar_init(&dpfull[1], 1);
-        ptx::mbar_init(dsfull, 8);
+        ptx::mbar_init(&dsfull[0], 8);
+        ptx::mbar_init(&dsfull[1], 8);
         ptx::mbar_init(accfull, 1);
         ptx::mbar_init(toguard, 1);
         ptx::mbar_init(guarded, 1);
@@ -440,7 +441,7 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
                         sum(DV, S, rb, st, i > 0);
                         ptx::umma_commit(&bempty[st]);
                         if (i + 1 < items && !(ok = first(i + 1))) break;
-                        if (!(ok = wait(dsfull, i))) break;
+                        if (!(ok = wait(&dsfull[0], i))) break;
                         sum(DK, DPT, ra, st, i > 0);
                         ptx::umma_commit(&aempty[st]);
                         if (i + 1 < items) ok = second(i + 1);
@@ -467,7 +468,9 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
                             if (!(ok = wait(sread, i))) break;
                             if (!(ok = both(i + 1))) break;
                         }
-                        if (!(ok = wait(dsfull, i))) break;
+                        // one barrier for each dP buffer: a warp may be a tile ahead of another, and its
+                        // arrival for i + 1 must not stand in for the other's for i
+                        if (!(ok = wait(&dsfull[i & 1], i >> 1))) break;
                         if (look) {
                             if (!(ok = wait(guarded, ng))) break;
                             ++ng;
@@ -660,7 +663,7 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
             ptx::tmem_wait_st();
             ptx::tc_fence_before();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(dsfull);
+            if (lane == 0) ptx::mbar_arrive(&dsfull[buf]);
         }
         bool have = items > 0 && ok;
         if (have) have = ptx::wait_bounded(accfull, 0, abort, status, WAIT_NS);

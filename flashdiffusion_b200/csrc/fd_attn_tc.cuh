@@ -93,6 +93,12 @@ __device__ __forceinline__ int warp_max(int x) { return __reduce_max_sync(~0u, x
 // Launchers of the tensor-core kernels.
 bool tc_applies(const Prob& a, int dtype, bool backward);
 int tc_forward(const Prob& a, int dtype, cudaStream_t s);
+// Few rows against many keys (fd_attn_rows.cu), where tc_applies: up to MAX_ROWS query rows per key head; above,
+// the 128-row tcgen05 tiles are full enough.
+constexpr int MAX_ROWS = 64;
+bool rows_applies(const Prob& a);
+size_t rows_bytes(int dim);
+int rows_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
 size_t tc_backward_bytes(int64_t batch, int64_t heads, int64_t q_len);
 int tc_backward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
 
