@@ -20,7 +20,6 @@ key/value cache of which ``lengths`` rows are in use.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -86,10 +85,8 @@ def document_spans(offsets: torch.Tensor, rows: int, *, causal: bool = True, win
             raise ValueError("a prefix needs causal=True and no window")
     first = torch.empty((1, rows), dtype=torch.int32, device=offsets.device)
     end = torch.empty_like(first)
-    with torch.cuda.device(offsets.device):
-        native.check(native.load().fd_attention_document_spans(
-            native._ptr(offsets), offsets.numel() - 1, native._ptr(prefix), rows, int(causal), window,
-            native._ptr(first), native._ptr(end), native._stream(offsets.device)))
+    native.call(native.load().fd_attention_document_spans, offsets.device, offsets.data_ptr(), offsets.numel() - 1,
+                native._ptr(prefix), rows, int(causal), window, first.data_ptr(), end.data_ptr())
     return Spans(first, end)
 
 
@@ -100,10 +97,8 @@ def prefix_spans(prefix: torch.Tensor, q_len: int, k_len: int | None = None) -> 
     k_len = q_len if k_len is None else int(k_len)
     first = torch.empty((prefix.numel(), q_len), dtype=torch.int32, device=prefix.device)
     end = torch.empty_like(first)
-    with torch.cuda.device(prefix.device):
-        native.check(native.load().fd_attention_prefix_spans(native._ptr(prefix), prefix.numel(), q_len, k_len,
-                                                             native._ptr(first), native._ptr(end),
-                                                             native._stream(prefix.device)))
+    native.call(native.load().fd_attention_prefix_spans, prefix.device, prefix.data_ptr(), prefix.numel(), q_len, k_len,
+                first.data_ptr(), end.data_ptr())
     return Spans(first, end)
 
 
@@ -117,56 +112,51 @@ def _window(window, causal) -> int:
     return min(int(window), 2**31 - 1)
 
 
-def _strides(t: torch.Tensor):
-    # 0 where the extent is 1: a stride that is never taken may be anything
-    return native._L3(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
-
-
 def _loadable(t: torch.Tensor) -> torch.Tensor:
     """t as the kernels take it: contiguous coordinates, and 16-bit heads that the tensor-core kernels could take
     at 16-byte steps in memory.  A copy is made of what is not: it costs one pass over t."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    n0, n1, n2, d = t.shape
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 and d > 1:
         return t.contiguous()
-    if t.dtype == torch.float32 or t.shape[-1] % 8 or t.shape[-1] > 128:
+    if t.dtype == torch.float32 or d % 8 or d > 128:
         return t
-    if t.data_ptr() % 16 or any(t.shape[i] > 1 and (t.stride(i) == 0 or t.stride(i) % 8) for i in range(3)):
+    if (t.data_ptr() % 16 or n0 > 1 and (s0 % 8 or not s0) or n1 > 1 and (s1 % 8 or not s1)
+            or n2 > 1 and (s2 % 8 or not s2)):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _arguments(q, k, v, o, lse, how) -> native.AttentionArgs:
+_NO_GRADIENTS = (0,) * 16
+
+
+def _arguments(q, k, v, o, lse, how, gradients=_NO_GRADIENTS) -> bytes:
+    """fd_attention_args, packed."""
     spans, causal, window, lengths, slopes, scale, cap = how
-    a = native.AttentionArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=_strides(q),
-                             k_stride=_strides(k), v_stride=_strides(v), o=o.data_ptr(), o_stride=_strides(o),
-                             scale=scale, cap=cap, dtype=_DTYPES[q.dtype], causal=int(causal), window=window,
-                             batch=q.shape[0], q_len=q.shape[1], k_len=k.shape[1], heads=q.shape[2],
-                             kv_heads=k.shape[2], dim=q.shape[3])
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    if spans is not None:
-        a.first, a.end = spans.first.data_ptr(), spans.end.data_ptr()
-        a.span_stride = spans.q_len if spans.batch > 1 else 0
-    if lengths is not None:
-        a.lengths = lengths.data_ptr()
-    if slopes is not None:
-        a.slopes = slopes.data_ptr()
-    return a
+    b, sq, h, d = q.shape
+    if spans is None:
+        first = end = step = 0
+    else:
+        first, end, step = spans.first.data_ptr(), spans.end.data_ptr(), sq if spans.batch > 1 else 0
+    return native.PACK_ATTENTION(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], o.data_ptr(),
+        *o.stride()[:3], 0 if lse is None else lse.data_ptr(), first, end, step,
+        0 if lengths is None else lengths.data_ptr(), 0 if slopes is None else slopes.data_ptr(), scale, cap,
+        _DTYPES[q.dtype], causal, window, b, sq, k.shape[1], h, k.shape[2], d, *gradients)
 
 
-def _call(fn, a, backward, device):
-    lib = native.load()
-    # the caching allocator's own buffer per call: streams and captured graphs never share it
-    with torch.cuda.device(device):
-        nbytes = int(lib.fd_attention_workspace_bytes(ctypes.byref(a), backward))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        native.check(fn(ctypes.byref(a), native._ptr(ws), nbytes, native._stream(device)))
+def _call(fn, args, backward, q):
+    # the caching allocator's own buffer for each call: streams and captured graphs never share it
+    nbytes = native.load().fd_attention_workspace_bytes(args, backward)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    native.call(fn, q.device, args, ws.data_ptr() if nbytes else 0, nbytes)
 
 
 def _forward(q, k, v, how, want_lse):
-    q, k, v = (_loadable(t) for t in (q, k, v))
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if want_lse else None
-    _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, how), 0, q.device)
+    """(output, lse or None) of heads that are loadable."""
+    o = q.new_empty(q.shape)
+    lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32) if want_lse else None
+    _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, how), 0, q)
     return o, lse
 
 
@@ -187,12 +177,11 @@ class _Attend(torch.autograd.Function):
     def backward(ctx, do, _):
         q, k, v, o, lse = ctx.saved_tensors[:5]
         do = _loadable(do)
-        a = _arguments(q, k, v, o, lse, ctx.how)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        a.d_o, a.do_stride = do.data_ptr(), _strides(do)
-        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        a.dq_stride, a.dk_stride, a.dv_stride = _strides(dq), _strides(dk), _strides(dv)
-        _call(native.load().fd_attention_backward, a, 1, q.device)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        args = _arguments(q, k, v, o, lse, ctx.how,
+                          (do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                           *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
+        _call(native.load().fd_attention_backward, args, 1, q)
         return dq, dk, dv, None
 
 
@@ -264,7 +253,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         o, lse = _Attend.apply(q, k, v, how)
     else:
-        o, lse = _forward(q, k, v, how, return_lse)
+        o, lse = _forward(_loadable(q), _loadable(k), _loadable(v), how, return_lse)
     if flat:
         o, lse = o[0], None if lse is None else lse[0]
     return (o, lse) if return_lse else o
@@ -290,5 +279,6 @@ def attend_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("attend_cached has no gradient: detach its inputs, or use attend")
     slopes = None if slopes is None else slopes.contiguous()
-    o, lse = _forward(q, k_cache, v_cache, (None, True, _window(window, True), lengths, slopes, scale, cap), return_lse)
+    o, lse = _forward(_loadable(q), _loadable(k_cache), _loadable(v_cache),
+                      (None, True, _window(window, True), lengths, slopes, scale, cap), return_lse)
     return (o, lse) if return_lse else o

@@ -47,7 +47,10 @@ __global__ void prefix_spans_kernel(const int32_t* __restrict__ prefix, int q_le
     end[(int64_t)b * q_len + i] = min(max(e, 0), k_len);
 }
 
-static View view(const void* p, const int64_t* s) { return {const_cast<void*>(p), s[0], s[1], s[2]}; }
+// A stride that is never taken (extent 1) may be anything: it becomes 0.
+static View view(const void* p, const int64_t* s, int batch, int rows, int heads) {
+    return {const_cast<void*>(p), batch > 1 ? s[0] : 0, rows > 1 ? s[1] : 0, heads > 1 ? s[2] : 0};
+}
 
 static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     FD_CHECK_ARG(r, "fd_attention: null arguments");
@@ -66,14 +69,14 @@ static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     FD_CHECK_ARG(!r->first || (!r->causal && !r->window), "fd_attention: spans replace causal and window");
     FD_CHECK_ARG(r->window == 0 || r->causal, "fd_attention: a window needs causal");
     Prob a{};
-    a.q = view(r->q, r->q_stride);
-    a.k = view(r->k, r->k_stride);
-    a.v = view(r->v, r->v_stride);
-    a.o = view(r->o, r->o_stride);
-    a.d_o = view(r->d_o, r->do_stride);
-    a.dq = view(r->dq, r->dq_stride);
-    a.dk = view(r->dk, r->dk_stride);
-    a.dv = view(r->dv, r->dv_stride);
+    a.q = view(r->q, r->q_stride, r->batch, r->q_len, r->heads);
+    a.k = view(r->k, r->k_stride, r->batch, r->k_len, r->kv_heads);
+    a.v = view(r->v, r->v_stride, r->batch, r->k_len, r->kv_heads);
+    a.o = view(r->o, r->o_stride, r->batch, r->q_len, r->heads);
+    a.d_o = view(r->d_o, r->do_stride, r->batch, r->q_len, r->heads);
+    a.dq = view(r->dq, r->dq_stride, r->batch, r->q_len, r->heads);
+    a.dk = view(r->dk, r->dk_stride, r->batch, r->k_len, r->kv_heads);
+    a.dv = view(r->dv, r->dv_stride, r->batch, r->k_len, r->kv_heads);
     a.lse = r->lse;
     a.first = r->first;
     a.end = r->end;

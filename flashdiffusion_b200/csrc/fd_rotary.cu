@@ -193,11 +193,14 @@ extern "C" int fd_rotary(const fd_rotary_args* r, void* stream) {
     rotary::Args a{};
     a.side[0] = {r->q, r->qo, {}, {}, r->heads};
     a.side[1] = {r->k, r->ko, {}, {}, r->kv_heads};
+    // a stride that is never taken (extent 1) may be anything: it becomes 0
     for (int i = 0; i < 3; ++i) {
-        a.side[0].xs[i] = r->q_stride[i];
-        a.side[0].ys[i] = r->qo_stride[i];
-        a.side[1].xs[i] = r->k_stride[i];
-        a.side[1].ys[i] = r->ko_stride[i];
+        const bool lone = (i == 0 && r->batch == 1) || (i == 1 && r->tokens == 1);
+        const bool q1 = lone || (i == 2 && r->heads == 1), k1 = lone || (i == 2 && r->kv_heads == 1);
+        a.side[0].xs[i] = q1 ? 0 : r->q_stride[i];
+        a.side[0].ys[i] = q1 ? 0 : r->qo_stride[i];
+        a.side[1].xs[i] = k1 ? 0 : r->k_stride[i];
+        a.side[1].ys[i] = k1 ? 0 : r->ko_stride[i];
     }
     a.pos = r->positions;
     a.ps[0] = r->position_stride[0];

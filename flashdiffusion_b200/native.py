@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -85,6 +86,11 @@ class RotaryArgs(ctypes.Structure):
                 ("rot", _I)]
 
 
+# The same two structures as packers: one pack() instead of some thirty field stores for each call.
+PACK_ROTARY = struct.Struct("@4P12qP2qPd4i2q4i").pack
+PACK_ATTENTION = struct.Struct("@3P9qP3q3PqPPdd9iP3q3P9q").pack
+
+
 class AttentionArgs(ctypes.Structure):
     """fd_attention_args."""
 
@@ -140,8 +146,13 @@ def _stream(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_devices = {}      # devices found fit, by index
+
+
 def require_device(device=None) -> torch.device:
     """The CUDA device to run on; raises unless it is a B200-class (sm_100) GPU."""
+    if isinstance(device, torch.device) and device.type == "cuda" and device.index in _devices:
+        return _devices[device.index]
     if not torch.cuda.is_available():
         raise RuntimeError("flashdiffusion_b200 needs a CUDA B200 (sm_100a) device; none is visible")
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
@@ -151,7 +162,18 @@ def require_device(device=None) -> torch.device:
     if not load().fd_device_supported(idx):
         cap = torch.cuda.get_device_capability(idx)
         raise RuntimeError(f"device {idx} has compute capability {cap}; libfd_sm100 needs 10.x (B200)")
-    return torch.device("cuda", idx)
+    return _devices.setdefault(idx, torch.device("cuda", idx))
+
+
+def call(fn, device: torch.device, *args) -> None:
+    """fn(*args, current stream of the device) with that device current; raises on an error code."""
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != FD_OK:
+        check(rc)
 
 
 class _Workspace:

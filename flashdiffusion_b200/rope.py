@@ -25,7 +25,6 @@ frequencies scaled for long contexts (``rotary_frequencies``), with gradients.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import numpy as np
@@ -375,30 +374,26 @@ def rotary_magnitude(factor: float) -> float:
     return 0.1 * math.log(factor) + 1.0
 
 
-def _strides3(t: torch.Tensor):
-    """Batch, token and head strides; 0 where the extent is 1, so that nothing hangs on a stride that is never taken."""
-    return native._L3(*(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))
+_NO_STRIDES = (0, 0, 0)
 
 
 def _rotate_heads(xs, positions, freqs, layout, magnitude, inverse, inplace):
     """fd_rotary on one or two (B, S, H, D) tensors; returns the rotated tensors."""
     xs = [x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous() for x in xs]
-    outs = xs if inplace else [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    outs = xs if inplace else [x.new_empty(x.shape) for x in xs]
     q, qo = xs[0], outs[0]
-    k, ko = (xs[1], outs[1]) if len(xs) > 1 else (None, None)
-    a = native.RotaryArgs(q=q.data_ptr(), qo=qo.data_ptr(), q_stride=_strides3(q), qo_stride=_strides3(qo),
-                          positions=positions.data_ptr(),
-                          position_stride=native._L2(*(positions.stride(i) if positions.shape[i] > 1 else 0
-                                                       for i in range(2))),
-                          freqs=freqs.data_ptr(), magnitude=magnitude, dtype=_ROTARY_DTYPES[q.dtype],
-                          position_dtype=_POSITION_DTYPES[positions.dtype], layout=layout, inverse=int(inverse),
-                          batch=q.shape[0], tokens=q.shape[1], heads=q.shape[2], dim=q.shape[3],
-                          rot=2 * freqs.numel())
-    if k is not None:
-        a.k, a.ko, a.k_stride, a.ko_stride, a.kv_heads = (k.data_ptr(), ko.data_ptr(), _strides3(k), _strides3(ko),
-                                                          k.shape[2])
-    with torch.cuda.device(q.device):
-        native.check(native.load().fd_rotary(ctypes.byref(a), native._stream(q.device)))
+    b, s, h, d = q.shape
+    if len(xs) > 1:
+        k, ko = xs[1], outs[1]
+        kp, kop, ks, kos, hk = k.data_ptr(), ko.data_ptr(), k.stride()[:3], ko.stride()[:3], k.shape[2]
+    else:
+        kp = kop = hk = 0
+        ks = kos = _NO_STRIDES
+    args = native.PACK_ROTARY(q.data_ptr(), kp, qo.data_ptr(), kop, *q.stride()[:3], *ks, *qo.stride()[:3], *kos,
+                              positions.data_ptr(), *positions.stride(), freqs.data_ptr(), magnitude,
+                              _ROTARY_DTYPES[q.dtype], _POSITION_DTYPES[positions.dtype], layout, inverse,
+                              b, s, h, hk, d, 2 * freqs.numel())
+    native.call(native.load().fd_rotary, q.device, args)
     return outs
 
 

@@ -54,6 +54,26 @@ def test_spans_refuse():
         attention.prefix_spans(torch.zeros(2, 2, **i32), 10)
 
 
+def test_packed_arguments_are_the_c_structures():
+    """The packers and the ctypes structures lay the same values out the same way."""
+    a = native.AttentionArgs()
+    values = list(range(1, 100))
+    flat = []
+    for name, kind in native.AttentionArgs._fields_:
+        n = 3 if kind is native._L3 else 1
+        take, values = values[:n], values[n:]
+        setattr(a, name, native._L3(*take) if n > 1 else (float(take[0]) if kind is ctypes.c_double else take[0]))
+        flat += [float(x) if kind is ctypes.c_double else x for x in take]
+    assert native.PACK_ATTENTION(*flat) == bytes(a)
+    r, values, flat = native.RotaryArgs(), list(range(1, 100)), []
+    for name, kind in native.RotaryArgs._fields_:
+        n = {native._L3: 3, native._L2: 2}.get(kind, 1)
+        take, values = values[:n], values[n:]
+        setattr(r, name, kind(*take) if n > 1 else (float(take[0]) if kind is ctypes.c_double else take[0]))
+        flat += [float(x) if kind is ctypes.c_double else x for x in take]
+    assert native.PACK_ROTARY(*flat) == bytes(r)
+
+
 def _args(**kw):
     n = 4096
     a = native.AttentionArgs(q=n, k=n, v=n, o=n, scale=1.0, cap=0.0, dtype=native.DTYPE_BF16, batch=1, q_len=8,
