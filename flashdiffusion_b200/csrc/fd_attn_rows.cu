@@ -1,24 +1,24 @@
 // Softmax attention of few query rows against many keys: the newest tokens of
 // each sequence and a cache, and any call of at most MAX_ROWS query rows per key
 // head.  Bandwidth-bound: every visible key and value is read once, and the
-// arithmetic of up to 16 rows (the query heads that share a key head, times the
-// new tokens) rides on one mma.sync tile, whose 16 rows would leave 112 of a
-// tcgen05 tile empty.
+// arithmetic of up to 16 or 32 rows (the query heads that share a key head, times
+// the new tokens) rides on mma.sync tiles of 16 rows; a tcgen05 tile has 128.
 //
 // Work split: the keys in use come from device memory, so the split is made on
-// the device.  All (sequence, key head, row tile) pairs are cut into units of 64
-// keys, laid end to end, and every CTA of a fixed grid takes an equal run of
-// units; lengths from 1 to the longest fill the SMs evenly.  A pair cut between
-// CTAs leaves (m, l, O) partials that join_kernel sums in CTA order (the same
-// bits at every call); a pair inside one CTA is finished there.
+// the device.  The keys of all (sequence, key head, row tile) pairs are cut into
+// units of 64, laid end to end with SETUP units more for each pair (what its
+// start and end cost), and every CTA of a fixed grid takes an equal run: lengths
+// from 1 to the longest fill the SMs evenly.  A pair cut between CTAs leaves
+// (m, l, O) partials that join_kernel sums in CTA order (the same bits at every
+// call); a pair inside one CTA is finished there.
 //
-// Loads go from global memory to registers in 16-byte pieces and are MMA
-// fragments as they are: the order of the contracted coordinate in Q K^T is free
-// (Q is loaded the same way), and so is the order of output coordinates in P V;
-// the pairs of keys that a P V fragment wants are put together by byte
-// permutes.  No shared memory, no barrier in the loop.  P is split in two
-// 16-bit parts, so that it adds no rounding of its own: the second product is
-// hidden behind the loads.
+// Each warp copies its own 16-key blocks with cp.async into a ring of its own,
+// STAGES - 1 blocks ahead and across the ends of pairs, and reads MMA fragments
+// from it in 16-byte pieces: the order of the contracted coordinate in Q K^T is
+// free (Q is loaded the same way), and so is the order of output coordinates in
+// P V; the pairs of keys that a P V fragment wants are put together by byte
+// permutes.  P is split in two 16-bit parts, so that it adds no rounding of its
+// own: the second product hides behind the loads.
 #include <algorithm>
 
 #include "fd_attn_tc.cuh"
@@ -30,6 +30,8 @@ namespace rows {
 constexpr int WARPS = 4;
 constexpr int UNIT = 16 * WARPS;      // keys of a unit: 16 per warp
 constexpr int CTAS_PER_SM = 2;
+constexpr int STAGES = 3;
+constexpr int SETUP = 2;
 
 struct Range {
     int lo, hi;   // keys seen by any row of the sequence, lo on a multiple of 16
@@ -54,9 +56,9 @@ __device__ __forceinline__ Range key_range(const Prob& a, int b) {
     return {lo & ~15, hi};
 }
 
-__device__ __forceinline__ int64_t units_of(const Prob& a, int b) {
-    const Range r = key_range(a, b);
-    return (r.hi - r.lo + UNIT - 1) / UNIT;
+// Units of one pair of this range, its SETUP included; 0 for an empty range.
+__device__ __forceinline__ int units_of(const Range& r) {
+    return r.hi > r.lo ? (r.hi - r.lo + UNIT - 1) / UNIT + SETUP : 0;
 }
 
 struct Plan {
@@ -65,23 +67,34 @@ struct Plan {
     int ctas;
 };
 
-__device__ __forceinline__ int64_t cut(int64_t total, int ctas, int c) { return total * c / ctas; }
+// Equal runs of `total` units for `ctas` CTAs: the first `more` take one more than `each`.
+struct Cut {
+    int64_t total, each, more;
+    int ctas;          // CTAs that have work
+    __device__ Cut(int64_t t, int n) : total(t), ctas((int)min((int64_t)n, t)) {
+        each = ctas ? t / ctas : 0;
+        more = ctas ? t - each * ctas : 0;
+    }
+    __device__ int64_t start(int c) const { return c >= ctas ? total : each * c + min((int64_t)c, more); }
+    __device__ int owner(int64_t u) const {
+        const int64_t wide = more * (each + 1);
+        return (int)(u < wide ? u / (each + 1) : more + (u - wide) / each);
+    }
+};
 
 struct Place {
     int b;             // sequence
     int64_t before;    // units of the sequences before it
-    int64_t total;
 };
 
-// Sum of the units of all sequences, and either the sequence that holds CTA c's
-// first unit (c >= 0) or the units before sequence b (c < 0).  Every warp does it
-// for itself: no barrier.
-__device__ Place find(const Prob& a, const Plan& p, int c, int b) {
+// The units of all sequences and, by `c`, where CTA c's run starts (c >= 0) or
+// the units before sequence b (c < 0).  Every warp does it for itself: no barrier.
+__device__ Cut find(const Prob& a, const Plan& p, int c, int b, Place& at) {
     const int lane = threadIdx.x & 31;
     const int per = (a.batch + 31) / 32, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
     int64_t sum = 0, part = 0;
     for (int i = b0; i < b1; ++i) {
-        const int64_t u = units_of(a, i) * p.pairs;
+        const int64_t u = (int64_t)units_of(key_range(a, i)) * p.pairs;
         sum += u;
         if (i < b) part += u;
     }
@@ -90,29 +103,59 @@ __device__ Place find(const Prob& a, const Plan& p, int c, int b) {
         const int64_t x = __shfl_up_sync(~0u, incl, o);
         if (lane >= o) incl += x;
     }
-    Place r;
-    r.total = __shfl_sync(~0u, incl, 31);
+    const Cut cut(__shfl_sync(~0u, incl, 31), p.ctas);
     if (c < 0) {
         for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(~0u, part, o);
-        r.b = b;
-        r.before = part;
-        return r;
+        at = {b, part};
+        return cut;
     }
-    const int64_t u = cut(r.total, p.ctas, c);
+    const int64_t u = cut.start(c);
     int64_t before = incl - sum;
     const bool mine = u >= before && u < incl;
-    int at = b0;
+    int x = b0;
     if (mine)
-        for (;; ++at) {
-            const int64_t x = units_of(a, at) * p.pairs;
-            if (u < before + x) break;
-            before += x;
+        for (;; ++x) {
+            const int64_t n = (int64_t)units_of(key_range(a, x)) * p.pairs;
+            if (u < before + n) break;
+            before += n;
         }
     const int src = __ffs(__ballot_sync(~0u, mine)) - 1;
-    r.b = src < 0 ? a.batch : __shfl_sync(~0u, at, src);
-    r.before = src < 0 ? r.total : __shfl_sync(~0u, before, src);
-    return r;
+    at.b = src < 0 ? a.batch : __shfl_sync(~0u, x, src);
+    at.before = src < 0 ? cut.total : __shfl_sync(~0u, before, src);
+    return cut;
 }
+
+// A CTA's run, pair by pair.
+struct Walk {
+    Place at;
+    int64_t u, u1;     // next unit, end of the run
+    int b, pair;       // the current pair and its keys [k0, k1) in this run
+    int k0, k1;
+    bool whole, front; // all of the pair; at the front of the run
+    __device__ bool next(const Prob& a, const Plan& p, int64_t u0) {
+        while (u < u1 && at.b < a.batch) {
+            const Range r = key_range(a, at.b);
+            const int ub = units_of(r);
+            const int64_t here = (int64_t)ub * p.pairs, off = u - at.before;
+            if (off >= here) {
+                at.before += here;
+                ++at.b;
+                continue;
+            }
+            pair = (uint64_t)off >> 32 ? (int)(off / ub) : (int)((uint32_t)off / (uint32_t)ub);
+            const int blk = (int)(off - (int64_t)pair * ub);
+            const int take = (int)min((int64_t)(ub - blk), u1 - u);
+            b = at.b;
+            k0 = r.lo + max(blk - SETUP, 0) * UNIT;
+            k1 = min(r.hi, r.lo + max(blk + take - SETUP, 0) * UNIT);
+            whole = blk == 0 && take == ub;
+            front = u == u0;
+            u += take;
+            if (k1 > k0) return true;   // else the run ends inside the pair's SETUP units
+        }
+        return false;
+    }
+};
 
 template <bool F16>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -142,9 +185,19 @@ __device__ __forceinline__ uint4 load16(const uint16_t* p, bool there) {
     return there ? __ldg((const uint4*)p) : make_uint4(0, 0, 0, 0);
 }
 
-// Floats of one partial: O of 16 rows, then their m and l.
-template <int DP>
-constexpr int PART = 16 * DP + 32;
+// 16 bytes to shared memory, zeros where `there` is false (nothing is read then)
+__device__ __forceinline__ void copy16(uint32_t dst, const uint16_t* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// Floats of one partial: O of 16 MT rows, then their m and l.
+template <int DP, int MT>
+constexpr int PART = 16 * MT * (DP + 2);
 
 // out[gr, d .. d + 8) = acc / l, and the row's lse with its first piece
 template <bool F16>
@@ -163,323 +216,450 @@ __device__ __forceinline__ void store_row(const Prob& a, int b, int hk, int gr, 
     if (d == 0 && a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
+template <int DP>
+struct Smem {
+    static constexpr uint32_t HALF = 16 * DP * 2;                 // K or V of a block
+    static constexpr uint32_t RING = WARPS * STAGES * 2 * HALF;
+    static constexpr int PIECES = DP / 8 + 1;                     // 16-byte pieces of one lane's sums: O, and m and l
+    static constexpr uint32_t BYTES = RING + 2 * PIECES * 32 * 16;
+    // two CTAs to an SM: 228 KB, of which each takes 1 KB for itself
+    static_assert(CTAS_PER_SM * (BYTES + 1024) <= 228 * 1024, "shared memory budget");
+};
+
 // Row r of a pair: query i = r / group, head hk * group + r % group.
-template <int DP, bool F16>
+template <int DP, bool F16, int MT>
 __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
 rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, float* __restrict__ parts) {
-    constexpr int KI = DP / 32, VB = DP / 64;
-    __shared__ float so[WARPS][16][DP + 4];
-    __shared__ float sm[WARPS][16], sl[WARPS][16];
+    using S = Smem<DP>;
+    constexpr int KI = DP / 32, VB = DP / 64, CH = DP / 8;   // 16-byte pieces of a row: CH
+    extern __shared__ __align__(16) uint8_t smem[];
+    float4* meet = (float4*)(smem + S::RING);                 // [2][PIECES][lane]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    Place at = find(a, p, blockIdx.x, 0);
-    int64_t u = cut(at.total, p.ctas, blockIdx.x);
-    const int64_t u0 = u, u1 = cut(at.total, p.ctas, blockIdx.x + 1);
+    asm volatile("griddepcontrol.launch_dependents;");
+    Walk w;
+    const Cut cut = find(a, p, blockIdx.x, 0, w.at);
+    if ((int)blockIdx.x >= cut.ctas) return;
+    const int64_t u0 = cut.start(blockIdx.x);
+    w.u = u0;
+    w.u1 = cut.start(blockIdx.x + 1);
     const float c = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
-    while (u < u1 && at.b < a.batch) {
-        const int b = at.b;
-        const Range kr = key_range(a, b);
-        const int64_t ub = (kr.hi - kr.lo + UNIT - 1) / UNIT;
-        if (u >= at.before + ub * p.pairs) {
-            at.before += ub * p.pairs;
-            ++at.b;
-            continue;
-        }
-        const int pair = (int)((u - at.before) / ub);
-        const int blk = (int)((u - at.before) - (int64_t)pair * ub);
-        const int take = (int)min(ub - blk, u1 - u);
-        const bool whole = blk == 0 && take == ub;
-        const int hk = pair / p.row_tiles, rt = pair - hk * p.row_tiles;
-        const int n = keys_of(a, b);
+    const uint32_t ring = ptx::smem_u32(smem) + warp * STAGES * 2 * S::HALF;
 
-        // this thread's rows: g and g + 8 of the tile
-        uint32_t q[2][KI][4];
-        int2 sp[2];
-        int pos[2];
-        float slope2[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int r = rt * 16 + g + 8 * z;
-            const bool real = r < p.rows;
-            const int i = real ? r / a.group : 0, h = hk * a.group + (real ? r % a.group : 0);
-            sp[z] = real ? row_span(a, b, i, n) : make_int2(0, 0);
-            pos[z] = n - a.q_len + i;
-            slope2[z] = a.slopes ? a.slopes[h] * LOG2E : 0.f;
-            const uint16_t* qr = (const uint16_t*)a.q.p + b * a.q.sb + i * a.q.ss + h * a.q.sh;
-#pragma unroll
-            for (int k = 0; k < KI; ++k) {
-                const int d = 32 * k + 8 * t;
-                const uint4 x = load16(qr + d, real && d < a.dim);
-                q[z][k][0] = x.x;
-                q[z][k][1] = x.y;
-                q[z][k][2] = x.z;
-                q[z][k][3] = x.w;
+    // ---- the copies run ahead: block `ahead` of pair `f`
+    Walk f = w;
+    int fk = 0, fend = 0, wr = 0;
+    const uint16_t *fkp = nullptr, *fvp = nullptr;
+    auto fetch = [&]() {
+        while (fk >= fend) {
+            if (!f.next(a, p, u0)) {
+                fk = 0x7fffffff;
+                fend = 0x7fffffff;
+                break;
             }
+            const int hk = f.pair / p.row_tiles;
+            fk = f.k0 + warp * 16;
+            fend = f.k1;
+            fkp = (const uint16_t*)a.k.p + f.b * a.k.sb + hk * a.k.sh;
+            fvp = (const uint16_t*)a.v.p + f.b * a.v.sb + hk * a.v.sh;
         }
-        // keys that every real row sees: [flo, fhi)
-        int flo = max(sp[0].y > sp[0].x ? sp[0].x : 0, sp[1].y > sp[1].x ? sp[1].x : 0);
-        int fhi = 0x7fffffff;
+        if (fk < fend) {
+            const uint32_t dst = ring + wr * 2 * S::HALF;
+#pragma unroll
+            for (int x = 0; x < 16 * CH / 32; ++x) {
+                const int at = x * 32 + lane, r = at / CH, ch = at % CH, key = fk + r;
+                const bool there = key < fend && ch * 8 < a.dim;
+                const int64_t kk = there ? key : fk, cc = there ? ch * 8 : 0;
+                // pieces are swapped within 128 bytes so that the fragment reads below hit every bank once
+                copy16(dst + (r * CH + (ch ^ ((r & 1) << 2))) * 16, fkp + kk * a.k.ss + cc, there);
+                copy16(dst + S::HALF + (r * CH + (ch ^ (r & 6))) * 16, fvp + kk * a.v.ss + cc, there);
+            }
+            fk += UNIT;
+            wr = wr + 1 == STAGES ? 0 : wr + 1;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int x = 0; x < STAGES - 1; ++x) fetch();
+    int rd = 0;
+
+    while (w.next(a, p, u0)) {
+        const int b = w.b, hk = w.pair / p.row_tiles, rt = w.pair - hk * p.row_tiles;
+        const int n = keys_of(a, b);
+        // this thread's rows: g and g + 8 of each 16-row tile
+        uint32_t q[MT][2][KI][4];
+        int2 sp[MT][2];
+        int pos[MT][2];
+        float slope2[MT][2], m[MT][2], l[MT][2];
+        int flo = 0, fhi = 0x7fffffff;   // keys that every row sees: [flo, fhi)
         bool hole = false;
 #pragma unroll
-        for (int z = 0; z < 2; ++z)
-            if (rt * 16 + g + 8 * z < p.rows) {
-                fhi = min(fhi, sp[z].y);
-                hole = hole || sp[z].y <= sp[z].x;
+        for (int y = 0; y < MT; ++y)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int r = (rt * MT + y) * 16 + g + 8 * z;
+                const bool real = r < p.rows;
+                const int i = real ? r / a.group : 0, h = hk * a.group + (real ? r % a.group : 0);
+                sp[y][z] = real ? row_span(a, b, i, n) : make_int2(0, 0);
+                pos[y][z] = n - a.q_len + i;
+                slope2[y][z] = a.slopes ? a.slopes[h] * LOG2E : 0.f;
+                m[y][z] = -INFINITY;
+                l[y][z] = 0.f;
+                const uint16_t* qr = (const uint16_t*)a.q.p + b * a.q.sb + i * a.q.ss + h * a.q.sh;
+#pragma unroll
+                for (int k = 0; k < KI; ++k) {
+                    const int d = 32 * k + 8 * t;
+                    const uint4 x = load16(qr + d, real && d < a.dim);
+                    q[y][z][k][0] = x.x;
+                    q[y][z][k][1] = x.y;
+                    q[y][z][k][2] = x.z;
+                    q[y][z][k][3] = x.w;
+                }
+                if (real) {
+                    if (sp[y][z].y > sp[y][z].x) flo = max(flo, sp[y][z].x);
+                    else hole = true;
+                    fhi = min(fhi, sp[y][z].y);
+                }
             }
         flo = warp_max(flo);
         fhi = warp_min(fhi);
         hole = __any_sync(~0u, hole);
-
-        const uint16_t* kb = (const uint16_t*)a.k.p + b * a.k.sb + hk * a.k.sh;
-        const uint16_t* vb = (const uint16_t*)a.v.p + b * a.v.sb + hk * a.v.sh;
-        float o[VB][8][4];
+        float o[MT][VB][8][4];
 #pragma unroll
-        for (int i = 0; i < VB; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-                for (int z = 0; z < 4; ++z) o[i][e][z] = 0.f;
-
-        const int k_begin = kr.lo + blk * UNIT + warp * 16, k_end = min(kr.hi, kr.lo + (blk + take) * UNIT);
-        uint4 kx[2][KI];
-        auto load_k = [&](int k0) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int key = k0 + 8 * j + g;
-#pragma unroll
-                for (int k = 0; k < KI; ++k)
-                    kx[j][k] = load16(kb + (int64_t)key * a.k.ss + 32 * k + 8 * t, key < k_end && 32 * k + 8 * t < a.dim);
-            }
-        };
-        if (k_begin < k_end) load_k(k_begin);
-#pragma unroll 1
-        for (int k0 = k_begin; k0 < k_end; k0 += UNIT) {
-            uint4 vx[4][VB];
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const int key = k0 + 2 * t + (z & 1) + 8 * (z >> 1);
-#pragma unroll
-                for (int i = 0; i < VB; ++i)
-                    vx[z][i] = load16(vb + (int64_t)key * a.v.ss + 64 * i + 8 * g, key < k_end && 64 * i + 8 * g < a.dim);
-            }
-            float s[2][4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int z = 0; z < 4; ++z) s[j][z] = 0.f;
-#pragma unroll
-                for (int k = 0; k < KI; ++k) {
-                    mma<F16>(s[j], q[0][k][0], q[1][k][0], q[0][k][1], q[1][k][1], kx[j][k].x, kx[j][k].y);
-                    mma<F16>(s[j], q[0][k][2], q[1][k][2], q[0][k][3], q[1][k][3], kx[j][k].z, kx[j][k].w);
-                }
-            }
-            if (k0 + UNIT < k_end) load_k(k0 + UNIT);
-            const bool edge = k0 < flo || k0 + 16 > fhi || hole;
-            // s[j][z]: row g + 8 (z / 2), key k0 + 8 j + 2 t + z % 2
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    const int key = k0 + 8 * j + 2 * t + (z & 1);
-                    float x = s[j][z] * c;
-                    if (cap2 > 0.f) {
-                        const float e = ptx::ex2_mufu(x * (2.f * LOG2E));
-                        x = cap2 * fmaf(-2.f, ptx::rcp_mufu(1.f + e), 1.f);
-                    }
-                    x = fmaf(-slope2[z >> 1], fabsf((float)(pos[z >> 1] - key)), x);
-                    if (edge && (key < sp[z >> 1].x || key >= sp[z >> 1].y)) x = -INFINITY;
-                    s[j][z] = x;
-                }
-            uint32_t ph[2][2], pl[2][2];   // [row g / g + 8][key block]
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                float top = fmaxf(fmaxf(s[0][2 * z], s[0][2 * z + 1]), fmaxf(s[1][2 * z], s[1][2 * z + 1]));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                const float mn = fmaxf(m[z], top), base = mn == -INFINITY ? 0.f : mn;
-                const float fix = ptx::ex2_mufu(m[z] - base);
-                if (__any_sync(~0u, top > m[z])) {
-#pragma unroll
-                    for (int i = 0; i < VB; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            o[i][e][2 * z] *= fix;
-                            o[i][e][2 * z + 1] *= fix;
-                        }
-                }
-                m[z] = mn;
-                l[z] *= fix;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float e0 = ptx::ex2_mufu(s[j][2 * z] - base), e1 = ptx::ex2_mufu(s[j][2 * z + 1] - base);
-                    l[z] += e0 + e1;
-                    ph[z][j] = ptx::pack16<F16>(e0, e1);
-                    const float2 hi = unpack16<F16>(ph[z][j]);
-                    pl[z][j] = ptx::pack16<F16>(e0 - hi.x, e1 - hi.y);
-                }
-            }
-            bool bad = false;
-            if (edge) {
-                // zero times a NaN or an infinity of a masked place would reach the row: such elements of V
-                // become zeros here and are given back below to the rows that see them
-                constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
-#pragma unroll
-                for (int z = 0; z < 4; ++z)
-#pragma unroll
-                    for (int i = 0; i < VB; ++i) {
-                        uint32_t(&w)[4] = reinterpret_cast<uint32_t(&)[4]>(vx[z][i]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if ((w[e] & EXP) == EXP) { w[e] &= 0xffff0000u; bad = true; }
-                            if (((w[e] >> 16) & EXP) == EXP) { w[e] &= 0xffffu; bad = true; }
-                        }
-                    }
-                bad = __any_sync(~0u, bad);
-            }
+        for (int y = 0; y < MT; ++y)
 #pragma unroll
             for (int i = 0; i < VB; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t w0 = reinterpret_cast<uint32_t(&)[4]>(vx[0][i])[e], w1 = reinterpret_cast<uint32_t(&)[4]>(vx[1][i])[e];
-                    const uint32_t w2 = reinterpret_cast<uint32_t(&)[4]>(vx[2][i])[e], w3 = reinterpret_cast<uint32_t(&)[4]>(vx[3][i])[e];
+                for (int e = 0; e < 8; ++e)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const uint32_t b0 = __byte_perm(w0, w1, y ? 0x7632 : 0x5410), b1 = __byte_perm(w2, w3, y ? 0x7632 : 0x5410);
-                        mma<F16>(o[i][2 * e + y], ph[0][0], ph[1][0], ph[0][1], ph[1][1], b0, b1);
-                        mma<F16>(o[i][2 * e + y], pl[0][0], pl[1][0], pl[0][1], pl[1][1], b0, b1);
+                    for (int z = 0; z < 4; ++z) o[y][i][e][z] = 0.f;
+
+#pragma unroll 1
+        for (int k0 = w.k0 + warp * 16; k0 < w.k1; k0 += UNIT) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();
+            const uint32_t sk = ring + rd * 2 * S::HALF, sv = sk + S::HALF;
+            rd = rd + 1 == STAGES ? 0 : rd + 1;
+            float s[MT][2][4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int y = 0; y < MT; ++y)
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) s[y][j][z] = 0.f;
+#pragma unroll
+                for (int k = 0; k < KI; ++k) {
+                    const int r = 8 * j + g;
+                    const uint4 x = lds16(sk + (r * CH + ((4 * k + t) ^ ((r & 1) << 2))) * 16);
+#pragma unroll
+                    for (int y = 0; y < MT; ++y) {
+                        mma<F16>(s[y][j], q[y][0][k][0], q[y][1][k][0], q[y][0][k][1], q[y][1][k][1], x.x, x.y);
+                        mma<F16>(s[y][j], q[y][0][k][2], q[y][1][k][2], q[y][0][k][3], q[y][1][k][3], x.z, x.w);
                     }
                 }
-            if (bad) {
-                for (int key = k0; key < min(k0 + 16, k_end); ++key) {
+            }
+            fetch();
+            const bool edge = k0 < flo || k0 + 16 > fhi || hole;
+            uint32_t ph[MT][2][2], pl[MT][2][2];   // [row g / g + 8][key block]
+#pragma unroll
+            for (int y = 0; y < MT; ++y) {
+                // s[y][j][z]: row g + 8 (z / 2), key k0 + 8 j + 2 t + z % 2
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const int key = k0 + 8 * j + 2 * t + (z & 1);
+                        float x = s[y][j][z] * c;
+                        if (cap2 > 0.f) {
+                            const float e = ptx::ex2_mufu(x * (2.f * LOG2E));
+                            x = cap2 * fmaf(-2.f, ptx::rcp_mufu(1.f + e), 1.f);
+                        }
+                        x = fmaf(-slope2[y][z >> 1], fabsf((float)(pos[y][z >> 1] - key)), x);
+                        if (edge && (key < sp[y][z >> 1].x || key >= sp[y][z >> 1].y)) x = -INFINITY;
+                        s[y][j][z] = x;
+                    }
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    float top = fmaxf(fmaxf(s[y][0][2 * z], s[y][0][2 * z + 1]), fmaxf(s[y][1][2 * z], s[y][1][2 * z + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+                    if (__any_sync(~0u, top > m[y][z])) {
+                        const float mn = fmaxf(m[y][z], top);
+                        const float fix = mn == -INFINITY ? 0.f : ptx::ex2_mufu(m[y][z] - mn);
+                        m[y][z] = mn;
+                        l[y][z] *= fix;
+#pragma unroll
+                        for (int i = 0; i < VB; ++i)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                o[y][i][e][2 * z] *= fix;
+                                o[y][i][e][2 * z + 1] *= fix;
+                            }
+                    }
+                    const float base = m[y][z] == -INFINITY ? 0.f : m[y][z];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float e0 = ptx::ex2_mufu(s[y][j][2 * z] - base), e1 = ptx::ex2_mufu(s[y][j][2 * z + 1] - base);
+                        l[y][z] += e0 + e1;
+                        ph[y][z][j] = ptx::pack16<F16>(e0, e1);
+                        const float2 hi = unpack16<F16>(ph[y][z][j]);
+                        pl[y][z][j] = ptx::pack16<F16>(e0 - hi.x, e1 - hi.y);
+                    }
+                }
+            }
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < VB; ++i) {
+                uint32_t v[4][4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const int r = 2 * t + (z & 1) + 8 * (z >> 1);
+                    const uint4 x = lds16(sv + (r * CH + ((8 * i + g) ^ (r & 6))) * 16);
+                    v[z][0] = x.x;
+                    v[z][1] = x.y;
+                    v[z][2] = x.z;
+                    v[z][3] = x.w;
+                }
+                if (edge) {
+                    // zero times a NaN or an infinity of a masked place would reach the row: such elements
+                    // of V become zeros here and are given back below to the rows that see them
+                    constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if ((v[z][e] & EXP) == EXP) { v[z][e] &= 0xffff0000u; bad = true; }
+                            if (((v[z][e] >> 16) & EXP) == EXP) { v[z][e] &= 0xffffu; bad = true; }
+                        }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t b0 = __byte_perm(v[0][e], v[1][e], x ? 0x7632 : 0x5410);
+                        const uint32_t b1 = __byte_perm(v[2][e], v[3][e], x ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int y = 0; y < MT; ++y) {
+                            mma<F16>(o[y][i][2 * e + x], ph[y][0][0], ph[y][1][0], ph[y][0][1], ph[y][1][1], b0, b1);
+                            mma<F16>(o[y][i][2 * e + x], pl[y][0][0], pl[y][1][0], pl[y][0][1], pl[y][1][1], b0, b1);
+                        }
+                    }
+            }
+            if (__any_sync(~0u, bad)) {
+                const uint16_t* vb = (const uint16_t*)a.v.p + b * a.v.sb + hk * a.v.sh;
+                for (int key = k0; key < min(k0 + 16, w.k1); ++key) {
                     const uint16_t* vr = vb + (int64_t)key * a.v.ss;
 #pragma unroll
                     for (int i = 0; i < VB; ++i)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
 #pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                const int d = 64 * i + 16 * t + 8 * y + e;
+                            for (int x = 0; x < 2; ++x) {
+                                const int d = 64 * i + 16 * t + 8 * x + e;
                                 if (d >= a.dim) continue;
                                 constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
-                                const uint16_t w = vr[d];
-                                if ((w & EXP) != EXP) continue;
-                                if (key >= sp[0].x && key < sp[0].y) o[i][e][y] += one16<F16>(w);
-                                if (key >= sp[1].x && key < sp[1].y) o[i][e][2 + y] += one16<F16>(w);
+                                const uint16_t h = vr[d];
+                                if ((h & EXP) != EXP) continue;
+#pragma unroll
+                                for (int y = 0; y < MT; ++y) {
+                                    if (key >= sp[y][0].x && key < sp[y][0].y) o[y][i][e][x] += one16<F16>(h);
+                                    if (key >= sp[y][1].x && key < sp[y][1].y) o[y][i][e][2 + x] += one16<F16>(h);
+                                }
                             }
                 }
             }
         }
-        // ---- the four warps' sums meet
+        // ---- the four warps' sums meet: 2 and 3 hand theirs to 0 and 1, then 1 to 0
+        float* part = parts + ((int64_t)blockIdx.x * 2 + (w.front ? 0 : 1)) * PART<DP, MT>;
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            l[z] += __shfl_xor_sync(~0u, l[z], 1);
-            l[z] += __shfl_xor_sync(~0u, l[z], 2);
-            if (t == 0) {
-                sm[warp][g + 8 * z] = m[z];
-                sl[warp][g + 8 * z] = l[z];
-            }
+        for (int y = 0; y < MT; ++y) {
 #pragma unroll
-            for (int i = 0; i < VB; ++i)
+            for (int from = 2; from; from >>= 1) {
+                if (warp >= from && warp < 2 * from) {
+                    float4* to = meet + (warp - from) * S::PIECES * 32 + lane;
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
+                    for (int i = 0; i < VB; ++i)
 #pragma unroll
-                    for (int e = 0; e < 8; e += 4)
-                        *(float4*)&so[warp][g + 8 * z][64 * i + 16 * t + 8 * y + e] =
-                            make_float4(o[i][e][2 * z + y], o[i][e + 1][2 * z + y], o[i][e + 2][2 * z + y], o[i][e + 3][2 * z + y]);
-        }
-        __syncthreads();
-        float* part = parts + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * PART<DP>;
-        for (int x = threadIdx.x; x < 16 * (DP / 8); x += WARPS * 32) {
-            const int r = x / (DP / 8), d = x % (DP / 8) * 8, gr = rt * 16 + r;
-            if (gr >= p.rows) continue;
-            float top = sm[0][r];
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm[w][r]);
-            const float base = top == -INFINITY ? 0.f : top;
-            float acc[8] = {}, lsum = 0.f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float f = ptx::ex2_mufu(sm[w][r] - base);
-                lsum = fmaf(f, sl[w][r], lsum);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, so[w][r][d + e], acc[e]);
-            }
-            if (!whole) {
-                *(float4*)(part + r * DP + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                *(float4*)(part + r * DP + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                if (d == 0) {
-                    part[16 * DP + r] = top;
-                    part[16 * DP + 16 + r] = lsum;
+                        for (int e = 0; e < 8; ++e)
+                            to[(i * 8 + e) * 32] = make_float4(o[y][i][e][0], o[y][i][e][1], o[y][i][e][2], o[y][i][e][3]);
+                    to[VB * 8 * 32] = make_float4(m[y][0], m[y][1], l[y][0], l[y][1]);
                 }
-                continue;
+                __syncthreads();
+                if (warp < from) {
+                    const float4* in = meet + warp * S::PIECES * 32 + lane;
+                    const float4 ml = in[VB * 8 * 32];
+                    const float mo[2] = {ml.x, ml.y}, lo[2] = {ml.z, ml.w};
+                    float f0[2], f1[2];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const float mn = fmaxf(m[y][z], mo[z]), base = mn == -INFINITY ? 0.f : mn;
+                        f0[z] = ptx::ex2_mufu(m[y][z] - base);
+                        f1[z] = ptx::ex2_mufu(mo[z] - base);
+                        m[y][z] = mn;
+                        l[y][z] = l[y][z] * f0[z] + lo[z] * f1[z];
+                    }
+#pragma unroll
+                    for (int i = 0; i < VB; ++i)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float4 v = in[(i * 8 + e) * 32];
+                            o[y][i][e][0] = o[y][i][e][0] * f0[0] + v.x * f1[0];
+                            o[y][i][e][1] = o[y][i][e][1] * f0[0] + v.y * f1[0];
+                            o[y][i][e][2] = o[y][i][e][2] * f0[1] + v.z * f1[1];
+                            o[y][i][e][3] = o[y][i][e][3] * f0[1] + v.w * f1[1];
+                        }
+                }
+                __syncthreads();
             }
-            store_row<F16>(a, b, hk, gr, d, acc, top, lsum);
+            if (warp == 0) {
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const int pr = y * 16 + g + 8 * z, gr = rt * MT * 16 + pr;
+                    float ls = l[y][z];
+                    ls += __shfl_xor_sync(~0u, ls, 1);
+                    ls += __shfl_xor_sync(~0u, ls, 2);
+                    if (gr >= p.rows) continue;
+#pragma unroll
+                    for (int i = 0; i < VB; ++i)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int d = 64 * i + 16 * t + 8 * x;
+                            float acc[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) acc[e] = o[y][i][e][2 * z + x];
+                            if (w.whole) {
+                                store_row<F16>(a, b, hk, gr, d, acc, m[y][z], ls);
+                            } else {
+                                *(float4*)(part + pr * DP + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                                *(float4*)(part + pr * DP + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                            }
+                        }
+                    if (!w.whole && t == 0) {
+                        part[16 * MT * DP + pr] = m[y][z];
+                        part[16 * MT * (DP + 1) + pr] = ls;
+                    }
+                }
+            }
         }
-        __syncthreads();
-        u += take;
     }
 }
 
-// Pairs that were cut: their partials in CTA order.  Pairs that see no key: zeros.
-template <int DP, bool F16>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p,
+// Pairs that were cut: their partials, in CTA order.  Pairs that see no key: zeros.
+// Block: one pair after another; up to 256 threads share the (row, 8 coordinates)
+// pieces of it, and where those are fewer the partials too (summed in group order).
+template <int DP, bool F16, int MT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p,
                                                    const float* __restrict__ parts, int64_t per_block) {
+    constexpr int CH = DP / 8;
+    __shared__ float sacc[256][9];
+    __shared__ float sml[256][2];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t all = (int64_t)a.batch * p.pairs;
     const int64_t p0 = min(blockIdx.x * per_block, all), p1 = min(p0 + per_block, all);
     if (p0 >= p1) return;
-    Place at = find(a, p, -1, (int)(p0 / p.pairs));
-    auto owner = [&](int64_t u) {
-        int c = (int)min((int64_t)p.ctas - 1, u * p.ctas / at.total);
-        while (c + 1 < p.ctas && cut(at.total, p.ctas, c + 1) <= u) ++c;
-        while (c > 0 && cut(at.total, p.ctas, c) > u) --c;
-        return c;
-    };
+    Place at;
+    const Cut cut = find(a, p, -1, (int)(p0 / p.pairs), at);
     for (int64_t x = p0; x < p1; ++x) {
         const int b = (int)(x / p.pairs), pair = (int)(x - (int64_t)b * p.pairs);
-        const int64_t ub = units_of(a, b);
         if (b != at.b) {
-            at.before += units_of(a, at.b) * p.pairs;
+            at.before += (int64_t)units_of(key_range(a, at.b)) * p.pairs;
             at.b = b;
         }
+        const int ub = units_of(key_range(a, b));
         const int hk = pair / p.row_tiles, rt = pair - hk * p.row_tiles;
-        const int64_t ua = at.before + pair * ub, uz = ua + ub;
-        const int c0 = ub ? owner(ua) : 0, c1 = ub ? owner(uz - 1) : 0;
-        if (ub && c0 == c1) continue;
-        for (int y = threadIdx.x; y < 16 * (DP / 8); y += 128) {
-            const int r = y / (DP / 8), d = y % (DP / 8) * 8, gr = rt * 16 + r;
-            if (gr >= p.rows) continue;
+        const int64_t ua = at.before + (int64_t)pair * ub;
+        int c0 = 0, nc = 0;
+        bool first_behind = false;   // the first CTA's run began before this pair
+        if (ub) {
+            c0 = cut.owner(ua + SETUP);
+            nc = cut.owner(ua + ub - 1) - c0 + 1;
+            first_behind = cut.start(c0) < ua;
+            // one CTA has it all and finished it, unless it began inside the pair's SETUP units
+            if (nc == 1 && cut.start(c0) <= ua) continue;
+        }
+        const int live = min(p.rows - rt * 16 * MT, 16 * MT), pieces = live * CH;
+        const int groups = max(1, 256 / pieces);
+        for (int y0 = 0; y0 < pieces; y0 += 256) {
+            const int y = y0 + (groups > 1 ? threadIdx.x % pieces : threadIdx.x);
+            const int grp = groups > 1 ? threadIdx.x / pieces : 0;
+            const int r = y / CH, d = y % CH * 8;
+            const bool busy = y < pieces && grp < groups;
             float acc[8] = {}, m = -INFINITY, l = 0.f;
-            for (int cc = c0; ub && cc <= c1; ++cc) {
-                const int64_t start = cut(at.total, p.ctas, cc);
-                if (start == cut(at.total, p.ctas, cc + 1)) continue;
-                const float* part = parts + ((int64_t)cc * 2 + (start >= ua ? 0 : 1)) * PART<DP>;
-                const float pm = part[16 * DP + r], pl = part[16 * DP + 16 + r];
-                const float4 v0 = *(const float4*)(part + r * DP + d), v1 = *(const float4*)(part + r * DP + d + 4);
-                const float mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.f : mn;
-                const float f0 = ptx::ex2_mufu(m - base), f1 = ptx::ex2_mufu(pm - base);
-                m = mn;
-                l = fmaf(l, f0, pl * f1);
-                const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+            if (busy) {
+                auto part_of = [&](int i) {
+                    return parts + ((int64_t)(c0 + i) * 2 + (i == 0 && first_behind ? 1 : 0)) * PART<DP, MT>;
+                };
+#pragma unroll 4
+                for (int i = grp; i < nc; i += groups) m = fmaxf(m, part_of(i)[16 * MT * DP + r]);
+                const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+                for (int i = grp; i < nc; i += groups) {
+                    const float* pt = part_of(i);
+                    const float fx = ptx::ex2_mufu(pt[16 * MT * DP + r] - base);
+                    l = fmaf(fx, pt[16 * MT * (DP + 1) + r], l);
+                    const float4 v0 = *(const float4*)(pt + r * DP + d), v1 = *(const float4*)(pt + r * DP + d + 4);
+                    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], f0, v[e] * f1);
+                    for (int e = 0; e < 8; ++e) acc[e] = fmaf(fx, v[e], acc[e]);
+                }
             }
-            store_row<F16>(a, b, hk, gr, d, acc, m, l);
+            if (groups > 1) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sacc[threadIdx.x][e] = acc[e];
+                sml[threadIdx.x][0] = m;
+                sml[threadIdx.x][1] = l;
+                __syncthreads();
+                if (busy && grp == 0) {
+                    for (int i = 1; i < groups; ++i) m = fmaxf(m, sml[threadIdx.x + i * pieces][0]);
+                    const float base = m == -INFINITY ? 0.f : m;
+                    l = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+                    for (int i = 0; i < groups; ++i) {
+                        const int s = threadIdx.x + i * pieces;
+                        const float fx = ptx::ex2_mufu(sml[s][0] - base);
+                        l = fmaf(fx, sml[s][1], l);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[e] = fmaf(fx, sacc[s][e], acc[e]);
+                    }
+                }
+                __syncthreads();
+            }
+            if (busy && grp == 0) store_row<F16>(a, b, hk, rt * 16 * MT + r, d, acc, m, l);
         }
     }
 }
 
-template <int DP, bool F16>
+template <int DP, bool F16, int MT>
 int launch(const Prob& a, float* parts, cudaStream_t s) {
     Plan p;
     p.rows = a.group * a.q_len;
-    p.row_tiles = (int)cdiv(p.rows, 16);
+    p.row_tiles = (int)cdiv(p.rows, 16 * MT);
     p.pairs = a.kv_heads * p.row_tiles;
     p.ctas = num_sms() * CTAS_PER_SM;
-    rows_kernel<DP, F16><<<p.ctas, WARPS * 32, 0, s>>>(a, p, parts);
+    using S = Smem<DP>;
+    auto fn = rows_kernel<DP, F16, MT>;
+    FD_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+    fn<<<p.ctas, WARPS * 32, S::BYTES, s>>>(a, p, parts);
     FD_CUDA_TRY(cudaGetLastError());
-    const int64_t all = (int64_t)a.batch * p.pairs, blocks = std::min<int64_t>(all, 8 * num_sms());
-    join_kernel<DP, F16><<<(unsigned)blocks, 128, 0, s>>>(a, p, parts, cdiv(all, blocks));
-    FD_CUDA_TRY(cudaGetLastError());
+    const int64_t all = (int64_t)a.batch * p.pairs, blocks = std::min<int64_t>(all, 4 * num_sms());
+    // launched while the rows kernel runs; it waits (griddepcontrol) for that grid's end before it reads
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const float* in = parts;
+    FD_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<DP, F16, MT>, a, p, in, cdiv(all, blocks)));
     return FD_OK;
+}
+
+template <int DP, bool F16>
+int by_rows(const Prob& a, float* parts, cudaStream_t s) {
+    return a.group * a.q_len <= 16 ? launch<DP, F16, 1>(a, parts, s) : launch<DP, F16, 2>(a, parts, s);
 }
 
 }  // namespace rows
@@ -487,14 +667,14 @@ int launch(const Prob& a, float* parts, cudaStream_t s) {
 bool rows_applies(const Prob& a) { return (int64_t)a.group * a.q_len <= MAX_ROWS; }
 
 size_t rows_bytes(int dim) {
-    return sizeof(float) * 2 * (size_t)num_sms() * rows::CTAS_PER_SM * (dim <= 64 ? rows::PART<64> : rows::PART<128>);
+    return sizeof(float) * 2 * (size_t)num_sms() * rows::CTAS_PER_SM * (dim <= 64 ? rows::PART<64, 2> : rows::PART<128, 2>);
 }
 
 int rows_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
     float* parts = (float*)workspace;
     if (dtype == FD_DTYPE_F16)
-        return a.dim <= 64 ? rows::launch<64, true>(a, parts, s) : rows::launch<128, true>(a, parts, s);
-    return a.dim <= 64 ? rows::launch<64, false>(a, parts, s) : rows::launch<128, false>(a, parts, s);
+        return a.dim <= 64 ? rows::by_rows<64, true>(a, parts, s) : rows::by_rows<128, true>(a, parts, s);
+    return a.dim <= 64 ? rows::by_rows<64, false>(a, parts, s) : rows::by_rows<128, false>(a, parts, s);
 }
 
 }  // namespace attn
