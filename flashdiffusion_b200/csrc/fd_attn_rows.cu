@@ -1,24 +1,29 @@
 // Softmax attention of few query rows against many keys: the newest tokens of
 // each sequence and a cache, and any call of at most MAX_ROWS query rows per key
 // head.  Bandwidth-bound: every visible key and value is read once, and the
-// arithmetic of up to 16 or 32 rows (the query heads that share a key head, times
-// the new tokens) rides on mma.sync tiles of 16 rows; a tcgen05 tile has 128.
+// arithmetic of 8, 16 or 32 rows (the query heads that share a key head, times
+// the new tokens) rides on mma.sync tiles with keys as their 16 rows and queries
+// as their 8 columns; a tcgen05 tile would have 128 rows.
+//
+//   S^T = K Q^T,  P^T = 2^(x - m),  O^T += V^T P^T
 //
 // Work split: the keys in use come from device memory, so the split is made on
 // the device.  The keys of all (sequence, key head, row tile) pairs are cut into
-// units of 64, laid end to end with SETUP units more for each pair (what its
-// start and end cost), and every CTA of a fixed grid takes an equal run: lengths
-// from 1 to the longest fill the SMs evenly.  A pair cut between CTAs leaves
-// (m, l, O) partials that join_kernel sums in CTA order (the same bits at every
-// call); a pair inside one CTA is finished there.
+// units, laid end to end with SETUP units more for each pair (what its start and
+// end cost), and every CTA of a fixed grid takes an equal run: lengths from 1 to
+// the longest fill the SMs evenly.  A pair cut between CTAs leaves (m, l, O)
+// partials that join_kernel sums in CTA order (the same bits at every call); a
+// pair inside one CTA is finished there.
 //
-// Each warp copies its own 16-key blocks with cp.async into a ring of its own,
+// Each warp copies its own blocks of keys with cp.async into a ring of its own,
 // STAGES - 1 blocks ahead and across the ends of pairs, and reads MMA fragments
-// from it in 16-byte pieces: the order of the contracted coordinate in Q K^T is
+// from it in 16-byte pieces: the order of the contracted coordinate in K Q^T is
 // free (Q is loaded the same way), and so is the order of output coordinates in
-// P V; the pairs of keys that a P V fragment wants are put together by byte
-// permutes.  P is split in two 16-bit parts, so that it adds no rounding of its
-// own: the second product hides behind the loads.
+// V^T P^T; the pairs of keys that a V^T fragment wants are put together by byte
+// permutes, and P^T is turned from accumulator to operand by movmatrix.  P is
+// split in two 16-bit parts, so that it adds no rounding of its own.  m is raised
+// only when a score exceeds it by more than 8, so the usual block needs no
+// exchange between lanes.
 #include <algorithm>
 
 #include "fd_attn_tc.cuh"
@@ -28,7 +33,6 @@ namespace attn {
 namespace rows {
 
 constexpr int WARPS = 4;
-constexpr int UNIT = 16 * WARPS;      // keys of a unit: 16 per warp
 constexpr int CTAS_PER_SM = 2;
 constexpr int STAGES = 3;
 constexpr int SETUP = 2;
@@ -56,16 +60,17 @@ __device__ __forceinline__ Range key_range(const Prob& a, int b) {
     return {lo & ~15, hi};
 }
 
-// Units of one pair of this range, its SETUP included; 0 for an empty range.
-__device__ __forceinline__ int units_of(const Range& r) {
-    return r.hi > r.lo ? (r.hi - r.lo + UNIT - 1) / UNIT + SETUP : 0;
-}
-
 struct Plan {
     int pairs;        // (key head, row tile) pairs of a sequence
     int row_tiles, rows;
     int ctas;
+    int unit;         // keys of a unit: a block for each warp
 };
+
+// Units of one pair of this range, its SETUP included; 0 for an empty range.
+__device__ __forceinline__ int units_of(const Range& r, const Plan& p) {
+    return r.hi > r.lo ? (r.hi - r.lo + p.unit - 1) / p.unit + SETUP : 0;
+}
 
 // Equal runs of `total` units for `ctas` CTAs: the first `more` take one more than `each`.
 struct Cut {
@@ -94,7 +99,7 @@ __device__ Cut find(const Prob& a, const Plan& p, int c, int b, Place& at) {
     const int per = (a.batch + 31) / 32, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
     int64_t sum = 0, part = 0;
     for (int i = b0; i < b1; ++i) {
-        const int64_t u = (int64_t)units_of(key_range(a, i)) * p.pairs;
+        const int64_t u = (int64_t)units_of(key_range(a, i), p) * p.pairs;
         sum += u;
         if (i < b) part += u;
     }
@@ -115,7 +120,7 @@ __device__ Cut find(const Prob& a, const Plan& p, int c, int b, Place& at) {
     int x = b0;
     if (mine)
         for (;; ++x) {
-            const int64_t n = (int64_t)units_of(key_range(a, x)) * p.pairs;
+            const int64_t n = (int64_t)units_of(key_range(a, x), p) * p.pairs;
             if (u < before + n) break;
             before += n;
         }
@@ -135,7 +140,7 @@ struct Walk {
     __device__ bool next(const Prob& a, const Plan& p, int64_t u0) {
         while (u < u1 && at.b < a.batch) {
             const Range r = key_range(a, at.b);
-            const int ub = units_of(r);
+            const int ub = units_of(r, p);
             const int64_t here = (int64_t)ub * p.pairs, off = u - at.before;
             if (off >= here) {
                 at.before += here;
@@ -146,8 +151,8 @@ struct Walk {
             const int blk = (int)(off - (int64_t)pair * ub);
             const int take = (int)min((int64_t)(ub - blk), u1 - u);
             b = at.b;
-            k0 = r.lo + max(blk - SETUP, 0) * UNIT;
-            k1 = min(r.hi, r.lo + max(blk + take - SETUP, 0) * UNIT);
+            k0 = r.lo + max(blk - SETUP, 0) * p.unit;
+            k1 = min(r.hi, r.lo + max(blk + take - SETUP, 0) * p.unit);
             whole = blk == 0 && take == ub;
             front = u == u0;
             u += take;
@@ -189,15 +194,21 @@ __device__ __forceinline__ uint4 load16(const uint16_t* p, bool there) {
 __device__ __forceinline__ void copy16(uint32_t dst, const uint16_t* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+// 8 x 8 16-bit matrix, rows over the lanes' quads -> its transpose in the same places
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
-// Floats of one partial: O of 16 MT rows, then their m and l.
-template <int DP, int MT>
-constexpr int PART = 16 * MT * (DP + 2);
+// Floats of one partial: O of 8 NT rows, then their m and l.
+template <int DP, int NT>
+constexpr int PART = 8 * NT * (DP + 2);
 
 // out[gr, d .. d + 8) = acc / l, and the row's lse with its first piece
 template <bool F16>
@@ -218,21 +229,23 @@ __device__ __forceinline__ void store_row(const Prob& a, int b, int hk, int gr, 
 
 template <int DP>
 struct Smem {
-    static constexpr uint32_t HALF = 16 * DP * 2;                 // K or V of a block
+    static constexpr int KEYS = 2048 / DP;                        // keys of a block: 16 or 32
+    static constexpr uint32_t HALF = KEYS * DP * 2;               // K or V of a block, 4 KB
     static constexpr uint32_t RING = WARPS * STAGES * 2 * HALF;
-    static constexpr int PIECES = DP / 8 + 1;                     // 16-byte pieces of one lane's sums: O, and m and l
+    static constexpr int PIECES = DP / 16 + 1;                    // 16-byte pieces of one lane's sums: O, and m and l
     static constexpr uint32_t BYTES = RING + 2 * PIECES * 32 * 16;
-    // two CTAs to an SM: 228 KB, of which each takes 1 KB for itself
+    // 228 KB to an SM, of which each CTA takes 1 KB for itself
     static_assert(CTAS_PER_SM * (BYTES + 1024) <= 228 * 1024, "shared memory budget");
 };
 
 // Row r of a pair: query i = r / group, head hk * group + r % group.
-template <int DP, bool F16, int MT>
+template <int DP, bool F16, int NT>
 __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
 rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, float* __restrict__ parts) {
     using S = Smem<DP>;
+    constexpr int KEYS = S::KEYS, KT = KEYS / 16, UNIT = KEYS * WARPS;
     constexpr int KI = DP / 32, VB = DP / 64, CH = DP / 8;   // 16-byte pieces of a row: CH
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     float4* meet = (float4*)(smem + S::RING);                 // [2][PIECES][lane]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;");
@@ -245,35 +258,41 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
     const float c = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
     const uint32_t ring = ptx::smem_u32(smem) + warp * STAGES * 2 * S::HALF;
 
-    // ---- the copies run ahead: block `ahead` of pair `f`
+    // ---- the copies run ahead: lane (lr, ch) copies piece ch of rows lr, lr + RP, ... of each block
+    constexpr int RP = 32 / CH;
+    const int lr = lane / CH, ch = lane % CH;
+    const bool col = ch * 8 < a.dim;
     Walk f = w;
     int fk = 0, fend = 0, wr = 0;
-    const uint16_t *fkp = nullptr, *fvp = nullptr;
+    const uint16_t *pk = nullptr, *pv = nullptr;
     auto fetch = [&]() {
         while (fk >= fend) {
             if (!f.next(a, p, u0)) {
-                fk = 0x7fffffff;
-                fend = 0x7fffffff;
+                fk = fend = 0x7fffffff;
                 break;
             }
             const int hk = f.pair / p.row_tiles;
-            fk = f.k0 + warp * 16;
+            fk = f.k0 + warp * KEYS;
             fend = f.k1;
-            fkp = (const uint16_t*)a.k.p + f.b * a.k.sb + hk * a.k.sh;
-            fvp = (const uint16_t*)a.v.p + f.b * a.v.sb + hk * a.v.sh;
+            pk = (const uint16_t*)a.k.p + f.b * a.k.sb + hk * a.k.sh + (int64_t)(fk + lr) * a.k.ss + (col ? ch * 8 : 0);
+            pv = (const uint16_t*)a.v.p + f.b * a.v.sb + hk * a.v.sh + (int64_t)(fk + lr) * a.v.ss + (col ? ch * 8 : 0);
         }
         if (fk < fend) {
-            const uint32_t dst = ring + wr * 2 * S::HALF;
+            // pieces are swapped within 128 bytes (by bit 0 of the row for K, bits 1 and 2 for V) so that the
+            // fragment reads below hit every bank once
+            const uint32_t dst = ring + wr * 2 * S::HALF + lr * CH * 16;
+            const uint32_t dk = dst + (ch ^ ((lr & 1) << 2)) * 16, dv = dst + S::HALF + (ch ^ (lr & 6)) * 16;
+            const int left = fend - fk - lr;     // this lane's rows before the end
 #pragma unroll
-            for (int x = 0; x < 16 * CH / 32; ++x) {
-                const int at = x * 32 + lane, r = at / CH, ch = at % CH, key = fk + r;
-                const bool there = key < fend && ch * 8 < a.dim;
-                const int64_t kk = there ? key : fk, cc = there ? ch * 8 : 0;
-                // pieces are swapped within 128 bytes so that the fragment reads below hit every bank once
-                copy16(dst + (r * CH + (ch ^ ((r & 1) << 2))) * 16, fkp + kk * a.k.ss + cc, there);
-                copy16(dst + S::HALF + (r * CH + (ch ^ (r & 6))) * 16, fvp + kk * a.v.ss + cc, there);
+            for (int x = 0; x < KEYS / RP; ++x) {
+                const bool there = x * RP < left && col;
+                copy16(dk + x * RP * CH * 16, there ? pk + x * RP * a.k.ss : (const uint16_t*)a.k.p, there);
+                copy16((dv ^ (((x * RP) & 6) << 4)) + x * RP * CH * 16, there ? pv + x * RP * a.v.ss : (const uint16_t*)a.v.p,
+                       there);
             }
             fk += UNIT;
+            pk += UNIT * a.k.ss;
+            pv += UNIT * a.v.ss;
             wr = wr + 1 == STAGES ? 0 : wr + 1;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -283,210 +302,250 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
     int rd = 0;
 
     while (w.next(a, p, u0)) {
-        const int b = w.b, hk = w.pair / p.row_tiles, rt = w.pair - hk * p.row_tiles;
+        const int b = w.b, hk = w.pair / p.row_tiles, r0 = (w.pair - hk * p.row_tiles) * NT * 8;
         const int n = keys_of(a, b);
-        // this thread's rows: g and g + 8 of each 16-row tile
-        uint32_t q[MT][2][KI][4];
-        int2 sp[MT][2];
-        int pos[MT][2];
-        float slope2[MT][2], m[MT][2], l[MT][2];
+        // operand rows: query r0 + 8 y + g; accumulator columns: queries r0 + 8 y + 2 t + z
+        uint32_t q[NT][KI][4];
+        int2 sp[NT][2];
+        float at[NT][2], slope2[NT][2], m[NT][2], l[NT][2];
         int flo = 0, fhi = 0x7fffffff;   // keys that every row sees: [flo, fhi)
         bool hole = false;
 #pragma unroll
-        for (int y = 0; y < MT; ++y)
+        for (int y = 0; y < NT; ++y) {
+            const int rq = r0 + 8 * y + g;
+            const uint16_t* qr = (const uint16_t*)a.q.p + b * a.q.sb + (int64_t)(rq < p.rows ? rq / a.group : 0) * a.q.ss +
+                                 (hk * a.group + (rq < p.rows ? rq % a.group : 0)) * a.q.sh;
+#pragma unroll
+            for (int k = 0; k < KI; ++k) {
+                const int d = 32 * k + 8 * t;
+                const uint4 x = load16(qr + d, rq < p.rows && d < a.dim);
+                q[y][k][0] = x.x;
+                q[y][k][1] = x.y;
+                q[y][k][2] = x.z;
+                q[y][k][3] = x.w;
+            }
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
-                const int r = (rt * MT + y) * 16 + g + 8 * z;
+                const int r = r0 + 8 * y + 2 * t + z;
                 const bool real = r < p.rows;
                 const int i = real ? r / a.group : 0, h = hk * a.group + (real ? r % a.group : 0);
                 sp[y][z] = real ? row_span(a, b, i, n) : make_int2(0, 0);
-                pos[y][z] = n - a.q_len + i;
+                at[y][z] = (float)(n - a.q_len + i - g - w.k0 - warp * KEYS);   // distance to this lane's first key
                 slope2[y][z] = a.slopes ? a.slopes[h] * LOG2E : 0.f;
                 m[y][z] = -INFINITY;
                 l[y][z] = 0.f;
-                const uint16_t* qr = (const uint16_t*)a.q.p + b * a.q.sb + i * a.q.ss + h * a.q.sh;
-#pragma unroll
-                for (int k = 0; k < KI; ++k) {
-                    const int d = 32 * k + 8 * t;
-                    const uint4 x = load16(qr + d, real && d < a.dim);
-                    q[y][z][k][0] = x.x;
-                    q[y][z][k][1] = x.y;
-                    q[y][z][k][2] = x.z;
-                    q[y][z][k][3] = x.w;
-                }
                 if (real) {
                     if (sp[y][z].y > sp[y][z].x) flo = max(flo, sp[y][z].x);
                     else hole = true;
                     fhi = min(fhi, sp[y][z].y);
                 }
             }
+        }
         flo = warp_max(flo);
         fhi = warp_min(fhi);
         hole = __any_sync(~0u, hole);
-        float o[MT][VB][8][4];
+        float o[NT][VB * 4][4];
 #pragma unroll
-        for (int y = 0; y < MT; ++y)
+        for (int y = 0; y < NT; ++y)
 #pragma unroll
-            for (int i = 0; i < VB; ++i)
+            for (int e = 0; e < VB * 4; ++e)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) o[y][i][e][z] = 0.f;
+                for (int z = 0; z < 4; ++z) o[y][e][z] = 0.f;
 
+        const int kfirst = w.k0 + warp * KEYS;
 #pragma unroll 1
-        for (int k0 = w.k0 + warp * 16; k0 < w.k1; k0 += UNIT) {
+        for (int k0 = kfirst; k0 < w.k1; k0 += UNIT) {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             __syncwarp();
             const uint32_t sk = ring + rd * 2 * S::HALF, sv = sk + S::HALF;
             rd = rd + 1 == STAGES ? 0 : rd + 1;
-            float s[MT][2][4];
+            // s[y][k][z]: query 2 t + z % 2 of column tile y, key k0 + 16 k + g + 8 (z / 2)
+            float s[NT][KT][4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int k = 0; k < KT; ++k) {
 #pragma unroll
-                for (int y = 0; y < MT; ++y)
+                for (int y = 0; y < NT; ++y)
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) s[y][j][z] = 0.f;
+                    for (int z = 0; z < 4; ++z) s[y][k][z] = 0.f;
 #pragma unroll
-                for (int k = 0; k < KI; ++k) {
-                    const int r = 8 * j + g;
-                    const uint4 x = lds16(sk + (r * CH + ((4 * k + t) ^ ((r & 1) << 2))) * 16);
+                for (int i = 0; i < KI; ++i) {
+                    const uint32_t at_k = sk + ((16 * k + g) * CH + ((4 * i + t) ^ ((g & 1) << 2))) * 16;
+                    const uint4 x0 = lds16(at_k), x1 = lds16(at_k + 8 * CH * 16);
 #pragma unroll
-                    for (int y = 0; y < MT; ++y) {
-                        mma<F16>(s[y][j], q[y][0][k][0], q[y][1][k][0], q[y][0][k][1], q[y][1][k][1], x.x, x.y);
-                        mma<F16>(s[y][j], q[y][0][k][2], q[y][1][k][2], q[y][0][k][3], q[y][1][k][3], x.z, x.w);
+                    for (int y = 0; y < NT; ++y) {
+                        mma<F16>(s[y][k], x0.x, x1.x, x0.y, x1.y, q[y][i][0], q[y][i][1]);
+                        mma<F16>(s[y][k], x0.z, x1.z, x0.w, x1.w, q[y][i][2], q[y][i][3]);
                     }
                 }
             }
             fetch();
-            const bool edge = k0 < flo || k0 + 16 > fhi || hole;
-            uint32_t ph[MT][2][2], pl[MT][2][2];   // [row g / g + 8][key block]
+            const bool edge = k0 < flo || k0 + KEYS > fhi || hole;
+            const float step = (float)(k0 - kfirst);
+            bool raise = false;
 #pragma unroll
-            for (int y = 0; y < MT; ++y) {
-                // s[y][j][z]: row g + 8 (z / 2), key k0 + 8 j + 2 t + z % 2
+            for (int y = 0; y < NT; ++y)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int k = 0; k < KT; ++k)
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) {
-                        const int key = k0 + 8 * j + 2 * t + (z & 1);
-                        float x = s[y][j][z] * c;
-                        if (cap2 > 0.f) {
-                            const float e = ptx::ex2_mufu(x * (2.f * LOG2E));
-                            x = cap2 * fmaf(-2.f, ptx::rcp_mufu(1.f + e), 1.f);
+                    for (int z = 0; z < 4; ++z) s[y][k][z] *= c;
+            if (cap2 > 0.f) {
+#pragma unroll
+                for (int y = 0; y < NT; ++y)
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            const float e = ptx::ex2_mufu(s[y][k][z] * (2.f * LOG2E));
+                            s[y][k][z] = cap2 * fmaf(-2.f, ptx::rcp_mufu(1.f + e), 1.f);
                         }
-                        x = fmaf(-slope2[y][z >> 1], fabsf((float)(pos[y][z >> 1] - key)), x);
-                        if (edge && (key < sp[y][z >> 1].x || key >= sp[y][z >> 1].y)) x = -INFINITY;
-                        s[y][j][z] = x;
-                    }
+            }
+            if (a.slopes) {
+#pragma unroll
+                for (int y = 0; y < NT; ++y)
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            const float far = at[y][z & 1] - step - (float)(16 * k + 8 * (z >> 1));
+                            s[y][k][z] = fmaf(-slope2[y][z & 1], fabsf(far), s[y][k][z]);
+                        }
+            }
+            if (edge) {
+#pragma unroll
+                for (int y = 0; y < NT; ++y)
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            const int key = k0 + 16 * k + g + 8 * (z >> 1);
+                            if (key < sp[y][z & 1].x || key >= sp[y][z & 1].y) s[y][k][z] = -INFINITY;
+                        }
+            }
+            float top[NT][2];
+#pragma unroll
+            for (int y = 0; y < NT; ++y)
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    float top = fmaxf(fmaxf(s[y][0][2 * z], s[y][0][2 * z + 1]), fmaxf(s[y][1][2 * z], s[y][1][2 * z + 1]));
-                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                    if (__any_sync(~0u, top > m[y][z])) {
-                        const float mn = fmaxf(m[y][z], top);
+                    top[y][z] = fmaxf(s[y][0][z], s[y][0][2 + z]);
+#pragma unroll
+                    for (int k = 1; k < KT; ++k) top[y][z] = fmaxf(top[y][z], fmaxf(s[y][k][z], s[y][k][2 + z]));
+                    raise = raise || top[y][z] > m[y][z] + 8.f;
+                }
+            if (__any_sync(~0u, raise)) {
+#pragma unroll
+                for (int y = 0; y < NT; ++y)
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        float tp = top[y][z];
+                        tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 4));
+                        tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 8));
+                        tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 16));
+                        const float mn = fmaxf(m[y][z], tp);
                         const float fix = mn == -INFINITY ? 0.f : ptx::ex2_mufu(m[y][z] - mn);
                         m[y][z] = mn;
                         l[y][z] *= fix;
 #pragma unroll
-                        for (int i = 0; i < VB; ++i)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                o[y][i][e][2 * z] *= fix;
-                                o[y][i][e][2 * z + 1] *= fix;
-                            }
+                        for (int e = 0; e < VB * 4; ++e) {
+                            o[y][e][z] *= fix;
+                            o[y][e][2 + z] *= fix;
+                        }
                     }
-                    const float base = m[y][z] == -INFINITY ? 0.f : m[y][z];
+            }
+            // P^T as B operand: keys along the contracted index
+            uint32_t ph[NT][KT][2], pl[NT][KT][2];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float e0 = ptx::ex2_mufu(s[y][j][2 * z] - base), e1 = ptx::ex2_mufu(s[y][j][2 * z + 1] - base);
-                        l[y][z] += e0 + e1;
-                        ph[y][z][j] = ptx::pack16<F16>(e0, e1);
-                        const float2 hi = unpack16<F16>(ph[y][z][j]);
-                        pl[y][z][j] = ptx::pack16<F16>(e0 - hi.x, e1 - hi.y);
+            for (int y = 0; y < NT; ++y) {
+                const float b0 = m[y][0] == -INFINITY ? 0.f : m[y][0], b1 = m[y][1] == -INFINITY ? 0.f : m[y][1];
+#pragma unroll
+                for (int k = 0; k < KT; ++k)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float e0 = ptx::ex2_mufu(s[y][k][2 * x] - b0), e1 = ptx::ex2_mufu(s[y][k][2 * x + 1] - b1);
+                        l[y][0] += e0;
+                        l[y][1] += e1;
+                        const uint32_t hi = ptx::pack16<F16>(e0, e1);
+                        const float2 hf = unpack16<F16>(hi);
+                        ph[y][k][x] = transpose8x8(hi);
+                        pl[y][k][x] = transpose8x8(ptx::pack16<F16>(e0 - hf.x, e1 - hf.y));
                     }
-                }
             }
             bool bad = false;
 #pragma unroll
-            for (int i = 0; i < VB; ++i) {
-                uint32_t v[4][4];
+            for (int k = 0; k < KT; ++k)
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    const int r = 2 * t + (z & 1) + 8 * (z >> 1);
-                    const uint4 x = lds16(sv + (r * CH + ((8 * i + g) ^ (r & 6))) * 16);
-                    v[z][0] = x.x;
-                    v[z][1] = x.y;
-                    v[z][2] = x.z;
-                    v[z][3] = x.w;
-                }
-                if (edge) {
-                    // zero times a NaN or an infinity of a masked place would reach the row: such elements
-                    // of V become zeros here and are given back below to the rows that see them
-                    constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+                for (int i = 0; i < VB; ++i) {
+                    uint32_t v[4][4];
 #pragma unroll
-                    for (int z = 0; z < 4; ++z)
+                    for (int z = 0; z < 4; ++z) {
+                        const int r = 16 * k + 2 * t + (z & 1) + 8 * (z >> 1);
+                        const uint4 x = lds16(sv + (r * CH + ((8 * i + g) ^ (2 * t))) * 16);
+                        v[z][0] = x.x;
+                        v[z][1] = x.y;
+                        v[z][2] = x.z;
+                        v[z][3] = x.w;
+                    }
+                    if (edge) {
+                        // zero times a NaN or an infinity of a masked place would reach the row: such elements
+                        // of V become zeros here and are given back below to the rows that see them
+                        constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if ((v[z][e] & EXP) == EXP) { v[z][e] &= 0xffff0000u; bad = true; }
-                            if (((v[z][e] >> 16) & EXP) == EXP) { v[z][e] &= 0xffffu; bad = true; }
-                        }
-                }
+                        for (int z = 0; z < 4; ++z)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                            for (int e = 0; e < 4; ++e) {
+                                if ((v[z][e] & EXP) == EXP) { v[z][e] &= 0xffff0000u; bad = true; }
+                                if (((v[z][e] >> 16) & EXP) == EXP) { v[z][e] &= 0xffffu; bad = true; }
+                            }
+                    }
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t b0 = __byte_perm(v[0][e], v[1][e], x ? 0x7632 : 0x5410);
-                        const uint32_t b1 = __byte_perm(v[2][e], v[3][e], x ? 0x7632 : 0x5410);
+                    for (int e = 0; e < 4; ++e) {
+                        // rows g and g + 8 of the tile: coordinates 64 i + 8 g + 2 e and the next one
+                        const uint32_t a0 = __byte_perm(v[0][e], v[1][e], 0x5410), a1 = __byte_perm(v[0][e], v[1][e], 0x7632);
+                        const uint32_t a2 = __byte_perm(v[2][e], v[3][e], 0x5410), a3 = __byte_perm(v[2][e], v[3][e], 0x7632);
 #pragma unroll
-                        for (int y = 0; y < MT; ++y) {
-                            mma<F16>(o[y][i][2 * e + x], ph[y][0][0], ph[y][1][0], ph[y][0][1], ph[y][1][1], b0, b1);
-                            mma<F16>(o[y][i][2 * e + x], pl[y][0][0], pl[y][1][0], pl[y][0][1], pl[y][1][1], b0, b1);
+                        for (int y = 0; y < NT; ++y) {
+                            mma<F16>(o[y][i * 4 + e], a0, a1, a2, a3, ph[y][k][0], ph[y][k][1]);
+                            mma<F16>(o[y][i * 4 + e], a0, a1, a2, a3, pl[y][k][0], pl[y][k][1]);
                         }
                     }
-            }
+                }
             if (__any_sync(~0u, bad)) {
                 const uint16_t* vb = (const uint16_t*)a.v.p + b * a.v.sb + hk * a.v.sh;
-                for (int key = k0; key < min(k0 + 16, w.k1); ++key) {
+                for (int key = k0; key < min(k0 + KEYS, w.k1); ++key) {
                     const uint16_t* vr = vb + (int64_t)key * a.v.ss;
 #pragma unroll
-                    for (int i = 0; i < VB; ++i)
+                    for (int e = 0; e < VB * 4; ++e)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
+                        for (int x = 0; x < 2; ++x) {
+                            const int d = 64 * (e / 4) + 8 * g + 2 * (e % 4) + x;
+                            if (d >= a.dim) continue;
+                            constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
+                            const uint16_t h = vr[d];
+                            if ((h & EXP) != EXP) continue;
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const int d = 64 * i + 16 * t + 8 * x + e;
-                                if (d >= a.dim) continue;
-                                constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
-                                const uint16_t h = vr[d];
-                                if ((h & EXP) != EXP) continue;
+                            for (int y = 0; y < NT; ++y)
 #pragma unroll
-                                for (int y = 0; y < MT; ++y) {
-                                    if (key >= sp[y][0].x && key < sp[y][0].y) o[y][i][e][x] += one16<F16>(h);
-                                    if (key >= sp[y][1].x && key < sp[y][1].y) o[y][i][e][2 + x] += one16<F16>(h);
-                                }
-                            }
+                                for (int z = 0; z < 2; ++z)
+                                    if (key >= sp[y][z].x && key < sp[y][z].y) o[y][e][2 * x + z] += one16<F16>(h);
+                        }
                 }
             }
         }
         // ---- the four warps' sums meet: 2 and 3 hand theirs to 0 and 1, then 1 to 0
-        float* part = parts + ((int64_t)blockIdx.x * 2 + (w.front ? 0 : 1)) * PART<DP, MT>;
+        float* part = parts + ((int64_t)blockIdx.x * 2 + (w.front ? 0 : 1)) * PART<DP, NT>;
 #pragma unroll
-        for (int y = 0; y < MT; ++y) {
+        for (int y = 0; y < NT; ++y) {
 #pragma unroll
             for (int from = 2; from; from >>= 1) {
                 if (warp >= from && warp < 2 * from) {
                     float4* to = meet + (warp - from) * S::PIECES * 32 + lane;
 #pragma unroll
-                    for (int i = 0; i < VB; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            to[(i * 8 + e) * 32] = make_float4(o[y][i][e][0], o[y][i][e][1], o[y][i][e][2], o[y][i][e][3]);
-                    to[VB * 8 * 32] = make_float4(m[y][0], m[y][1], l[y][0], l[y][1]);
+                    for (int e = 0; e < VB * 4; ++e) to[e * 32] = make_float4(o[y][e][0], o[y][e][1], o[y][e][2], o[y][e][3]);
+                    to[VB * 4 * 32] = make_float4(m[y][0], m[y][1], l[y][0], l[y][1]);
                 }
                 __syncthreads();
                 if (warp < from) {
                     const float4* in = meet + warp * S::PIECES * 32 + lane;
-                    const float4 ml = in[VB * 8 * 32];
+                    const float4 ml = in[VB * 4 * 32];
                     const float mo[2] = {ml.x, ml.y}, lo[2] = {ml.z, ml.w};
                     float f0[2], f1[2];
 #pragma unroll
@@ -498,44 +557,41 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                         l[y][z] = l[y][z] * f0[z] + lo[z] * f1[z];
                     }
 #pragma unroll
-                    for (int i = 0; i < VB; ++i)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float4 v = in[(i * 8 + e) * 32];
-                            o[y][i][e][0] = o[y][i][e][0] * f0[0] + v.x * f1[0];
-                            o[y][i][e][1] = o[y][i][e][1] * f0[0] + v.y * f1[0];
-                            o[y][i][e][2] = o[y][i][e][2] * f0[1] + v.z * f1[1];
-                            o[y][i][e][3] = o[y][i][e][3] * f0[1] + v.w * f1[1];
-                        }
+                    for (int e = 0; e < VB * 4; ++e) {
+                        const float4 v = in[e * 32];
+                        o[y][e][0] = o[y][e][0] * f0[0] + v.x * f1[0];
+                        o[y][e][1] = o[y][e][1] * f0[1] + v.y * f1[1];
+                        o[y][e][2] = o[y][e][2] * f0[0] + v.z * f1[0];
+                        o[y][e][3] = o[y][e][3] * f0[1] + v.w * f1[1];
+                    }
                 }
                 __syncthreads();
             }
             if (warp == 0) {
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    const int pr = y * 16 + g + 8 * z, gr = rt * MT * 16 + pr;
+                    const int pr = 8 * y + 2 * t + z, gr = r0 + pr;
                     float ls = l[y][z];
-                    ls += __shfl_xor_sync(~0u, ls, 1);
-                    ls += __shfl_xor_sync(~0u, ls, 2);
+                    ls += __shfl_xor_sync(~0u, ls, 4);
+                    ls += __shfl_xor_sync(~0u, ls, 8);
+                    ls += __shfl_xor_sync(~0u, ls, 16);
                     if (gr >= p.rows) continue;
 #pragma unroll
-                    for (int i = 0; i < VB; ++i)
+                    for (int i = 0; i < VB; ++i) {
+                        const int d = 64 * i + 8 * g;
+                        float acc[8];
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const int d = 64 * i + 16 * t + 8 * x;
-                            float acc[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) acc[e] = o[y][i][e][2 * z + x];
-                            if (w.whole) {
-                                store_row<F16>(a, b, hk, gr, d, acc, m[y][z], ls);
-                            } else {
-                                *(float4*)(part + pr * DP + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                                *(float4*)(part + pr * DP + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                            }
+                        for (int e = 0; e < 8; ++e) acc[e] = o[y][i * 4 + e / 2][2 * (e & 1) + z];
+                        if (w.whole) {
+                            store_row<F16>(a, b, hk, gr, d, acc, m[y][z], ls);
+                        } else {
+                            *(float4*)(part + pr * DP + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                            *(float4*)(part + pr * DP + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
                         }
-                    if (!w.whole && t == 0) {
-                        part[16 * MT * DP + pr] = m[y][z];
-                        part[16 * MT * (DP + 1) + pr] = ls;
+                    }
+                    if (!w.whole && g == 0) {
+                        part[8 * NT * DP + pr] = m[y][z];
+                        part[8 * NT * (DP + 1) + pr] = ls;
                     }
                 }
             }
@@ -546,7 +602,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
 // Pairs that were cut: their partials, in CTA order.  Pairs that see no key: zeros.
 // Block: one pair after another; up to 256 threads share the (row, 8 coordinates)
 // pieces of it, and where those are fewer the partials too (summed in group order).
-template <int DP, bool F16, int MT>
+template <int DP, bool F16, int NT>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p,
                                                    const float* __restrict__ parts, int64_t per_block) {
     constexpr int CH = DP / 8;
@@ -561,10 +617,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
     for (int64_t x = p0; x < p1; ++x) {
         const int b = (int)(x / p.pairs), pair = (int)(x - (int64_t)b * p.pairs);
         if (b != at.b) {
-            at.before += (int64_t)units_of(key_range(a, at.b)) * p.pairs;
+            at.before += (int64_t)units_of(key_range(a, at.b), p) * p.pairs;
             at.b = b;
         }
-        const int ub = units_of(key_range(a, b));
+        const int ub = units_of(key_range(a, b), p);
         const int hk = pair / p.row_tiles, rt = pair - hk * p.row_tiles;
         const int64_t ua = at.before + (int64_t)pair * ub;
         int c0 = 0, nc = 0;
@@ -576,7 +632,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
             // one CTA has it all and finished it, unless it began inside the pair's SETUP units
             if (nc == 1 && cut.start(c0) <= ua) continue;
         }
-        const int live = min(p.rows - rt * 16 * MT, 16 * MT), pieces = live * CH;
+        const int live = min(p.rows - rt * 8 * NT, 8 * NT), pieces = live * CH;
         const int groups = max(1, 256 / pieces);
         for (int y0 = 0; y0 < pieces; y0 += 256) {
             const int y = y0 + (groups > 1 ? threadIdx.x % pieces : threadIdx.x);
@@ -586,16 +642,16 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
             float acc[8] = {}, m = -INFINITY, l = 0.f;
             if (busy) {
                 auto part_of = [&](int i) {
-                    return parts + ((int64_t)(c0 + i) * 2 + (i == 0 && first_behind ? 1 : 0)) * PART<DP, MT>;
+                    return parts + ((int64_t)(c0 + i) * 2 + (i == 0 && first_behind ? 1 : 0)) * PART<DP, NT>;
                 };
 #pragma unroll 4
-                for (int i = grp; i < nc; i += groups) m = fmaxf(m, part_of(i)[16 * MT * DP + r]);
+                for (int i = grp; i < nc; i += groups) m = fmaxf(m, part_of(i)[8 * NT * DP + r]);
                 const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 4
                 for (int i = grp; i < nc; i += groups) {
                     const float* pt = part_of(i);
-                    const float fx = ptx::ex2_mufu(pt[16 * MT * DP + r] - base);
-                    l = fmaf(fx, pt[16 * MT * (DP + 1) + r], l);
+                    const float fx = ptx::ex2_mufu(pt[8 * NT * DP + r] - base);
+                    l = fmaf(fx, pt[8 * NT * (DP + 1) + r], l);
                     const float4 v0 = *(const float4*)(pt + r * DP + d), v1 = *(const float4*)(pt + r * DP + d + 4);
                     const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
@@ -624,20 +680,21 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
                 }
                 __syncthreads();
             }
-            if (busy && grp == 0) store_row<F16>(a, b, hk, rt * 16 * MT + r, d, acc, m, l);
+            if (busy && grp == 0) store_row<F16>(a, b, hk, rt * 8 * NT + r, d, acc, m, l);
         }
     }
 }
 
-template <int DP, bool F16, int MT>
+template <int DP, bool F16, int NT>
 int launch(const Prob& a, float* parts, cudaStream_t s) {
     Plan p;
     p.rows = a.group * a.q_len;
-    p.row_tiles = (int)cdiv(p.rows, 16 * MT);
+    p.row_tiles = (int)cdiv(p.rows, 8 * NT);
     p.pairs = a.kv_heads * p.row_tiles;
     p.ctas = num_sms() * CTAS_PER_SM;
+    p.unit = Smem<DP>::KEYS * WARPS;
     using S = Smem<DP>;
-    auto fn = rows_kernel<DP, F16, MT>;
+    auto fn = rows_kernel<DP, F16, NT>;
     FD_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
     fn<<<p.ctas, WARPS * 32, S::BYTES, s>>>(a, p, parts);
     FD_CUDA_TRY(cudaGetLastError());
@@ -653,13 +710,16 @@ int launch(const Prob& a, float* parts, cudaStream_t s) {
     cfg.attrs = &early;
     cfg.numAttrs = 1;
     const float* in = parts;
-    FD_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<DP, F16, MT>, a, p, in, cdiv(all, blocks)));
+    FD_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<DP, F16, NT>, a, p, in, cdiv(all, blocks)));
     return FD_OK;
 }
 
 template <int DP, bool F16>
 int by_rows(const Prob& a, float* parts, cudaStream_t s) {
-    return a.group * a.q_len <= 16 ? launch<DP, F16, 1>(a, parts, s) : launch<DP, F16, 2>(a, parts, s);
+    const int rows = a.group * a.q_len;
+    return rows <= 8    ? launch<DP, F16, 1>(a, parts, s)
+           : rows <= 16 ? launch<DP, F16, 2>(a, parts, s)
+                        : launch<DP, F16, 4>(a, parts, s);
 }
 
 }  // namespace rows
@@ -667,7 +727,7 @@ int by_rows(const Prob& a, float* parts, cudaStream_t s) {
 bool rows_applies(const Prob& a) { return (int64_t)a.group * a.q_len <= MAX_ROWS; }
 
 size_t rows_bytes(int dim) {
-    return sizeof(float) * 2 * (size_t)num_sms() * rows::CTAS_PER_SM * (dim <= 64 ? rows::PART<64, 2> : rows::PART<128, 2>);
+    return sizeof(float) * 2 * (size_t)num_sms() * rows::CTAS_PER_SM * (dim <= 64 ? rows::PART<64, 4> : rows::PART<128, 4>);
 }
 
 int rows_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
