@@ -64,12 +64,15 @@ struct Plan {
     int pairs;        // (key head, row tile) pairs of a sequence
     int row_tiles, rows;
     int ctas;
-    int unit;         // keys of a unit: a block for each warp
+    int unit;         // log2 of the keys of a unit: a block for each warp
+    int magic;        // r / group = r magic >> 16 for the rows of a pair (r, group <= 64: off by less than 1 / 600)
+    __device__ int query(int r) const { return r * magic >> 16; }
+    __device__ int head(int pair) const { return row_tiles == 1 ? pair : pair / row_tiles; }
 };
 
 // Units of one pair of this range, its SETUP included; 0 for an empty range.
 __device__ __forceinline__ int units_of(const Range& r, const Plan& p) {
-    return r.hi > r.lo ? (r.hi - r.lo + p.unit - 1) / p.unit + SETUP : 0;
+    return r.hi > r.lo ? ((r.hi - r.lo - 1) >> p.unit) + 1 + SETUP : 0;
 }
 
 // Equal runs of `total` units for `ctas` CTAs: the first `more` take one more than `each`.
@@ -147,12 +150,12 @@ struct Walk {
                 ++at.b;
                 continue;
             }
-            pair = (uint64_t)off >> 32 ? (int)(off / ub) : (int)((uint32_t)off / (uint32_t)ub);
+            pair = off < ub ? 0 : (uint64_t)off >> 32 ? (int)(off / ub) : (int)((uint32_t)off / (uint32_t)ub);
             const int blk = (int)(off - (int64_t)pair * ub);
             const int take = (int)min((int64_t)(ub - blk), u1 - u);
             b = at.b;
-            k0 = r.lo + max(blk - SETUP, 0) * p.unit;
-            k1 = min(r.hi, r.lo + max(blk + take - SETUP, 0) * p.unit);
+            k0 = r.lo + (max(blk - SETUP, 0) << p.unit);
+            k1 = (int)min((int64_t)r.hi, r.lo + ((int64_t)max(blk + take - SETUP, 0) << p.unit));
             whole = blk == 0 && take == ub;
             front = u == u0;
             u += take;
@@ -212,9 +215,9 @@ constexpr int PART = 8 * NT * (DP + 2);
 
 // out[gr, d .. d + 8) = acc / l, and the row's lse with its first piece
 template <bool F16>
-__device__ __forceinline__ void store_row(const Prob& a, int b, int hk, int gr, int d, const float (&acc)[8], float m,
-                                          float l) {
-    const int i = gr / a.group, h = hk * a.group + gr % a.group;
+__device__ __forceinline__ void store_row(const Prob& a, const Plan& p, int b, int hk, int gr, int d,
+                                          const float (&acc)[8], float m, float l) {
+    const int i = p.query(gr), h = hk * a.group + gr - i * a.group;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (d < a.dim) {
         uint4 w;
@@ -263,21 +266,22 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
     const int lr = lane / CH, ch = lane % CH;
     const bool col = ch * 8 < a.dim;
     Walk f = w;
-    int fk = 0, fend = 0, wr = 0;
+    // blocks flast, flast + UNIT, ... below fend, the last first: the nearest keys have the largest scores
+    // where a bias falls with distance, and m then rises once
+    auto last_block = [](int lo, int end) { return end > lo ? lo + (end - lo - 1) / UNIT * UNIT : lo - UNIT; };
+    int fk = -1, flast = 0, fend = 0, wr = 0;
     const uint16_t *pk = nullptr, *pv = nullptr;
     auto fetch = [&]() {
-        while (fk >= fend) {
-            if (!f.next(a, p, u0)) {
-                fk = fend = 0x7fffffff;
-                break;
-            }
-            const int hk = f.pair / p.row_tiles;
-            fk = f.k0 + warp * KEYS;
+        while (fk < flast) {
+            if (!f.next(a, p, u0)) break;
+            const int hk = p.head(f.pair);
+            flast = f.k0 + warp * KEYS;
             fend = f.k1;
+            fk = last_block(flast, fend);
             pk = (const uint16_t*)a.k.p + f.b * a.k.sb + hk * a.k.sh + (int64_t)(fk + lr) * a.k.ss + (col ? ch * 8 : 0);
             pv = (const uint16_t*)a.v.p + f.b * a.v.sb + hk * a.v.sh + (int64_t)(fk + lr) * a.v.ss + (col ? ch * 8 : 0);
         }
-        if (fk < fend) {
+        if (fk >= flast) {
             // pieces are swapped within 128 bytes (by bit 0 of the row for K, bits 1 and 2 for V) so that the
             // fragment reads below hit every bank once
             const uint32_t dst = ring + wr * 2 * S::HALF + lr * CH * 16;
@@ -290,9 +294,9 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                 copy16((dv ^ (((x * RP) & 6) << 4)) + x * RP * CH * 16, there ? pv + x * RP * a.v.ss : (const uint16_t*)a.v.p,
                        there);
             }
-            fk += UNIT;
-            pk += UNIT * a.k.ss;
-            pv += UNIT * a.v.ss;
+            fk -= UNIT;
+            pk -= UNIT * a.k.ss;
+            pv -= UNIT * a.v.ss;
             wr = wr + 1 == STAGES ? 0 : wr + 1;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -302,7 +306,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
     int rd = 0;
 
     while (w.next(a, p, u0)) {
-        const int b = w.b, hk = w.pair / p.row_tiles, r0 = (w.pair - hk * p.row_tiles) * NT * 8;
+        const int b = w.b, hk = p.head(w.pair), r0 = (w.pair - hk * p.row_tiles) * NT * 8;
         const int n = keys_of(a, b);
         // operand rows: query r0 + 8 y + g; accumulator columns: queries r0 + 8 y + 2 t + z
         uint32_t q[NT][KI][4];
@@ -313,8 +317,8 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
 #pragma unroll
         for (int y = 0; y < NT; ++y) {
             const int rq = r0 + 8 * y + g;
-            const uint16_t* qr = (const uint16_t*)a.q.p + b * a.q.sb + (int64_t)(rq < p.rows ? rq / a.group : 0) * a.q.ss +
-                                 (hk * a.group + (rq < p.rows ? rq % a.group : 0)) * a.q.sh;
+            const int qi = rq < p.rows ? p.query(rq) : 0, qh = rq < p.rows ? rq - qi * a.group : 0;
+            const uint16_t* qr = (const uint16_t*)a.q.p + b * a.q.sb + qi * a.q.ss + (hk * a.group + qh) * a.q.sh;
 #pragma unroll
             for (int k = 0; k < KI; ++k) {
                 const int d = 32 * k + 8 * t;
@@ -328,7 +332,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
             for (int z = 0; z < 2; ++z) {
                 const int r = r0 + 8 * y + 2 * t + z;
                 const bool real = r < p.rows;
-                const int i = real ? r / a.group : 0, h = hk * a.group + (real ? r % a.group : 0);
+                const int i = real ? p.query(r) : 0, h = hk * a.group + (real ? r - i * a.group : 0);
                 sp[y][z] = real ? row_span(a, b, i, n) : make_int2(0, 0);
                 at[y][z] = (float)(n - a.q_len + i - g - w.k0 - warp * KEYS);   // distance to this lane's first key
                 slope2[y][z] = a.slopes ? a.slopes[h] * LOG2E : 0.f;
@@ -354,7 +358,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
 
         const int kfirst = w.k0 + warp * KEYS;
 #pragma unroll 1
-        for (int k0 = kfirst; k0 < w.k1; k0 += UNIT) {
+        for (int k0 = last_block(kfirst, w.k1); k0 >= kfirst; k0 -= UNIT) {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             __syncwarp();
             const uint32_t sk = ring + rd * 2 * S::HALF, sv = sk + S::HALF;
@@ -583,7 +587,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
 #pragma unroll
                         for (int e = 0; e < 8; ++e) acc[e] = o[y][i * 4 + e / 2][2 * (e & 1) + z];
                         if (w.whole) {
-                            store_row<F16>(a, b, hk, gr, d, acc, m[y][z], ls);
+                            store_row<F16>(a, p, b, hk, gr, d, acc, m[y][z], ls);
                         } else {
                             *(float4*)(part + pr * DP + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
                             *(float4*)(part + pr * DP + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
@@ -600,20 +604,25 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
 }
 
 // Pairs that were cut: their partials, in CTA order.  Pairs that see no key: zeros.
-// Block: one pair after another; up to 256 threads share the (row, 8 coordinates)
-// pieces of it, and where those are fewer the partials too (summed in group order).
+// A block takes one slice of a pair, 32 pieces of a row and 8 coordinates; its
+// eight warps share the partials (warp v takes v, v + 8, ...), and their sums are
+// added in warp order.
 template <int DP, bool F16, int NT>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p,
-                                                   const float* __restrict__ parts, int64_t per_block) {
-    constexpr int CH = DP / 8;
-    __shared__ float sacc[256][9];
-    __shared__ float sml[256][2];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t all = (int64_t)a.batch * p.pairs;
-    const int64_t p0 = min(blockIdx.x * per_block, all), p1 = min(p0 + per_block, all);
-    if (p0 >= p1) return;
+                                                   const float* __restrict__ parts) {
+    constexpr int CH = DP / 8, SLICES = 8 * NT * CH / 32;
+    __shared__ float sacc[8][8][32];
+    __shared__ float sml[8][2][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int slice = blockIdx.x % SLICES;
+    const int64_t all = (int64_t)a.batch * p.pairs, blocks = gridDim.x / SLICES;
+    const int64_t per_block = (all + blocks - 1) / blocks;
+    const int64_t p0 = min(blockIdx.x / SLICES * per_block, all), p1 = min(p0 + per_block, all);
     Place at;
+    // only lengths and spans are read before the rows kernel is known to have ended
     const Cut cut = find(a, p, -1, (int)(p0 / p.pairs), at);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int y = slice * 32 + lane, r = y / CH, d = y % CH * 8;
     for (int64_t x = p0; x < p1; ++x) {
         const int b = (int)(x / p.pairs), pair = (int)(x - (int64_t)b * p.pairs);
         if (b != at.b) {
@@ -621,7 +630,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
             at.b = b;
         }
         const int ub = units_of(key_range(a, b), p);
-        const int hk = pair / p.row_tiles, rt = pair - hk * p.row_tiles;
+        const int hk = p.head(pair), gr = (pair - hk * p.row_tiles) * 8 * NT + r;
+        if (__all_sync(~0u, gr >= p.rows)) continue;        // the same for all warps: no barrier is missed
         const int64_t ua = at.before + (int64_t)pair * ub;
         int c0 = 0, nc = 0;
         bool first_behind = false;   // the first CTA's run began before this pair
@@ -632,56 +642,46 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
             // one CTA has it all and finished it, unless it began inside the pair's SETUP units
             if (nc == 1 && cut.start(c0) <= ua) continue;
         }
-        const int live = min(p.rows - rt * 8 * NT, 8 * NT), pieces = live * CH;
-        const int groups = max(1, 256 / pieces);
-        for (int y0 = 0; y0 < pieces; y0 += 256) {
-            const int y = y0 + (groups > 1 ? threadIdx.x % pieces : threadIdx.x);
-            const int grp = groups > 1 ? threadIdx.x / pieces : 0;
-            const int r = y / CH, d = y % CH * 8;
-            const bool busy = y < pieces && grp < groups;
-            float acc[8] = {}, m = -INFINITY, l = 0.f;
-            if (busy) {
-                auto part_of = [&](int i) {
-                    return parts + ((int64_t)(c0 + i) * 2 + (i == 0 && first_behind ? 1 : 0)) * PART<DP, NT>;
-                };
+        float acc[8] = {}, m = -INFINITY, l = 0.f;
+        const float* first = parts + ((int64_t)c0 * 2 + (first_behind ? 1 : 0)) * PART<DP, NT>;
+        const float* rest = parts + (int64_t)c0 * 2 * PART<DP, NT>;
+        if (gr < p.rows) {
 #pragma unroll 4
-                for (int i = grp; i < nc; i += groups) m = fmaxf(m, part_of(i)[8 * NT * DP + r]);
-                const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-                for (int i = grp; i < nc; i += groups) {
-                    const float* pt = part_of(i);
-                    const float fx = ptx::ex2_mufu(pt[8 * NT * DP + r] - base);
-                    l = fmaf(fx, pt[8 * NT * (DP + 1) + r], l);
-                    const float4 v0 = *(const float4*)(pt + r * DP + d), v1 = *(const float4*)(pt + r * DP + d + 4);
-                    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+            for (int i = warp; i < nc; i += 8) {
+                const float* pt = i ? rest + (int64_t)i * 2 * PART<DP, NT> : first;
+                const float pm = pt[8 * NT * DP + r], pl = pt[8 * NT * (DP + 1) + r];
+                const float4 v0 = *(const float4*)(pt + r * DP + d), v1 = *(const float4*)(pt + r * DP + d + 4);
+                const float mn = fmaxf(m, pm), base = mn == -INFINITY ? 0.f : mn;
+                const float f0 = ptx::ex2_mufu(m - base), f1 = ptx::ex2_mufu(pm - base);
+                m = mn;
+                l = l * f0 + pl * f1;
+                const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) acc[e] = fmaf(fx, v[e], acc[e]);
-                }
+                for (int e = 0; e < 8; ++e) acc[e] = acc[e] * f0 + v[e] * f1;
             }
-            if (groups > 1) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sacc[threadIdx.x][e] = acc[e];
-                sml[threadIdx.x][0] = m;
-                sml[threadIdx.x][1] = l;
-                __syncthreads();
-                if (busy && grp == 0) {
-                    for (int i = 1; i < groups; ++i) m = fmaxf(m, sml[threadIdx.x + i * pieces][0]);
-                    const float base = m == -INFINITY ? 0.f : m;
-                    l = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-                    for (int i = 0; i < groups; ++i) {
-                        const int s = threadIdx.x + i * pieces;
-                        const float fx = ptx::ex2_mufu(sml[s][0] - base);
-                        l = fmaf(fx, sml[s][1], l);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) acc[e] = fmaf(fx, sacc[s][e], acc[e]);
-                    }
-                }
-                __syncthreads();
-            }
-            if (busy && grp == 0) store_row<F16>(a, b, hk, rt * 8 * NT + r, d, acc, m, l);
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sacc[warp][e][lane] = acc[e];
+        sml[warp][0][lane] = m;
+        sml[warp][1][lane] = l;
+        __syncthreads();
+        if (warp == 0) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m = fmaxf(m, sml[i][0][lane]);
+            const float base = m == -INFINITY ? 0.f : m;
+            l = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float fx = ptx::ex2_mufu(sml[i][0][lane] - base);
+                l = fmaf(fx, sml[i][1][lane], l);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] = fmaf(fx, sacc[i][e][lane], acc[e]);
+            }
+            if (gr < p.rows) store_row<F16>(a, p, b, hk, gr, d, acc, m, l);
+        }
+        __syncthreads();
     }
 }
 
@@ -692,13 +692,16 @@ int launch(const Prob& a, float* parts, cudaStream_t s) {
     p.row_tiles = (int)cdiv(p.rows, 8 * NT);
     p.pairs = a.kv_heads * p.row_tiles;
     p.ctas = num_sms() * CTAS_PER_SM;
-    p.unit = Smem<DP>::KEYS * WARPS;
+    p.unit = DP == 64 ? 7 : 6;
+    static_assert(Smem<DP>::KEYS * WARPS == (DP == 64 ? 128 : 64), "unit");
+    p.magic = (65536 + a.group - 1) / a.group;
     using S = Smem<DP>;
     auto fn = rows_kernel<DP, F16, NT>;
     FD_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
     fn<<<p.ctas, WARPS * 32, S::BYTES, s>>>(a, p, parts);
     FD_CUDA_TRY(cudaGetLastError());
-    const int64_t all = (int64_t)a.batch * p.pairs, blocks = std::min<int64_t>(all, 4 * num_sms());
+    constexpr int slices = 8 * NT * DP / 8 / 32;
+    const int64_t blocks = std::min<int64_t>((int64_t)a.batch * p.pairs, 4 * num_sms()) * slices;
     // launched while the rows kernel runs; it waits (griddepcontrol) for that grid's end before it reads
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -710,7 +713,7 @@ int launch(const Prob& a, float* parts, cudaStream_t s) {
     cfg.attrs = &early;
     cfg.numAttrs = 1;
     const float* in = parts;
-    FD_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<DP, F16, NT>, a, p, in, cdiv(all, blocks)));
+    FD_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<DP, F16, NT>, a, p, in));
     return FD_OK;
 }
 
