@@ -14,12 +14,14 @@
 // CTA: two compute warpgroups that share the 128 rows of the accumulators (64
 // columns of each score tile apiece), and a warpgroup with a TMA producer, an
 // MMA issuer and a guard.
-//   key side    rows = keys.  TMEM: S^T | dP^T | dV | dK.  While the exponentials
-//               of tile i + 1 wait for S^T, the tensor core runs dV(i), S(i+1),
-//               and while dS(i) is made ... : P^T and dS^T go back to TMEM over
-//               the scores they came from and are the A operands.
+//   key side    rows = keys.  TMEM: S^T | dP^T | dV | dK.  P^T and dS^T go back to
+//               TMEM over the scores they came from and are the A operands.  The
+//               tensor core runs dV(i) and S(i + 1) while dS(i) is made, dK(i) and
+//               dP(i + 1) while P(i + 1) is.
 //   query side  rows = queries.  TMEM: S | dP, dP | dQ (dP in two buffers, so that
 //               the next tile's products do not wait for dS).
+#include <climits>
+
 #include "fd_attn_tc.cuh"
 
 namespace fd {
@@ -42,8 +44,9 @@ struct Bounds {
 
 // What prep_kernel leaves for the gradient kernel.
 struct Work {
-    float* delta;        // [batch * heads][rows padded to 128]
-    float* lse2;         // the same, base 2 (less P_SHIFT_F16 for fp16); +inf for rows that see nothing and for the padding
+    float* delta;        // -delta, [batch * heads][rows padded to 128]
+    float* lse2;         // -lse in base 2 (plus P_SHIFT_F16 for fp16); -inf for rows that see nothing and for the padding
+    int2* spans;         // [batch][rows padded to 128]
     Bounds* bounds;      // [batch][query tiles]
     unsigned* top;       // fp16: bits of the largest |dO row|^2 and |V row|^2
 };
@@ -57,9 +60,10 @@ __host__ __device__ inline size_t work_layout(Work* w, void* base, int64_t bh, i
     };
     char* a = take(sizeof(float) * bh * n_qt * T);
     char* b = take(sizeof(float) * bh * n_qt * T);
-    char* c = take(sizeof(Bounds) * batch * n_qt);
-    char* d = take(2 * sizeof(unsigned));
-    if (w) *w = {(float*)a, (float*)b, (Bounds*)c, (unsigned*)d};
+    char* c = take(sizeof(int2) * batch * n_qt * T);
+    char* d = take(sizeof(Bounds) * batch * n_qt);
+    char* e = take(2 * sizeof(unsigned));
+    if (w) *w = {(float*)a, (float*)b, (int2*)c, (Bounds*)d, (unsigned*)e};
     return at;
 }
 
@@ -111,6 +115,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
             const int i = t * T + threadIdx.x;
             const bool real = i < a.q_len;
             const int2 sp = real ? row_span(a, b, i, n) : make_int2(0, 0);
+            w.spans[((int64_t)b * n_qt + t) * T + threadIdx.x] = sp;
             const bool some = sp.y > sp.x;
             if (some) {
                 atomicMin(&sb[0], sp.x);
@@ -148,8 +153,8 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
         const bool some = lse != -INFINITY;
         if (F16 && some && s < INFINITY) top = fmaxf(top, s);
         if (piece == 0) {
-            w.delta[base + i] = some ? d : 0.f;
-            w.lse2[base + i] = some ? lse * LOG2E - (F16 ? P_SHIFT_F16 : 0.f) : INFINITY;
+            w.delta[base + i] = some ? -d : 0.f;
+            w.lse2[base + i] = some ? (F16 ? P_SHIFT_F16 : 0.f) - lse * LOG2E : -INFINITY;
         }
     }
     if (F16) {
@@ -162,13 +167,18 @@ template <int DP>
 struct Cfg {
     static constexpr int BOXES = DP / 64;
     static constexpr uint32_t TILE = BOXES * BOX_BYTES;
-    static constexpr int STAGES = 2;
-    static constexpr uint32_t RING_OFF = 2 * TILE;                       // behind the resident pair
-    static constexpr uint32_t VEC_OFF = RING_OFF + 2 * STAGES * TILE;    // lse2 and delta of each stage
-    static constexpr uint32_t BAR_OFF = VEC_OFF + STAGES * 2 * T * 4;
-    static constexpr int NBARS = 32;
+    // ring A: Q (key side) or K (query side), needed until the last product of a tile; ring B: dO or V, needed
+    // for less long, with lse2 and delta on the key side
+    static constexpr int SA = DP == 128 ? 3 : 4, SB = DP == 128 ? 2 : 4;
+    static constexpr uint32_t A_OFF = 2 * TILE;                       // behind the resident pair
+    static constexpr uint32_t B_OFF = A_OFF + SA * TILE;
+    static constexpr uint32_t VEC_OFF = B_OFF + SB * TILE;
+    static constexpr uint32_t BAR_OFF = VEC_OFF + SB * 2 * T * 4;
+    // opfull, afull[SA], aempty[SA], bfull[SB], bempty[SB], sfull, sread, pfull, dpfull[2], dsfull[2], accfull,
+    // toguard, guarded
+    static constexpr int NBARS = 1 + 2 * SA + 2 * SB + 10;
     static constexpr uint32_t MISC_OFF = BAR_OFF + NBARS * 8;
-    static constexpr uint32_t SMEM = MISC_OFF + 64 + 1024;
+    static constexpr uint32_t SMEM = MISC_OFF + 32;                   // 1024-byte aligned: nothing lies before it
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
 
@@ -182,34 +192,8 @@ struct Misc {
 struct Args {
     Prob a;
     Work w;
-    int n_qt, n_kt, n_key;   // query tiles, key tiles, CTAs of the key side
+    int n_qt, n_key;   // query tiles, CTAs of the key side
 };
-
-// A tile in shared memory: elements that are NaN or infinite become zeros; true if there were any.
-template <bool F16>
-__device__ __forceinline__ bool clear_bad(uint8_t* tile, int bytes, int lane) {
-    constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
-    bool bad = false;
-#pragma unroll 8
-    for (int i = lane; i < bytes / 16; i += 32) {
-        const uint4 x = ((uint4*)tile)[i];
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bad = bad || (w[e] & EXP) == EXP || ((w[e] >> 16) & EXP) == EXP;
-    }
-    bad = __any_sync(~0u, bad);
-    if (bad) {
-        for (int i = lane; i < bytes / 4; i += 32) {
-            uint32_t x = ((uint32_t*)tile)[i];
-            if ((x & EXP) == EXP) x &= 0xffff0000u;
-            if (((x >> 16) & EXP) == EXP) x &= 0xffffu;
-            ((uint32_t*)tile)[i] = x;
-        }
-        ptx::fence_async_shared();
-        __syncwarp();
-    }
-    return bad;
-}
 
 // Store N columns of one accumulator row, times f, as 16-bit values behind column c0 of `out`.
 template <int N, bool F16>
@@ -237,63 +221,520 @@ __device__ __forceinline__ void store_cols(uint32_t taddr, float f, uint8_t* out
     }
 }
 
+// What every role of a CTA knows.
+struct Cta {
+    const Prob& a;
+    const Work& w;
+    bool key_side;
+    int tile, b, h;        // h: key head on the key side, query head on the query side
+    int r0, n, n_qt;       // first row of this CTA, keys in use, query tiles
+    int t0, nt, items;     // the other side's tiles t0 .. t0 + nt, walked items / nt times (once for each head of the group)
+    Bounds own;            // query side: this tile's bounds
+    const Bounds* bounds;
+};
+
+// Item i of a CTA: its tile, and the query head on the key side.
+struct Item {
+    int i, t, head;
+    __device__ explicit Item(const Cta& c) : i(0), t(c.t0), head(c.key_side ? c.h * c.a.group : c.h) {}
+    __device__ void next(const Cta& c) {
+        ++i;
+        if (++t == c.t0 + c.nt) {
+            t = c.t0;
+            ++head;
+        }
+    }
+    // some pair of the tile is masked
+    __device__ bool partial(const Cta& c) const {
+        if (!c.key_side) return t * T < c.own.flo || (t + 1) * T > c.own.fhi;
+        const Bounds o = c.bounds[t];
+        return c.r0 < o.flo || c.r0 + T > o.fhi;
+    }
+};
+
+struct Bars {
+    uint64_t *opfull, *afull, *aempty, *bfull, *bempty, *sfull, *sread, *pfull, *dpfull, *dsfull, *accfull, *toguard, *guarded;
+};
+
+// Stage and phase of a ring of N slots.
+template <int N>
+struct Slot {
+    int at = 0;
+    uint32_t ph = 0;
+    __device__ void next() {
+        if (++at == N) {
+            at = 0;
+            ph ^= 1;
+        }
+    }
+};
+
+template <int DP, bool F16>
+__device__ __forceinline__ void produce(const Cta& c, const Bars& br, uint8_t* base, const CUtensorMap* tmq,
+                                        const CUtensorMap* tmk, const CUtensorMap* tmv, const CUtensorMap* tmdo,
+                                        volatile int* abort, int* status) {
+    using C = Cfg<DP>;
+    auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int t, int hh) {
+        for (int x = 0; x < C::BOXES; ++x) ptx::tma_load_4d(dst + x * BOX_BYTES, m, bar, x * 64, t * T, hh, c.b);
+    };
+    ptx::mbar_expect_tx(br.opfull, 2 * C::TILE);
+    load(base, c.key_side ? tmk : tmq, br.opfull, c.tile, c.h);
+    load(base + C::TILE, c.key_side ? tmv : tmdo, br.opfull, c.tile, c.h);
+    const int hk = c.h / c.a.group;      // query side
+    Slot<C::SA> sa;
+    Slot<C::SB> sb;
+    int na = 0, nb = 0;
+    for (Item it(c); it.i < c.items; it.next(c)) {
+        const int hh = c.key_side ? it.head : hk;
+        if (!ptx::wait_bounded(&br.aempty[sa.at], sa.ph ^ 1, abort, status, WAIT_NS)) break;
+        ptx::mbar_expect_tx(&br.afull[sa.at], C::TILE);
+        load(base + C::A_OFF + sa.at * C::TILE, c.key_side ? tmq : tmk, &br.afull[sa.at], it.t, hh);
+        sa.next();
+        ++na;
+        if (!ptx::wait_bounded(&br.bempty[sb.at], sb.ph ^ 1, abort, status, WAIT_NS)) break;
+        ptx::mbar_expect_tx(&br.bfull[sb.at], C::TILE + (c.key_side ? 2 * T * 4 : 0));
+        load(base + C::B_OFF + sb.at * C::TILE, c.key_side ? tmdo : tmv, &br.bfull[sb.at], it.t, hh);
+        if (c.key_side) {
+            float* vec = (float*)(base + C::VEC_OFF) + sb.at * 2 * T;
+            const int64_t at = (((int64_t)c.b * c.a.heads + hh) * c.n_qt + it.t) * T;
+            ptx::bulk_load(vec, c.w.lse2 + at, T * 4, &br.bfull[sb.at]);
+            ptx::bulk_load(vec + T, c.w.delta + at, T * 4, &br.bfull[sb.at]);
+        }
+        sb.next();
+        ++nb;
+    }
+    if (*abort) {   // the copies in flight still write into this block's memory
+        wait_landed(br.opfull, 0);
+        for (int z = max(0, na - C::SA); z < na; ++z) wait_landed(&br.afull[z % C::SA], (z / C::SA) & 1);
+        for (int z = max(0, nb - C::SB); z < nb; ++z) wait_landed(&br.bfull[z % C::SB], (z / C::SB) & 1);
+    }
+}
+
+template <int DP, bool F16>
+__device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* base, uint32_t tmem, volatile int* abort,
+                                      int* status) {
+    using C = Cfg<DP>;
+    const int kd = (c.a.dim + 15) / 16;
+    const uint32_t id_s = ptx::idesc_f32acc(T, T, F16);
+    const uint32_t id_acc = ptx::idesc_f32acc(T, kd * 16, F16) | ptx::IDESC_B_MN;
+    const uint32_t op0 = ptx::smem_u32(base), op1 = op0 + C::TILE, ra = op0 + C::A_OFF, rb = op0 + C::B_OFF;
+    auto wait = [&](uint64_t* bar, uint32_t ph) { return ptx::wait_bounded(bar, ph & 1, abort, status, WAIT_NS); };
+    // D[128 x 128] = resident operand . ring operand^T
+    auto scores = [&](uint32_t d, uint32_t op, uint32_t rg) {
+        ptx::tc_fence_after();
+        for (int ks = 0; ks < kd; ++ks) ptx::umma_ss(d, kmajor(op, ks), kmajor(rg, ks), id_s, ks > 0);
+    };
+    // acc[128 x dim] += (16-bit tile in TMEM, 64 columns of it at `src`, 64 at `src` + 64) . ring tile
+    auto sum = [&](uint32_t acc, uint32_t src, uint32_t rg, bool more) {
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < T / 16; ++ks)
+            ptx::umma_ts(acc, src + (ks >> 2) * 64 + (ks & 3) * 8, mnmajor(rg, ks), id_acc, more || ks > 0);
+    };
+    uint32_t ng = 0;
+    bool ok = wait(br.opfull, 0);
+    if (c.key_side) {
+        const uint32_t S = tmem, DPT = tmem + 128, DV = tmem + 256, DK = tmem + 384;
+        Slot<C::SA> sa, da;      // next S, current dK
+        Slot<C::SB> sb, db;      // next dP, current dV
+        Item ahead(c);           // tile of the next dP
+        bool look = false;
+        auto first = [&]() {     // S^T
+            if (!wait(&br.afull[sa.at], sa.ph)) return false;
+            scores(S, op0, ra + sa.at * C::TILE);
+            ptx::umma_commit(br.sfull);
+            sa.next();
+            return true;
+        };
+        auto second = [&]() {    // dP^T
+            if (!wait(&br.bfull[sb.at], sb.ph)) return false;
+            scores(DPT, op1, rb + sb.at * C::TILE);
+            ptx::umma_commit(&br.dpfull[0]);
+            look = ahead.partial(c);
+            if (look) ptx::mbar_arrive(br.toguard);
+            sb.next();
+            ahead.next(c);
+            return true;
+        };
+        ok = ok && first() && second();
+        for (int i = 0; i < c.items && ok; ++i) {
+            if (!(ok = wait(br.pfull, i))) break;
+            if (look) {
+                if (!(ok = wait(br.guarded, ng))) break;
+                ++ng;
+            }
+            sum(DV, S, rb + db.at * C::TILE, i > 0);
+            ptx::umma_commit(&br.bempty[db.at]);
+            db.next();
+            if (i + 1 < c.items && !(ok = first())) break;
+            if (!(ok = wait(&br.dsfull[0], i))) break;
+            sum(DK, DPT, ra + da.at * C::TILE, i > 0);
+            ptx::umma_commit(&br.aempty[da.at]);
+            da.next();
+            if (i + 1 < c.items) ok = second();
+        }
+    } else {
+        const uint32_t S = tmem, DQ = tmem + 384;
+        Slot<C::SA> sa, da;
+        Slot<C::SB> sb;
+        int made = 0;
+        auto both = [&]() {       // S and dP of the next tile
+            if (!wait(&br.afull[sa.at], sa.ph)) return false;
+            scores(S, op0, ra + sa.at * C::TILE);
+            ptx::umma_commit(br.sfull);
+            if (!wait(&br.bfull[sb.at], sb.ph)) return false;
+            scores(tmem + 128 + (made & 1) * 128, op1, rb + sb.at * C::TILE);
+            ptx::umma_commit(&br.dpfull[made & 1]);
+            ptx::umma_commit(&br.bempty[sb.at]);
+            sa.next();
+            sb.next();
+            ++made;
+            return true;
+        };
+        ok = ok && both();
+        for (Item it(c); it.i < c.items && ok; it.next(c)) {
+            const bool look = it.partial(c);
+            if (look) ptx::mbar_arrive(br.toguard);
+            if (it.i + 1 < c.items) {
+                if (!(ok = wait(br.sread, it.i))) break;
+                if (!(ok = both())) break;
+            }
+            // one barrier for each dP buffer: a warp may be a tile ahead of another, and its arrival for the
+            // next tile must not stand in for the other's for this one
+            if (!(ok = wait(&br.dsfull[it.i & 1], it.i >> 1))) break;
+            if (look) {
+                if (!(ok = wait(br.guarded, ng))) break;
+                ++ng;
+            }
+            sum(DQ, tmem + 128 + (it.i & 1) * 128, ra + da.at * C::TILE, it.i > 0);
+            ptx::umma_commit(&br.aempty[da.at]);
+            da.next();
+        }
+    }
+    ptx::umma_commit(br.accfull);
+    if (!ok) wait_landed(br.accfull, 0);
+}
+
+// Masked pairs have P = dS = 0, and zero times a NaN or an infinity of the other operand would reach the sum: in
+// partly visible tiles such elements become zeros before the product.  What a visible pair loses with them is NaN
+// already through lse (Q, K) or delta (dO) of its row, except for dV, where a visible row's bad dO elements are put
+// back at the end (`poison`).
+template <int DP, bool F16>
+__device__ __forceinline__ void watch(const Cta& c, const Bars& br, uint8_t* base, int lane, int* poison,
+                                      volatile int* abort, int* status) {
+    using C = Cfg<DP>;
+    uint32_t ng = 0;
+    Slot<C::SA> sa;
+    Slot<C::SB> sb;
+    for (Item it(c); it.i < c.items; it.next(c), sa.next(), sb.next()) {
+        if (!it.partial(c)) continue;
+        // not before the issuer has seen the tile: see the forward kernel's guard
+        if (!ptx::wait_bounded(br.toguard, ng & 1, abort, status, WAIT_NS)) return;
+        ++ng;
+        if (!ptx::wait_bounded(&br.afull[sa.at], sa.ph, abort, status, WAIT_NS)) return;
+        clear_bad<F16>(base + C::A_OFF + sa.at * C::TILE, C::TILE, lane);
+        if (c.key_side) {
+            if (!ptx::wait_bounded(&br.bfull[sb.at], sb.ph, abort, status, WAIT_NS)) return;
+            if (clear_bad<F16>(base + C::B_OFF + sb.at * C::TILE, C::TILE, lane) && lane == 0) *poison = 1;
+            __syncwarp();
+        }
+        if (lane == 0) ptx::mbar_arrive(br.guarded);
+    }
+}
+
+// Raw products of one row, 32 columns, to weights: x = 2^(score + add); with a cap, bend = 1 - tanh^2.
+template <bool GEN, int POLY>
+__device__ __forceinline__ void weights32(uint64_t (&x)[16], const uint64_t (&add)[16], const Score& sc, float slope2,
+                                          float dist, float by, int side, uint64_t (&bend)[GEN ? 16 : 1]) {
+    if (GEN && sc.capped) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = ptx::mul2(x[e], sc.c);
+        tanh32(x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            bend[e] = ptx::fma2(ptx::mul2(x[e], ptx::both2(-1.f)), x[e], ptx::both2(1.f));
+            x[e] = ptx::fma2(x[e], sc.cap2, add[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = ptx::fma2(x[e], sc.c, add[e]);
+    }
+    if (GEN && slope2 != 0.f) add_bias(x, slope2, dist, by, side);
+    exp32<POLY>(x);
+}
+
+template <int DP, bool F16, bool GEN>
+__device__ __forceinline__ bool compute_key(const Cta& c, const Bars& br, const uint8_t* base, uint32_t lanes, int half,
+                                            int row, float up_p, volatile int* abort, int* status) {
+    using C = Cfg<DP>;
+    const Prob& a = c.a;
+    const int lane = threadIdx.x & 31;
+    const Score sc(a);
+    const int shift = c.n - a.q_len;              // position of query i: shift + i
+    const int2* spans = c.w.spans + (int64_t)c.b * c.n_qt * T;
+    Slot<C::SB> sb;
+    float slope2 = 0.f;
+    int head = -1;
+    Item it(c);
+    bool masked = it.i < c.items && it.partial(c);
+    for (; it.i < c.items;) {
+        const int t = it.t, q0 = t * T + half * 64;          // this thread's first column
+        if (GEN && a.slopes && head != it.head) {
+            head = it.head;
+            slope2 = a.slopes[head] * LOG2E;
+        }
+        const int side = GEN ? side_of(a, shift + t * T, c.r0) : 1;
+        const uint32_t i = it.i;
+        const float* vec = (const float*)(base + C::VEC_OFF) + sb.at * 2 * T + half * 64;
+        if (!ptx::wait_bounded(&br.bfull[sb.at], sb.ph, abort, status, WAIT_NS)) return false;
+        uint64_t add[2][16];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) ptx::lds_pairs(vec + g * 32 + 2 * e, add[g][e], add[g][e + 1]);
+        if (!ptx::wait_bounded(br.sfull, i & 1, abort, status, WAIT_NS)) return false;
+        ptx::tc_fence_after();
+        uint64_t x[2][16];
+        {
+            uint32_t r[2][32];
+            ptx::tmem_ld32(lanes + half * 64, r[0]);
+            ptx::tmem_ld32(lanes + half * 64 + 32, r[1]);
+            ptx::tmem_wait_ld(r[0]);
+            ptx::tmem_wait_ld(r[1]);
+            pairs32(r[0], x[0]);
+            pairs32(r[1], x[1]);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            uint64_t bend[GEN ? 16 : 1];
+            weights32<GEN, 1>(x[g], add[g], sc, slope2, (float)(shift + q0 + g * 32 - row), 1.f, side, bend);
+            if (masked) {
+                if (!a.first) {
+                    // the queries that see this key are a run: i >= row - shift, and i < that + window
+                    const int lo = a.causal ? row - shift : row < c.n ? INT_MIN / 2 : INT_MAX / 2;
+                    const int64_t hi = row >= c.n ? lo : a.window ? (int64_t)row - shift + a.window : a.q_len;
+                    const int l0 = max(lo, 0) - (q0 + g * 32), l1 = (int)min(hi, (int64_t)a.q_len) - (q0 + g * 32);
+                    mask32(x[g], l0, (uint32_t)max(l1 - l0, 0), 0.f);
+                } else {
+                    const int4* sp = (const int4*)(spans + q0 + g * 32);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int4 s = sp[e];
+                        x[g][e] = ptx::pack2(row >= s.x && row < s.y ? ptx::lo2(x[g][e]) : 0.f,
+                                             row >= s.z && row < s.w ? ptx::hi2(x[g][e]) : 0.f);
+                    }
+                }
+            }
+            uint32_t p[16];
+            round32<F16>(x[g], p);
+            ptx::tmem_st16(lanes + half * 64 + g * 16, p);
+            if (GEN && sc.capped) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
+            }
+        }
+        // delta leaves the stage before it may be refilled (after dV of this tile)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) ptx::lds_pairs(vec + T + g * 32 + 2 * e, add[g][e], add[g][e + 1]);
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(br.pfull);
+        sb.next();
+        it.next(c);
+        const bool next_masked = it.i < c.items && it.partial(c);
+        if (!ptx::wait_bounded(&br.dpfull[0], i & 1, abort, status, WAIT_NS)) return false;
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            uint32_t r[32];
+            ptx::tmem_ld32(lanes + 128 + half * 64 + g * 32, r);
+            ptx::tmem_wait_ld(r);
+            uint64_t d[16];
+            pairs32(r, d);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) d[e] = ptx::mul2(x[g][e], ptx::add2(d[e], add[g][e]));
+            if (masked) {   // zero, whatever dP of a masked pair holds
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    d[e] = ptx::pack2(ptx::lo2(x[g][e]) == 0.f ? 0.f : ptx::lo2(d[e]), ptx::hi2(x[g][e]) == 0.f ? 0.f : ptx::hi2(d[e]));
+            }
+            if (F16) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) d[e] = ptx::mul2(d[e], ptx::both2(up_p));
+            }
+            uint32_t p[16];
+            round32<F16>(d, p);
+            ptx::tmem_st16(lanes + 128 + half * 64 + g * 16, p);
+        }
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&br.dsfull[0]);
+        masked = next_masked;
+    }
+    return true;
+}
+
+template <int DP, bool F16, bool GEN>
+__device__ __forceinline__ bool compute_query(const Cta& c, const Bars& br, uint32_t lanes, int half, int row, float up_p,
+                                              volatile int* abort, int* status) {
+    const Prob& a = c.a;
+    const int lane = threadIdx.x & 31;
+    const Score sc(a);
+    const int64_t at = (((int64_t)c.b * a.heads + c.h) * c.n_qt) * T + row;
+    const uint64_t nlse = ptx::both2(c.w.lse2[at]), ndelta = ptx::both2(c.w.delta[at]);
+    // rows behind the last query have no weight, and are not stored
+    const int2 span = row < a.q_len ? c.w.spans[(int64_t)c.b * c.n_qt * T + row] : make_int2(0, INT_MAX);
+    const float slope2 = GEN && a.slopes ? a.slopes[c.h] * LOG2E : 0.f;
+    const int shift = c.n - a.q_len;
+    uint64_t add[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) add[e] = nlse;
+    for (Item it(c); it.i < c.items; it.next(c)) {
+        const int k0 = it.t * T + half * 64;                 // this thread's first column
+        const uint32_t i = it.i, buf = i & 1;
+        const bool masked = it.partial(c);
+        const int side = GEN ? side_of(a, shift + c.r0, it.t * T) : 1;
+        if (!ptx::wait_bounded(br.sfull, i & 1, abort, status, WAIT_NS)) return false;
+        ptx::tc_fence_after();
+        uint64_t x[2][16];
+        {
+            uint32_t r[2][32];
+            ptx::tmem_ld32(lanes + half * 64, r[0]);
+            ptx::tmem_ld32(lanes + half * 64 + 32, r[1]);
+            ptx::tmem_wait_ld(r[0]);
+            ptx::tmem_wait_ld(r[1]);
+            pairs32(r[0], x[0]);
+            pairs32(r[1], x[1]);
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(br.sread);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            uint64_t bend[GEN ? 16 : 1];
+            weights32<GEN, 1>(x[g], add, sc, slope2, (float)(shift + row - k0 - g * 32), -1.f, side, bend);
+            if (masked) mask32(x[g], span.x - k0 - g * 32, (uint32_t)(span.y - span.x), 0.f);
+            if (GEN && sc.capped) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
+            }
+        }
+        const uint32_t dp = lanes + 128 + buf * 128 + half * 64;
+        if (!ptx::wait_bounded(&br.dpfull[buf], (i >> 1) & 1, abort, status, WAIT_NS)) return false;
+        ptx::tc_fence_after();
+        uint32_t r[2][32];
+        ptx::tmem_ld32(dp, r[0]);
+        ptx::tmem_ld32(dp + 32, r[1]);
+        ptx::tmem_wait_ld(r[0]);
+        ptx::tmem_wait_ld(r[1]);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            uint64_t d[16];
+            pairs32(r[g], d);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) d[e] = ptx::mul2(x[g][e], ptx::add2(d[e], ndelta));
+            if (masked) {   // zero, whatever dP of a masked pair holds
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    d[e] = ptx::pack2(ptx::lo2(x[g][e]) == 0.f ? 0.f : ptx::lo2(d[e]), ptx::hi2(x[g][e]) == 0.f ? 0.f : ptx::hi2(d[e]));
+            }
+            if (F16) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) d[e] = ptx::mul2(d[e], ptx::both2(up_p));
+            }
+            uint32_t p[16];
+            round32<F16>(d, p);
+            ptx::tmem_st16(dp + g * 16, p);
+        }
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&br.dsfull[buf]);
+    }
+    return true;
+}
+
+// dV row `out`: the NaN and infinite dO elements that the guard took out, of the queries that see this key.
+template <bool F16>
+__device__ void put_back(const Cta& c, uint8_t* out, int row) {
+    const Prob& a = c.a;
+    for (Item it(c); it.i < c.items; it.next(c)) {
+        if (!it.partial(c)) continue;
+        const int q1 = min((it.t + 1) * T, a.q_len);
+        for (int q = it.t * T; q < q1; ++q) {
+            const int2 sp = row_span(a, c.b, q, c.n);
+            if (row < sp.x || row >= sp.y) continue;
+            const uint16_t* g = (const uint16_t*)a.d_o.p + c.b * a.d_o.sb + (int64_t)q * a.d_o.ss + it.head * a.d_o.sh;
+            constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
+            for (int d = 0; d < a.dim; ++d)
+                if ((g[d] & EXP) == EXP) {
+                    uint16_t* o = (uint16_t*)out + d;
+                    const float2 f = pair_of<F16>((uint32_t)*o | ((uint32_t)g[d] << 16));
+                    *o = (uint16_t)ptx::pack16<F16>(f.x + f.y, 0.f);
+                }
+        }
+    }
+}
+
 template <int DP, bool F16, bool GEN>
 __global__ void __launch_bounds__(NTHREADS, 1)
 gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmdo,
                 const __grid_constant__ Args args, int* __restrict__ status) {
     using C = Cfg<DP>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = (uint64_t*)(base + C::BAR_OFF);
-    // ring A: Q (key side) or K (query side), needed until the last product of a tile;
-    // ring B: dO or V
-    uint64_t *opfull = bars, *afull = bars + 1, *aempty = afull + C::STAGES, *bfull = aempty + C::STAGES,
-             *bempty = bfull + C::STAGES, *sfull = bempty + C::STAGES, *sread = sfull + 1, *pfull = sread + 1,
-             *dpfull = pfull + 1, *dsfull = dpfull + 2, *accfull = dsfull + 2, *toguard = accfull + 1,
-             *guarded = toguard + 1;
+    extern __shared__ __align__(1024) uint8_t base[];
+    if (ptx::smem_u32(base) & 1023) {   // the swizzled tiles need it, and there is no room to round up
+        if (threadIdx.x == 0) atomicExch(status, FD_ERR_UNSUPPORTED);
+        return;
+    }
+    Bars br;
+    br.opfull = (uint64_t*)(base + C::BAR_OFF);
+    br.afull = br.opfull + 1;
+    br.aempty = br.afull + C::SA;
+    br.bfull = br.aempty + C::SA;
+    br.bempty = br.bfull + C::SB;
+    br.sfull = br.bempty + C::SB;
+    br.sread = br.sfull + 1;
+    br.pfull = br.sread + 1;
+    br.dpfull = br.pfull + 1;
+    br.dsfull = br.dpfull + 2;
+    br.accfull = br.dsfull + 2;
+    br.toguard = br.accfull + 1;
+    br.guarded = br.toguard + 1;
     Misc& ms = *(Misc*)(base + C::MISC_OFF);
     volatile int* abort = &ms.abort;
     const Prob& a = args.a;
     const Work& w = args.w;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool key_side = (int)blockIdx.x < args.n_key;
-    int tile, b, h;     // h: key head on the key side, query head on the query side
-    if (key_side) {
+    Cta c{a, w};
+    c.key_side = (int)blockIdx.x < args.n_key;
+    if (c.key_side) {
         // earlier key tiles are seen by more queries under a causal mask: they start first
         const int nh = a.kv_heads * a.batch;
-        tile = blockIdx.x / nh;
-        b = blockIdx.x % nh / a.kv_heads;
-        h = blockIdx.x % nh % a.kv_heads;
+        c.tile = blockIdx.x / nh;
+        c.b = blockIdx.x % nh / a.kv_heads;
+        c.h = blockIdx.x % nh % a.kv_heads;
     } else {
         const int nh = a.heads * a.batch, u = blockIdx.x - args.n_key;
-        tile = args.n_qt - 1 - u / nh;
-        b = u % nh / a.heads;
-        h = u % nh % a.heads;
+        c.tile = args.n_qt - 1 - u / nh;
+        c.b = u % nh / a.heads;
+        c.h = u % nh % a.heads;
     }
-    const int r0 = tile * T;                     // first row of this CTA
-    const int n = keys_of(a, b);
-    const Bounds* bounds = w.bounds + (int64_t)b * args.n_qt;
+    c.r0 = c.tile * T;
+    c.n = keys_of(a, c.b);
+    c.n_qt = args.n_qt;
+    c.bounds = w.bounds + (int64_t)c.b * args.n_qt;
 
     if (threadIdx.x == 0) {
-        ptx::mbar_init(opfull, 1);
-        for (int i = 0; i < C::STAGES; ++i) {
-            ptx::mbar_init(&afull[i], 1);
-            ptx::mbar_init(&aempty[i], 1);
-            ptx::mbar_init(&bfull[i], 1);
-            ptx::mbar_init(&bempty[i], 1);
+        for (int i = 0; i < C::NBARS; ++i) {
+            uint64_t* bar = br.opfull + i;
+            ptx::mbar_init(bar, bar == br.sread || bar == br.pfull || (bar >= br.dsfull && bar < br.dsfull + 2) ? 8 : 1);
         }
-        ptx::mbar_init(sfull, 1);
-        ptx::mbar_init(sread, 8);
-        ptx::mbar_init(pfull, 8);
-        ptx::mbar_init(&dpfull[0], 1);
-        ptx::mbar_init(&dpfull[1], 1);
-        ptx::mbar_init(&dsfull[0], 8);
-        ptx::mbar_init(&dsfull[1], 8);
-        ptx::mbar_init(accfull, 1);
-        ptx::mbar_init(toguard, 1);
-        ptx::mbar_init(guarded, 1);
         ms.abort = 0;
         ms.poison = 0;
         ms.lo = 0x7fffffff;
@@ -311,10 +752,10 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         ptx::prefetch_tmap(&tmdo);
     }
     __syncthreads();
-    if (key_side) {
+    if (c.key_side) {
         int lo = 0x7fffffff, hi = 0;
         for (int t = threadIdx.x; t < args.n_qt; t += NTHREADS)
-            if (bounds[t].hi > r0 && bounds[t].lo < r0 + T) {
+            if (c.bounds[t].hi > c.r0 && c.bounds[t].lo < c.r0 + T) {
                 lo = min(lo, t);
                 hi = max(hi, t + 1);
             }
@@ -329,377 +770,55 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = ms.tmem;
-    // the other side's tiles, t0 .. t0 + nt, walked `items / nt` times (once for each head of the group)
-    int t0, nt;
-    Bounds own = {0, 0, 0, 0};
-    if (key_side) {
-        t0 = ms.lo;
-        nt = ms.hi > ms.lo ? ms.hi - ms.lo : 0;
+    c.own = {0, 0, 0, 0};
+    if (c.key_side) {
+        c.t0 = ms.lo;
+        c.nt = ms.hi > ms.lo ? ms.hi - ms.lo : 0;
     } else {
-        own = bounds[tile];
-        t0 = own.lo / T;
-        nt = own.hi > own.lo ? (own.hi + T - 1) / T - t0 : 0;
+        c.own = c.bounds[c.tile];
+        c.t0 = c.own.lo / T;
+        c.nt = c.own.hi > c.own.lo ? (c.own.hi + T - 1) / T - c.t0 : 0;
     }
-    const int items = key_side ? nt * a.group : nt;
-    auto tile_of = [&](int i) { return t0 + (key_side ? i % nt : i); };
-    auto head_of = [&](int i) { return h * a.group + i / nt; };
-    // some pair of the tile is masked
-    auto partial = [&](int i) {
-        const int t = tile_of(i);
-        if (!key_side) return t * T < own.flo || (t + 1) * T > own.fhi;
-        const Bounds o = bounds[t];
-        return r0 < o.flo || r0 + T > o.fhi;
-    };
+    c.items = c.key_side ? c.nt * a.group : c.nt;
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        uint8_t* ring_a = base + C::RING_OFF;
-        uint8_t* ring_b = ring_a + C::STAGES * C::TILE;
         if (warp == TMA_WARP) {
-            if (lane == 0 && items > 0) {
-                auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int t, int hh) {
-                    for (int c = 0; c < C::BOXES; ++c) ptx::tma_load_4d(dst + c * BOX_BYTES, m, bar, c * 64, t * T, hh, b);
-                };
-                ptx::mbar_expect_tx(opfull, 2 * C::TILE);
-                const int hk = key_side ? h : h / a.group;
-                load(base, key_side ? &tmk : &tmq, opfull, tile, h);
-                load(base + C::TILE, key_side ? &tmv : &tmdo, opfull, tile, h);
-                int i = 0, ib = 0;
-                for (; i < items; ++i, ++ib) {
-                    const int st = i % C::STAGES, ph = (i / C::STAGES) & 1;
-                    const int t = tile_of(i), hh = key_side ? head_of(i) : hk;
-                    if (!ptx::wait_bounded(&aempty[st], ph ^ 1, abort, status, WAIT_NS)) break;
-                    ptx::mbar_expect_tx(&afull[st], C::TILE + (key_side ? 2 * T * 4 : 0));
-                    load(ring_a + st * C::TILE, key_side ? &tmq : &tmk, &afull[st], t, hh);
-                    if (key_side) {
-                        float* vec = (float*)(base + C::VEC_OFF) + st * 2 * T;
-                        const int64_t at = (((int64_t)b * a.heads + hh) * args.n_qt + t) * T;
-                        ptx::bulk_load(vec, w.lse2 + at, T * 4, &afull[st]);
-                        ptx::bulk_load(vec + T, w.delta + at, T * 4, &afull[st]);
-                    }
-                    if (!ptx::wait_bounded(&bempty[st], ph ^ 1, abort, status, WAIT_NS)) { ++i; break; }
-                    ptx::mbar_expect_tx(&bfull[st], C::TILE);
-                    load(ring_b + st * C::TILE, key_side ? &tmdo : &tmv, &bfull[st], t, hh);
-                }
-                if (*abort) {   // the copies in flight still write into this block's memory
-                    wait_landed(opfull, 0);
-                    for (int z = max(0, i - C::STAGES); z < i; ++z) wait_landed(&afull[z % C::STAGES], (z / C::STAGES) & 1);
-                    for (int z = max(0, ib - C::STAGES); z < ib; ++z) wait_landed(&bfull[z % C::STAGES], (z / C::STAGES) & 1);
-                }
-            }
+            if (lane == 0 && c.items > 0) produce<DP, F16>(c, br, base, &tmq, &tmk, &tmv, &tmdo, abort, status);
         } else if (warp == MMA_WARP) {
-            if (lane == 0 && items > 0) {
-                const int kd = (a.dim + 15) / 16;
-                const uint32_t id_s = ptx::idesc_f32acc(T, T, F16);
-                const uint32_t id_acc = ptx::idesc_f32acc(T, kd * 16, F16) | ptx::IDESC_B_MN;
-                const uint32_t op0 = ptx::smem_u32(base), op1 = op0 + C::TILE;
-                const uint32_t ra = ptx::smem_u32(ring_a), rb = ptx::smem_u32(ring_b);
-                auto wait = [&](uint64_t* bar, int ph) { return ptx::wait_bounded(bar, ph & 1, abort, status, WAIT_NS); };
-                // D[128 x 128] = resident operand . ring operand^T
-                auto scores = [&](uint32_t d, uint32_t op, uint32_t rg, int st) {
-                    ptx::tc_fence_after();
-                    for (int ks = 0; ks < kd; ++ks)
-                        ptx::umma_ss(d, kmajor(op, ks), kmajor(rg + st * C::TILE, ks), id_s, ks > 0);
-                };
-                // acc[128 x dim] += (16-bit tile in TMEM, 64 columns of it at `src`, 64 at `src` + 64) . ring tile
-                auto sum = [&](uint32_t acc, uint32_t src, uint32_t rg, int st, bool more) {
-                    ptx::tc_fence_after();
-#pragma unroll
-                    for (int ks = 0; ks < T / 16; ++ks)
-                        ptx::umma_ts(acc, src + (ks >> 2) * 64 + (ks & 3) * 8, mnmajor(rg + st * C::TILE, ks), id_acc,
-                                     more || ks > 0);
-                };
-                uint32_t ng = 0;
-                bool ok = wait(opfull, 0);
-                if (key_side) {
-                    const uint32_t S = tmem, DPT = tmem + 128, DV = tmem + 256, DK = tmem + 384;
-                    bool look = false;
-                    auto first = [&](int i) {      // S^T(i)
-                        const int st = i % C::STAGES;
-                        if (!wait(&afull[st], i / C::STAGES)) return false;
-                        scores(S, op0, ra, st);
-                        ptx::umma_commit(sfull);
-                        return true;
-                    };
-                    auto second = [&](int i) {     // dP^T(i)
-                        const int st = i % C::STAGES;
-                        if (!wait(&bfull[st], i / C::STAGES)) return false;
-                        scores(DPT, op1, rb, st);
-                        ptx::umma_commit(&dpfull[0]);
-                        look = partial(i);
-                        if (look) ptx::mbar_arrive(toguard);
-                        return true;
-                    };
-                    ok = ok && first(0) && second(0);
-                    for (int i = 0; i < items && ok; ++i) {
-                        const int st = i % C::STAGES;
-                        if (!(ok = wait(pfull, i))) break;
-                        if (look) {
-                            if (!(ok = wait(guarded, ng))) break;
-                            ++ng;
-                        }
-                        sum(DV, S, rb, st, i > 0);
-                        ptx::umma_commit(&bempty[st]);
-                        if (i + 1 < items && !(ok = first(i + 1))) break;
-                        if (!(ok = wait(&dsfull[0], i))) break;
-                        sum(DK, DPT, ra, st, i > 0);
-                        ptx::umma_commit(&aempty[st]);
-                        if (i + 1 < items) ok = second(i + 1);
-                    }
-                } else {
-                    const uint32_t S = tmem, DQ = tmem + 384;
-                    auto both = [&](int i) {       // S(i), dP(i)
-                        const int st = i % C::STAGES;
-                        if (!wait(&afull[st], i / C::STAGES)) return false;
-                        scores(S, op0, ra, st);
-                        ptx::umma_commit(sfull);
-                        if (!wait(&bfull[st], i / C::STAGES)) return false;
-                        scores(tmem + 128 + (i & 1) * 128, op1, rb, st);
-                        ptx::umma_commit(&dpfull[i & 1]);
-                        ptx::umma_commit(&bempty[st]);
-                        return true;
-                    };
-                    ok = ok && both(0);
-                    for (int i = 0; i < items && ok; ++i) {
-                        const int st = i % C::STAGES;
-                        const bool look = partial(i);
-                        if (look) ptx::mbar_arrive(toguard);
-                        if (i + 1 < items) {
-                            if (!(ok = wait(sread, i))) break;
-                            if (!(ok = both(i + 1))) break;
-                        }
-                        // one barrier for each dP buffer: a warp may be a tile ahead of another, and its
-                        // arrival for i + 1 must not stand in for the other's for i
-                        if (!(ok = wait(&dsfull[i & 1], i >> 1))) break;
-                        if (look) {
-                            if (!(ok = wait(guarded, ng))) break;
-                            ++ng;
-                        }
-                        sum(DQ, tmem + 128 + (i & 1) * 128, ra, st, i > 0);
-                        ptx::umma_commit(&aempty[st]);
-                    }
-                }
-                ptx::umma_commit(accfull);
-                if (!ok) wait_landed(accfull, 0);
-            }
+            if (lane == 0 && c.items > 0) issue<DP, F16>(c, br, base, tmem, abort, status);
         } else if (warp == GUARD_WARP) {
-            // Masked pairs have P = dS = 0, and zero times a NaN or an infinity of the other operand would
-            // reach the sum: in partly visible tiles such elements become zeros before the product.  What a
-            // visible pair loses with them is NaN already through lse (Q, K) or delta (dO) of its row, except
-            // for dV, where a visible row's bad dO elements are put back at the end.
-            uint32_t ng = 0;
-            for (int i = 0; i < items; ++i) {
-                if (!partial(i)) continue;
-                const int st = i % C::STAGES, ph = (i / C::STAGES) & 1;
-                // not before the issuer has seen the tile: see the forward kernel's guard
-                if (!ptx::wait_bounded(toguard, ng & 1, abort, status, WAIT_NS)) break;
-                ++ng;
-                if (!ptx::wait_bounded(&afull[st], ph, abort, status, WAIT_NS)) break;
-                clear_bad<F16>(ring_a + st * C::TILE, C::TILE, lane);
-                if (key_side) {
-                    if (!ptx::wait_bounded(&bfull[st], ph, abort, status, WAIT_NS)) break;
-                    if (clear_bad<F16>(ring_b + st * C::TILE, C::TILE, lane) && lane == 0) ms.poison = 1;
-                    __syncwarp();
-                }
-                if (lane == 0) ptx::mbar_arrive(guarded);
-            }
+            watch<DP, F16>(c, br, base, lane, &ms.poison, abort, status);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(COMPUTE_REGS));
         const int half = warp >> 2;                 // columns 64 half .. of each score tile
-        const int lrow = threadIdx.x & 127;
-        const int row = r0 + lrow;                  // this thread's key (key side) or query
+        const int row = c.r0 + (threadIdx.x & 127); // this thread's key (key side) or query
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-        Score sc;
-        sc.cap2 = a.cap * LOG2E;
-        sc.c = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E;
-        sc.slope2 = 0.f;
-        const bool sloped = GEN && a.slopes;
         // fp16 keeps 2^-14 .. 65504: dS is scaled by a power of two that brings its bound 2 |dO| |V| to
         // 2^14 .. 2^15, and the accumulator is scaled back at the end
-        float up = 1.f, up_p = 1.f, p_back = 1.f;
+        float up = 1.f, p_back = 1.f;
         if (F16) {
             const float m2 = __uint_as_float(w.top[0]) * __uint_as_float(w.top[1]);
             if (m2 > 0.f && m2 < INFINITY) up = exp2f(14.f - ceilf(0.5f * log2f(m2)));
             up = fminf(fmaxf(up, 0x1p-60f), 0x1p60f);
             p_back = exp2f(-P_SHIFT_F16);
-            up_p = up * p_back;
         }
-        int2 span = make_int2(0, 0x7fffffff);
-        float my_lse2 = 0.f, my_delta = 0.f;
-        if (!key_side) {
-            const int64_t at = (((int64_t)b * a.heads + h) * args.n_qt + tile) * T + lrow;
-            my_lse2 = w.lse2[at];
-            my_delta = w.delta[at];
-            if (row < a.q_len) span = row_span(a, b, row, n);
-            if (sloped) sc.slope2 = a.slopes[h] * LOG2E;
-        }
-        const int shift = n - a.q_len;              // position of query i: shift + i
-        bool ok = true;
-        for (int i = 0; i < items; ++i) {
-            const int t = tile_of(i);
-            const float* vec = (const float*)(base + C::VEC_OFF) + (i % C::STAGES) * 2 * T + half * 64;
-            if (key_side && sloped) sc.slope2 = a.slopes[head_of(i)] * LOG2E;
-            const bool masked = partial(i);
-            if (!ptx::wait_bounded(sfull, i & 1, abort, status, WAIT_NS)) { ok = false; break; }
-            // the stage's lse2 and delta came with Q: sfull implies it
-            ptx::tc_fence_after();
-            uint32_t x[2][32];
-            ptx::tmem_ld32(lanes + half * 64, x[0]);
-            ptx::tmem_ld32(lanes + half * 64 + 32, x[1]);
-            ptx::tmem_wait_ld(x[0]);
-            ptx::tmem_wait_ld(x[1]);
-            float(&v)[2][32] = reinterpret_cast<float(&)[2][32]>(x);
-            if (!key_side) {
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(sread);
-            }
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int c0 = half * 64 + g * 32;   // column of v[g][0]
-                float bend[GEN ? 32 : 1];
-                if (GEN) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[g][e] *= sc.c;
-                    if (sc.cap2 > 0.f) {
-                        tanh_n(v[g]);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            bend[e] = fmaf(-v[g][e], v[g][e], 1.f);
-                            v[g][e] *= sc.cap2;
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) bend[e] = 1.f;
-                    }
-                    if (sc.slope2 != 0.f) {
-                        // distance of column e from this row, as |at -+ e|: symmetric, one form for both sides
-                        const float at = key_side ? (float)(row - shift - t * T - c0) : (float)(shift + row - t * T - c0);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[g][e] = fmaf(-sc.slope2, fabsf(at - (float)e), v[g][e]);
-                    }
-                }
-                const float c = GEN ? 1.f : sc.c;
-                if (key_side) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 l4 = *(const float4*)(vec + g * 32 + e);
-                        v[g][e] = ptx::ex2_mufu(fmaf(v[g][e], c, -l4.x));
-                        v[g][e + 1] = ptx::ex2_mufu(fmaf(v[g][e + 1], c, -l4.y));
-                        v[g][e + 2] = ptx::ex2_mufu(fmaf(v[g][e + 2], c, -l4.z));
-                        v[g][e + 3] = ptx::ex2_mufu(fmaf(v[g][e + 3], c, -l4.w));
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const int q = t * T + c0 + e;
-                            const int2 sp = q < a.q_len ? row_span(a, b, q, n) : make_int2(0, 0);
-                            if (row < sp.x || row >= sp.y) v[g][e] = 0.f;
-                        }
-                    }
-                    uint32_t p[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) p[e] = ptx::pack16<F16>(v[g][2 * e], v[g][2 * e + 1]);
-                    ptx::tmem_st16(lanes + half * 64 + g * 16, p);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[g][e] = ptx::ex2_mufu(fmaf(v[g][e], c, -my_lse2));
-                    if (masked) {
-                        const int lo = span.x - t * T - c0;
-                        const uint32_t len = (uint32_t)(span.y - span.x);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if ((uint32_t)(e - lo) >= len) v[g][e] = 0.f;
-                    }
-                }
-                if (GEN) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[g][e] *= bend[e];
-                }
-            }
-            if (key_side) {
-                ptx::tmem_wait_st();
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(pfull);
-            }
-            const int buf = key_side ? 0 : i & 1;
-            const uint32_t dp_addr = lanes + 128 + buf * 128 + half * 64;
-            if (!ptx::wait_bounded(&dpfull[buf], key_side ? i & 1 : (i >> 1) & 1, abort, status, WAIT_NS)) { ok = false; break; }
-            ptx::tc_fence_after();
-            uint32_t y[2][32];
-            ptx::tmem_ld32(dp_addr, y[0]);
-            ptx::tmem_ld32(dp_addr + 32, y[1]);
-            ptx::tmem_wait_ld(y[0]);
-            ptx::tmem_wait_ld(y[1]);
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                float(&d)[32] = reinterpret_cast<float(&)[32]>(y[g]);
-                if (key_side) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 d4 = *(const float4*)(vec + T + g * 32 + e);
-                        d[e] = v[g][e] * (d[e] - d4.x);
-                        d[e + 1] = v[g][e + 1] * (d[e + 1] - d4.y);
-                        d[e + 2] = v[g][e + 2] * (d[e + 2] - d4.z);
-                        d[e + 3] = v[g][e + 3] * (d[e + 3] - d4.w);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) d[e] = v[g][e] * (d[e] - my_delta);
-                }
-                if (masked) {   // zero, whatever dP of a masked pair holds
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (v[g][e] == 0.f) d[e] = 0.f;
-                }
-                uint32_t p[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    p[e] = F16 ? ptx::pack16<F16>(d[2 * e] * up_p, d[2 * e + 1] * up_p) : ptx::pack16<F16>(d[2 * e], d[2 * e + 1]);
-                ptx::tmem_st16(dp_addr + g * 16, p);
-            }
-            ptx::tmem_wait_st();
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&dsfull[buf]);
-        }
-        bool have = items > 0 && ok;
-        if (have) have = ptx::wait_bounded(accfull, 0, abort, status, WAIT_NS);
+        const bool ok = c.key_side ? compute_key<DP, F16, GEN>(c, br, base, lanes, half, row, up * p_back, abort, status)
+                                   : compute_query<DP, F16, GEN>(c, br, lanes, half, row, up * p_back, abort, status);
+        const bool have = c.items > 0 && ok && ptx::wait_bounded(br.accfull, 0, abort, status, WAIT_NS);
         ptx::tc_fence_after();
         const float back = a.scale / up;
-        if (key_side) {
-            const bool live = row < a.k_len;
-            if (half == 0) {
-                uint8_t* out = (uint8_t*)a.dv.p + 2 * (b * a.dv.sb + (int64_t)row * a.dv.ss + h * a.dv.sh);
-                store_cols<DP, F16>(lanes + 256, p_back, out, 0, a.dim, live, have);
-                if (have && live && *(volatile int*)&ms.poison) {
-                    for (int i = 0; i < items; ++i) {
-                        if (!partial(i)) continue;
-                        const int q1 = min((tile_of(i) + 1) * T, a.q_len);
-                        for (int q = tile_of(i) * T; q < q1; ++q) {
-                            const int2 sp = row_span(a, b, q, n);
-                            if (row < sp.x || row >= sp.y) continue;
-                            const uint16_t* g = (const uint16_t*)a.d_o.p + b * a.d_o.sb + (int64_t)q * a.d_o.ss + head_of(i) * a.d_o.sh;
-                            constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
-                            for (int c = 0; c < a.dim; ++c)
-                                if ((g[c] & EXP) == EXP) {
-                                    uint16_t* o = (uint16_t*)out + c;
-                                    const uint32_t pr = (uint32_t)*o | ((uint32_t)g[c] << 16);
-                                    const float2 f = pair_of<F16>(pr);
-                                    *o = (uint16_t)ptx::pack16<F16>(f.x + f.y, 0.f);
-                                }
-                        }
-                    }
-                }
-            } else {
-                uint8_t* out = (uint8_t*)a.dk.p + 2 * (b * a.dk.sb + (int64_t)row * a.dk.ss + h * a.dk.sh);
-                store_cols<DP, F16>(lanes + 384, back, out, 0, a.dim, live, have);
-            }
-        } else {
-            uint8_t* out = (uint8_t*)a.dq.p + 2 * (b * a.dq.sb + (int64_t)row * a.dq.ss + h * a.dq.sh);
+        if (!c.key_side) {
+            uint8_t* out = (uint8_t*)a.dq.p + 2 * (c.b * a.dq.sb + (int64_t)row * a.dq.ss + c.h * a.dq.sh);
             store_cols<DP / 2, F16>(lanes + 384 + half * (DP / 2), back, out, half * (DP / 2), a.dim, row < a.q_len, have);
+        } else if (half == 0) {
+            uint8_t* out = (uint8_t*)a.dv.p + 2 * (c.b * a.dv.sb + (int64_t)row * a.dv.ss + c.h * a.dv.sh);
+            store_cols<DP, F16>(lanes + 256, p_back, out, 0, a.dim, row < a.k_len, have);
+            if (have && row < a.k_len && *(volatile int*)&ms.poison) put_back<F16>(c, out, row);
+        } else {
+            uint8_t* out = (uint8_t*)a.dk.p + 2 * (c.b * a.dk.sb + (int64_t)row * a.dk.ss + c.h * a.dk.sh);
+            store_cols<DP, F16>(lanes + 384, back, out, 0, a.dim, row < a.k_len, have);
         }
         ptx::tc_fence_before();
     }
@@ -723,12 +842,12 @@ int launch(const Prob& a, const Work& w, cudaStream_t s) {
     args.a = a;
     args.w = w;
     args.n_qt = (int)cdiv(a.q_len, T);
-    args.n_kt = (int)cdiv(a.k_len, T);
-    const int64_t keys = (int64_t)args.n_kt * a.kv_heads * a.batch;
+    const int n_kt = (int)cdiv(a.k_len, T);
+    const int64_t keys = (int64_t)n_kt * a.kv_heads * a.batch;
     const int64_t blocks = keys + (int64_t)args.n_qt * a.heads * a.batch;
     FD_CHECK_ARG(blocks <= 0x7fffffff && cdiv(a.q_len, T) + cdiv(a.k_len, T) <= 0x7fffffff, "fd_attention: too many tiles");
     args.n_key = (int)keys;
-    const int v_blocks = F16 ? args.n_kt : 0;
+    const int v_blocks = F16 ? n_kt : 0;
     if (F16) FD_CUDA_TRY(cudaMemsetAsync(w.top, 0, 2 * sizeof(unsigned), s));
     prep_kernel<F16><<<dim3(args.n_qt + v_blocks, a.heads, a.batch), 256, 0, s>>>(a, w, args.n_qt);
     FD_CUDA_TRY(cudaGetLastError());

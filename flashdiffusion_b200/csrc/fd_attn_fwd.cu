@@ -250,28 +250,8 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             if (!ptx::wait_bounded(toguard, ng & 1, abort, status, WAIT_NS)) break;
             ++ng;
             if (!ptx::wait_bounded(&full[slot], (item / C::SLOTS) & 1, abort, status, WAIT_NS)) break;
-            uint4* v = (uint4*)(ring + slot * C::TILE);
-            constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
-            bool bad = false;
-#pragma unroll 8
-            for (int i = lane; i < (int)C::TILE / 16; i += 32) {
-                const uint4 x = v[i];
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    bad = bad || (w[e] & EXP) == EXP || ((w[e] >> 16) & EXP) == EXP;
-            }
-            if (__any_sync(~0u, bad)) {
-                for (int i = lane; i < (int)C::TILE / 4; i += 32) {
-                    uint32_t x = ((uint32_t*)v)[i];
-                    if ((x & EXP) == EXP) x &= 0xffff0000u;
-                    if (((x >> 16) & EXP) == EXP) x &= 0xffffu;
-                    ((uint32_t*)v)[i] = x;
-                }
-                ptx::fence_async_shared();
-                if (lane == 0) ms.poison = 1;
-                __syncwarp();
-            }
+            if (clear_bad<F16>(ring + slot * C::TILE, C::TILE, lane) && lane == 0) ms.poison = 1;
+            __syncwarp();
             if (lane == 0) ptx::mbar_arrive(guarded);
         }
     }
@@ -280,13 +260,11 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         // ---- softmax: one query row per thread
         const uint32_t s_addr = tmem + ((uint32_t)(warp & 3) << 21) + sub * T;
         const uint32_t o_addr = tmem + ((uint32_t)(warp & 3) << 21) + C::O_COL + sub * DP;
-        Score sc;
-        sc.cap2 = a.cap * LOG2E;
-        sc.c = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E;
-        sc.slope2 = GEN && a.slopes ? a.slopes[h] * LOG2E : 0.f;
+        const Score sc(a);
+        const float slope2 = GEN && a.slopes ? a.slopes[h] * LOG2E : 0.f;
         // plain scores stay raw until the exponential's own multiply-add
-        const float c = GEN ? 1.f : sc.c;
-        const float room = GEN ? 8.f : 8.f / sc.c;
+        const float c = GEN ? 1.f : ptx::lo2(sc.c);
+        const float room = GEN ? 8.f : 8.f / c;
         const int pos = n - a.q_len + row;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
@@ -294,46 +272,47 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         for (int j = ta[sub]; j < tb[sub]; ++j, ++it) {
             if (!ptx::wait_bounded(&sfull[sub], it & 1, abort, status, WAIT_NS)) { ok = false; break; }
             ptx::tc_fence_after();
-            uint32_t x[4][32];
+            uint64_t x[4][16];
+            {
+                uint32_t r[4][32];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) ptx::tmem_ld32(s_addr + g * 32, x[g]);
+                for (int g = 0; g < 4; ++g) ptx::tmem_ld32(s_addr + g * 32, r[g]);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) ptx::tmem_wait_ld(x[g]);
-            float(&v)[4][32] = reinterpret_cast<float(&)[4][32]>(x);
+                for (int g = 0; g < 4; ++g) ptx::tmem_wait_ld(r[g]);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) pairs32(r[g], x[g]);
+            }
             if (GEN) {
-                const float at = (float)(pos - j * T);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[g][i] *= sc.c;
-                    if (sc.cap2 > 0.f) {
-                        tanh_n(v[g]);
+                    for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.c);
+                    if (sc.capped) {
+                        tanh32(x[g]);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[g][i] *= sc.cap2;
+                        for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.cap2);
                     }
-                    if (sc.slope2 != 0.f) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[g][i] = fmaf(-sc.slope2, fabsf(at - (float)(g * 32 + i)), v[g][i]);
-                    }
+                    if (slope2 != 0.f)
+                        add_bias(x[g], slope2, (float)(pos - j * T - g * 32), -1.f,
+                                 side_of(a, n - a.q_len + q0 + sub * T, j * T));
                 }
             }
             const int lo = span.x - j * T, len = span.y - span.x;
-            if (!__all_sync(~0u, lo <= 0 && (int64_t)lo + len >= T)) {
+            const bool masked = !__all_sync(~0u, lo <= 0 && (int64_t)lo + len >= T);
+            if (masked) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if ((uint32_t)(g * 32 + i - lo) >= (uint32_t)len) v[g][i] = -INFINITY;
+                for (int g = 0; g < 4; ++g) mask32(x[g], lo - g * 32, (uint32_t)len, -INFINITY);
             }
+            // a NaN among the visible scores becomes the row's m, and with it the whole row NaN
             float top[4];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                top[g] = v[g][0];
+                top[g] = max_nan(ptx::lo2(x[g][0]), ptx::hi2(x[g][0]));
 #pragma unroll
-                for (int i = 1; i < 32; ++i) top[g] = fmaxf(top[g], v[g][i]);
+                for (int i = 1; i < 16; ++i) top[g] = max_nan(top[g], max_nan(ptx::lo2(x[g][i]), ptx::hi2(x[g][i])));
             }
-            const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            const bool raise = mt > m + room;
+            const float mt = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+            const bool raise = !(mt <= m + room);
             if (__any_sync(~0u, raise)) {
                 const float mn = raise ? mt : m;
                 const float fix = m == -INFINITY ? 0.f : ptx::ex2_mufu((m - mn) * c);
@@ -352,21 +331,23 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                     }
                 }
             }
-            const float off = m == -INFINITY ? 0.f : fmaf(-m, c, P_SHIFT);
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t off = ptx::both2(m == -INFINITY ? 0.f : fmaf(-m, c, P_SHIFT));
+            const uint64_t c2 = ptx::both2(c);
+            uint64_t part[2] = {0, 0};
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                uint32_t p[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e0 = ptx::ex2_mufu(fmaf(v[g][2 * i], c, off));
-                    const float e1 = ptx::ex2_mufu(fmaf(v[g][2 * i + 1], c, off));
-                    part[g] += e0 + e1;
-                    p[i] = ptx::pack16<F16>(e0, e1);
-                }
+                for (int i = 0; i < 16; ++i) x[g][i] = GEN ? ptx::add2(x[g][i], off) : ptx::fma2(x[g][i], c2, off);
+                if (masked) exp32<0>(x[g]);
+                else exp32<1>(x[g]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part[i & 1] = ptx::add2(part[i & 1], x[g][i]);
+                uint32_t p[16];
+                round32<F16>(x[g], p);
                 ptx::tmem_st16(s_addr + g * 16, p);
             }
-            l += (part[0] + part[1]) + (part[2] + part[3]);
+            part[0] = ptx::add2(part[0], part[1]);
+            l += ptx::lo2(part[0]) + ptx::hi2(part[0]);
             ptx::tmem_wait_st();
             ptx::tc_fence_before();
             __syncwarp();

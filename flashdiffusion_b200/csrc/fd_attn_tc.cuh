@@ -34,49 +34,139 @@ __device__ __forceinline__ uint64_t mnmajor(uint32_t base, int ks) {
     return ptx::sw128_mnmajor_desc(base + (uint32_t)ks * 2048, BOX_BYTES);
 }
 
-// Scores in base 2 from the raw products: x = c s, or with a cap
-// x = cap log2(e) tanh(s scale / cap), minus slope log2(e) |distance|.
+// Scores in base 2 from the raw products, 32 columns of a row as 16 packed pairs:
+//   x = c s + add                       (no cap; c = scale log2(e))
+//   x = cap2 tanh(c s) + add            (c = scale / cap, cap2 = cap log2(e))
+// minus slope2 |distance| (slope2 = slope log2(e)).
 struct Score {
-    float c;            // scale log2(e); with a cap: scale / cap
-    float cap2;         // cap log2(e), 0 without a cap
-    float slope2;       // slope log2(e)
+    uint64_t c, cap2;    // both halves the same
+    bool capped;
+    __device__ explicit Score(const Prob& a) {
+        capped = a.cap > 0.f;
+        c = ptx::both2(capped ? a.scale / a.cap : a.scale * LOG2E);
+        cap2 = ptx::both2(a.cap * LOG2E);
+    }
 };
 
-// tanh of N arguments.  |u| <= 0.6 for all 32 lanes (scores well inside their cap,
-// the usual case): an odd degree-9 polynomial on the FMA pipe in packed pairs,
-// absolute error 8.5e-8 (least-squares fit on Chebyshev nodes).  Otherwise
-// 1 - 2 / (1 + e^2u) with two MUFU operations, absolute error 2e-7: three MUFU
-// operations per pair with the softmax's own would make MUFU the bound.
-template <int N>
-__device__ __forceinline__ void tanh_n(float (&u)[N]) {
+// tanh of 32 arguments.  |u| <= 0.6 for the whole warp (scores well inside their
+// cap, the usual case): an odd degree-9 polynomial on the FMA pipe in packed
+// pairs, absolute error 8.5e-8 (least-squares fit on Chebyshev nodes).  Otherwise
+// 1 - 2 / (1 + e^2u) with two MUFU operations, absolute error 2e-7: with the
+// softmax's own that makes three MUFU operations a pair, and MUFU the bound.
+__device__ __forceinline__ void tanh32(uint64_t (&u)[16]) {
     float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(u[i]));
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(ptx::lo2(u[i])), fabsf(ptx::hi2(u[i]))));
     if (__all_sync(~0u, top <= 0.6f)) {
-        const uint64_t c4 = ptx::pack2(0.01548669f, 0.01548669f), c3 = ptx::pack2(-0.052109625f, -0.052109625f);
-        const uint64_t c2 = ptx::pack2(0.13310358f, 0.13310358f), c1 = ptx::pack2(-0.33332324f, -0.33332324f);
-        const uint64_t c0 = ptx::pack2(0.99999994f, 0.99999994f), zero = ptx::pack2(0.f, 0.f);
+        const uint64_t c4 = ptx::both2(0.01548669f), c3 = ptx::both2(-0.052109625f), c2 = ptx::both2(0.13310358f),
+                       c1 = ptx::both2(-0.33332324f), c0 = ptx::both2(0.99999994f);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const uint64_t x = ptx::pack2(u[i], u[i + 1]);
-            const uint64_t y = ptx::fma2(x, x, zero);
+        for (int i = 0; i < 16; ++i) {
+            const uint64_t y = ptx::mul2(u[i], u[i]);
             uint64_t p = ptx::fma2(c4, y, c3);
             p = ptx::fma2(p, y, c2);
             p = ptx::fma2(p, y, c1);
             p = ptx::fma2(p, y, c0);
-            p = ptx::fma2(p, x, zero);
-            uint32_t a, b;
-            ptx::unpack2(p, a, b);
-            u[i] = __uint_as_float(a);
-            u[i + 1] = __uint_as_float(b);
+            u[i] = ptx::mul2(p, u[i]);
         }
     } else {
+        // e^2u overflows to infinity (tanh 1) and underflows to 0 (tanh -1); NaN stays NaN
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            // e^2u overflows to infinity (tanh 1) and underflows to 0 (tanh -1); NaN stays NaN
-            const float e = ptx::ex2_mufu(u[i] * (2.f * LOG2E));
-            u[i] = fmaf(-2.f, ptx::rcp_mufu(1.f + e), 1.f);
+        for (int i = 0; i < 16; ++i) {
+            const float e0 = ptx::ex2_mufu(ptx::lo2(u[i]) * (2.f * LOG2E)), e1 = ptx::ex2_mufu(ptx::hi2(u[i]) * (2.f * LOG2E));
+            u[i] = ptx::pack2(fmaf(-2.f, ptx::rcp_mufu(1.f + e0), 1.f), fmaf(-2.f, ptx::rcp_mufu(1.f + e1), 1.f));
         }
+    }
+}
+
+// x[i] += from + by * (2 i, 2 i + 1), four independent chains
+__device__ __forceinline__ void add_line(uint64_t (&x)[16], float from, float by) {
+    uint64_t l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l[j] = ptx::pack2(fmaf(by, (float)(2 * j), from), fmaf(by, (float)(2 * j + 1), from));
+    const uint64_t step = ptx::both2(8.f * by);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[i + j] = ptx::add2(x[i + j], l[j]);
+            if (i < 12) l[j] = ptx::add2(l[j], step);
+        }
+}
+
+// x[i] -= slope2 |dist + by * (2 i, 2 i + 1)|, by = 1 or -1: the distances of 32
+// pairs.  `side` says what is known of their sign in the whole tile: 1 none is
+// negative where it matters, -1 none positive, 0 both.
+__device__ __forceinline__ void add_bias(uint64_t (&x)[16], float slope2, float dist, float by, int side) {
+    if (side != 0) {
+        const float f = side > 0 ? -slope2 : slope2;
+        add_line(x, f * dist, f * by);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float d0 = fabsf(fmaf(by, (float)(2 * i), dist)), d1 = fabsf(fmaf(by, (float)(2 * i + 1), dist));
+        x[i] = ptx::pack2(fmaf(-slope2, d0, ptx::lo2(x[i])), fmaf(-slope2, d1, ptx::hi2(x[i])));
+    }
+}
+
+// Sign of pos - key over positions [p0, p0 + T) and keys [k0, k0 + T), as add_bias takes it.
+__device__ __forceinline__ int side_of(const Prob& a, int p0, int k0) {
+    if (a.causal || p0 >= k0 + T - 1) return 1;   // causal: pairs with a negative distance are masked
+    return p0 + T - 1 <= k0 ? -1 : 0;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// 2^x of a pair on the FMA pipe, as exp2_poly2 of the tile kernels has it (2^j 2^f,
+// degree-4 polynomial, relative error 3.6e-6, never below 2^-125), but a NaN does
+// not come out as a number that could pass for a weight.
+__device__ __forceinline__ uint64_t exp2_fma2(uint64_t x) {
+    const uint64_t X = ptx::pack2(max_nan(ptx::lo2(x), -125.f), max_nan(ptx::hi2(x), -125.f));
+    const uint64_t SH = ptx::both2(12582912.0f);
+    const uint64_t T = ptx::add2(X, SH);
+    const uint64_t F = ptx::sub2(X, ptx::sub2(T, SH));
+    uint64_t P = ptx::fma2(ptx::both2(0.009782912f), F, ptx::both2(0.055976883f));
+    P = ptx::fma2(P, F, ptx::both2(0.2402071f));
+    P = ptx::fma2(P, F, ptx::both2(0.6931136f));
+    P = ptx::fma2(P, F, ptx::both2(1.0f));
+    uint32_t p0, p1, t0, t1;
+    ptx::unpack2(P, p0, p1);
+    ptx::unpack2(T, t0, t1);
+    return ptx::pack2(__uint_as_float(p0 + (t0 << 23)), __uint_as_float(p1 + (t1 << 23)));
+}
+
+// 2^x of 16 pairs; POLY of every 4 go to the FMA pipe: MUFU, 16 exponentials a
+// clock and SM, is the bound of the softmax.  POLY = 0 where zeros must be zeros.
+template <int POLY>
+__device__ __forceinline__ void exp32(uint64_t (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if (i % 4 >= 4 - POLY) x[i] = exp2_fma2(x[i]);
+        else x[i] = ptx::pack2(ptx::ex2_mufu(ptx::lo2(x[i])), ptx::ex2_mufu(ptx::hi2(x[i])));
+    }
+}
+
+// A row's 32 TMEM columns as pairs.
+__device__ __forceinline__ void pairs32(const uint32_t (&r)[32], uint64_t (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = ptx::pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+}
+template <bool F16>
+__device__ __forceinline__ void round32(const uint64_t (&x)[16], uint32_t (&p)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = ptx::pack16<F16>(ptx::lo2(x[i]), ptx::hi2(x[i]));
+}
+// Pairs outside columns [lo, lo + len) become `value`.
+__device__ __forceinline__ void mask32(uint64_t (&x)[16], int lo, uint32_t len, float value) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const bool a = (uint32_t)(2 * i - lo) < len, b = (uint32_t)(2 * i + 1 - lo) < len;
+        x[i] = ptx::pack2(a ? ptx::lo2(x[i]) : value, b ? ptx::hi2(x[i]) : value);
     }
 }
 
@@ -85,6 +175,32 @@ __device__ __forceinline__ void wait_landed(uint64_t* b, uint32_t parity) {
     const uint64_t t0 = ptx::globaltimer();
     while (!ptx::mbar_try_wait(b, parity) && ptx::globaltimer() - t0 < WAIT_NS) {
     }
+}
+
+// A tile in shared memory: elements that are NaN or infinite become zeros; true (in all lanes) if there were any.
+template <bool F16>
+__device__ __forceinline__ bool clear_bad(uint8_t* tile, int bytes, int lane) {
+    constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+#pragma unroll 8
+    for (int i = lane; i < bytes / 16; i += 32) {
+        const uint4 x = ((uint4*)tile)[i];
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad = bad || (w[e] & EXP) == EXP || ((w[e] >> 16) & EXP) == EXP;
+    }
+    bad = __any_sync(~0u, bad);
+    if (bad) {
+        for (int i = lane; i < bytes / 4; i += 32) {
+            uint32_t x = ((uint32_t*)tile)[i];
+            if ((x & EXP) == EXP) x &= 0xffff0000u;
+            if (((x >> 16) & EXP) == EXP) x &= 0xffffu;
+            ((uint32_t*)tile)[i] = x;
+        }
+        ptx::fence_async_shared();
+        __syncwarp();
+    }
+    return bad;
 }
 
 __device__ __forceinline__ int warp_min(int x) { return __reduce_min_sync(~0u, x); }

@@ -309,6 +309,22 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t both2(float x) { return pack2(x, x); }
+__device__ __forceinline__ float lo2(uint64_t v) {
+    uint32_t a, b;
+    unpack2(v, a, b);
+    return __uint_as_float(a);
+}
+__device__ __forceinline__ float hi2(uint64_t v) {
+    uint32_t a, b;
+    unpack2(v, a, b);
+    return __uint_as_float(b);
+}
 // Two consecutive fp32 pairs from shared memory (16-byte aligned).
 __device__ __forceinline__ void lds_pairs(const float* p, uint64_t& a, uint64_t& b) {
     asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(smem_u32(p)));
