@@ -314,22 +314,22 @@ template <int DP, bool F16>
 __device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* base, uint32_t tmem, volatile int* abort,
                                       int* status) {
     using C = Cfg<DP>;
+    const uint32_t lead = elect_lane();
     const int kd = (c.a.dim + 15) / 16;
     const uint32_t id_s = ptx::idesc_f32acc(T, T, F16);
     const uint32_t id_acc = ptx::idesc_f32acc(T, kd * 16, F16) | ptx::IDESC_B_MN;
     const uint32_t op0 = ptx::smem_u32(base), op1 = op0 + C::TILE, ra = op0 + C::A_OFF, rb = op0 + C::B_OFF;
-    auto wait = [&](uint64_t* bar, uint32_t ph) { return ptx::wait_bounded(bar, ph & 1, abort, status, WAIT_NS); };
+    auto wait = [&](uint64_t* bar, uint32_t ph) { return wait_warp(bar, ph & 1, abort, status); };
+    auto commit = [&](uint64_t* bar) { mma_commit(lead, bar); };
     // D[128 x 128] = resident operand . ring operand^T
     auto scores = [&](uint32_t d, uint32_t op, uint32_t rg) {
         ptx::tc_fence_after();
-        for (int ks = 0; ks < kd; ++ks) ptx::umma_ss(d, kmajor(op, ks), kmajor(rg, ks), id_s, ks > 0);
+        product_rows<DP>(lead, d, op, rg, id_s, kd);
     };
     // acc[128 x dim] += (16-bit tile in TMEM, 64 columns of it at `src`, 64 at `src` + 64) . ring tile
     auto sum = [&](uint32_t acc, uint32_t src, uint32_t rg, bool more) {
         ptx::tc_fence_after();
-#pragma unroll
-        for (int ks = 0; ks < T / 16; ++ks)
-            ptx::umma_ts(acc, src + (ks >> 2) * 64 + (ks & 3) * 8, mnmajor(rg, ks), id_acc, more || ks > 0);
+        product_sum<64>(lead, acc, src, rg, id_acc, more);
     };
     uint32_t ng = 0;
     bool ok = wait(br.opfull, 0);
@@ -342,16 +342,16 @@ __device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* bas
         auto first = [&]() {     // S^T
             if (!wait(&br.afull[sa.at], sa.ph)) return false;
             scores(S, op0, ra + sa.at * C::TILE);
-            ptx::umma_commit(br.sfull);
+            commit(br.sfull);
             sa.next();
             return true;
         };
         auto second = [&]() {    // dP^T
             if (!wait(&br.bfull[sb.at], sb.ph)) return false;
             scores(DPT, op1, rb + sb.at * C::TILE);
-            ptx::umma_commit(&br.dpfull[0]);
+            commit(&br.dpfull[0]);
             look = ahead.partial(c);
-            if (look) ptx::mbar_arrive(br.toguard);
+            if (look && lead) ptx::mbar_arrive(br.toguard);
             sb.next();
             ahead.next(c);
             return true;
@@ -364,12 +364,12 @@ __device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* bas
                 ++ng;
             }
             sum(DV, S, rb + db.at * C::TILE, i > 0);
-            ptx::umma_commit(&br.bempty[db.at]);
+            commit(&br.bempty[db.at]);
             db.next();
             if (i + 1 < c.items && !(ok = first())) break;
             if (!(ok = wait(&br.dsfull[0], i))) break;
             sum(DK, DPT, ra + da.at * C::TILE, i > 0);
-            ptx::umma_commit(&br.aempty[da.at]);
+            commit(&br.aempty[da.at]);
             da.next();
             if (i + 1 < c.items) ok = second();
         }
@@ -381,11 +381,11 @@ __device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* bas
         auto both = [&]() {       // S and dP of the next tile
             if (!wait(&br.afull[sa.at], sa.ph)) return false;
             scores(S, op0, ra + sa.at * C::TILE);
-            ptx::umma_commit(br.sfull);
+            commit(br.sfull);
             if (!wait(&br.bfull[sb.at], sb.ph)) return false;
             scores(tmem + 128 + (made & 1) * 128, op1, rb + sb.at * C::TILE);
-            ptx::umma_commit(&br.dpfull[made & 1]);
-            ptx::umma_commit(&br.bempty[sb.at]);
+            commit(&br.dpfull[made & 1]);
+            commit(&br.bempty[sb.at]);
             sa.next();
             sb.next();
             ++made;
@@ -394,7 +394,7 @@ __device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* bas
         ok = ok && both();
         for (Item it(c); it.i < c.items && ok; it.next(c)) {
             const bool look = it.partial(c);
-            if (look) ptx::mbar_arrive(br.toguard);
+            if (look && lead) ptx::mbar_arrive(br.toguard);
             if (it.i + 1 < c.items) {
                 if (!(ok = wait(br.sread, it.i))) break;
                 if (!(ok = both())) break;
@@ -407,11 +407,11 @@ __device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* bas
                 ++ng;
             }
             sum(DQ, tmem + 128 + (it.i & 1) * 128, ra + da.at * C::TILE, it.i > 0);
-            ptx::umma_commit(&br.aempty[da.at]);
+            commit(&br.aempty[da.at]);
             da.next();
         }
     }
-    ptx::umma_commit(br.accfull);
+    commit(br.accfull);
     if (!ok) wait_landed(br.accfull, 0);
 }
 
@@ -786,7 +786,7 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         if (warp == TMA_WARP) {
             if (lane == 0 && c.items > 0) produce<DP, F16>(c, br, base, &tmq, &tmk, &tmv, &tmdo, abort, status);
         } else if (warp == MMA_WARP) {
-            if (lane == 0 && c.items > 0) issue<DP, F16>(c, br, base, tmem, abort, status);
+            if (c.items > 0) issue<DP, F16>(c, br, base, tmem, abort, status);
         } else if (warp == GUARD_WARP) {
             watch<DP, F16>(c, br, base, lane, &ms.poison, abort, status);
         }

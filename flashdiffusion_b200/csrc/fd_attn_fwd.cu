@@ -181,57 +181,55 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             }
         }
     } else if (warp == MMA_WARP) {
-        if (lane == 0 && t1 > t0) {
+        if (t1 > t0) {
+            const uint32_t lead = elect_lane();
             const int ks_qk = (a.dim + 15) / 16;
             const uint32_t id_qk = ptx::idesc_f32acc(T, T, F16);
             const uint32_t id_pv = ptx::idesc_f32acc(T, ks_qk * 16, F16) | ptx::IDESC_B_MN;
             const uint32_t q_base = ptx::smem_u32(sQ), r_base = ptx::smem_u32(ring);
             auto slot_of = [&](int item) { return item % C::SLOTS; };
             auto wait_full = [&](int item) {
-                return ptx::wait_bounded(&full[slot_of(item)], (item / C::SLOTS) & 1, abort, status, WAIT_NS);
+                return wait_warp(&full[slot_of(item)], (item / C::SLOTS) & 1, abort, status);
             };
             auto issue_qk = [&](int s, int item) {
                 ptx::tc_fence_after();
-                const uint32_t kb = r_base + slot_of(item) * C::TILE, qb = q_base + s * C::TILE;
-                for (int ks = 0; ks < ks_qk; ++ks)
-                    ptx::umma_ss(tmem + s * T, kmajor(qb, ks), kmajor(kb, ks), id_qk, ks > 0);
-                ptx::umma_commit(&sfull[s]);
+                product_rows<DP>(lead, tmem + s * T, q_base + s * C::TILE, r_base + slot_of(item) * C::TILE, id_qk, ks_qk);
+                mma_commit(lead, &sfull[s]);
             };
-            bool ok = ptx::wait_bounded(qfull, 0, abort, status, WAIT_NS) && wait_full(0);
+            bool ok = wait_warp(qfull, 0, abort, status) && wait_full(0);
             if (ok) {
                 for (int s = 0; s < 2; ++s)
                     if (active(s, t0)) issue_qk(s, 0);
-                ptx::umma_commit(&empty[0]);
+                mma_commit(lead, &empty[0]);
             }
             uint32_t np[2] = {0, 0}, ng = 0;
             for (int j = t0; j < t1 && ok; ++j) {
                 const int iv = 2 * (j - t0) + 1, ik = iv + 1;
                 ok = wait_full(iv) && (j + 1 == t1 || wait_full(ik));
                 bool look = ok && partial(j);
-                if (look) ptx::mbar_arrive(toguard);
-                for (int s = 0; s < 2 && ok; ++s) {
+                if (look && lead) ptx::mbar_arrive(toguard);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    if (!ok) break;
                     if (active(s, j)) {
-                        ok = ptx::wait_bounded(&pfull[s], np[s] & 1, abort, status, WAIT_NS);
+                        ok = wait_warp(&pfull[s], np[s] & 1, abort, status);
                         if (!ok) break;
                         ++np[s];
                         if (look) {
-                            ok = ptx::wait_bounded(guarded, ng & 1, abort, status, WAIT_NS);
+                            ok = wait_warp(guarded, ng & 1, abort, status);
                             if (!ok) break;
                             ++ng;
                             look = false;
                         }
                         ptx::tc_fence_after();
-                        const uint32_t vb = r_base + slot_of(iv) * C::TILE;
-#pragma unroll
-                        for (int ks = 0; ks < T / 16; ++ks)
-                            ptx::umma_ts(tmem + C::O_COL + s * DP, tmem + s * T + ks * 8, mnmajor(vb, ks), id_pv,
-                                         j > ta[s] || ks > 0);
-                        if (j + 1 == tb[s]) ptx::umma_commit(&ofull[s]);
+                        product_sum<32>(lead, tmem + C::O_COL + s * DP, tmem + s * T, r_base + slot_of(iv) * C::TILE, id_pv,
+                                        j > ta[s]);
+                        if (j + 1 == tb[s]) mma_commit(lead, &ofull[s]);
                     }
                     if (j + 1 < t1 && active(s, j + 1)) issue_qk(s, ik);
                 }
-                ptx::umma_commit(&empty[slot_of(iv)]);
-                if (j + 1 < t1) ptx::umma_commit(&empty[slot_of(ik)]);
+                mma_commit(lead, &empty[slot_of(iv)]);
+                if (j + 1 < t1) mma_commit(lead, &empty[slot_of(ik)]);
             }
         }
     } else if (warp == GUARD_WARP) {

@@ -26,12 +26,58 @@ inline bool tma_view(const View& v, const int64_t (&extent)[3]) {
 // 4-D map (coordinate, row, head, batch) of one operand, boxes of 64 x 128 x 1 x 1.
 int make_head_map(CUtensorMap* map, const View& v, int64_t rows, int heads, int batch, int dim, bool f16);
 
-__device__ __forceinline__ uint64_t kmajor(uint32_t base, int ks) {
-    return ptx::sw128_kmajor_desc(base + (uint32_t)(ks >> 2) * BOX_BYTES + (uint32_t)(ks & 3) * 32);
+// ---- tensor-core products, issued by a whole warp with one elected lane.
+// Everything but the instruction itself is the same in all 32 lanes and stays in
+// uniform registers, where tcgen05.mma wants its operands: under `if (lane == 0)`
+// every descriptor word is moved there first, and issuing cost about 115 cycles an
+// instruction (3,700 of the 4,800 cycles of a gradient tile) against the 64 that
+// the tensor core needs for it.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p;
 }
-// The same tile with its rows as the contracted index: step ks covers rows 16 ks .. 16 ks + 15.
-__device__ __forceinline__ uint64_t mnmajor(uint32_t base, int ks) {
-    return ptx::sw128_mnmajor_desc(base + (uint32_t)ks * 2048, BOX_BYTES);
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t more) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(more), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t more) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(more), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t lead, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(ptx::smem_u32(bar)), "r"(lead)
+        : "memory");
+}
+// A wait of the whole warp, with an answer that is the same in all lanes.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+    return __all_sync(~0u, ptx::wait_bounded(bar, parity, abort, status, WAIT_NS));
+}
+
+// D[128 x 128] = A B^T over DP coordinates (`kd` steps of 16 are not zero), both tiles as TMA left them.
+template <int DP>
+__device__ __forceinline__ void product_rows(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int kd) {
+    const uint64_t da = ptx::sw128_kmajor_desc(a), db = ptx::sw128_kmajor_desc(b);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        const uint32_t off = ((ks >> 2) * BOX_BYTES + (ks & 3) * 32) >> 4;
+        if (ks < kd) mma_ss(lead, d, da + off, db + off, idesc, ks > 0);
+    }
+}
+// D[128 x N] (+)= P B: P 16-bit in TMEM, its columns 16 ks .. at p + STEP4 (ks / 4) + 8 (ks % 4); the rows of B, as
+// TMA left them, are the contracted index.
+template <int STEP4>
+__device__ __forceinline__ void product_sum(uint32_t lead, uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool more) {
+    const uint64_t db = ptx::sw128_mnmajor_desc(b, BOX_BYTES);
+#pragma unroll
+    for (int ks = 0; ks < T / 16; ++ks)
+        mma_ts(lead, d, p + (ks >> 2) * STEP4 + (ks & 3) * 8, db + ks * (2048 >> 4), idesc, more || ks > 0);
 }
 
 // Scores in base 2 from the raw products, 32 columns of a row as 16 packed pairs:
@@ -181,14 +227,33 @@ __device__ __forceinline__ void wait_landed(uint64_t* b, uint32_t parity) {
 template <bool F16>
 __device__ __forceinline__ bool clear_bad(uint8_t* tile, int bytes, int lane) {
     constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
-    bool bad = false;
+    // zero times x is NaN for a NaN or an infinity and zero for a number: one packed multiply-add for two elements
+    float seen = 0.f;
+    if (F16) {
+        __half2 z[4] = {};
 #pragma unroll 8
-    for (int i = lane; i < bytes / 16; i += 32) {
-        const uint4 x = ((uint4*)tile)[i];
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int i = lane; i < bytes / 16; i += 32) {
+            const uint4 x = ((uint4*)tile)[i];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bad = bad || (w[e] & EXP) == EXP || ((w[e] >> 16) & EXP) == EXP;
+            for (int e = 0; e < 4; ++e) z[e] = __hfma2(*(__half2*)&w[e], __half2half2(__ushort_as_half(0)), z[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen += __low2float(z[e]) + __high2float(z[e]);
+    } else {
+        __nv_bfloat162 z[4] = {};
+#pragma unroll 8
+        for (int i = lane; i < bytes / 16; i += 32) {
+            const uint4 x = ((uint4*)tile)[i];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                z[e] = __hfma2(*(__nv_bfloat162*)&w[e], __bfloat162bfloat162(__ushort_as_bfloat16(0)), z[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen += __low2float(z[e]) + __high2float(z[e]);
     }
+    bool bad = seen != 0.f;      // NaN differs from everything
     bad = __any_sync(~0u, bad);
     if (bad) {
         for (int i = lane; i < bytes / 4; i += 32) {
