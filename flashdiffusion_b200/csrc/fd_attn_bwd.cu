@@ -329,7 +329,7 @@ __device__ __forceinline__ void issue(const Cta& c, const Bars& br, uint8_t* bas
     // acc[128 x dim] += (16-bit tile in TMEM, 64 columns of it at `src`, 64 at `src` + 64) . ring tile
     auto sum = [&](uint32_t acc, uint32_t src, uint32_t rg, bool more) {
         ptx::tc_fence_after();
-        product_sum<64>(lead, acc, src, rg, id_acc, more);
+        product_sum<2, 64>(lead, acc, src, rg, id_acc, more);
     };
     uint32_t ng = 0;
     bool ok = wait(br.opfull, 0);

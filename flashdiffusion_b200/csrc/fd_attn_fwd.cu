@@ -13,20 +13,23 @@
 // CTA = 256 query rows of one head (two subtiles of 128) against a stream of
 // 128-key tiles; both subtiles use a K/V tile while it is in shared memory, and
 // the tensor core works on one subtile's products while the other's
-// exponentials are made.  Three warpgroups: two for the softmax (one row per
-// thread), one with a TMA producer, an MMA issuer and a guard that looks at the
-// V tiles of which some row sees only a part (see `guard`).
+// exponentials are made.  Five warpgroups: four for the softmax, one with a TMA
+// producer, an MMA issuer and a guard that looks at the V tiles of which some row
+// sees only a part (see `guard`).  Two softmax threads share a row, 64 columns
+// each, and exchange their maxima through shared memory: with one thread a row
+// (8 warps) the SM issued an instruction in 0.35 of its cycles, two warps a
+// scheduler being too few for the latencies of TMEM, MUFU and FMA chains.
 #include "fd_attn_tc.cuh"
 
 namespace fd {
 namespace attn {
 namespace fwd {
 
-constexpr int TMA_WARP = 8, MMA_WARP = 9, GUARD_WARP = 10;
-constexpr int NTHREADS = 12 * 32;
-// Registers: 168 a thread at launch (64512 in all); the softmax warpgroups hold a row of 128 scores each and
-// take 208, the third gives up what it does not use: 256 * 208 + 128 * 80 = 63488.
-constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 80;
+constexpr int TMA_WARP = 16, MMA_WARP = 17, GUARD_WARP = 18;
+constexpr int NTHREADS = 20 * 32;
+// Registers: 96 a thread at launch (61440 in all); the softmax threads hold 64 scores each and take 104, the others
+// give up what they do not use: 512 * 104 + 128 * 56 = 60416.
+constexpr int SOFTMAX_REGS = 104, OTHER_REGS = 56;
 constexpr uint32_t TMEM_COLS = 512;
 
 template <int DP>
@@ -39,7 +42,9 @@ struct Cfg {
     // qfull, full[SLOTS], empty[SLOTS], sfull[2], pfull[2], ofull[2], toguard, guarded
     static constexpr int NBARS = 1 + 2 * SLOTS + 6 + 2;
     static constexpr uint32_t MISC_OFF = BAR_OFF + NBARS * 8;
-    static constexpr uint32_t SMEM = MISC_OFF + 64 + 1024;
+    // maxima and, at the end, sums of a row's two threads: [2 subtiles][2 halves][128]
+    static constexpr uint32_t MEET_OFF = (MISC_OFF + 64 + 15) / 16 * 16;
+    static constexpr uint32_t SMEM = MEET_OFF + 4 * T * 4;            // 1024-byte aligned: nothing lies before it
     static constexpr uint32_t O_COL = 256;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
     static_assert(O_COL + 2 * DP <= TMEM_COLS, "TMEM budget");
@@ -60,8 +65,11 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                int* __restrict__ status) {
     using C = Cfg<DP>;
     constexpr float P_SHIFT = F16 ? 7.f : 0.f;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) uint8_t base[];
+    if (ptx::smem_u32(base) & 1023) {   // the swizzled tiles need it, and there is no room to round up
+        if (threadIdx.x == 0) atomicExch(status, FD_ERR_UNSUPPORTED);
+        return;
+    }
     uint8_t* sQ = base;
     uint8_t* ring = base + C::Q_BYTES;
     uint64_t* qfull = (uint64_t*)(base + C::BAR_OFF);
@@ -92,7 +100,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&sfull[i], 1);
-            ptx::mbar_init(&pfull[i], 4);
+            ptx::mbar_init(&pfull[i], 8);
             ptx::mbar_init(&ofull[i], 1);
             ms.lo[i] = 0x7fffffff;
             ms.hi[i] = 0;
@@ -116,8 +124,8 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     }
     __syncthreads();
 
-    const int sub = warp >> 2;                   // softmax warpgroup = query subtile
-    const int row = q0 + threadIdx.x;            // softmax threads: their query row
+    const int sub = warp >> 3, half = (warp >> 2) & 1;   // softmax warps: query subtile, columns 64 half ..
+    const int lrow = threadIdx.x & 127, row = q0 + sub * T + lrow;
     int2 span = make_int2(0, 0);
     if (sub < 2) {
         const bool real = row < a.q_len;
@@ -222,7 +230,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                             look = false;
                         }
                         ptx::tc_fence_after();
-                        product_sum<32>(lead, tmem + C::O_COL + s * DP, tmem + s * T, r_base + slot_of(iv) * C::TILE, id_pv,
+                        product_sum<1, 32>(lead, tmem + C::O_COL + s * DP, tmem + s * T, r_base + slot_of(iv) * C::TILE, id_pv,
                                         j > ta[s]);
                         if (j + 1 == tb[s]) mma_commit(lead, &ofull[s]);
                     }
@@ -255,9 +263,19 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
-        // ---- softmax: one query row per thread
-        const uint32_t s_addr = tmem + ((uint32_t)(warp & 3) << 21) + sub * T;
-        const uint32_t o_addr = tmem + ((uint32_t)(warp & 3) << 21) + C::O_COL + sub * DP;
+        // ---- softmax: two threads a query row
+        const uint32_t s_addr = tmem + ((uint32_t)(warp & 3) << 21) + sub * T + half * 64;
+        const uint32_t o_addr = tmem + ((uint32_t)(warp & 3) << 21) + C::O_COL + sub * DP + half * (DP / 2);
+        float* meet = (float*)(base + C::MEET_OFF) + (sub * 2 + half) * T + lrow;
+        const float* other = (const float*)(base + C::MEET_OFF) + (sub * 2 + (half ^ 1)) * T + lrow;
+        // the threads of a subtile meet; true if `good` is true in all of them, so that they leave the loop together
+        auto both_here = [&](bool good) {
+            uint32_t all;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, 256, p;\n\t"
+                "selp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)good), "r"(1 + sub) : "memory");
+            return all != 0;
+        };
         const Score sc(a);
         const float slope2 = GEN && a.slopes ? a.slopes[h] * LOG2E : 0.f;
         // plain scores stay raw until the exponential's own multiply-add
@@ -268,21 +286,22 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         bool ok = true;
         int it = 0;
         for (int j = ta[sub]; j < tb[sub]; ++j, ++it) {
-            if (!ptx::wait_bounded(&sfull[sub], it & 1, abort, status, WAIT_NS)) { ok = false; break; }
+            ok = ptx::wait_bounded(&sfull[sub], it & 1, abort, status, WAIT_NS);
             ptx::tc_fence_after();
-            uint64_t x[4][16];
+            uint64_t x[2][16];
             {
-                uint32_t r[4][32];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) ptx::tmem_ld32(s_addr + g * 32, r[g]);
-#pragma unroll
-                for (int g = 0; g < 4; ++g) ptx::tmem_wait_ld(r[g]);
-#pragma unroll
-                for (int g = 0; g < 4; ++g) pairs32(r[g], x[g]);
+                uint32_t r[2][32];
+                ptx::tmem_ld32(s_addr, r[0]);
+                ptx::tmem_ld32(s_addr + 32, r[1]);
+                ptx::tmem_wait_ld(r[0]);
+                ptx::tmem_wait_ld(r[1]);
+                pairs32(r[0], x[0]);
+                pairs32(r[1], x[1]);
             }
+            const int k0 = j * T + half * 64;
             if (GEN) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int g = 0; g < 2; ++g) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.c);
                     if (sc.capped) {
@@ -291,25 +310,31 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                         for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.cap2);
                     }
                     if (slope2 != 0.f)
-                        add_bias(x[g], slope2, (float)(pos - j * T - g * 32), -1.f,
+                        add_bias(x[g], slope2, (float)(pos - k0 - g * 32), -1.f,
                                  side_of(a, n - a.q_len + q0 + sub * T, j * T));
                 }
             }
-            const int lo = span.x - j * T, len = span.y - span.x;
-            const bool masked = !__all_sync(~0u, lo <= 0 && (int64_t)lo + len >= T);
+            const int lo = span.x - k0, len = span.y - span.x;
+            const bool masked = !__all_sync(~0u, lo <= 0 && (int64_t)lo + len >= 64);
             if (masked) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) mask32(x[g], lo - g * 32, (uint32_t)len, -INFINITY);
+                for (int g = 0; g < 2; ++g) mask32(x[g], lo - g * 32, (uint32_t)len, -INFINITY);
             }
             // a NaN among the visible scores becomes the row's m, and with it the whole row NaN
             float top[4];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                top[g] = max_nan(ptx::lo2(x[g][0]), ptx::hi2(x[g][0]));
+                top[g] = max_nan(ptx::lo2(x[g / 2][g % 2 * 8]), ptx::hi2(x[g / 2][g % 2 * 8]));
 #pragma unroll
-                for (int i = 1; i < 16; ++i) top[g] = max_nan(top[g], max_nan(ptx::lo2(x[g][i]), ptx::hi2(x[g][i])));
+                for (int i = 1; i < 8; ++i)
+                    top[g] = max_nan(top[g], max_nan(ptx::lo2(x[g / 2][g % 2 * 8 + i]), ptx::hi2(x[g / 2][g % 2 * 8 + i])));
             }
-            const float mt = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+            float mt = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+            // the next tile's scores come only after every thread here has read this and handed over its P
+            meet[0] = mt;
+            ok = both_here(ok);
+            if (!ok) break;
+            mt = max_nan(mt, other[0]);
             const bool raise = !(mt <= m + room);
             if (__any_sync(~0u, raise)) {
                 const float mn = raise ? mt : m;
@@ -317,9 +342,9 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                 m = mn;
                 l *= fix;
                 if (it > 0) {
-                    // S's commit also covered the previous P V, so O is at rest
+                    // S's commit also covered the previous P V, so O is at rest; each thread takes half its columns
 #pragma unroll 1
-                    for (int g = 0; g < DP; g += 16) {
+                    for (int g = 0; g < DP / 2; g += 16) {
                         uint32_t o[16];
                         ptx::tmem_ld16(o_addr + g, o);
                         ptx::tmem_wait_ld16(o);
@@ -333,7 +358,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             const uint64_t c2 = ptx::both2(c);
             uint64_t part[2] = {0, 0};
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+            for (int g = 0; g < 2; ++g) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[g][i] = GEN ? ptx::add2(x[g][i], off) : ptx::fma2(x[g][i], c2, off);
                 if (masked) exp32<0>(x[g]);
@@ -342,7 +367,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                 for (int i = 0; i < 16; ++i) part[i & 1] = ptx::add2(part[i & 1], x[g][i]);
                 uint32_t p[16];
                 round32<F16>(x[g], p);
-                ptx::tmem_st16(s_addr + g * 16, p);
+                ptx::tmem_st16(s_addr + g * 32, p);
             }
             part[0] = ptx::add2(part[0], part[1]);
             l += ptx::lo2(part[0]) + ptx::hi2(part[0]);
@@ -353,29 +378,34 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         }
         if (it > 0 && ok) ok = ptx::wait_bounded(&ofull[sub], 0, abort, status, WAIT_NS);
         ptx::tc_fence_after();
+        both_here(ok);
+        meet[0] = l;
+        both_here(ok);
+        l += other[0];
         const bool real = row < a.q_len;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint8_t* out = (uint8_t*)a.o.p + 2 * (b * a.o.sb + (int64_t)row * a.o.ss + h * a.o.sh);
         const bool poison = it > 0 && *(volatile int*)&ms.poison;
 #pragma unroll 1
-        for (int g = 0; g < DP; g += 32) {
-            uint32_t o[32];
+        for (int g = 0; g < DP / 2; g += 16) {
+            const int c0 = half * (DP / 2) + g;
+            uint32_t o[16];
             if (it > 0 && ok) {
-                ptx::tmem_ld32(o_addr + g, o);
-                ptx::tmem_wait_ld(o);
+                ptx::tmem_ld16(o_addr + g, o);
+                ptx::tmem_wait_ld16(o);
             }
-            float(&f)[32] = reinterpret_cast<float(&)[32]>(o);
+            float(&f)[16] = reinterpret_cast<float(&)[16]>(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = l == 0.f ? 0.f : f[i] * inv;
+            for (int i = 0; i < 16; ++i) f[i] = l == 0.f ? 0.f : f[i] * inv;
             if (poison && real && l != 0.f) {
                 // put back what the guard took out, for the keys that this row sees
                 for (int j = ta[sub]; j < tb[sub]; ++j) {
                     if (!partial(j)) continue;
                     for (int k = max(span.x, j * T); k < min(span.y, (j + 1) * T); ++k) {
-                        const uint16_t* vr = (const uint16_t*)a.v.p + b * a.v.sb + (int64_t)k * a.v.ss + hk * a.v.sh + g;
+                        const uint16_t* vr = (const uint16_t*)a.v.p + b * a.v.sb + (int64_t)k * a.v.ss + hk * a.v.sh + c0;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (g + i >= a.dim) continue;
+                        for (int i = 0; i < 16; ++i) {
+                            if (c0 + i >= a.dim) continue;
                             const uint16_t w = vr[i];
                             constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
                             if ((w & EXP) == EXP) f[i] += F16 ? __half2float(__ushort_as_half(w))
@@ -386,18 +416,18 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             }
             if (real) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (g + i * 8 >= a.dim) continue;
+                for (int i = 0; i < 2; ++i) {
+                    if (c0 + i * 8 >= a.dim) continue;
                     uint4 w;
                     w.x = ptx::pack16<F16>(f[8 * i], f[8 * i + 1]);
                     w.y = ptx::pack16<F16>(f[8 * i + 2], f[8 * i + 3]);
                     w.z = ptx::pack16<F16>(f[8 * i + 4], f[8 * i + 5]);
                     w.w = ptx::pack16<F16>(f[8 * i + 6], f[8 * i + 7]);
-                    *(uint4*)(out + 2 * (g + i * 8)) = w;
+                    *(uint4*)(out + 2 * (c0 + i * 8)) = w;
                 }
             }
         }
-        if (real && a.lse)
+        if (half == 0 && real && a.lse)
             a.lse[((int64_t)b * a.heads + h) * a.q_len + row] = l == 0.f ? -INFINITY : (m * c + (log2f(l) - P_SHIFT)) * LN2;
         ptx::tc_fence_before();
     }

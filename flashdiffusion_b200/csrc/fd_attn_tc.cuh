@@ -70,14 +70,14 @@ __device__ __forceinline__ void product_rows(uint32_t lead, uint32_t d, uint32_t
         if (ks < kd) mma_ss(lead, d, da + off, db + off, idesc, ks > 0);
     }
 }
-// D[128 x N] (+)= P B: P 16-bit in TMEM, its columns 16 ks .. at p + STEP4 (ks / 4) + 8 (ks % 4); the rows of B, as
-// TMA left them, are the contracted index.
-template <int STEP4>
+// D[128 x N] (+)= P B: P 16-bit in TMEM, the words of keys 32 x .. 32 x + 31 at p + (x / PER) * STEP + (x % PER) * 16;
+// the rows of B, as TMA left them, are the contracted index.
+template <int PER, int STEP>
 __device__ __forceinline__ void product_sum(uint32_t lead, uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool more) {
     const uint64_t db = ptx::sw128_mnmajor_desc(b, BOX_BYTES);
 #pragma unroll
     for (int ks = 0; ks < T / 16; ++ks)
-        mma_ts(lead, d, p + (ks >> 2) * STEP4 + (ks & 3) * 8, db + ks * (2048 >> 4), idesc, more || ks > 0);
+        mma_ts(lead, d, p + (ks / 2 / PER) * STEP + (ks / 2 % PER) * 16 + (ks & 1) * 8, db + ks * (2048 >> 4), idesc, more || ks > 0);
 }
 
 // Scores in base 2 from the raw products, 32 columns of a row as 16 packed pairs:
