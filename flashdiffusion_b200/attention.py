@@ -127,6 +127,10 @@ def _loadable(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 _NO_GRADIENTS = (0,) * 16
 
 
@@ -154,7 +158,7 @@ def _call(fn, args, backward, q):
 
 def _forward(q, k, v, how, want_lse):
     """(output, lse or None) of heads that are loadable."""
-    o = q.new_empty(q.shape)
+    o = _like(q)
     lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32) if want_lse else None
     _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, how), 0, q)
     return o, lse
@@ -162,32 +166,63 @@ def _forward(q, k, v, how, want_lse):
 
 class _Attend(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, how):
-        q, k, v = (_loadable(t) for t in (q, k, v))
+    def forward(ctx, q, k, v, how, return_lse):
+        q, k, v = _loadable(q), _loadable(k), _loadable(v)
         o, lse = _forward(q, k, v, how, True)
-        spans, _, _, _, slopes, _, _ = how
-        masks = () if spans is None else (spans.first, spans.end)
-        ctx.save_for_backward(q, k, v, o, lse, *masks, *(() if slopes is None else (slopes,)))
+        spans, slopes = how[0], how[4]
+        if spans is None and slopes is None:
+            ctx.save_for_backward(q, k, v, o, lse)
+        else:    # what the gradients read again: autograd notices if it was changed in between
+            ctx.save_for_backward(q, k, v, o, lse, *(() if spans is None else (spans.first, spans.end)),
+                                  *(() if slopes is None else (slopes,)))
         ctx.how = how
+        if not return_lse:
+            return o
         ctx.mark_non_differentiable(lse)
         return o, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do, _):
+    def backward(ctx, do, *_):
+        if torch.is_grad_enabled():
+            raise RuntimeError("attend has no second derivative: call backward without create_graph")
         q, k, v, o, lse = ctx.saved_tensors[:5]
         do = _loadable(do)
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        dq, dk, dv = _like(q), _like(k), _like(v)
         args = _arguments(q, k, v, o, lse, ctx.how,
                           (do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                            *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
         _call(native.load().fd_attention_backward, args, 1, q)
-        return dq, dk, dv, None
+        return dq, dk, dv, None, None
 
 
 def _check(q, k, v, slopes, scale, cap, names):
+    # the usual call is found in order by these comparisons; _explain says what is wrong with any other
+    qs, ks = q.shape, k.shape
+    if not (ks == v.shape and q.dtype is k.dtype is v.dtype and q.dtype in _DTYPES and q.device == k.device == v.device
+            and len(qs) == len(ks) and 3 <= len(qs) <= 4 and qs[-1] == ks[-1] and qs[:-3] == ks[:-3]
+            and 1 <= qs[-1] <= MAX_DIM and ks[-2] >= 1 and qs[-2] >= 1 and qs[-2] % ks[-2] == 0):
+        _explain(q, k, v, names)
+    h = qs[-2]
+    if slopes is not None:
+        if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or tuple(slopes.shape) != (h,):
+            raise ValueError(f"slopes must be a float32 tensor of {h} values")
+        if slopes.device != q.device:
+            raise ValueError("slopes must be on the device of the heads")
+        if slopes.requires_grad:
+            raise ValueError("there is no gradient for slopes: detach them")
+    scale = qs[-1] ** -0.5 if scale is None else float(scale)
+    cap = 0.0 if cap is None else float(cap)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite (got {scale})")
+    if cap and not 1e-3 <= cap < math.inf:
+        raise ValueError(f"cap must be None or at least 1e-3 (got {cap})")
+    native.require_device(q.device)
+    return scale, cap
+
+
+def _explain(q, k, v, names):
     for name, t in zip(names, (q, k, v)):
-        if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES:
+        if t.dtype not in _DTYPES:
             raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
         if t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"{names[0]}, {names[1]} and {names[2]} must have one type and device")
@@ -199,24 +234,13 @@ def _check(q, k, v, slopes, scale, cap, names):
         raise ValueError(f"{names[0]} {tuple(q.shape)} and {names[1]} {tuple(k.shape)} differ in batch or head size")
     if not 1 <= q.shape[-1] <= MAX_DIM:
         raise ValueError(f"heads of 1 to {MAX_DIM} coordinates (got {q.shape[-1]})")
-    h, hk = q.shape[-2], k.shape[-2]
-    if hk < 1 or h < 1 or h % hk:
-        raise ValueError(f"{h} query heads are no multiple of {hk} key heads")
-    if slopes is not None:
-        if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or tuple(slopes.shape) != (h,):
-            raise ValueError(f"slopes must be a float32 tensor of {h} values")
-        if slopes.device != q.device:
-            raise ValueError("slopes must be on the device of the heads")
-        if slopes.requires_grad:
-            raise ValueError("there is no gradient for slopes: detach them")
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    cap = 0.0 if cap is None else float(cap)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite (got {scale})")
-    if not (math.isfinite(cap) and cap >= 0) or (cap and cap < 1e-3):
-        raise ValueError(f"cap must be None or at least 1e-3 (got {cap})")
-    native.require_device(q.device)
-    return scale, cap
+    raise ValueError(f"{q.shape[-2]} query heads are no multiple of {k.shape[-2]} key heads")
+
+
+def _tensors(names, ts):
+    for name, t in zip(names, ts):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | None = None, causal: bool = False,
@@ -236,6 +260,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     Returns the output (as q), or (output, lse): lse (B, H, Sq) float32 is the natural log of the sum of
     exp(scores), -inf for rows that see nothing; it carries no gradient.
     """
+    _tensors(("q", "k", "v"), (q, k, v))
     scale, cap = _check(q, k, v, slopes, scale, cap, ("q", "k", "v"))
     flat = q.dim() == 3
     if flat:
@@ -251,7 +276,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     slopes = None if slopes is None else slopes.contiguous()
     how = (spans, bool(causal), _window(window, causal), None, slopes, scale, cap)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o, lse = _Attend.apply(q, k, v, how)
+        o = _Attend.apply(q, k, v, how, return_lse)
+        o, lse = o if return_lse else (o, None)
     else:
         o, lse = _forward(_loadable(q), _loadable(k), _loadable(v), how, return_lse)
     if flat:
@@ -270,6 +296,7 @@ def attend_cached(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     Rows of the cache behind lengths[b] are never looked at.  scale, window, cap, slopes and return_lse as in
     ``attend``.
     """
+    _tensors(("q", "k_cache", "v_cache"), (q, k_cache, v_cache))
     scale, cap = _check(q, k_cache, v_cache, slopes, scale, cap, ("q", "k_cache", "v_cache"))
     if q.dim() != 4:
         raise ValueError(f"q must be (B, N, H, D) (got {tuple(q.shape)})")

@@ -1,9 +1,25 @@
 // Softmax attention over key spans: what the kernels of fd_attn_*.cu share.
 #pragma once
+#include <atomic>
+
 #include "fd_common.cuh"
 
 namespace fd {
 namespace attn {
+
+// Allow kernel FN `bytes` of dynamic shared memory on the current device: set once
+// for each device (the call costs a microsecond and more).
+template <auto FN>
+inline int allow_smem(uint32_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    FD_CUDA_TRY(cudaGetDevice(&dev));
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return FD_OK;
+    FD_CUDA_TRY(cudaFuncSetAttribute(FN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return FD_OK;
+}
 
 struct View {
     void* p;

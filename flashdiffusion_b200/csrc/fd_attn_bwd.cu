@@ -851,9 +851,8 @@ int launch(const Prob& a, const Work& w, cudaStream_t s) {
     if (F16) FD_CUDA_TRY(cudaMemsetAsync(w.top, 0, 2 * sizeof(unsigned), s));
     prep_kernel<F16><<<dim3(args.n_qt + v_blocks, a.heads, a.batch), 256, 0, s>>>(a, w, args.n_qt);
     FD_CUDA_TRY(cudaGetLastError());
-    auto fn = gradient_kernel<DP, F16, GEN>;
-    FD_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM));
-    fn<<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, g, args, status);
+    FD_TRY((allow_smem<gradient_kernel<DP, F16, GEN>>(Cfg<DP>::SMEM)));
+    gradient_kernel<DP, F16, GEN><<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, g, args, status);
     FD_CUDA_TRY(cudaGetLastError());
     return FD_OK;
 }

@@ -446,12 +446,11 @@ int launch(const Prob& a, cudaStream_t s) {
     FD_TRY(make_head_map(&v, a.v, a.k_len, a.kv_heads, a.batch, a.dim, F16));
     int* status = nullptr;
     FD_TRY(status_word(&status));
-    auto fn = forward_kernel<DP, F16, GEN>;
-    FD_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM));
+    FD_TRY((allow_smem<forward_kernel<DP, F16, GEN>>(Cfg<DP>::SMEM)));
     const int n_qt = (int)cdiv(a.q_len, 2 * T);
     const int64_t blocks = (int64_t)n_qt * a.heads * a.batch;
     FD_CHECK_ARG(blocks <= 0x7fffffff, "fd_attention: too many query tiles");
-    fn<<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, a, n_qt, status);
+    forward_kernel<DP, F16, GEN><<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, a, n_qt, status);
     FD_CUDA_TRY(cudaGetLastError());
     return FD_OK;
 }

@@ -696,9 +696,8 @@ int launch(const Prob& a, float* parts, cudaStream_t s) {
     static_assert(Smem<DP>::KEYS * WARPS == (DP == 64 ? 128 : 64), "unit");
     p.magic = (65536 + a.group - 1) / a.group;
     using S = Smem<DP>;
-    auto fn = rows_kernel<DP, F16, NT>;
-    FD_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
-    fn<<<p.ctas, WARPS * 32, S::BYTES, s>>>(a, p, parts);
+    FD_TRY((allow_smem<rows_kernel<DP, F16, NT>>(S::BYTES)));
+    rows_kernel<DP, F16, NT><<<p.ctas, WARPS * 32, S::BYTES, s>>>(a, p, parts);
     FD_CUDA_TRY(cudaGetLastError());
     constexpr int slices = 8 * NT * DP / 8 / 32;
     const int64_t blocks = std::min<int64_t>((int64_t)a.batch * p.pairs, 4 * num_sms()) * slices;

@@ -623,6 +623,15 @@ __global__ void tcw_fixup_kernel(const double* __restrict__ part, Sched sc, int6
 // ---- host side -----------------------------------------------------------------
 
 int get_encode(EncodeTiledFn* fn) {
+    // The driver call below wants a context on the calling thread.  The runtime binds one at its own first call
+    // there, which need not have come yet: an autograd worker may start with a gradient.
+    static thread_local bool bound = false;
+    if (!bound) {
+        int dev = 0;
+        FD_CUDA_TRY(cudaGetDevice(&dev));
+        FD_CUDA_TRY(cudaSetDevice(dev));
+        bound = true;
+    }
     static EncodeTiledFn cached = nullptr;
     if (!cached) {
         cudaDriverEntryPointQueryResult q;

@@ -380,7 +380,7 @@ _NO_STRIDES = (0, 0, 0)
 def _rotate_heads(xs, positions, freqs, layout, magnitude, inverse, inplace):
     """fd_rotary on one or two (B, S, H, D) tensors; returns the rotated tensors."""
     xs = [x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous() for x in xs]
-    outs = xs if inplace else [x.new_empty(x.shape) for x in xs]
+    outs = xs if inplace else [torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
     q, qo = xs[0], outs[0]
     b, s, h, d = q.shape
     if len(xs) > 1:
@@ -405,8 +405,9 @@ class _Rotary(torch.autograd.Function):
         return tuple(_rotate_heads(xs, positions, freqs, layout, magnitude, inverse, False))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
+        if torch.is_grad_enabled():
+            raise RuntimeError("apply_rotary has no second derivative: call backward without create_graph")
         positions, freqs = ctx.saved_tensors
         layout, magnitude, inverse = ctx.how
         return (None,) * 5 + tuple(_rotate_heads(grads, positions, freqs, layout, magnitude, not inverse, False))
@@ -425,39 +426,40 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: t
     scales the rotated coordinates, ``inverse`` turns the other way.  ``inplace`` overwrites q and k (no
     gradients).  Returns the rotated q, or (q, k).
     """
-    xs = [q] if k is None else [q, k]
+    xs = (q,) if k is None else (q, k)
     for name, x in zip("qk", xs):
         if not isinstance(x, torch.Tensor) or x.dtype not in _ROTARY_DTYPES:
             raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
-        if x.dim() not in (3, 4) or x.dim() != q.dim() or x.dtype != q.dtype or x.device != q.device:
-            raise ValueError("q and k must be (S, H, D) or (B, S, H, D) tensors of one type on one device")
-        if x.shape[:-2] != q.shape[:-2] or x.shape[-1] != q.shape[-1]:
-            raise ValueError(f"q {tuple(q.shape)} and k {tuple(x.shape)} may differ in their heads only")
+    shape, device = q.shape, q.device
+    if not 3 <= len(shape) <= 4 or k is not None and (len(k.shape) != len(shape) or k.dtype != q.dtype or k.device != device):
+        raise ValueError("q and k must be (S, H, D) or (B, S, H, D) tensors of one type on one device")
+    if k is not None and (k.shape[:-2] != shape[:-2] or k.shape[-1] != shape[-1]):
+        raise ValueError(f"q {tuple(shape)} and k {tuple(k.shape)} may differ in their heads only")
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be 'half' or 'interleaved' (got {layout!r})")
     if not isinstance(freqs, torch.Tensor) or freqs.dtype != torch.float64 or freqs.dim() != 1:
         raise TypeError("freqs must be a one-dimensional float64 tensor")
-    if not 1 <= freqs.numel() <= q.shape[-1] // 2:
-        raise ValueError(f"freqs has {freqs.numel()} pairs, a head of {q.shape[-1]} coordinates takes 1 to "
-                         f"{q.shape[-1] // 2}")
+    if not 1 <= freqs.shape[0] <= shape[-1] // 2:
+        raise ValueError(f"freqs has {freqs.shape[0]} pairs, a head of {shape[-1]} coordinates takes 1 to "
+                         f"{shape[-1] // 2}")
     if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_DTYPES:
         raise TypeError("positions must be an int32, int64, float32 or float64 tensor")
     if not math.isfinite(magnitude):
         raise ValueError(f"magnitude must be finite (got {magnitude})")
-    lead = tuple(q.shape[:-2])
-    if tuple(positions.shape) not in (lead, lead[-1:]):
-        raise ValueError(f"positions {tuple(positions.shape)} must be {lead} or {lead[-1:]}")
-    if positions.device != q.device or freqs.device != q.device:
+    lead = shape[:-2]
+    if positions.shape != lead and positions.shape != lead[-1:]:
+        raise ValueError(f"positions {tuple(positions.shape)} must be {tuple(lead)} or {tuple(lead[-1:])}")
+    if positions.device != device or freqs.device != device:
         raise ValueError("q, positions and freqs must be on one device")
     if positions.requires_grad or freqs.requires_grad:
         raise ValueError("apply_rotary has no gradient for positions and freqs: detach them")
-    native.require_device(q.device)
-    grad = torch.is_grad_enabled() and any(x.requires_grad for x in xs)
+    native.require_device(device)
+    grad = torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad)
     if inplace and grad:
         raise ValueError("inplace=True has no gradient: detach q and k, or rotate out of place")
-    flat = q.dim() == 3
-    x4 = [x[None] if flat else x for x in xs]
-    pos = positions if positions.dim() == 2 else positions[None].expand(x4[0].shape[0], -1)
+    flat = len(shape) == 3
+    x4 = [x[None] for x in xs] if flat else xs
+    pos = positions if len(positions.shape) == 2 else positions[None].expand(x4[0].shape[0], -1)
     freqs = freqs.contiguous()
     if inplace:
         if any(x.stride(-1) != 1 and x.shape[-1] > 1 for x in x4):
@@ -467,5 +469,6 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: t
                 raise ValueError("inplace=True cannot write to an expanded tensor")
     args = (pos, freqs, _LAYOUTS[layout], float(magnitude), bool(inverse))
     out = _Rotary.apply(*args, *x4) if grad else _rotate_heads(x4, *args, inplace)
-    out = [o[0] for o in out] if flat else list(out)
+    if flat:
+        out = [o[0] for o in out]
     return out[0] if k is None else (out[0], out[1])

@@ -330,6 +330,43 @@ def test_cached_long_and_strided():
     assert torch.equal(attend_cached(q, big[:, :, 1:3, 64:192], v, n.cuda()), a)
 
 
+def test_from_a_thread_that_has_no_context_yet():
+    """The first CUDA call of a new thread may be the operator's own (an autograd worker's is)."""
+    import ctypes
+    import threading
+
+    from flashdiffusion_b200 import attention as A
+    from flashdiffusion_b200 import native
+    q, k, v, _ = _inputs(1, 130, 130, 2, 1, 64, BF)
+    want = A.attend(q, k, v)
+    o = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    args = A._arguments(q, k, v, o, None, (None, False, 0, None, None, 64 ** -0.5, 0.0))
+    stream = torch.cuda.current_stream().cuda_stream
+    got = []
+
+    def work():
+        got.append(native.load().fd_attention_forward(args, None, 0, ctypes.c_void_p(stream)))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert got == [native.FD_OK] and torch.equal(o, want)
+
+
+def test_no_second_derivative():
+    from flashdiffusion_b200.attention import attend
+    from flashdiffusion_b200.rope import apply_rotary, rotary_frequencies
+    q, k, v, do = _inputs(1, 8, 8, 2, 1, 64, BF)
+    a = q.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(attend(a, k, v), a, do, create_graph=True)
+    r = apply_rotary(a, positions=torch.arange(8, device="cuda"), freqs=rotary_frequencies(64))
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(r, a, do, create_graph=True)
+
+
 def test_refuses_on_the_device():
     from flashdiffusion_b200.attention import Spans, attend, attend_cached
     q, k, v, _ = _inputs(2, 8, 8, 4, 2, 64, BF)
