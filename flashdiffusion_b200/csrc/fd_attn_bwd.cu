@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
     const int h = blockIdx.y, b = blockIdx.z, t = blockIdx.x;
     const int piece = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     float top = 0.f;
+    asm volatile("griddepcontrol.launch_dependents;");   // the gradient kernel sets itself up and waits
     if (t >= n_qt) {
         if (h >= a.kv_heads) return;
         for (int r = r0; r < T; r += 16) {
@@ -130,31 +131,39 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
         if (threadIdx.x == 0) w.bounds[(int64_t)b * n_qt + t] = {sb[0], sb[1], sb[3], sb[2]};
     }
     const int64_t base = ((int64_t)b * a.heads + h) * n_qt * T;
-    for (int r = r0; r < T; r += 16) {
-        const int64_t i = (int64_t)t * T + r;
-        float d = 0.f, s = 0.f;
-        const bool real = i < a.q_len;
-        if (real && piece * 8 < a.dim) {
-            const uint4 x = *(const uint4*)((const uint16_t*)a.d_o.p + b * a.d_o.sb + i * a.d_o.ss + h * a.d_o.sh + piece * 8);
-            const uint4 y = *(const uint4*)((const uint16_t*)a.o.p + b * a.o.sb + i * a.o.ss + h * a.o.sh + piece * 8);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    uint4 x[8], y[8];
+    float lse[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = pair_of<F16>(xs[e]), g = pair_of<F16>(ys[e]);
-                d = fmaf(f.x, g.x, fmaf(f.y, g.y, d));
-                if (F16) s = fmaf(f.x, f.x, fmaf(f.y, f.y, s));
-            }
+    for (int j = 0; j < 8; ++j) {
+        const int64_t i = (int64_t)t * T + r0 + 16 * j;
+        const bool real = i < a.q_len;
+        x[j] = y[j] = make_uint4(0, 0, 0, 0);
+        if (real && piece * 8 < a.dim) {
+            x[j] = *(const uint4*)((const uint16_t*)a.d_o.p + b * a.d_o.sb + i * a.d_o.ss + h * a.d_o.sh + piece * 8);
+            y[j] = *(const uint4*)((const uint16_t*)a.o.p + b * a.o.sb + i * a.o.ss + h * a.o.sh + piece * 8);
+        }
+        lse[j] = real ? a.lse[((int64_t)b * a.heads + h) * a.q_len + i] : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float d = 0.f, s = 0.f;
+        const uint32_t xs[4] = {x[j].x, x[j].y, x[j].z, x[j].w}, ys[4] = {y[j].x, y[j].y, y[j].z, y[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = pair_of<F16>(xs[e]), g = pair_of<F16>(ys[e]);
+            d = fmaf(f.x, g.x, fmaf(f.y, g.y, d));
+            if (F16) s = fmaf(f.x, f.x, fmaf(f.y, f.y, s));
         }
         for (int o = 8; o; o >>= 1) {
             d += __shfl_xor_sync(~0u, d, o);
             if (F16) s += __shfl_xor_sync(~0u, s, o);
         }
-        const float lse = real ? a.lse[((int64_t)b * a.heads + h) * a.q_len + i] : -INFINITY;
-        const bool some = lse != -INFINITY;
+        const bool some = lse[j] != -INFINITY;
         if (F16 && some && s < INFINITY) top = fmaxf(top, s);
         if (piece == 0) {
-            w.delta[base + i] = some ? -d : 0.f;
-            w.lse2[base + i] = some ? (F16 ? P_SHIFT_F16 : 0.f) - lse * LOG2E : -INFINITY;
+            const int64_t at = base + (int64_t)t * T + r0 + 16 * j;
+            w.delta[at] = some ? -d : 0.f;
+            w.lse2[at] = some ? (F16 ? P_SHIFT_F16 : 0.f) - lse[j] * LOG2E : -INFINITY;
         }
     }
     if (F16) {
@@ -443,24 +452,44 @@ __device__ __forceinline__ void watch(const Cta& c, const Bars& br, uint8_t* bas
 }
 
 // Raw products of one row, 32 columns, to weights: x = 2^(score + add); with a cap, bend = 1 - tanh^2.
-template <bool GEN, int POLY>
+template <bool GEN>
 __device__ __forceinline__ void weights32(uint64_t (&x)[16], const uint64_t (&add)[16], const Score& sc, float slope2,
                                           float dist, float by, int side, uint64_t (&bend)[GEN ? 16 : 1]) {
     if (GEN && sc.capped) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = ptx::mul2(x[e], sc.c);
-        tanh32(x);
+        cap32(x, sc);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            bend[e] = ptx::fma2(ptx::mul2(x[e], ptx::both2(-1.f)), x[e], ptx::both2(1.f));
-            x[e] = ptx::fma2(x[e], sc.cap2, add[e]);
+            bend[e] = ptx::fma2(ptx::mul2(x[e], sc.shrink), x[e], ptx::both2(1.f));
+            x[e] = ptx::add2(x[e], add[e]);
         }
     } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = ptx::fma2(x[e], sc.c, add[e]);
     }
     if (GEN && slope2 != 0.f) add_bias(x, slope2, dist, by, side);
-    exp32<POLY>(x);
+    if (GEN && sc.capped) exp32<0>(x);     // a cap keeps the FMA pipe busy enough
+    else exp32<1>(x);
+}
+
+// Keep the places of x whose bit is set.
+__device__ __forceinline__ void keep32(uint64_t (&x)[16], uint32_t bits) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        x[e] = ptx::pack2(bits >> (2 * e) & 1 ? ptx::lo2(x[e]) : 0.f, bits >> (2 * e + 1) & 1 ? ptx::hi2(x[e]) : 0.f);
+}
+
+// Which of 32 queries see which of the warp's 32 keys from `k0` on: lane e brings query e's span; bit e of the answer
+// of lane l: query e sees key k0 + l.
+__device__ __forceinline__ uint32_t seen32(int2 span, int k0, int lane) {
+    if (__all_sync(~0u, span.x <= k0 && span.y >= k0 + 32)) return ~0u;
+    if (!__any_sync(~0u, span.x < k0 + 32 && span.y > k0)) return 0;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int l = 0; l < 32; ++l) {
+        const uint32_t b = __ballot_sync(~0u, span.x <= k0 + l && span.y > k0 + l);
+        if (lane == l) bits = b;
+    }
+    return bits;
 }
 
 template <int DP, bool F16, bool GEN>
@@ -486,6 +515,11 @@ __device__ __forceinline__ bool compute_key(const Cta& c, const Bars& br, const 
         const int side = GEN ? side_of(a, shift + t * T, c.r0) : 1;
         const uint32_t i = it.i;
         const float* vec = (const float*)(base + C::VEC_OFF) + sb.at * 2 * T + half * 64;
+        int2 see[2] = {};
+        if (masked && a.first) {
+            see[0] = spans[q0 + lane];
+            see[1] = spans[q0 + 32 + lane];
+        }
         if (!ptx::wait_bounded(&br.bfull[sb.at], sb.ph, abort, status, WAIT_NS)) return false;
         uint64_t add[2][16];
 #pragma unroll
@@ -507,22 +541,17 @@ __device__ __forceinline__ bool compute_key(const Cta& c, const Bars& br, const 
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             uint64_t bend[GEN ? 16 : 1];
-            weights32<GEN, 1>(x[g], add[g], sc, slope2, (float)(shift + q0 + g * 32 - row), 1.f, side, bend);
+            weights32<GEN>(x[g], add[g], sc, slope2, (float)(shift + q0 + g * 32 - row), 1.f, side, bend);
             if (masked) {
                 if (!a.first) {
                     // the queries that see this key are a run: i >= row - shift, and i < that + window
                     const int lo = a.causal ? row - shift : row < c.n ? INT_MIN / 2 : INT_MAX / 2;
                     const int64_t hi = row >= c.n ? lo : a.window ? (int64_t)row - shift + a.window : a.q_len;
                     const int l0 = max(lo, 0) - (q0 + g * 32), l1 = (int)min(hi, (int64_t)a.q_len) - (q0 + g * 32);
-                    mask32(x[g], l0, (uint32_t)max(l1 - l0, 0), 0.f);
+                    if (!__all_sync(~0u, l0 <= 0 && l1 >= 32)) mask32(x[g], l0, (uint32_t)max(l1 - l0, 0), 0.f);
                 } else {
-                    const int4* sp = (const int4*)(spans + q0 + g * 32);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int4 s = sp[e];
-                        x[g][e] = ptx::pack2(row >= s.x && row < s.y ? ptx::lo2(x[g][e]) : 0.f,
-                                             row >= s.z && row < s.w ? ptx::hi2(x[g][e]) : 0.f);
-                    }
+                    const uint32_t bits = seen32(see[g], row - lane, lane);
+                    if (!__all_sync(~0u, bits == ~0u)) keep32(x[g], bits);
                 }
             }
             uint32_t p[16];
@@ -616,8 +645,12 @@ __device__ __forceinline__ bool compute_query(const Cta& c, const Bars& br, uint
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             uint64_t bend[GEN ? 16 : 1];
-            weights32<GEN, 1>(x[g], add, sc, slope2, (float)(shift + row - k0 - g * 32), -1.f, side, bend);
-            if (masked) mask32(x[g], span.x - k0 - g * 32, (uint32_t)(span.y - span.x), 0.f);
+            weights32<GEN>(x[g], add, sc, slope2, (float)(shift + row - k0 - g * 32), -1.f, side, bend);
+            if (masked) {
+                const int lo = span.x - k0 - g * 32;
+                if (!__all_sync(~0u, lo <= 0 && (int64_t)lo + (span.y - span.x) >= 32))
+                    mask32(x[g], lo, (uint32_t)(span.y - span.x), 0.f);
+            }
             if (GEN && sc.capped) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
@@ -751,6 +784,7 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         ptx::prefetch_tmap(&tmv);
         ptx::prefetch_tmap(&tmdo);
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // prep_kernel's results from here on
     __syncthreads();
     if (c.key_side) {
         int lo = 0x7fffffff, hi = 0;
@@ -852,7 +886,17 @@ int launch(const Prob& a, const Work& w, cudaStream_t s) {
     prep_kernel<F16><<<dim3(args.n_qt + v_blocks, a.heads, a.batch), 256, 0, s>>>(a, w, args.n_qt);
     FD_CUDA_TRY(cudaGetLastError());
     FD_TRY((allow_smem<gradient_kernel<DP, F16, GEN>>(Cfg<DP>::SMEM)));
-    gradient_kernel<DP, F16, GEN><<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, g, args, status);
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(NTHREADS);
+    cfg.dynamicSmemBytes = Cfg<DP>::SMEM;
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    FD_CUDA_TRY(cudaLaunchKernelEx(&cfg, gradient_kernel<DP, F16, GEN>, q, k, v, g, args, status));
     FD_CUDA_TRY(cudaGetLastError());
     return FD_OK;
 }

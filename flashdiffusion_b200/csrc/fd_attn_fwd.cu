@@ -299,37 +299,62 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                 pairs32(r[1], x[1]);
             }
             const int k0 = j * T + half * 64;
-            if (GEN) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.c);
-                    if (sc.capped) {
-                        tanh32(x[g]);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.cap2);
-                    }
-                    if (slope2 != 0.f)
-                        add_bias(x[g], slope2, (float)(pos - k0 - g * 32), -1.f,
-                                 side_of(a, n - a.q_len + q0 + sub * T, j * T));
-                }
-            }
             const int lo = span.x - k0, len = span.y - span.x;
             const bool masked = !__all_sync(~0u, lo <= 0 && (int64_t)lo + len >= 64);
-            if (masked) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g) mask32(x[g], lo - g * 32, (uint32_t)len, -INFINITY);
-            }
+            // A cap alone, well inside its range: it is monotone, so the largest score comes from the largest (or
+            // smallest) raw product, and the polynomial goes straight into the exponential's argument.
+            bool direct = GEN && sc.capped && slope2 == 0.f && !masked;
             // a NaN among the visible scores becomes the row's m, and with it the whole row NaN
-            float top[4];
+            float mt;
+            if (direct) {
+                float hi[2], bo[2];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                top[g] = max_nan(ptx::lo2(x[g / 2][g % 2 * 8]), ptx::hi2(x[g / 2][g % 2 * 8]));
+                for (int g = 0; g < 2; ++g) {
+                    hi[g] = max_nan(ptx::lo2(x[g][0]), ptx::hi2(x[g][0]));
+                    bo[g] = fminf(ptx::lo2(x[g][0]), ptx::hi2(x[g][0]));
 #pragma unroll
-                for (int i = 1; i < 8; ++i)
-                    top[g] = max_nan(top[g], max_nan(ptx::lo2(x[g / 2][g % 2 * 8 + i]), ptx::hi2(x[g / 2][g % 2 * 8 + i])));
+                    for (int i = 1; i < 16; ++i) {
+                        hi[g] = max_nan(hi[g], max_nan(ptx::lo2(x[g][i]), ptx::hi2(x[g][i])));
+                        bo[g] = fminf(bo[g], fminf(ptx::lo2(x[g][i]), ptx::hi2(x[g][i])));
+                    }
+                }
+                mt = max_nan(hi[0], hi[1]);
+                const float mb = fminf(bo[0], bo[1]);
+                direct = __all_sync(~0u, mt <= sc.limit && mb >= -sc.limit);
+                if (direct) {
+                    const float end = ptx::lo2(sc.c) > 0.f ? mt : mb;
+                    mt = end * ptx::lo2(sc.ratio(ptx::both2(end)));
+                }
             }
-            float mt = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+            if (!direct) {
+                if (GEN) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        if (sc.capped) {
+                            cap32(x[g], sc);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.c);
+                        }
+                        if (slope2 != 0.f)
+                            add_bias(x[g], slope2, (float)(pos - k0 - g * 32), -1.f,
+                                     side_of(a, n - a.q_len + q0 + sub * T, j * T));
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) mask32(x[g], lo - g * 32, (uint32_t)len, -INFINITY);
+                }
+                float top[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    top[g] = max_nan(ptx::lo2(x[g / 2][g % 2 * 8]), ptx::hi2(x[g / 2][g % 2 * 8]));
+#pragma unroll
+                    for (int i = 1; i < 8; ++i)
+                        top[g] = max_nan(top[g], max_nan(ptx::lo2(x[g / 2][g % 2 * 8 + i]), ptx::hi2(x[g / 2][g % 2 * 8 + i])));
+                }
+                mt = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+            }
             // the next tile's scores come only after every thread here has read this and handed over its P
             meet[0] = mt;
             ok = both_here(ok);
@@ -359,9 +384,15 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             uint64_t part[2] = {0, 0};
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
+                if (direct) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[g][i] = GEN ? ptx::add2(x[g][i], off) : ptx::fma2(x[g][i], c2, off);
-                if (masked) exp32<0>(x[g]);
+                    for (int i = 0; i < 16; ++i) x[g][i] = ptx::fma2(sc.ratio(x[g][i]), x[g][i], off);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[g][i] = GEN ? ptx::add2(x[g][i], off) : ptx::fma2(x[g][i], c2, off);
+                }
+                // masked places must be zeros; a cap keeps the FMA pipe busy enough
+                if (masked || direct) exp32<0>(x[g]);
                 else exp32<1>(x[g]);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) part[i & 1] = ptx::add2(part[i & 1], x[g][i]);

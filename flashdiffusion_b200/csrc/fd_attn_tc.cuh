@@ -84,43 +84,57 @@ __device__ __forceinline__ void product_sum(uint32_t lead, uint32_t d, uint32_t 
 //   x = c s + add                       (no cap; c = scale log2(e))
 //   x = cap2 tanh(c s) + add            (c = scale / cap, cap2 = cap log2(e))
 // minus slope2 |distance| (slope2 = slope log2(e)).
+//
+// The tanh has two forms.  |c s| <= 0.45 for the whole warp (scores well inside
+// their cap, the usual case): an odd degree-7 polynomial in the raw product, with
+// c and cap2 in its coefficients, on the FMA pipe in packed pairs (absolute error
+// of the tanh 9e-8; weighted least squares on Chebyshev nodes).  Otherwise
+// 1 - 2 / (1 + e^2u) with two MUFU operations, absolute error 2e-7: with the
+// softmax's own that makes three MUFU operations a pair, and MUFU the bound.
 struct Score {
-    uint64_t c, cap2;    // both halves the same
+    uint64_t c, cap2;            // both halves the same
+    uint64_t b0, b1, b2, b3;     // cap2 tanh(c s) = s (b0 + b1 s^2 + b2 s^4 + b3 s^6)
+    uint64_t shrink;             // -1 / cap2^2: 1 - tanh^2 = 1 + shrink x^2
+    float limit;                 // |s| up to which it holds
     bool capped;
     __device__ explicit Score(const Prob& a) {
         capped = a.cap > 0.f;
-        c = ptx::both2(capped ? a.scale / a.cap : a.scale * LOG2E);
-        cap2 = ptx::both2(a.cap * LOG2E);
+        const float f = capped ? a.scale / a.cap : a.scale * LOG2E, top = a.cap * LOG2E;
+        c = ptx::both2(f);
+        cap2 = ptx::both2(top);
+        b0 = ptx::both2(0.99999905f * f * top);
+        b1 = ptx::both2(-0.33326662f * f * f * f * top);
+        b2 = ptx::both2(0.13208261f * f * f * f * f * f * top);
+        b3 = ptx::both2(-0.04522878f * f * f * f * f * f * f * f * top);
+        shrink = ptx::both2(capped ? -1.f / (top * top) : 0.f);
+        // steep enough for a coefficient to overflow: the polynomial is never taken
+        limit = !(fabsf(ptx::lo2(b3)) < INFINITY) ? -1.f : f != 0.f ? 0.45f / fabsf(f) : INFINITY;
+    }
+    // the factor of s in the polynomial
+    __device__ __forceinline__ uint64_t ratio(uint64_t s) const {
+        const uint64_t y = ptx::mul2(s, s);
+        return ptx::fma2(ptx::fma2(ptx::fma2(b3, y, b2), y, b1), y, b0);
     }
 };
 
-// tanh of 32 arguments.  |u| <= 0.6 for the whole warp (scores well inside their
-// cap, the usual case): an odd degree-9 polynomial on the FMA pipe in packed
-// pairs, absolute error 8.5e-8 (least-squares fit on Chebyshev nodes).  Otherwise
-// 1 - 2 / (1 + e^2u) with two MUFU operations, absolute error 2e-7: with the
-// softmax's own that makes three MUFU operations a pair, and MUFU the bound.
-__device__ __forceinline__ void tanh32(uint64_t (&u)[16]) {
+__device__ __forceinline__ bool inside32(const uint64_t (&s)[16], float limit) {
     float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(ptx::lo2(u[i])), fabsf(ptx::hi2(u[i]))));
-    if (__all_sync(~0u, top <= 0.6f)) {
-        const uint64_t c4 = ptx::both2(0.01548669f), c3 = ptx::both2(-0.052109625f), c2 = ptx::both2(0.13310358f),
-                       c1 = ptx::both2(-0.33332324f), c0 = ptx::both2(0.99999994f);
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(ptx::lo2(s[i])), fabsf(ptx::hi2(s[i]))));
+    return __all_sync(~0u, top <= limit);
+}
+// x = cap2 tanh(c x)
+__device__ __forceinline__ void cap32(uint64_t (&x)[16], const Score& sc) {
+    if (inside32(x, sc.limit)) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint64_t y = ptx::mul2(u[i], u[i]);
-            uint64_t p = ptx::fma2(c4, y, c3);
-            p = ptx::fma2(p, y, c2);
-            p = ptx::fma2(p, y, c1);
-            p = ptx::fma2(p, y, c0);
-            u[i] = ptx::mul2(p, u[i]);
-        }
+        for (int i = 0; i < 16; ++i) x[i] = ptx::mul2(sc.ratio(x[i]), x[i]);
     } else {
         // e^2u overflows to infinity (tanh 1) and underflows to 0 (tanh -1); NaN stays NaN
+        const float c = ptx::lo2(sc.c) * (2.f * LOG2E), top = ptx::lo2(sc.cap2);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float e0 = ptx::ex2_mufu(ptx::lo2(u[i]) * (2.f * LOG2E)), e1 = ptx::ex2_mufu(ptx::hi2(u[i]) * (2.f * LOG2E));
-            u[i] = ptx::pack2(fmaf(-2.f, ptx::rcp_mufu(1.f + e0), 1.f), fmaf(-2.f, ptx::rcp_mufu(1.f + e1), 1.f));
+            const float e0 = ptx::ex2_mufu(ptx::lo2(x[i]) * c), e1 = ptx::ex2_mufu(ptx::hi2(x[i]) * c);
+            x[i] = ptx::pack2(fmaf(-2.f * top, ptx::rcp_mufu(1.f + e0), top), fmaf(-2.f * top, ptx::rcp_mufu(1.f + e1), top));
         }
     }
 }

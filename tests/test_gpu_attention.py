@@ -83,6 +83,16 @@ def test_scores(kw, d, dtype):
     _compare(out, ref, dtype)
 
 
+@pytest.mark.parametrize("scale", [1e-12, 1e9])
+def test_cap_with_extreme_scales(scale):
+    """Products that vanish under the cap, and a slope of the tanh whose powers leave fp32 (rows of zeros among them)."""
+    q, k, v, do = _inputs(1, 140, 140, 2, 1, 64, BF, seed=9)
+    q[:, 5], k[:, 9] = 0, 0
+    lo, hi, pos = spans_of(140, 140, 1)
+    out = _run(q, k, v, do, cap=2.0, scale=scale, grad=False)
+    _compare(out, reference(q, k, v, lo, hi, pos, cap=2.0, scale=scale), BF)
+
+
 def test_large_scores_and_cap_at_its_ends():
     """Scores of hundreds: without a cap one key takes all, with one the tanh is flat at both ends."""
     q, k, v, do = _inputs(1, 150, 150, 2, 2, 64, BF, seed=3)
