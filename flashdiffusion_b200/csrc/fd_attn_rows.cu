@@ -310,8 +310,11 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
         const int n = keys_of(a, b);
         // operand rows: query r0 + 8 y + g; accumulator columns: queries r0 + 8 y + 2 t + z
         uint32_t q[NT][KI][4];
-        int2 sp[NT][2];
         float at[NT][2], slope2[NT][2], m[NT][2], l[NT][2];
+        auto span_of = [&](int y, int z) {       // of this lane's column, made again where a block is not wholly seen
+            const int r = r0 + 8 * y + 2 * t + z;
+            return r < p.rows ? row_span(a, b, p.query(r), n) : make_int2(0, 0);
+        };
         int flo = 0, fhi = 0x7fffffff;   // keys that every row sees: [flo, fhi)
         bool hole = false;
 #pragma unroll
@@ -333,15 +336,15 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                 const int r = r0 + 8 * y + 2 * t + z;
                 const bool real = r < p.rows;
                 const int i = real ? p.query(r) : 0, h = hk * a.group + (real ? r - i * a.group : 0);
-                sp[y][z] = real ? row_span(a, b, i, n) : make_int2(0, 0);
                 at[y][z] = (float)(n - a.q_len + i - g - w.k0 - warp * KEYS);   // distance to this lane's first key
                 slope2[y][z] = a.slopes ? a.slopes[h] * LOG2E : 0.f;
                 m[y][z] = -INFINITY;
                 l[y][z] = 0.f;
                 if (real) {
-                    if (sp[y][z].y > sp[y][z].x) flo = max(flo, sp[y][z].x);
+                    const int2 sp = row_span(a, b, i, n);
+                    if (sp.y > sp.x) flo = max(flo, sp.x);
                     else hole = true;
-                    fhi = min(fhi, sp[y][z].y);
+                    fhi = min(fhi, sp.y);
                 }
             }
         }
@@ -385,13 +388,6 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
             fetch();
             const bool edge = k0 < flo || k0 + KEYS > fhi || hole;
             const float step = (float)(k0 - kfirst);
-            bool raise = false;
-#pragma unroll
-            for (int y = 0; y < NT; ++y)
-#pragma unroll
-                for (int k = 0; k < KT; ++k)
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) s[y][k][z] *= c;
             if (cap2 > 0.f) {
 #pragma unroll
                 for (int y = 0; y < NT; ++y)
@@ -399,41 +395,43 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                     for (int k = 0; k < KT; ++k)
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const float e = ptx::ex2_mufu(s[y][k][z] * (2.f * LOG2E));
-                            s[y][k][z] = cap2 * fmaf(-2.f, ptx::rcp_mufu(1.f + e), 1.f);
+                            const float e = ptx::ex2_mufu(s[y][k][z] * (c * 2.f * LOG2E));
+                            s[y][k][z] = fmaf(-2.f * cap2, ptx::rcp_mufu(1.f + e), cap2);
                         }
             }
-            if (a.slopes) {
-#pragma unroll
-                for (int y = 0; y < NT; ++y)
-#pragma unroll
-                    for (int k = 0; k < KT; ++k)
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float far = at[y][z & 1] - step - (float)(16 * k + 8 * (z >> 1));
-                            s[y][k][z] = fmaf(-slope2[y][z & 1], fabsf(far), s[y][k][z]);
-                        }
-            }
-            if (edge) {
-#pragma unroll
-                for (int y = 0; y < NT; ++y)
-#pragma unroll
-                    for (int k = 0; k < KT; ++k)
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const int key = k0 + 16 * k + g + 8 * (z >> 1);
-                            if (key < sp[y][z & 1].x || key >= sp[y][z & 1].y) s[y][k][z] = -INFINITY;
-                        }
-            }
+            // s becomes score - m (score itself while m is not yet a number)
+            const float mul = cap2 > 0.f ? 1.f : c;
             float top[NT][2];
+            bool raise = false;
 #pragma unroll
             for (int y = 0; y < NT; ++y)
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
+                    const float nb = m[y][z] == -INFINITY ? 0.f : -m[y][z];
+                    const float sl = slope2[y][z], far = at[y][z] - step, from = fmaf(-sl, far, nb);
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float off = (float)(16 * k + 8 * x);
+                            // causal: the key is never ahead of the query, but where it is masked
+                            const float add = !a.slopes ? nb : a.causal ? fmaf(sl, off, from) : fmaf(-sl, fabsf(far - off), nb);
+                            s[y][k][2 * x + z] = fmaf(s[y][k][2 * x + z], mul, add);
+                        }
+                    if (edge) {
+                        const int2 sp = span_of(y, z);
+#pragma unroll
+                        for (int k = 0; k < KT; ++k)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int key = k0 + 16 * k + g + 8 * x;
+                                if (key < sp.x || key >= sp.y) s[y][k][2 * x + z] = -INFINITY;
+                            }
+                    }
                     top[y][z] = fmaxf(s[y][0][z], s[y][0][2 + z]);
 #pragma unroll
                     for (int k = 1; k < KT; ++k) top[y][z] = fmaxf(top[y][z], fmaxf(s[y][k][z], s[y][k][2 + z]));
-                    raise = raise || top[y][z] > m[y][z] + 8.f;
+                    raise = raise || top[y][z] > (m[y][z] == -INFINITY ? -INFINITY : 8.f);
                 }
             if (__any_sync(~0u, raise)) {
 #pragma unroll
@@ -444,10 +442,17 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 4));
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 8));
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 16));
-                        const float mn = fmaxf(m[y][z], tp);
-                        const float fix = mn == -INFINITY ? 0.f : ptx::ex2_mufu(m[y][z] - mn);
-                        m[y][z] = mn;
+                        const bool fresh = m[y][z] == -INFINITY;
+                        if (!fresh) tp = fmaxf(tp, 0.f);
+                        if (tp == -INFINITY) continue;            // still nothing seen
+                        const float fix = fresh ? 0.f : ptx::ex2_mufu(-tp);
+                        m[y][z] = fresh ? tp : m[y][z] + tp;
                         l[y][z] *= fix;
+#pragma unroll
+                        for (int k = 0; k < KT; ++k) {
+                            s[y][k][z] -= tp;
+                            s[y][k][2 + z] -= tp;
+                        }
 #pragma unroll
                         for (int e = 0; e < VB * 4; ++e) {
                             o[y][e][z] *= fix;
@@ -458,13 +463,12 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
             // P^T as B operand: keys along the contracted index
             uint32_t ph[NT][KT][2], pl[NT][KT][2];
 #pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                const float b0 = m[y][0] == -INFINITY ? 0.f : m[y][0], b1 = m[y][1] == -INFINITY ? 0.f : m[y][1];
+            for (int y = 0; y < NT; ++y)
 #pragma unroll
                 for (int k = 0; k < KT; ++k)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float e0 = ptx::ex2_mufu(s[y][k][2 * x] - b0), e1 = ptx::ex2_mufu(s[y][k][2 * x + 1] - b1);
+                        const float e0 = ptx::ex2_mufu(s[y][k][2 * x]), e1 = ptx::ex2_mufu(s[y][k][2 * x + 1]);
                         l[y][0] += e0;
                         l[y][1] += e1;
                         const uint32_t hi = ptx::pack16<F16>(e0, e1);
@@ -472,7 +476,6 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                         ph[y][k][x] = transpose8x8(hi);
                         pl[y][k][x] = transpose8x8(ptx::pack16<F16>(e0 - hf.x, e1 - hf.y));
                     }
-            }
             bool bad = false;
 #pragma unroll
             for (int k = 0; k < KT; ++k)
@@ -528,8 +531,10 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
 #pragma unroll
                             for (int y = 0; y < NT; ++y)
 #pragma unroll
-                                for (int z = 0; z < 2; ++z)
-                                    if (key >= sp[y][z].x && key < sp[y][z].y) o[y][e][2 * x + z] += one16<F16>(h);
+                                for (int z = 0; z < 2; ++z) {
+                                    const int2 sp = span_of(y, z);
+                                    if (key >= sp.x && key < sp.y) o[y][e][2 * x + z] += one16<F16>(h);
+                                }
                         }
                 }
             }
