@@ -16,7 +16,7 @@
 // pair inside one CTA is finished there.
 //
 // Each warp copies its own blocks of keys with cp.async into a ring of its own,
-// STAGES - 1 blocks ahead and across the ends of pairs, and reads MMA fragments
+// one or two blocks ahead and across the ends of pairs, and reads MMA fragments
 // from it in 16-byte pieces: the order of the contracted coordinate in K Q^T is
 // free (Q is loaded the same way), and so is the order of output coordinates in
 // V^T P^T; the pairs of keys that a V^T fragment wants are put together by byte
@@ -33,9 +33,12 @@ namespace attn {
 namespace rows {
 
 constexpr int WARPS = 4;
-constexpr int CTAS_PER_SM = 2;
-constexpr int STAGES = 3;
-constexpr int SETUP = 2;
+constexpr int SETUP = 3;
+// CTAs to an SM and blocks of a warp's ring, by column tiles: registers allow three CTAs for up to 8 rows, shared
+// memory then two blocks for each warp (48 ragged lengths to 8192 of 32 / 8 heads of 128: 50 us with two CTAs and
+// three blocks, 44 so), else two.
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+__host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 2 : 3; }
 
 struct Range {
     int lo, hi;   // keys seen by any row of the sequence, lo on a multiple of 16
@@ -230,22 +233,24 @@ __device__ __forceinline__ void store_row(const Prob& a, const Plan& p, int b, i
     if (d == 0 && a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
-template <int DP>
+template <int DP, int NT>
 struct Smem {
+    static constexpr int STAGES = stages(NT), CTAS = ctas_per_sm(NT);
     static constexpr int KEYS = 2048 / DP;                        // keys of a block: 16 or 32
     static constexpr uint32_t HALF = KEYS * DP * 2;               // K or V of a block, 4 KB
     static constexpr uint32_t RING = WARPS * STAGES * 2 * HALF;
     static constexpr int PIECES = DP / 16 + 1;                    // 16-byte pieces of one lane's sums: O, and m and l
     static constexpr uint32_t BYTES = RING + 2 * PIECES * 32 * 16;
     // 228 KB to an SM, of which each CTA takes 1 KB for itself
-    static_assert(CTAS_PER_SM * (BYTES + 1024) <= 228 * 1024, "shared memory budget");
+    static_assert(CTAS * (BYTES + 1024) <= 228 * 1024, "shared memory budget");
 };
 
 // Row r of a pair: query i = r / group, head hk * group + r % group.
 template <int DP, bool F16, int NT>
-__global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
+__global__ void __launch_bounds__(WARPS * 32, ctas_per_sm(NT))
 rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, float* __restrict__ parts) {
-    using S = Smem<DP>;
+    using S = Smem<DP, NT>;
+    constexpr int STAGES = S::STAGES;
     constexpr int KEYS = S::KEYS, KT = KEYS / 16, UNIT = KEYS * WARPS;
     constexpr int KI = DP / 32, VB = DP / 64, CH = DP / 8;   // 16-byte pieces of a row: CH
     extern __shared__ __align__(128) uint8_t smem[];
@@ -696,11 +701,11 @@ int launch(const Prob& a, float* parts, cudaStream_t s) {
     p.rows = a.group * a.q_len;
     p.row_tiles = (int)cdiv(p.rows, 8 * NT);
     p.pairs = a.kv_heads * p.row_tiles;
-    p.ctas = num_sms() * CTAS_PER_SM;
+    p.ctas = num_sms() * ctas_per_sm(NT);
     p.unit = DP == 64 ? 7 : 6;
-    static_assert(Smem<DP>::KEYS * WARPS == (DP == 64 ? 128 : 64), "unit");
+    static_assert(Smem<DP, NT>::KEYS * WARPS == (DP == 64 ? 128 : 64), "unit");
     p.magic = (65536 + a.group - 1) / a.group;
-    using S = Smem<DP>;
+    using S = Smem<DP, NT>;
     FD_TRY((allow_smem<rows_kernel<DP, F16, NT>>(S::BYTES)));
     rows_kernel<DP, F16, NT><<<p.ctas, WARPS * 32, S::BYTES, s>>>(a, p, parts);
     FD_CUDA_TRY(cudaGetLastError());
@@ -734,7 +739,8 @@ int by_rows(const Prob& a, float* parts, cudaStream_t s) {
 bool rows_applies(const Prob& a) { return (int64_t)a.group * a.q_len <= MAX_ROWS; }
 
 size_t rows_bytes(int dim) {
-    return sizeof(float) * 2 * (size_t)num_sms() * rows::CTAS_PER_SM * (dim <= 64 ? rows::PART<64, 4> : rows::PART<128, 4>);
+    static_assert(rows::ctas_per_sm(4) * 4 >= rows::ctas_per_sm(1), "the widest kernel has the largest partials");
+    return sizeof(float) * 2 * (size_t)num_sms() * rows::ctas_per_sm(4) * (dim <= 64 ? rows::PART<64, 4> : rows::PART<128, 4>);
 }
 
 int rows_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
