@@ -134,7 +134,7 @@ def _like(t):
 _NO_GRADIENTS = (0,) * 16
 
 
-def _arguments(q, k, v, o, lse, how, gradients=_NO_GRADIENTS) -> bytes:
+def _arguments(q, k, v, o, lse, low, how, gradients=_NO_GRADIENTS) -> bytes:
     """fd_attention_args, packed."""
     spans, causal, window, lengths, slopes, scale, cap = how
     b, sq, h, d = q.shape
@@ -144,7 +144,7 @@ def _arguments(q, k, v, o, lse, how, gradients=_NO_GRADIENTS) -> bytes:
         first, end, step = spans.first.data_ptr(), spans.end.data_ptr(), sq if spans.batch > 1 else 0
     return native.PACK_ATTENTION(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], o.data_ptr(),
-        *o.stride()[:3], 0 if lse is None else lse.data_ptr(), first, end, step,
+        *o.stride()[:3], 0 if lse is None else lse.data_ptr(), 0 if low is None else low.data_ptr(), first, end, step,
         0 if lengths is None else lengths.data_ptr(), 0 if slopes is None else slopes.data_ptr(), scale, cap,
         _DTYPES[q.dtype], causal, window, b, sq, k.shape[1], h, k.shape[2], d, *gradients)
 
@@ -156,11 +156,11 @@ def _call(fn, args, backward, q):
     native.call(fn, q.device, args, ws.data_ptr() if nbytes else 0, nbytes)
 
 
-def _forward(q, k, v, how, want_lse):
+def _forward(q, k, v, how, want_lse, low=None):
     """(output, lse or None) of heads that are loadable."""
     o = _like(q)
     lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32) if want_lse else None
-    _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, how), 0, q)
+    _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, low, how), 0, q)
     return o, lse
 
 
@@ -168,7 +168,11 @@ class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, how, return_lse):
         q, k, v = _loadable(q), _loadable(k), _loadable(v)
-        o, lse = _forward(q, k, v, how, True)
+        # 16-bit heads on the tensor cores: eight more bits of o for the backward pass
+        low = (torch.empty(q.shape, dtype=torch.int8, device=q.device)
+               if q.dtype is not torch.float32 and q.shape[-1] % 8 == 0 and q.shape[-1] <= 128 else None)
+        o, lse = _forward(q, k, v, how, True, low)
+        ctx.low = low
         spans, slopes = how[0], how[4]
         if spans is None and slopes is None:
             ctx.save_for_backward(q, k, v, o, lse)
@@ -188,7 +192,7 @@ class _Attend(torch.autograd.Function):
         q, k, v, o, lse = ctx.saved_tensors[:5]
         do = _loadable(do)
         dq, dk, dv = _like(q), _like(k), _like(v)
-        args = _arguments(q, k, v, o, lse, ctx.how,
+        args = _arguments(q, k, v, o, lse, ctx.low, ctx.how,
                           (do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                            *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
         _call(native.load().fd_attention_backward, args, 1, q)

@@ -78,6 +78,7 @@ static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     a.dk = view(r->dk, r->dk_stride, r->batch, r->k_len, r->kv_heads);
     a.dv = view(r->dv, r->dv_stride, r->batch, r->k_len, r->kv_heads);
     a.lse = r->lse;
+    a.o_low = r->o_low;
     a.first = r->first;
     a.end = r->end;
     a.span_stride = r->span_stride;

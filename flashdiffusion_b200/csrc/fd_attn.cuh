@@ -29,6 +29,7 @@ struct View {
 struct Prob {
     View q, k, v, o, d_o, dq, dk, dv;
     float* lse;
+    int8_t* o_low;
     const int32_t *first, *end;
     int64_t span_stride;
     const int32_t* lengths;

@@ -67,12 +67,6 @@ __host__ __device__ inline size_t work_layout(Work* w, void* base, int64_t bh, i
     return at;
 }
 
-template <bool F16>
-__device__ __forceinline__ float2 pair_of(uint32_t w) {
-    if (F16) return __half22float2(*(__half2*)&w);
-    return __bfloat1622float2(*(__nv_bfloat162*)&w);
-}
-
 // Block (t, h, b): delta and lse2 of 128 rows, 16 lanes a row (one 16-byte piece
 // each); head 0 also makes the tile's bounds.  fp16: the largest row norms of dO
 // and, in the blocks behind the query tiles, of V.  Bandwidth-bound: dO and o are
@@ -132,15 +126,18 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
     }
     const int64_t base = ((int64_t)b * a.heads + h) * n_qt * T;
     uint4 x[8], y[8];
+    uint2 low[8];
     float lse[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int64_t i = (int64_t)t * T + r0 + 16 * j;
         const bool real = i < a.q_len;
         x[j] = y[j] = make_uint4(0, 0, 0, 0);
+        low[j] = make_uint2(0, 0);
         if (real && piece * 8 < a.dim) {
             x[j] = *(const uint4*)((const uint16_t*)a.d_o.p + b * a.d_o.sb + i * a.d_o.ss + h * a.d_o.sh + piece * 8);
             y[j] = *(const uint4*)((const uint16_t*)a.o.p + b * a.o.sb + i * a.o.ss + h * a.o.sh + piece * 8);
+            if (a.o_low) low[j] = *(const uint2*)(a.o_low + (((int64_t)b * a.q_len + i) * a.heads + h) * a.dim + piece * 8);
         }
         lse[j] = real ? a.lse[((int64_t)b * a.heads + h) * a.q_len + i] : -INFINITY;
     }
@@ -151,7 +148,9 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 f = pair_of<F16>(xs[e]), g = pair_of<F16>(ys[e]);
-            d = fmaf(f.x, g.x, fmaf(f.y, g.y, d));
+            const uint32_t l = e < 2 ? low[j].x : low[j].y;
+            const float g0 = with_low<F16>(g.x, (int8_t)(l >> (e % 2 * 16))), g1 = with_low<F16>(g.y, (int8_t)(l >> (e % 2 * 16 + 8)));
+            d = fmaf(f.x, g0, fmaf(f.y, g1, d));
             if (F16) s = fmaf(f.x, f.x, fmaf(f.y, f.y, s));
         }
         for (int o = 8; o; o >>= 1) {

@@ -416,6 +416,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         const bool real = row < a.q_len;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint8_t* out = (uint8_t*)a.o.p + 2 * (b * a.o.sb + (int64_t)row * a.o.ss + h * a.o.sh);
+        int8_t* low = a.o_low ? a.o_low + (((int64_t)b * a.q_len + row) * a.heads + h) * a.dim : nullptr;
         const bool poison = it > 0 && *(volatile int*)&ms.poison;
 #pragma unroll 1
         for (int g = 0; g < DP / 2; g += 16) {
@@ -449,12 +450,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (c0 + i * 8 >= a.dim) continue;
-                    uint4 w;
-                    w.x = ptx::pack16<F16>(f[8 * i], f[8 * i + 1]);
-                    w.y = ptx::pack16<F16>(f[8 * i + 2], f[8 * i + 3]);
-                    w.z = ptx::pack16<F16>(f[8 * i + 4], f[8 * i + 5]);
-                    w.w = ptx::pack16<F16>(f[8 * i + 6], f[8 * i + 7]);
-                    *(uint4*)(out + 2 * (c0 + i * 8)) = w;
+                    store8<F16>(out + 2 * (c0 + i * 8), low ? low + c0 + i * 8 : nullptr, f + 8 * i);
                 }
             }
         }

@@ -223,12 +223,11 @@ __device__ __forceinline__ void store_row(const Prob& a, const Plan& p, int b, i
     const int i = p.query(gr), h = hk * a.group + gr - i * a.group;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (d < a.dim) {
-        uint4 w;
-        w.x = ptx::pack16<F16>(acc[0] * inv, acc[1] * inv);
-        w.y = ptx::pack16<F16>(acc[2] * inv, acc[3] * inv);
-        w.z = ptx::pack16<F16>(acc[4] * inv, acc[5] * inv);
-        w.w = ptx::pack16<F16>(acc[6] * inv, acc[7] * inv);
-        *(uint4*)((uint16_t*)a.o.p + b * a.o.sb + (int64_t)i * a.o.ss + h * a.o.sh + d) = w;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = acc[e] * inv;
+        store8<F16>((uint16_t*)a.o.p + b * a.o.sb + (int64_t)i * a.o.ss + h * a.o.sh + d,
+                    a.o_low ? a.o_low + (((int64_t)b * a.q_len + i) * a.heads + h) * a.dim + d : nullptr, f);
     }
     if (d == 0 && a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }

@@ -285,6 +285,43 @@ __device__ __forceinline__ bool clear_bad(uint8_t* tile, int bytes, int lane) {
 __device__ __forceinline__ int warp_min(int x) { return __reduce_min_sync(~0u, x); }
 __device__ __forceinline__ int warp_max(int x) { return __reduce_max_sync(~0u, x); }
 
+// The eight bits below a rounded output, in units of 2^8 (bf16) or 2^5 (fp16) last places of fp32: `bits` is the
+// unrounded value, `back` the rounded one.  delta = d_o . o summed from rounded outputs would be the largest error of
+// dq and dk after their own rounding and that of dS.
+template <bool F16>
+__device__ __forceinline__ int low_bits(float f, float back) {
+    constexpr int SH = F16 ? 5 : 8;
+    if (!(fabsf(back) < INFINITY)) return 0;
+    return min(max((__float_as_int(f) - __float_as_int(back) + (1 << (SH - 1))) >> SH, -128), 127);
+}
+template <bool F16>
+__device__ __forceinline__ float with_low(float back, int low) {
+    return __int_as_float(__float_as_int(back) + low * (F16 ? 32 : 256));
+}
+template <bool F16>
+__device__ __forceinline__ float2 pair_of(uint32_t w) {
+    if (F16) return __half22float2(*(__half2*)&w);
+    return __bfloat1622float2(*(__nv_bfloat162*)&w);
+}
+// Eight outputs, 16-bit to `out` and their low bits to `low` (unless it is null).
+template <bool F16>
+__device__ __forceinline__ void store8(void* out, int8_t* low, const float* f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = ptx::pack16<F16>(f[2 * i], f[2 * i + 1]);
+    *(uint4*)out = make_uint4(w[0], w[1], w[2], w[3]);
+    if (low) {
+        uint32_t v[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 b = pair_of<F16>(w[i]);
+            v[i / 2] |= ((uint32_t)low_bits<F16>(f[2 * i], b.x) & 255) << (i % 2 * 16);
+            v[i / 2] |= ((uint32_t)low_bits<F16>(f[2 * i + 1], b.y) & 255) << (i % 2 * 16 + 8);
+        }
+        *(uint2*)low = make_uint2(v[0], v[1]);
+    }
+}
+
 // Launchers of the tensor-core kernels.
 bool tc_applies(const Prob& a, int dtype, bool backward);
 int tc_forward(const Prob& a, int dtype, cudaStream_t s);

@@ -88,14 +88,14 @@ class RotaryArgs(ctypes.Structure):
 
 # The same two structures as packers: one pack() instead of some thirty field stores for each call.
 PACK_ROTARY = struct.Struct("@4P12qP2qPd4i2q4i").pack
-PACK_ATTENTION = struct.Struct("@3P9qP3q3PqPPdd9iP3q3P9q").pack
+PACK_ATTENTION = struct.Struct("@3P9qP3q4PqPPdd9iP3q3P9q").pack
 
 
 class AttentionArgs(ctypes.Structure):
     """fd_attention_args."""
 
     _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_stride", _L3), ("k_stride", _L3), ("v_stride", _L3),
-                ("o", _P), ("o_stride", _L3), ("lse", _P), ("first", _P), ("end", _P), ("span_stride", _L),
+                ("o", _P), ("o_stride", _L3), ("lse", _P), ("o_low", _P), ("first", _P), ("end", _P), ("span_stride", _L),
                 ("lengths", _P), ("slopes", _P), ("scale", ctypes.c_double), ("cap", ctypes.c_double),
                 ("dtype", _I), ("causal", _I), ("window", _I), ("batch", _I), ("q_len", _I), ("k_len", _I),
                 ("heads", _I), ("kv_heads", _I), ("dim", _I),

@@ -351,7 +351,7 @@ def test_from_a_thread_that_has_no_context_yet():
     want = A.attend(q, k, v)
     o = torch.zeros_like(q)
     torch.cuda.synchronize()
-    args = A._arguments(q, k, v, o, None, (None, False, 0, None, None, 64 ** -0.5, 0.0))
+    args = A._arguments(q, k, v, o, None, None, (None, False, 0, None, None, 64 ** -0.5, 0.0))
     stream = torch.cuda.current_stream().cuda_stream
     got = []
 
