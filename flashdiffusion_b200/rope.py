@@ -424,7 +424,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: t
 
     layout "half" pairs coordinate p with p + R/2, "interleaved" 2p with 2p + 1 (as ROPE does).  ``magnitude``
     scales the rotated coordinates, ``inverse`` turns the other way.  ``inplace`` overwrites q and k (no
-    gradients).  Returns the rotated q, or (q, k).
+    gradients; q and k must not overlap).  Returns the rotated q, or (q, k).
     """
     xs = (q,) if k is None else (q, k)
     for name, x in zip("qk", xs):
@@ -467,8 +467,12 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: t
         for x in x4:
             if any(x.stride(i) == 0 and x.shape[i] > 1 for i in range(3)):
                 raise ValueError("inplace=True cannot write to an expanded tensor")
+        if k is not None and k.numel() and q.data_ptr() == k.data_ptr():
+            raise ValueError("inplace=True would rotate the same memory as q and as k")
     args = (pos, freqs, _LAYOUTS[layout], float(magnitude), bool(inverse))
     out = _Rotary.apply(*args, *x4) if grad else _rotate_heads(x4, *args, inplace)
+    if inplace:    # autograd sees the change, as of any operation in place
+        torch.autograd.graph.increment_version([x for x in xs if not x.is_inference()])
     if flat:
         out = [o[0] for o in out]
     return out[0] if k is None else (out[0], out[1])

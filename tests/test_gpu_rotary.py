@@ -129,3 +129,21 @@ def test_gradient_against_differences():
     # the map is linear: any step is exact up to fp32 rounding of 48 terms of size about 1
     diff = (loss(x.detach() + e) - loss(x.detach() - e)) / 2
     assert abs(float(diff) - float((g * e).double().sum())) < 48 * 2.0 ** -22 * 8
+
+
+def test_in_place_is_seen_by_autograd_and_refused_twice():
+    from flashdiffusion_b200.rope import apply_rotary, rotary_frequencies
+    x = torch.randn(1, 6, 4, 64, device="cuda")
+    pos, f = torch.arange(6, device="cuda"), rotary_frequencies(64)
+    w = torch.ones_like(x, requires_grad=True)
+    y = w * x                                       # saves x
+    with torch.no_grad():
+        apply_rotary(x[:, :, :2], x[:, :, 2:], positions=pos, freqs=f, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(ValueError, match="same memory"):
+        apply_rotary(x, x, positions=pos, freqs=f, inplace=True)
+    with torch.inference_mode():
+        z = torch.randn(1, 6, 4, 64, device="cuda")
+        want = apply_rotary(z, positions=pos, freqs=f)
+        assert torch.equal(apply_rotary(z, positions=pos, freqs=f, inplace=True), want)
