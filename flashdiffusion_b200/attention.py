@@ -16,6 +16,12 @@ whatever their memory holds.
 
 ``attend_cached`` is the form for the newest tokens of each sequence against a
 key/value cache of which ``lengths`` rows are in use.
+
+Everything runs on the current stream and may be captured into a graph.  Where a
+captured step takes gradients of leaves (``backward`` into ``.grad``), run its
+warm-up on a side stream, or drop every output of earlier eager steps first: a
+leaf whose gradient node was made on the default stream, and is kept alive by
+such an output, pulls that stream into the capture, which torch cannot do.
 """
 
 from __future__ import annotations
@@ -172,12 +178,11 @@ class _Attend(torch.autograd.Function):
         low = (torch.empty(q.shape, dtype=torch.int8, device=q.device)
                if q.dtype is not torch.float32 and q.shape[-1] % 8 == 0 and q.shape[-1] <= 128 else None)
         o, lse = _forward(q, k, v, how, True, low)
-        ctx.low = low
         spans, slopes = how[0], how[4]
         if spans is None and slopes is None:
-            ctx.save_for_backward(q, k, v, o, lse)
+            ctx.save_for_backward(q, k, v, o, lse, low)
         else:    # what the gradients read again: autograd notices if it was changed in between
-            ctx.save_for_backward(q, k, v, o, lse, *(() if spans is None else (spans.first, spans.end)),
+            ctx.save_for_backward(q, k, v, o, lse, low, *(() if spans is None else (spans.first, spans.end)),
                                   *(() if slopes is None else (slopes,)))
         ctx.how = how
         if not return_lse:
@@ -189,10 +194,10 @@ class _Attend(torch.autograd.Function):
     def backward(ctx, do, *_):
         if torch.is_grad_enabled():
             raise RuntimeError("attend has no second derivative: call backward without create_graph")
-        q, k, v, o, lse = ctx.saved_tensors[:5]
+        q, k, v, o, lse, low = ctx.saved_tensors[:6]
         do = _loadable(do)
         dq, dk, dv = _like(q), _like(k), _like(v)
-        args = _arguments(q, k, v, o, lse, ctx.low, ctx.how,
+        args = _arguments(q, k, v, o, lse, low, ctx.how,
                           (do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                            *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
         _call(native.load().fd_attention_backward, args, 1, q)

@@ -61,8 +61,8 @@ static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     FD_CHECK_ARG(r->dim >= 1 && r->dim <= 256, "fd_attention: dim=%d not in 1..256", r->dim);
     FD_CHECK_ARG(r->heads >= 1 && r->kv_heads >= 1 && r->heads % r->kv_heads == 0,
                  "fd_attention: heads=%d must be a multiple of kv_heads=%d", r->heads, r->kv_heads);
-    FD_CHECK_ARG((int64_t)r->batch * r->heads <= 65535, "fd_attention: batch * heads = %lld above 65535",
-                 (long long)r->batch * r->heads);
+    FD_CHECK_ARG(r->batch <= 65535 && r->heads <= 65535, "fd_attention: batch=%d or heads=%d above 65535", r->batch, r->heads);
+    FD_CHECK_ARG(((uintptr_t)r->o_low & 7) == 0, "fd_attention: o_low must be 8-byte aligned");
     FD_CHECK_ARG(r->scale == r->scale && r->cap >= 0.0, "fd_attention: scale and cap must be numbers, cap >= 0");
     FD_CHECK_ARG((r->first == nullptr) == (r->end == nullptr), "fd_attention: first and end come together");
     FD_CHECK_ARG(r->window >= 0, "fd_attention: window=%d", r->window);

@@ -63,9 +63,7 @@ __device__ __forceinline__ int2 row_span(const Prob& a, int b, int i, int n) {
 
 // Launchers (fd_attn_simt.cu).
 int simt_forward(const Prob& a, int dtype, cudaStream_t s);
-int simt_backward(const Prob& a, int dtype, float* delta, cudaStream_t s);
-// delta[b, h, i] = sum_c d_o o  (batch, heads, q_len)
-int launch_delta(const Prob& a, int dtype, float* delta, cudaStream_t s);
+int simt_backward(const Prob& a, int dtype, float* delta, cudaStream_t s);   // delta: batch * heads * q_len floats
 
 }  // namespace attn
 }  // namespace fd

@@ -8,8 +8,7 @@ Rounding model (u = half a step of the tensors' type, w = 2^-24):
             good to 4e-6, twice for numerator and sum), and rounded once to the tensors' type: u
   output    one rounding, u, of a sum of p v
   ds        p (dp - delta): delta is summed from the rounded output, dp like a score without the scale; rounded: u
-Sums of up to n terms in fp32 add 2 n w of their absolute sum; with n <= 4096 here that stays below 5e-4 and is
-counted as 2 sqrt-free n w.
+Sums of up to n terms in fp32 add 2 n w of their absolute sum; with n <= 4096 here that stays below 5e-4.
 """
 import torch
 

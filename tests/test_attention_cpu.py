@@ -85,7 +85,7 @@ def _args(**kw):
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=native.DTYPE_F64), dict(batch=-1), dict(q_len=-1), dict(k_len=-2), dict(dim=0), dict(dim=257),
-    dict(kv_heads=3), dict(kv_heads=0), dict(heads=0), dict(batch=20000), dict(scale=float("nan")), dict(cap=-1.0),
+    dict(kv_heads=3), dict(kv_heads=0), dict(heads=0), dict(batch=70000), dict(heads=65536 * 2), dict(o_low=4100), dict(scale=float("nan")), dict(cap=-1.0),
     dict(cap=float("nan")), dict(first=4096), dict(end=4096), dict(window=-1), dict(window=3),
     dict(first=4096, end=4096, causal=1), dict(q=None), dict(k=None), dict(o=None), dict(q_len=(1 << 30) + 1),
 ], ids=str)
@@ -115,6 +115,13 @@ def test_c_entries_check_workspace_and_gradients():
     # nothing to do is not an error
     empty = _args(batch=0)
     assert lib.fd_attention_forward(ctypes.byref(empty), None, 0, None) == native.FD_OK
+
+
+def test_rotary_c_entry_refuses_very_wide_heads():
+    lib = native.load()
+    a = native.RotaryArgs(q=4096, qo=4096, positions=4096, freqs=4096, magnitude=1.0, dtype=native.DTYPE_BF16,
+                          position_dtype=native.DTYPE_I64, batch=1, tokens=4, heads=2, dim=4098, rot=64)
+    assert lib.fd_rotary(ctypes.byref(a), None) == native.FD_ERR_ARG
 
 
 @pytest.mark.parametrize("bad", [

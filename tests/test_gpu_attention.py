@@ -427,6 +427,190 @@ def test_other_stream_and_captured_graph():
         assert all(torch.equal(x, y) for x, y in zip(outs, w))
 
 
+@pytest.mark.parametrize("dtype,d", [(SF, 64), (SF, 33), (SF, 128), (HF, 200), (BF, 256), (BF, 20)], ids=str)
+def test_general_path_tiles(dtype, d):
+    """More rows than the general path takes one by one: whole tiles, ends inside tiles, shared heads, a window, and
+    keys and rows outside the spans that hold anything."""
+    from flashdiffusion_b200.attention import Spans
+    b, sq, sk, h, hk = 2, 300, 333, 4, 2
+    q, k, v, do = _inputs(b, sq, sk, h, hk, d, dtype, seed=d)
+    lo, hi, pos = spans_of(sq, sk, b, causal=True, window=150)
+    ref = reference(q, k, v, lo, hi, pos, do=do)
+    _compare(_run(q, k, v, do, causal=True, window=150), ref, dtype)
+    g = torch.Generator().manual_seed(d)
+    lo = torch.randint(10, 200, (b, sq), generator=g).int()
+    hi = (lo + torch.randint(0, 140, (b, sq), generator=g)).clamp(max=321).int()
+    for x in range(b):
+        for t in (k, v):
+            t[x, :10], t[x, 321:] = float("nan"), float("inf")
+        q[x, hi[x] <= lo[x]] = float("nan")
+        do[x, hi[x] <= lo[x]] = float("inf")
+    ref = reference(q, k, v, lo, hi, pos, cap=9.0, do=do)
+    _compare(_run(q, k, v, do, spans=Spans(lo.cuda(), hi.cuda()), cap=9.0), ref, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 64), (SF, 16)], ids=str)
+def test_very_many_heads(dtype, d):
+    """More (sequence, head) pairs than a grid's second axis holds."""
+    from flashdiffusion_b200.attention import attend
+    q, k, v, _ = _inputs(2100, 1, 3, 32, 32, d, dtype)
+    o = attend(q, k, v).double()
+    s = torch.einsum("bihd,bjhd->bhij", q.double(), k.double()) * d ** -0.5
+    p = torch.softmax(s, -1)
+    u = torch.finfo(dtype).eps / 2
+    # the reference module's bound with scores of D + 8 roundings, their sum at most 8 sqrt(d) here
+    rel = u + 2 * (2 * (d + 8) * 2.0 ** -24 * 8 * d ** 0.5) + 2e-5
+    want, room = (torch.einsum("bhij,bjhd->bihd", p, x) for x in (v.double(), v.double().abs()))
+    assert float(s.abs().max()) < 8 * d ** 0.5
+    assert ((o - want).abs() <= u * want.abs() + rel * room + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, SF], ids=str)
+def test_one_tensor_in_every_place(dtype):
+    """attend(x, x, x): the gradient of x is the sum of the three."""
+    from flashdiffusion_b200.attention import attend
+    x, _, _, do = _inputs(1, 140, 140, 2, 2, 64, dtype, seed=51)
+    lo, hi, pos = spans_of(140, 140, 1, causal=True)
+    ref = reference(x, x, x, lo, hi, pos, do=do)
+    x.requires_grad_(True)
+    o = attend(x, x, x, causal=True)
+    dx, = torch.autograd.grad(o, x, do)
+    total = sum(ref[n] for n in ("dq", "dk", "dv"))
+    u = torch.finfo(dtype).eps / 2
+    # two additions of rounded gradients, each rounded again: partial sums stay below the three sizes' sum
+    size = sum(ref[n].abs() + ref[n + "_tol"] for n in ("dq", "dk", "dv"))
+    check("dx", dx, {"dx": total, "dx_tol": sum(ref[n + "_tol"] for n in ("dq", "dk", "dv")) + 2 * u * size})
+
+
+@pytest.mark.parametrize("d,dtype", [(64, BF), (64, SF)], ids=str)
+def test_offsets_beyond_32_bits(d, dtype):
+    """A cache of more than 2^31 elements: only its end is written, read and compared."""
+    from flashdiffusion_b200.attention import Spans, attend, attend_cached
+    rows = 2 ** 31 // d + 700
+    q, k, v, _ = _inputs(1, 3, 600, 4, 1, d, dtype, seed=53)
+    kc, vc = (torch.empty(1, rows, 1, d, dtype=dtype, device="cuda") for _ in "kv")
+    kc[:, -600:], vc[:, -600:] = k, v
+    n = torch.tensor([rows], dtype=torch.int32, device="cuda")
+    lo, hi, pos = spans_of(3, 600, 1, causal=True, window=500)
+    ref = reference(q, k, v, lo, hi, pos)
+    check("o", attend_cached(q, kc, vc, n, window=500), ref, FLOOR[dtype])
+    many = torch.randn(1, 1200, 4, d, device="cuda").to(dtype)
+    at = torch.arange(1200, device="cuda", dtype=torch.int32) % 100 + (rows - 300)
+    lo, hi, pos = spans_of(1200, 600, 1, first=(at - (rows - 600)).cpu(), end=(at - (rows - 600)).cpu() + 77)
+    ref = reference(many, k, v, lo, hi, pos)
+    check("o", attend(many, kc, vc, spans=Spans(at, at + 77)), ref, FLOOR[dtype])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF], ids=str)
+def test_two_streams_at_once(dtype):
+    """Training steps and cache reads in flight on two streams together give the bits that each gives alone."""
+    from flashdiffusion_b200.attention import attend, attend_cached
+    sets = [_inputs(2, 500, 500, 8, 2, 64, dtype, seed=s) for s in (55, 56)]
+    n = torch.tensor([500, 77], dtype=torch.int32, device="cuda")
+
+    def step(q, k, v, do):
+        a, b, c = (t.detach().requires_grad_(True) for t in (q, k, v))
+        o = attend(a, b, c, causal=True)
+        return (o.detach(), attend_cached(q[:, -2:], k, v, n), *torch.autograd.grad(o, (a, b, c), do))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(6):
+        for i, (stream, s) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(stream):
+                got[i].append(step(*s))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(x, y) for g in got[i] for x, y in zip(g, want[i]))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF], ids=str)
+def test_two_captured_graphs_of_one_pool(dtype):
+    """Two training steps captured into one memory pool and replayed in turn on changing inputs."""
+    from flashdiffusion_b200.attention import attend, attend_cached
+    sets = [_inputs(1, s, s, 4, 2, 128, dtype, seed=s) for s in (130, 390)]
+    n = torch.tensor([100], dtype=torch.int32, device="cuda")
+
+    def step(q, k, v, do):
+        a, b, c = (t.detach().requires_grad_(True) for t in (q, k, v))
+        o = attend(a, b, c, causal=True, cap=30.0)
+        return (o.detach(), attend_cached(q[:, -1:], k, v, n), *torch.autograd.grad(o, (a, b, c), do))
+
+    want = [[step(*s), step(*(t.flip(1) for t in s))] for s in sets]
+    ins = [[t.clone() for t in s] for s in sets]
+    pool, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for x in ins:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(step(*x))
+        graphs.append(g)
+    for turn in (0, 1, 0):
+        for i in (0, 1):
+            for t, x in zip(ins[i], sets[i]):
+                t.copy_(x.flip(1) if turn else x)
+            graphs[i].replay()
+            assert all(torch.equal(x, y) for x, y in zip(outs[i], want[i][turn]))
+
+
+@pytest.mark.filterwarnings("ignore:The AccumulateGrad node's stream")
+@pytest.mark.parametrize("dtype", [BF, SF], ids=str)
+def test_captured_while_a_warm_up_graph_of_the_same_leaves_lives(dtype):
+    """The warm-up ran on a side stream, as the documentation of capture asks, and its output is still referenced."""
+    from flashdiffusion_b200.attention import attend
+    q, k, v, do = _inputs(1, 200, 200, 4, 2, 128, dtype, seed=59)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = attend(*leaves, causal=True)
+        warm.backward(do)
+    torch.cuda.current_stream().wait_stream(side)
+    want = [t.grad.clone() for t in leaves]
+    for t in leaves:
+        t.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(*leaves, causal=True).backward(do)
+    graph.replay()
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    del warm
+
+
+def test_what_the_gradients_read_again_is_watched():
+    """Spans, slopes and heads changed in place between the passes are refused, not used."""
+    from flashdiffusion_b200.attention import Spans, attend
+    q, k, v, do = _inputs(1, 20, 20, 2, 1, 64, BF)
+    first, end = torch.zeros(20, dtype=torch.int32, device="cuda"), torch.full((20,), 20, dtype=torch.int32, device="cuda")
+    slopes = torch.ones(2, device="cuda")
+    for change in (lambda: end.fill_(3), lambda: slopes.zero_(), lambda: k.zero_()):
+        o = attend(q.requires_grad_(True), k, v, spans=Spans(first, end), slopes=slopes)
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            o.backward(do)
+
+
+def test_the_low_bits_of_the_output_serve_the_gradients():
+    """Rows that cancel: dq of one query that looks at two keys whose values differ little.  dS = P (dP - delta) is then
+    the small difference of large numbers; with delta from o rounded to bf16 it would be off by 2^-9 |dO . o|, with
+    eight more bits by 2^-17 of it."""
+    from flashdiffusion_b200.attention import attend
+    d = 64
+    q, k = (torch.randn(1, n, 1, d, device="cuda", generator=torch.Generator("cuda").manual_seed(57)).to(BF) for n in (1, 2))
+    v = torch.ones(1, 2, 1, d, device="cuda", dtype=BF)
+    v[0, 1] += 2.0 ** -6
+    do = torch.ones(1, 1, 1, d, device="cuda", dtype=BF)
+    lo, hi, pos = spans_of(1, 2, 1)
+    ref = reference(q, k, v, lo, hi, pos, do=do)
+    dq, = torch.autograd.grad(attend(q.requires_grad_(True), k, v), q, do)
+    p = 0.25                                               # the largest p (1 - p)
+    # ds = scale p0 p1 64 2^-6 <= p / 8; error of delta: 64 (2^-17 for the kept bits, 2^-20 for fp32 steps), of P: 2^-16
+    ds_tol = d ** -0.5 * (2 * p * 64 * (2.0 ** -17 + 2.0 ** -20) + p * 2.0 ** -15) + 2.0 ** -8 * d ** -0.5 * p
+    room = 2.0 ** -8 * ref["dq"].abs() + ds_tol * k.double().cpu().abs().sum(1, keepdim=True)
+    assert ((dq.double().cpu() - ref["dq"]).abs() <= room).all()
+
+
 def test_a_prompt_its_training_step_and_its_answers():
     """The operators together: rotate, attend over a packed prompt, gradients to the unrotated heads; then token by
     token against the cache, where each answer equals the prompt's row within both calls' rounding."""
