@@ -121,8 +121,10 @@ extern "C" {
 size_t fd_attention_workspace_bytes(const fd_attention_args* r, int backward) {
     if (!r || r->batch < 0 || r->q_len < 0 || r->k_len < 0 || r->heads < 1) return 0;
     if (backward) return std::max(attn::delta_bytes(r), attn::tc_backward_bytes(r->batch, r->heads, r->q_len));
-    const bool few = r->kv_heads > 0 && (int64_t)(r->heads / r->kv_heads) * r->q_len <= attn::MAX_ROWS;
-    return few && r->dtype != FD_DTYPE_F32 && r->dim <= 128 ? align256(attn::rows_bytes(r->dim)) : 0;
+    if (r->dtype == FD_DTYPE_F32 || r->dim < 1 || r->dim > 128 || r->kv_heads < 1) return 0;
+    const bool few = (int64_t)(r->heads / r->kv_heads) * r->q_len <= attn::MAX_ROWS;
+    return few ? align256(attn::rows_bytes(r->dim))
+               : attn::tc_forward_bytes(r->batch, r->heads, r->q_len, r->k_len, r->window, r->dim);
 }
 
 int fd_attention_forward(const fd_attention_args* r, void* workspace, size_t workspace_bytes, void* stream) {
@@ -136,7 +138,7 @@ int fd_attention_forward(const fd_attention_args* r, void* workspace, size_t wor
                  "fd_attention_forward: workspace must be 256-byte aligned");
     const bool tc = attn::tc_applies(a, r->dtype, false);
     if (tc && attn::rows_applies(a)) return attn::rows_forward(a, r->dtype, workspace, (cudaStream_t)stream);
-    if (tc) return attn::tc_forward(a, r->dtype, (cudaStream_t)stream);
+    if (tc) return attn::tc_forward(a, r->dtype, workspace, (cudaStream_t)stream);
     return attn::simt_forward(a, r->dtype, (cudaStream_t)stream);
 }
 

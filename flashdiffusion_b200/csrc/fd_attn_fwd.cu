@@ -19,6 +19,8 @@
 // each, and exchange their maxima through shared memory: with one thread a row
 // (8 warps) the SM issued an instruction in 0.35 of its cycles, two warps a
 // scheduler being too few for the latencies of TMEM, MUFU and FMA chains.
+#include <algorithm>
+
 #include "fd_attn_tc.cuh"
 
 namespace fd {
@@ -58,11 +60,18 @@ struct Misc {
     int flo[2], fhi[2];  // keys seen by every row: [flo, fhi)
 };
 
+// Keys cut into parts (parts > 1): each CTA leaves its normalised rows and their lse2 for join_kernel.
+struct Split {
+    int parts;
+    float* o;        // [part][batch][query][head][dim]
+    float* lse2;     // [part][batch][query][head], base 2
+};
+
 template <int DP, bool F16, bool GEN>
 __global__ void __launch_bounds__(NTHREADS, 1)
 forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
-               const __grid_constant__ CUtensorMap tmv, const __grid_constant__ Prob a, int n_qt,
-               int* __restrict__ status) {
+               const __grid_constant__ CUtensorMap tmv, const __grid_constant__ Prob a, const __grid_constant__ Split sp,
+               int n_qt, int* __restrict__ status) {
     using C = Cfg<DP>;
     constexpr float P_SHIFT = F16 ? 7.f : 0.f;
     extern __shared__ __align__(1024) uint8_t base[];
@@ -86,8 +95,8 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // later query tiles see more keys under a causal mask: they start first
     const int nh = a.heads * a.batch;
-    const int qt = n_qt - 1 - blockIdx.x / nh;
-    const int bh = blockIdx.x % nh;
+    const int qt = n_qt - 1 - blockIdx.x / (nh * sp.parts);
+    const int part = blockIdx.x / nh % sp.parts, bh = blockIdx.x % nh;
     const int b = bh / a.heads, h = bh - b * a.heads, hk = h / a.group;
     const int q0 = qt * 2 * T;
     const int n = keys_of(a, b);
@@ -155,8 +164,19 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         tb[s] = some ? (ms.hi[s] + T - 1) / T : 0;
     }
     // tiles of either subtile; an empty subtile takes no part
-    const int t0 = tb[0] == 0 ? ta[1] : tb[1] == 0 ? ta[0] : min(ta[0], ta[1]);
-    const int t1 = max(tb[0], tb[1]);
+    int t0 = tb[0] == 0 ? ta[1] : tb[1] == 0 ? ta[0] : min(ta[0], ta[1]);
+    int t1 = max(tb[0], tb[1]);
+    if (sp.parts > 1) {
+        const int n = t1 - t0, from = t0 + n * part / sp.parts, to = t0 + n * (part + 1) / sp.parts;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            ta[s] = max(ta[s], from);
+            tb[s] = min(tb[s], to);
+            if (ta[s] >= tb[s]) ta[s] = tb[s] = 0;
+        }
+        t0 = tb[0] == 0 ? ta[1] : tb[1] == 0 ? ta[0] : min(ta[0], ta[1]);
+        t1 = max(tb[0], tb[1]);
+    }
     auto active = [&](int s, int j) { return j >= ta[s] && j < tb[s]; };
     // some row of an active subtile sees only a part of tile j
     auto partial = [&](int j) {
@@ -446,7 +466,12 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                     }
                 }
             }
-            if (real) {
+            if (real && sp.parts > 1) {
+                float* to = sp.o + ((((int64_t)part * a.batch + b) * a.q_len + row) * a.heads + h) * a.dim + c0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c0 + i * 4 < a.dim) *(float4*)(to + 4 * i) = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+            } else if (real) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (c0 + i * 8 >= a.dim) continue;
@@ -454,8 +479,11 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                 }
             }
         }
-        if (half == 0 && real && a.lse)
-            a.lse[((int64_t)b * a.heads + h) * a.q_len + row] = l == 0.f ? -INFINITY : (m * c + (log2f(l) - P_SHIFT)) * LN2;
+        if (half == 0 && real) {
+            const float lse2 = l == 0.f ? -INFINITY : m * c + (log2f(l) - P_SHIFT);
+            if (sp.parts > 1) sp.lse2[(((int64_t)part * a.batch + b) * a.q_len + row) * a.heads + h] = lse2;
+            else if (a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + row] = lse2 * LN2;
+        }
         ptx::tc_fence_before();
     }
     __syncthreads();
@@ -465,8 +493,40 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     }
 }
 
+// The parts of a row, in order: o = sum_p 2^(lse2_p - lse2) o_p.  Thread: eight coordinates.
+template <bool F16>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob a, const __grid_constant__ Split sp) {
+    const int pieces = a.dim / 8;
+    const int64_t rows = (int64_t)a.batch * a.q_len * a.heads, x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (x >= rows * pieces) return;
+    const int64_t r = x / pieces;
+    const int d = (int)(x - r * pieces) * 8;
+    float m = -INFINITY;
+    for (int p = 0; p < sp.parts; ++p) m = fmaxf(m, sp.lse2[p * rows + r]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float sum = 0.f, acc[8] = {};
+#pragma unroll 4
+    for (int p = 0; p < sp.parts; ++p) {
+        const float w = exp2f(sp.lse2[p * rows + r] - base);
+        const float* o = sp.o + (p * rows + r) * a.dim + d;
+        const float4 u = *(const float4*)o, v = *(const float4*)(o + 4);
+        const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        sum += w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, f[e], acc[e]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= inv;
+    const int64_t t = r / a.heads, b = t / a.q_len, row = t - b * a.q_len;
+    const int h = (int)(r - t * a.heads);
+    store8<F16>((uint16_t*)a.o.p + b * a.o.sb + row * a.o.ss + h * a.o.sh + d, a.o_low ? a.o_low + r * a.dim + d : nullptr, acc);
+    if (d == 0 && a.lse)
+        a.lse[(b * a.heads + h) * a.q_len + row] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * LN2;
+}
+
 template <int DP, bool F16, bool GEN>
-int launch(const Prob& a, cudaStream_t s) {
+int launch(const Prob& a, const Split& sp, cudaStream_t s) {
     CUtensorMap q, k, v;
     FD_TRY(make_head_map(&q, a.q, a.q_len, a.heads, a.batch, a.dim, F16));
     FD_TRY(make_head_map(&k, a.k, a.k_len, a.kv_heads, a.batch, a.dim, F16));
@@ -475,19 +535,24 @@ int launch(const Prob& a, cudaStream_t s) {
     FD_TRY(status_word(&status));
     FD_TRY((allow_smem<forward_kernel<DP, F16, GEN>>(Cfg<DP>::SMEM)));
     const int n_qt = (int)cdiv(a.q_len, 2 * T);
-    const int64_t blocks = (int64_t)n_qt * a.heads * a.batch;
+    const int64_t blocks = (int64_t)n_qt * a.heads * a.batch * sp.parts;
     FD_CHECK_ARG(blocks <= 0x7fffffff, "fd_attention: too many query tiles");
-    forward_kernel<DP, F16, GEN><<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, a, n_qt, status);
+    forward_kernel<DP, F16, GEN><<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, a, sp, n_qt, status);
     FD_CUDA_TRY(cudaGetLastError());
+    if (sp.parts > 1) {
+        const int64_t threads = (int64_t)a.batch * a.q_len * a.heads * (a.dim / 8);
+        join_kernel<F16><<<(unsigned)cdiv(threads, 256), 256, 0, s>>>(a, sp);
+        FD_CUDA_TRY(cudaGetLastError());
+    }
     return FD_OK;
 }
 
 template <int DP>
-int by_type(const Prob& a, int dtype, cudaStream_t s) {
+int by_type(const Prob& a, int dtype, const Split& sp, cudaStream_t s) {
     // the plain kernel keeps raw scores and needs them to grow with the products
     const bool gen = a.cap > 0.f || a.slopes || !(a.scale > 0.f);
-    if (dtype == FD_DTYPE_F16) return gen ? launch<DP, true, true>(a, s) : launch<DP, true, false>(a, s);
-    return gen ? launch<DP, false, true>(a, s) : launch<DP, false, false>(a, s);
+    if (dtype == FD_DTYPE_F16) return gen ? launch<DP, true, true>(a, sp, s) : launch<DP, true, false>(a, sp, s);
+    return gen ? launch<DP, false, true>(a, sp, s) : launch<DP, false, false>(a, sp, s);
 }
 
 }  // namespace fwd
@@ -516,8 +581,27 @@ bool tc_applies(const Prob& a, int dtype, bool backward) {
     return tma_view(a.d_o, qe) && tma_view(a.dq, qe) && tma_view(a.dk, ke) && tma_view(a.dv, ke);
 }
 
-int tc_forward(const Prob& a, int dtype, cudaStream_t s) {
-    return a.dim <= 64 ? fwd::by_type<64>(a, dtype, s) : fwd::by_type<128>(a, dtype, s);
+// Parts of the key axis for each query tile: as many as the SMs hold, none with fewer than four key tiles, which cost
+// about what a part's start, its fp32 rows and the join do (8 / 2 bf16 heads of 128, 512 causal rows: against 16384
+// keys 267 us whole, 59 us in 9 parts; against 4096 keys 79 and 35 us; two heads of 128 rows against 640 keys are as
+// fast whole, 20.5 us, as in two parts).
+static int split_parts(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window) {
+    const int64_t ctas = cdiv(q_len, 2 * T) * heads * batch;
+    const int64_t keys = window > 0 ? std::min(k_len, window + 2 * T) : k_len;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(num_sms() / std::max<int64_t>(ctas, 1), cdiv(keys, T) / 4));
+}
+
+size_t tc_forward_bytes(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window, int64_t dim) {
+    const int64_t parts = split_parts(batch, heads, q_len, k_len, window);
+    return parts > 1 ? align256(sizeof(float) * parts * batch * q_len * heads * (dim + 1)) : 0;
+}
+
+int tc_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
+    fwd::Split sp{};
+    sp.parts = split_parts(a.batch, a.heads, a.q_len, a.k_len, a.window);
+    sp.o = (float*)workspace;
+    sp.lse2 = sp.o + (int64_t)sp.parts * a.batch * a.q_len * a.heads * a.dim;
+    return a.dim <= 64 ? fwd::by_type<64>(a, dtype, sp, s) : fwd::by_type<128>(a, dtype, sp, s);
 }
 
 }  // namespace attn

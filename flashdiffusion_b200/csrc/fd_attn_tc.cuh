@@ -324,7 +324,8 @@ __device__ __forceinline__ void store8(void* out, int8_t* low, const float* f) {
 
 // Launchers of the tensor-core kernels.
 bool tc_applies(const Prob& a, int dtype, bool backward);
-int tc_forward(const Prob& a, int dtype, cudaStream_t s);
+size_t tc_forward_bytes(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window, int64_t dim);
+int tc_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
 // Few rows against many keys (fd_attn_rows.cu), where tc_applies: up to MAX_ROWS query rows per key head; above,
 // the 128-row tcgen05 tiles are full enough.
 constexpr int MAX_ROWS = 64;
