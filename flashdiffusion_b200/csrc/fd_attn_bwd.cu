@@ -9,7 +9,9 @@
 // by another over its key tiles: seven products in the place of five, but every
 // sum has one owner and a fixed order (the same bits at every call), and no
 // fp32 gradient passes through memory.  Both kinds of CTA are one launch, the
-// longest first, so that the short ones fill the SMs at its end.
+// longest first, so that the short ones fill the SMs at its end.  Where there are
+// too few for that (few key heads, few query rows), a CTA's tiles are shared
+// between several, whose fp32 sums sum_kernel adds up in their order.
 //
 // CTA: two compute warpgroups that share the 128 rows of the accumulators (64
 // columns of each score tile apiece), and a warpgroup with a TMA producer, an
@@ -20,7 +22,9 @@
 //               dP(i + 1) while P(i + 1) is.
 //   query side  rows = queries.  TMEM: S | dP, dP | dQ (dP in two buffers, so that
 //               the next tile's products do not wait for dS).
+#include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "fd_attn_tc.cuh"
 
@@ -49,9 +53,38 @@ struct Work {
     int2* spans;         // [batch][rows padded to 128]
     Bounds* bounds;      // [batch][query tiles]
     unsigned* top;       // fp16: bits of the largest |dO row|^2 and |V row|^2
+    float *dq, *dk, *dv; // fp32 sums of each part, [part][batch][row][head][dim], where there are parts
 };
 
-__host__ __device__ inline size_t work_layout(Work* w, void* base, int64_t bh, int64_t batch, int64_t n_qt) {
+// What the sizes of a call say about its work.
+struct Shape {
+    int64_t batch, heads, kv_heads, q_len, k_len, dim, window;
+    bool causal;
+    int key_parts() const { return parts(tiles(q_len, k_len) * (heads / kv_heads)); }
+    int query_parts() const { return parts(tiles(k_len, q_len)); }
+    // tiles of one side that a tile of the other sees
+    int64_t tiles(int64_t of, int64_t by) const {
+        return window > 0 ? std::min(cdiv(of, T), window / T + 2) : cdiv(of, T);
+    }
+    // the share of score tiles that hold a visible pair
+    double visible() const {
+        if (window > 0) return (window / T + 1.0) / (window / T + 2.0);
+        return !causal ? 1.0 : q_len <= k_len ? 1.0 - 0.5 * q_len / k_len : 0.5 * k_len / q_len;
+    }
+    // A CTA of `items` score tiles is cut where it would outlast an SM's equal share of them all by more than a third,
+    // but into parts of no fewer than MIN_ITEMS, which cost about what a part's start, its fp32 rows and their join do.
+    // Whole and cut, causal, bf16: 7900 rows of 4 / 1 heads of 64 348 and 156 us; 1000 rows of 4 / 1 heads of 128 70 and
+    // 37 us; 512 rows of 8 / 2 heads against 16384 keys 178 and 119 us; 1000 rows of 4 / 4 heads, not cut, 29 us, 33 us
+    // in parts of four.
+    int parts(int64_t items) const {
+        const double share = 2 * visible() * cdiv(q_len, T) * heads * batch * tiles(k_len, q_len) / num_sms();
+        return (int)std::min(std::max(std::ceil(items / std::max(share, (double)MIN_ITEMS) - 0.35), 1.0), 64.0);
+    }
+    static constexpr int MIN_ITEMS = 8;
+};
+
+inline size_t work_layout(Work* w, void* base, const Shape& z) {
+    const int64_t bh = z.batch * z.heads, batch = z.batch, n_qt = cdiv(z.q_len, T);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -63,7 +96,11 @@ __host__ __device__ inline size_t work_layout(Work* w, void* base, int64_t bh, i
     char* c = take(sizeof(int2) * batch * n_qt * T);
     char* d = take(sizeof(Bounds) * batch * n_qt);
     char* e = take(2 * sizeof(unsigned));
-    if (w) *w = {(float*)a, (float*)b, (int2*)c, (Bounds*)d, (unsigned*)e};
+    auto sums = [&](int parts, int64_t rows) { return parts > 1 ? sizeof(float) * parts * batch * rows * z.dim : 0; };
+    char* f = take(sums(z.query_parts(), z.q_len * z.heads));
+    char* g = take(sums(z.key_parts(), z.k_len * z.kv_heads));
+    char* h = take(sums(z.key_parts(), z.k_len * z.kv_heads));
+    if (w) *w = {(float*)a, (float*)b, (int2*)c, (Bounds*)d, (unsigned*)e, (float*)f, (float*)g, (float*)h};
     return at;
 }
 
@@ -200,12 +237,15 @@ struct Misc {
 struct Args {
     Prob a;
     Work w;
-    int n_qt, n_key;   // query tiles, CTAs of the key side
+    int n_qt;                   // query tiles
+    int first, keys_first;      // CTAs of the side that starts first: the one with the longer CTAs
+    int key_parts, query_parts; // CTAs that share a key tile's, a query tile's items
 };
 
-// Store N columns of one accumulator row, times f, as 16-bit values behind column c0 of `out`.
+// Store N columns of one accumulator row, times f, behind column c0: as 16-bit values of `out`, or as fp32 of `sums`.
 template <int N, bool F16>
-__device__ __forceinline__ void store_cols(uint32_t taddr, float f, uint8_t* out, int c0, int dim, bool live, bool have) {
+__device__ __forceinline__ void store_cols(uint32_t taddr, float f, uint8_t* out, float* sums, int c0, int dim, bool live,
+                                           bool have) {
 #pragma unroll 1
     for (int g = 0; g < N; g += 32) {
         uint32_t o[32];
@@ -217,6 +257,15 @@ __device__ __forceinline__ void store_cols(uint32_t taddr, float f, uint8_t* out
             for (int i = 0; i < 32; ++i) o[i] = 0;
         }
         if (!live) continue;
+        if (sums) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+                if (c0 + g + i < dim)
+                    *(float4*)(sums + c0 + g + i) =
+                        make_float4(__uint_as_float(o[i]) * f, __uint_as_float(o[i + 1]) * f, __uint_as_float(o[i + 2]) * f,
+                                    __uint_as_float(o[i + 3]) * f);
+            continue;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (c0 + g + i * 8 >= dim) continue;
@@ -236,7 +285,8 @@ struct Cta {
     bool key_side;
     int tile, b, h;        // h: key head on the key side, query head on the query side
     int r0, n, n_qt;       // first row of this CTA, keys in use, query tiles
-    int t0, nt, items;     // the other side's tiles t0 .. t0 + nt, walked items / nt times (once for each head of the group)
+    int t0, nt;            // the other side's tiles t0 .. t0 + nt, walked once for each head of the group on the key side
+    int skip, items;       // this CTA's items of that walk
     Bounds own;            // query side: this tile's bounds
     const Bounds* bounds;
 };
@@ -244,7 +294,12 @@ struct Cta {
 // Item i of a CTA: its tile, and the query head on the key side.
 struct Item {
     int i, t, head;
-    __device__ explicit Item(const Cta& c) : i(0), t(c.t0), head(c.key_side ? c.h * c.a.group : c.h) {}
+    __device__ explicit Item(const Cta& c) : i(0), t(c.t0 + c.skip), head(c.key_side ? c.h * c.a.group : c.h) {
+        if (c.skip >= c.nt && c.nt > 0) {
+            t = c.t0 + c.skip % c.nt;
+            head += c.skip / c.nt;
+        }
+    }
     __device__ void next(const Cta& c) {
         ++i;
         if (++t == c.t0 + c.nt) {
@@ -557,6 +612,11 @@ __device__ __forceinline__ bool compute_key(const Cta& c, const Bars& br, const 
             round32<F16>(x[g], p);
             ptx::tmem_st16(lanes + half * 64 + g * 16, p);
             if (GEN && sc.capped) {
+                if (masked) {   // a masked pair's bend may be a NaN
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        bend[e] = ptx::pack2(ptx::lo2(x[g][e]) == 0.f ? 0.f : ptx::lo2(bend[e]), ptx::hi2(x[g][e]) == 0.f ? 0.f : ptx::hi2(bend[e]));
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
             }
@@ -645,14 +705,14 @@ __device__ __forceinline__ bool compute_query(const Cta& c, const Bars& br, uint
         for (int g = 0; g < 2; ++g) {
             uint64_t bend[GEN ? 16 : 1];
             weights32<GEN>(x[g], add, sc, slope2, (float)(shift + row - k0 - g * 32), -1.f, side, bend);
+            if (GEN && sc.capped) {   // before the mask: a masked pair's bend may be a NaN
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
+            }
             if (masked) {
                 const int lo = span.x - k0 - g * 32;
                 if (!__all_sync(~0u, lo <= 0 && (int64_t)lo + (span.y - span.x) >= 32))
                     mask32(x[g], lo, (uint32_t)(span.y - span.x), 0.f);
-            }
-            if (GEN && sc.capped) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
             }
         }
         const uint32_t dp = lanes + 128 + buf * 128 + half * 64;
@@ -690,9 +750,10 @@ __device__ __forceinline__ bool compute_query(const Cta& c, const Bars& br, uint
     return true;
 }
 
-// dV row `out`: the NaN and infinite dO elements that the guard took out, of the queries that see this key.
+// dV row `out` (or this part's `sums`): the NaN and infinite dO elements that the guard took out, of the queries that
+// see this key.
 template <bool F16>
-__device__ void put_back(const Cta& c, uint8_t* out, int row) {
+__device__ void put_back(const Cta& c, uint8_t* out, float* sums, int row) {
     const Prob& a = c.a;
     for (Item it(c); it.i < c.items; it.next(c)) {
         if (!it.partial(c)) continue;
@@ -704,6 +765,10 @@ __device__ void put_back(const Cta& c, uint8_t* out, int row) {
             constexpr uint16_t EXP = F16 ? 0x7c00 : 0x7f80;
             for (int d = 0; d < a.dim; ++d)
                 if ((g[d] & EXP) == EXP) {
+                    if (sums) {
+                        sums[d] += pair_of<F16>(g[d]).x;
+                        continue;
+                    }
                     uint16_t* o = (uint16_t*)out + d;
                     const float2 f = pair_of<F16>((uint32_t)*o | ((uint32_t)g[d] << 16));
                     *o = (uint16_t)ptx::pack16<F16>(f.x + f.y, 0.f);
@@ -744,18 +809,24 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Cta c{a, w};
-    c.key_side = (int)blockIdx.x < args.n_key;
+    int parts, part;
+    const int x = (int)blockIdx.x < args.first ? blockIdx.x : blockIdx.x - args.first;
+    c.key_side = ((int)blockIdx.x < args.first) == (args.keys_first != 0);
     if (c.key_side) {
         // earlier key tiles are seen by more queries under a causal mask: they start first
         const int nh = a.kv_heads * a.batch;
-        c.tile = blockIdx.x / nh;
-        c.b = blockIdx.x % nh / a.kv_heads;
-        c.h = blockIdx.x % nh % a.kv_heads;
+        parts = args.key_parts;
+        part = x / nh % parts;
+        c.tile = x / (nh * parts);
+        c.b = x % nh / a.kv_heads;
+        c.h = x % nh % a.kv_heads;
     } else {
-        const int nh = a.heads * a.batch, u = blockIdx.x - args.n_key;
-        c.tile = args.n_qt - 1 - u / nh;
-        c.b = u % nh / a.heads;
-        c.h = u % nh % a.heads;
+        const int nh = a.heads * a.batch;
+        parts = args.query_parts;
+        part = x / nh % parts;
+        c.tile = args.n_qt - 1 - x / (nh * parts);
+        c.b = x % nh / a.heads;
+        c.h = x % nh % a.heads;
     }
     c.r0 = c.tile * T;
     c.n = keys_of(a, c.b);
@@ -813,6 +884,11 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         c.nt = c.own.hi > c.own.lo ? (c.own.hi + T - 1) / T - c.t0 : 0;
     }
     c.items = c.key_side ? c.nt * a.group : c.nt;
+    c.skip = 0;
+    if (parts > 1) {
+        c.skip = (int)((int64_t)c.items * part / parts);
+        c.items = (int)((int64_t)c.items * (part + 1) / parts) - c.skip;
+    }
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
@@ -842,16 +918,22 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         const bool have = c.items > 0 && ok && ptx::wait_bounded(br.accfull, 0, abort, status, WAIT_NS);
         ptx::tc_fence_after();
         const float back = a.scale / up;
+        // this row's sums of this part, if there are parts
+        auto sums = [&](float* to, int rows, int heads) {
+            return parts > 1 ? to + ((((int64_t)part * a.batch + c.b) * rows + row) * heads + c.h) * a.dim : nullptr;
+        };
         if (!c.key_side) {
             uint8_t* out = (uint8_t*)a.dq.p + 2 * (c.b * a.dq.sb + (int64_t)row * a.dq.ss + c.h * a.dq.sh);
-            store_cols<DP / 2, F16>(lanes + 384 + half * (DP / 2), back, out, half * (DP / 2), a.dim, row < a.q_len, have);
+            store_cols<DP / 2, F16>(lanes + 384 + half * (DP / 2), back, out, sums(w.dq, a.q_len, a.heads), half * (DP / 2),
+                                    a.dim, row < a.q_len, have);
         } else if (half == 0) {
             uint8_t* out = (uint8_t*)a.dv.p + 2 * (c.b * a.dv.sb + (int64_t)row * a.dv.ss + c.h * a.dv.sh);
-            store_cols<DP, F16>(lanes + 256, p_back, out, 0, a.dim, row < a.k_len, have);
-            if (have && row < a.k_len && *(volatile int*)&ms.poison) put_back<F16>(c, out, row);
+            float* to = sums(w.dv, a.k_len, a.kv_heads);
+            store_cols<DP, F16>(lanes + 256, p_back, out, to, 0, a.dim, row < a.k_len, have);
+            if (have && row < a.k_len && *(volatile int*)&ms.poison) put_back<F16>(c, out, to, row);
         } else {
             uint8_t* out = (uint8_t*)a.dk.p + 2 * (c.b * a.dk.sb + (int64_t)row * a.dk.ss + c.h * a.dk.sh);
-            store_cols<DP, F16>(lanes + 384, back, out, 0, a.dim, row < a.k_len, have);
+            store_cols<DP, F16>(lanes + 384, back, out, sums(w.dk, a.k_len, a.kv_heads), 0, a.dim, row < a.k_len, have);
         }
         ptx::tc_fence_before();
     }
@@ -862,8 +944,44 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
     }
 }
 
+// One gradient's parts, in order.
+struct Sums {
+    const float* parts;
+    View out;
+    int n, rows, heads;
+};
+
+// Thread: eight coordinates of a row of dq, dk or dv.
+template <bool F16>
+__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ Sums dq, const __grid_constant__ Sums dk,
+                                                  const __grid_constant__ Sums dv, int batch, int dim) {
+    int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int pieces = dim / 8;
+    for (int g = 0; g < 3; ++g) {
+        const Sums& z = g == 0 ? dq : g == 1 ? dk : dv;
+        const int64_t rows = z.n > 1 ? (int64_t)batch * z.rows * z.heads : 0;
+        if (x >= rows * pieces) {
+            x -= rows * pieces;
+            continue;
+        }
+        const int64_t r = x / pieces, t = r / z.heads, b = t / z.rows;
+        const int d = (int)(x - r * pieces) * 8, h = (int)(r - t * z.heads);
+        float f[8] = {};
+#pragma unroll 4
+        for (int p = 0; p < z.n; ++p) {
+            const float* o = z.parts + (p * rows + r) * dim + d;
+            const float4 u = *(const float4*)o, v = *(const float4*)(o + 4);
+            const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] += e[i];
+        }
+        store8<F16>((uint16_t*)z.out.p + b * z.out.sb + (t - b * z.rows) * z.out.ss + h * z.out.sh + d, nullptr, f);
+        return;
+    }
+}
+
 template <int DP, bool F16, bool GEN>
-int launch(const Prob& a, const Work& w, cudaStream_t s) {
+int launch(const Prob& a, const Work& w, const Shape& z, cudaStream_t s) {
     CUtensorMap q, k, v, g;
     FD_TRY(make_head_map(&q, a.q, a.q_len, a.heads, a.batch, a.dim, F16));
     FD_TRY(make_head_map(&k, a.k, a.k_len, a.kv_heads, a.batch, a.dim, F16));
@@ -876,10 +994,13 @@ int launch(const Prob& a, const Work& w, cudaStream_t s) {
     args.w = w;
     args.n_qt = (int)cdiv(a.q_len, T);
     const int n_kt = (int)cdiv(a.k_len, T);
-    const int64_t keys = (int64_t)n_kt * a.kv_heads * a.batch;
-    const int64_t blocks = keys + (int64_t)args.n_qt * a.heads * a.batch;
+    args.key_parts = z.key_parts();
+    args.query_parts = z.query_parts();
+    const int64_t keys = (int64_t)n_kt * a.kv_heads * a.batch * args.key_parts;
+    const int64_t queries = (int64_t)args.n_qt * a.heads * a.batch * args.query_parts, blocks = keys + queries;
+    args.keys_first = z.tiles(a.q_len, a.k_len) * a.group * args.query_parts >= z.tiles(a.k_len, a.q_len) * args.key_parts;
     FD_CHECK_ARG(blocks <= 0x7fffffff && cdiv(a.q_len, T) + cdiv(a.k_len, T) <= 0x7fffffff, "fd_attention: too many tiles");
-    args.n_key = (int)keys;
+    args.first = (int)(args.keys_first ? keys : queries);
     const int v_blocks = F16 ? n_kt : 0;
     if (F16) FD_CUDA_TRY(cudaMemsetAsync(w.top, 0, 2 * sizeof(unsigned), s));
     prep_kernel<F16><<<dim3(args.n_qt + v_blocks, a.heads, a.batch), 256, 0, s>>>(a, w, args.n_qt);
@@ -896,27 +1017,36 @@ int launch(const Prob& a, const Work& w, cudaStream_t s) {
     cfg.attrs = &early;
     cfg.numAttrs = 1;
     FD_CUDA_TRY(cudaLaunchKernelEx(&cfg, gradient_kernel<DP, F16, GEN>, q, k, v, g, args, status));
+    const int64_t joined = (args.query_parts > 1 ? (int64_t)a.q_len * a.heads : 0) +
+                           (args.key_parts > 1 ? 2 * (int64_t)a.k_len * a.kv_heads : 0);
+    if (joined > 0) {
+        const Sums dq{w.dq, a.dq, args.query_parts, a.q_len, a.heads}, dk{w.dk, a.dk, args.key_parts, a.k_len, a.kv_heads},
+            dv{w.dv, a.dv, args.key_parts, a.k_len, a.kv_heads};
+        sum_kernel<F16><<<(unsigned)cdiv(joined * a.batch * (a.dim / 8), 256), 256, 0, s>>>(dq, dk, dv, a.batch, a.dim);
+    }
     FD_CUDA_TRY(cudaGetLastError());
     return FD_OK;
 }
 
 template <int DP>
-int by_type(const Prob& a, int dtype, const Work& w, cudaStream_t s) {
+int by_type(const Prob& a, int dtype, const Work& w, const Shape& z, cudaStream_t s) {
     const bool gen = a.cap > 0.f || a.slopes;
-    if (dtype == FD_DTYPE_F16) return gen ? launch<DP, true, true>(a, w, s) : launch<DP, true, false>(a, w, s);
-    return gen ? launch<DP, false, true>(a, w, s) : launch<DP, false, false>(a, w, s);
+    if (dtype == FD_DTYPE_F16) return gen ? launch<DP, true, true>(a, w, z, s) : launch<DP, true, false>(a, w, z, s);
+    return gen ? launch<DP, false, true>(a, w, z, s) : launch<DP, false, false>(a, w, z, s);
 }
 
 }  // namespace bwd
 
-size_t tc_backward_bytes(int64_t batch, int64_t heads, int64_t q_len) {
-    return bwd::work_layout(nullptr, nullptr, batch * heads, batch, cdiv(q_len, T));
+size_t tc_backward_bytes(const fd_attention_args* r) {
+    const bwd::Shape z{r->batch, r->heads, r->kv_heads, r->q_len, r->k_len, r->dim, r->window, r->causal != 0};
+    return bwd::work_layout(nullptr, nullptr, z);
 }
 
 int tc_backward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
+    const bwd::Shape z{a.batch, a.heads, a.kv_heads, a.q_len, a.k_len, a.dim, a.window, a.causal != 0};
     bwd::Work w;
-    bwd::work_layout(&w, workspace, (int64_t)a.batch * a.heads, a.batch, cdiv(a.q_len, T));
-    return a.dim <= 64 ? bwd::by_type<64>(a, dtype, w, s) : bwd::by_type<128>(a, dtype, w, s);
+    bwd::work_layout(&w, workspace, z);
+    return a.dim <= 64 ? bwd::by_type<64>(a, dtype, w, z, s) : bwd::by_type<128>(a, dtype, w, z, s);
 }
 
 }  // namespace attn

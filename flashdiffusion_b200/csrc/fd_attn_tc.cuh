@@ -332,7 +332,7 @@ constexpr int MAX_ROWS = 64;
 bool rows_applies(const Prob& a);
 size_t rows_bytes(int dim);
 int rows_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
-size_t tc_backward_bytes(int64_t batch, int64_t heads, int64_t q_len);
+size_t tc_backward_bytes(const fd_attention_args* r);
 int tc_backward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
 
 }  // namespace attn

@@ -223,6 +223,27 @@ def test_masked_places_hold_anything(dtype, d):
 
 
 @pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (SF, 48)], ids=str)
+def test_masked_places_hold_anything_under_a_cap(dtype, d):
+    """The same with capped scores, whose slope 1 - tanh^2 is a NaN in such places, and a bias."""
+    from flashdiffusion_b200.attention import Spans
+    s = 300
+    q, k, v, do = _inputs(1, s, s, 4, 2, d, dtype, seed=63)
+    first, end = torch.full((s,), 7, dtype=torch.int32), torch.arange(s).clamp(max=250).int()
+    slopes = torch.tensor([0.1, 0.0, 0.01, 0.5], device="cuda")
+    kw = dict(spans=Spans(first.cuda(), end.cuda()), cap=6.0, slopes=slopes)
+    want = _run(q, k, v, do, **kw)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        q2, k2, v2, do2 = (t.clone() for t in (q, k, v, do))
+        for t in (q2, do2):
+            t[:, :8] = bad                                 # rows that see nothing
+        for t in (k2, v2):
+            t[:, :7], t[:, 250:] = bad, bad                # keys that nobody sees
+        got = _run(q2, k2, v2, do2, **kw)
+        for n in got:
+            assert torch.equal(got[n], want[n]), (n, bad)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (SF, 48)], ids=str)
 def test_causal_future_holds_anything(dtype, d):
     """A NaN or infinity in a key or value reaches the rows that see it and no other."""
     s, at = 300, 170
@@ -447,6 +468,50 @@ def test_general_path_tiles(dtype, d):
         do[x, hi[x] <= lo[x]] = float("inf")
     ref = reference(q, k, v, lo, hi, pos, cap=9.0, do=do)
     _compare(_run(q, k, v, do, spans=Spans(lo.cuda(), hi.cuda()), cap=9.0), ref, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (BF, 80)], ids=str)
+@pytest.mark.parametrize("b,sq,sk,h,hk,window", [
+    (1, 300, 3001, 2, 1, None), (2, 130, 1100, 4, 1, 700), (1, 1500, 1500, 4, 1, None), (1, 2100, 140, 1, 1, None),
+    (1, 1400, 1400, 3, 1, 300),
+])
+def test_split_axes(b, sq, sk, h, hk, window, dtype, d):
+    """Few tiles for many SMs: keys (forward, dq) and queries (dk, dv) are cut into parts that are joined."""
+    q, k, v, do = _inputs(b, sq, sk, h, hk, d, dtype, seed=sk)
+    lo, hi, pos = spans_of(sq, sk, b, causal=True, window=window)
+    out = _run(q, k, v, do, causal=True, window=window)
+    _compare(out, reference(q, k, v, lo, hi, pos, do=do), dtype)
+    again = _run(q, k, v, do, causal=True, window=window)
+    assert all(torch.equal(out[n], again[n]) for n in out)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+def test_split_axes_with_anything_in_masked_places(dtype):
+    from flashdiffusion_b200.attention import Spans
+    b, sq, sk, h, hk, d = 1, 700, 2500, 3, 1, 128
+    q, k, v, do = _inputs(b, sq, sk, h, hk, d, dtype, seed=61)
+    g = torch.Generator().manual_seed(61)
+    lo = torch.randint(5, 1500, (b, sq), generator=g).int()
+    hi = (lo + torch.randint(0, 900, (b, sq), generator=g) * torch.randint(0, 2, (b, sq), generator=g)).int()
+    hi = hi.clamp(max=2390)
+    empty = hi[0] <= lo[0]
+    for t in (k, v):
+        t[0, :5], t[0, 2390:] = float("inf"), float("nan")
+    q[0, empty], do[0, empty] = float("nan"), float("inf")
+    pos = spans_of(sq, sk, b)[2]
+    slopes = torch.tensor([0.001, 0.0, 0.01], device="cuda")
+    kw = dict(spans=Spans(lo.cuda(), hi.cuda()), cap=8.0, slopes=slopes)
+    _compare(_run(q, k, v, do, **kw), reference(q, k, v, lo, hi, pos, cap=8.0, slopes=slopes, do=do), dtype)
+    # a visible infinity of dO reaches dV of the keys that its row sees, and no other's
+    clean = _run(q, k, v, do, **kw)
+    i = int((hi[0] - lo[0]).argmax())
+    do2 = do.clone()
+    do2[0, i, 1, 7] = float("inf")
+    got = _run(q, k, v, do2, **kw)["dv"]
+    inside = torch.zeros(sk, dtype=torch.bool, device="cuda")
+    inside[lo[0, i]:hi[0, i]] = True
+    assert not torch.isfinite(got[0, inside, 0, 7]).any()
+    assert torch.equal(got[0, ~inside], clean["dv"][0, ~inside])
 
 
 @pytest.mark.parametrize("dtype,d", [(BF, 64), (SF, 16)], ids=str)
