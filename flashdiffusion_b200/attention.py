@@ -141,7 +141,7 @@ _NO_GRADIENTS = (0,) * 16
 
 
 def _arguments(q, k, v, o, lse, low, how, gradients=_NO_GRADIENTS) -> bytes:
-    """fd_attention_args, packed."""
+    """fd_attention_args, packed; lse and low are addresses, 0 for none."""
     spans, causal, window, lengths, slopes, scale, cap = how
     b, sq, h, d = q.shape
     if spans is None:
@@ -150,7 +150,7 @@ def _arguments(q, k, v, o, lse, low, how, gradients=_NO_GRADIENTS) -> bytes:
         first, end, step = spans.first.data_ptr(), spans.end.data_ptr(), sq if spans.batch > 1 else 0
     return native.PACK_ATTENTION(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], o.data_ptr(),
-        *o.stride()[:3], 0 if lse is None else lse.data_ptr(), 0 if low is None else low.data_ptr(), first, end, step,
+        *o.stride()[:3], lse or 0, low or 0, first, end, step,
         0 if lengths is None else lengths.data_ptr(), 0 if slopes is None else slopes.data_ptr(), scale, cap,
         _DTYPES[q.dtype], causal, window, b, sq, k.shape[1], h, k.shape[2], d, *gradients)
 
@@ -162,27 +162,42 @@ def _call(fn, args, backward, q):
     native.call(fn, q.device, args, ws.data_ptr() if nbytes else 0, nbytes)
 
 
-def _forward(q, k, v, how, want_lse, low=None):
+def _forward(q, k, v, how, want_lse):
     """(output, lse or None) of heads that are loadable."""
     o = _like(q)
-    lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32) if want_lse else None
-    _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse, low, how), 0, q)
+    lse = _lse_like(q) if want_lse else None
+    _call(native.load().fd_attention_forward, _arguments(q, k, v, o, lse.data_ptr() if want_lse else 0, 0, how), 0, q)
     return o, lse
+
+
+def _lse_like(q):
+    return q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+
+
+def _kept(kept, lse, low_at):
+    """Addresses of lse and of o's low bits (0: none)."""
+    at = kept.data_ptr()
+    return at if lse is None else lse.data_ptr(), 0 if low_at is None else at + low_at
 
 
 class _Attend(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, how, return_lse):
         q, k, v = _loadable(q), _loadable(k), _loadable(v)
-        # 16-bit heads on the tensor cores: eight more bits of o for the backward pass
-        low = (torch.empty(q.shape, dtype=torch.int8, device=q.device)
-               if q.dtype is not torch.float32 and q.shape[-1] % 8 == 0 and q.shape[-1] <= 128 else None)
-        o, lse = _forward(q, k, v, how, True, low)
+        b, sq, h, d = q.shape
+        # one buffer for what the gradients want besides o: lse (unless it is an output), and for 16-bit heads on the
+        # tensor cores eight more bits of o
+        rows = b * sq * h
+        low = rows * d if q.dtype is not torch.float32 and d % 8 == 0 and d <= 128 else 0
+        ctx.low_at = (0 if return_lse else (rows + 1) // 2 * 8) if low else None
+        kept = torch.empty((0 if return_lse else (rows + 1) // 2 * 8) + low, dtype=torch.uint8, device=q.device)
+        o, lse = _like(q), _lse_like(q) if return_lse else None
+        _call(native.load().fd_attention_forward, _arguments(q, k, v, o, *_kept(kept, lse, ctx.low_at), how), 0, q)
         spans, slopes = how[0], how[4]
         if spans is None and slopes is None:
-            ctx.save_for_backward(q, k, v, o, lse, low)
+            ctx.save_for_backward(q, k, v, o, kept, lse)
         else:    # what the gradients read again: autograd notices if it was changed in between
-            ctx.save_for_backward(q, k, v, o, lse, low, *(() if spans is None else (spans.first, spans.end)),
+            ctx.save_for_backward(q, k, v, o, kept, lse, *(() if spans is None else (spans.first, spans.end)),
                                   *(() if slopes is None else (slopes,)))
         ctx.how = how
         if not return_lse:
@@ -194,10 +209,10 @@ class _Attend(torch.autograd.Function):
     def backward(ctx, do, *_):
         if torch.is_grad_enabled():
             raise RuntimeError("attend has no second derivative: call backward without create_graph")
-        q, k, v, o, lse, low = ctx.saved_tensors[:6]
+        q, k, v, o, kept, lse = ctx.saved_tensors[:6]
         do = _loadable(do)
         dq, dk, dv = _like(q), _like(k), _like(v)
-        args = _arguments(q, k, v, o, lse, low, ctx.how,
+        args = _arguments(q, k, v, o, *_kept(kept, lse, ctx.low_at), ctx.how,
                           (do.data_ptr(), *do.stride()[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                            *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]))
         _call(native.load().fd_attention_backward, args, 1, q)
