@@ -332,17 +332,25 @@ struct Slot {
     }
 };
 
+template <int DP>
+__device__ __forceinline__ void load_box(const Cta& c, uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int t, int head) {
+    for (int x = 0; x < Cfg<DP>::BOXES; ++x) ptx::tma_load_4d(dst + x * BOX_BYTES, m, bar, x * 64, t * T, head, c.b);
+}
+
+// This CTA's own pair of tiles: on its way before anything is known of the other side (a microsecond of each CTA's ten).
+template <int DP>
+__device__ __forceinline__ void load_resident(const Cta& c, const Bars& br, uint8_t* base, const CUtensorMap* tmq,
+                                              const CUtensorMap* tmk, const CUtensorMap* tmv, const CUtensorMap* tmdo) {
+    ptx::mbar_expect_tx(br.opfull, 2 * Cfg<DP>::TILE);
+    load_box<DP>(c, base, c.key_side ? tmk : tmq, br.opfull, c.tile, c.h);
+    load_box<DP>(c, base + Cfg<DP>::TILE, c.key_side ? tmv : tmdo, br.opfull, c.tile, c.h);
+}
+
 template <int DP, bool F16>
 __device__ __forceinline__ void produce(const Cta& c, const Bars& br, uint8_t* base, const CUtensorMap* tmq,
                                         const CUtensorMap* tmk, const CUtensorMap* tmv, const CUtensorMap* tmdo,
                                         volatile int* abort, int* status) {
     using C = Cfg<DP>;
-    auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int t, int hh) {
-        for (int x = 0; x < C::BOXES; ++x) ptx::tma_load_4d(dst + x * BOX_BYTES, m, bar, x * 64, t * T, hh, c.b);
-    };
-    ptx::mbar_expect_tx(br.opfull, 2 * C::TILE);
-    load(base, c.key_side ? tmk : tmq, br.opfull, c.tile, c.h);
-    load(base + C::TILE, c.key_side ? tmv : tmdo, br.opfull, c.tile, c.h);
     const int hk = c.h / c.a.group;      // query side
     Slot<C::SA> sa;
     Slot<C::SB> sb;
@@ -351,12 +359,12 @@ __device__ __forceinline__ void produce(const Cta& c, const Bars& br, uint8_t* b
         const int hh = c.key_side ? it.head : hk;
         if (!ptx::wait_bounded(&br.aempty[sa.at], sa.ph ^ 1, abort, status, WAIT_NS)) break;
         ptx::mbar_expect_tx(&br.afull[sa.at], C::TILE);
-        load(base + C::A_OFF + sa.at * C::TILE, c.key_side ? tmq : tmk, &br.afull[sa.at], it.t, hh);
+        load_box<DP>(c, base + C::A_OFF + sa.at * C::TILE, c.key_side ? tmq : tmk, &br.afull[sa.at], it.t, hh);
         sa.next();
         ++na;
         if (!ptx::wait_bounded(&br.bempty[sb.at], sb.ph ^ 1, abort, status, WAIT_NS)) break;
         ptx::mbar_expect_tx(&br.bfull[sb.at], C::TILE + (c.key_side ? 2 * T * 4 : 0));
-        load(base + C::B_OFF + sb.at * C::TILE, c.key_side ? tmdo : tmv, &br.bfull[sb.at], it.t, hh);
+        load_box<DP>(c, base + C::B_OFF + sb.at * C::TILE, c.key_side ? tmdo : tmv, &br.bfull[sb.at], it.t, hh);
         if (c.key_side) {
             float* vec = (float*)(base + C::VEC_OFF) + sb.at * 2 * T;
             const int64_t at = (((int64_t)c.b * c.a.heads + hh) * c.n_qt + it.t) * T;
@@ -854,8 +862,10 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         ptx::prefetch_tmap(&tmv);
         ptx::prefetch_tmap(&tmdo);
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // prep_kernel's results from here on
     __syncthreads();
+    if (warp == TMA_WARP && lane == 0) load_resident<DP>(c, br, base, &tmq, &tmk, &tmv, &tmdo);
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // prep_kernel's results from here on
     if (c.key_side) {
         int lo = 0x7fffffff, hi = 0;
         for (int t = threadIdx.x; t < args.n_qt; t += NTHREADS)
@@ -894,6 +904,7 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
         if (warp == TMA_WARP) {
             if (lane == 0 && c.items > 0) produce<DP, F16>(c, br, base, &tmq, &tmk, &tmv, &tmdo, abort, status);
+            if (lane == 0 && c.items == 0) wait_landed(br.opfull, 0);
         } else if (warp == MMA_WARP) {
             if (c.items > 0) issue<DP, F16>(c, br, base, tmem, abort, status);
         } else if (warp == GUARD_WARP) {

@@ -133,6 +133,13 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     }
     __syncthreads();
 
+    if (warp == TMA_WARP && lane == 0) {   // on their way before the spans are known
+        ptx::mbar_expect_tx(qfull, C::Q_BYTES);
+        for (int s = 0; s < 2; ++s)
+            for (int c = 0; c < C::BOXES; ++c)
+                ptx::tma_load_4d(sQ + s * C::TILE + c * BOX_BYTES, &tmq, qfull, c * 64, q0 + s * T, h, b);
+    }
+    __syncwarp();
     const int sub = warp >> 3, half = (warp >> 2) & 1;   // softmax warps: query subtile, columns 64 half ..
     const int lrow = threadIdx.x & 127, row = q0 + sub * T + lrow;
     int2 span = make_int2(0, 0);
@@ -189,10 +196,6 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
     if (warp == TMA_WARP) {
         if (lane == 0 && t1 > t0) {
-            ptx::mbar_expect_tx(qfull, C::Q_BYTES);
-            for (int s = 0; s < 2; ++s)
-                for (int c = 0; c < C::BOXES; ++c)
-                    ptx::tma_load_4d(sQ + s * C::TILE + c * BOX_BYTES, &tmq, qfull, c * 64, q0 + s * T, h, b);
             const int items = 2 * (t1 - t0);
             int i = 0;
             for (; i < items; ++i) {
@@ -207,6 +210,8 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                 wait_landed(qfull, 0);
                 for (int z = max(0, i - C::SLOTS); z < i; ++z) wait_landed(&full[z % C::SLOTS], (z / C::SLOTS) & 1);
             }
+        } else if (lane == 0) {
+            wait_landed(qfull, 0);   // nothing to do, but the copy is still under way
         }
     } else if (warp == MMA_WARP) {
         if (t1 > t0) {
