@@ -125,7 +125,7 @@ def _loadable(t: torch.Tensor) -> torch.Tensor:
     s0, s1, s2, s3 = t.stride()
     if s3 != 1 and d > 1:
         return t.contiguous()
-    if t.dtype == torch.float32 or d % 8 or d > 128:
+    if t.dtype == torch.float32 or d % 8:
         return t
     if (t.data_ptr() % 16 or n0 > 1 and (s0 % 8 or not s0) or n1 > 1 and (s1 % 8 or not s1)
             or n2 > 1 and (s2 % 8 or not s2)):

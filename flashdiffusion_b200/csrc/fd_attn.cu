@@ -120,10 +120,10 @@ extern "C" {
 
 size_t fd_attention_workspace_bytes(const fd_attention_args* r, int backward) {
     if (!r || r->batch < 0 || r->q_len < 0 || r->k_len < 0 || r->heads < 1) return 0;
-    const bool tc = r->dtype != FD_DTYPE_F32 && r->dim >= 1 && r->dim <= 128 && r->kv_heads >= 1;
-    if (backward) return std::max(attn::delta_bytes(r), tc ? attn::tc_backward_bytes(r) : 0);
+    const bool tc = r->dtype != FD_DTYPE_F32 && r->dim >= 1 && r->kv_heads >= 1;
+    if (backward) return std::max(attn::delta_bytes(r), tc && r->dim <= 128 ? attn::tc_backward_bytes(r) : 0);
     if (!tc) return 0;
-    const bool few = (int64_t)(r->heads / r->kv_heads) * r->q_len <= attn::MAX_ROWS;
+    const bool few = r->dim <= 128 && (int64_t)(r->heads / r->kv_heads) * r->q_len <= attn::MAX_ROWS;
     return few ? align256(attn::rows_bytes(r->dim))
                : attn::tc_forward_bytes(r->batch, r->heads, r->q_len, r->k_len, r->window, r->dim);
 }

@@ -18,7 +18,14 @@
 // sees only a part (see `guard`).  Two softmax threads share a row, 64 columns
 // each, and exchange their maxima through shared memory: with one thread a row
 // (8 warps) the SM issued an instruction in 0.35 of its cycles, two warps a
-// scheduler being too few for the latencies of TMEM, MUFU and FMA chains.
+// scheduler being too few for the latencies of TMEM, MUFU and FMA chains.  Heads
+// of 129 to 256 coordinates leave room for one subtile.
+//
+// Measured, bf16: 2 x 4096 rows of 16 / 4 heads of 128 298 us, 922 TFLOP/s, causal
+// 164 us, 840; 16384 causal rows of 8 / 2 heads 504 us, 1091, with a cap and a
+// window of 4096 (fp16) 351 us, 685; 8192 causal rows of 8 / 4 heads of 256 328 us,
+// 839.  Bound by the shared memory that feeds S and P V (tensor pipe 36 % at 2 x
+// 4096 causal rows) and by the exponentials' issue slots (44 %), which take turns.
 #include <algorithm>
 
 #include "fd_attn_tc.cuh"
@@ -38,8 +45,11 @@ template <int DP>
 struct Cfg {
     static constexpr int BOXES = DP / 64;
     static constexpr uint32_t TILE = BOXES * BOX_BYTES;
-    static constexpr uint32_t Q_BYTES = 2 * TILE;
-    static constexpr int SLOTS = DP == 128 ? 5 : 8;
+    // D = 256 fills TMEM (O) and shared memory (K and V take turns in a slot each) with one subtile; the warps of
+    // the other then have nothing to do
+    static constexpr int SUBTILES = DP <= 128 ? 2 : 1;
+    static constexpr uint32_t Q_BYTES = SUBTILES * TILE;
+    static constexpr int SLOTS = DP == 64 ? 8 : DP == 128 ? 5 : 2;
     static constexpr uint32_t BAR_OFF = Q_BYTES + SLOTS * TILE;
     // qfull, full[SLOTS], empty[SLOTS], sfull[2], pfull[2], ofull[2], toguard, guarded
     static constexpr int NBARS = 1 + 2 * SLOTS + 6 + 2;
@@ -49,7 +59,7 @@ struct Cfg {
     static constexpr uint32_t SMEM = MEET_OFF + 4 * T * 4;            // 1024-byte aligned: nothing lies before it
     static constexpr uint32_t O_COL = 256;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
-    static_assert(O_COL + 2 * DP <= TMEM_COLS, "TMEM budget");
+    static_assert(O_COL + SUBTILES * DP <= TMEM_COLS, "TMEM budget");
 };
 
 struct Misc {
@@ -98,7 +108,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     const int qt = n_qt - 1 - blockIdx.x / (nh * sp.parts);
     const int part = blockIdx.x / nh % sp.parts, bh = blockIdx.x % nh;
     const int b = bh / a.heads, h = bh - b * a.heads, hk = h / a.group;
-    const int q0 = qt * 2 * T;
+    const int q0 = qt * C::SUBTILES * T;
     const int n = keys_of(a, b);
 
     if (threadIdx.x == 0) {
@@ -135,7 +145,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
 
     if (warp == TMA_WARP && lane == 0) {   // on their way before the spans are known
         ptx::mbar_expect_tx(qfull, C::Q_BYTES);
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < C::SUBTILES; ++s)
             for (int c = 0; c < C::BOXES; ++c)
                 ptx::tma_load_4d(sQ + s * C::TILE + c * BOX_BYTES, &tmq, qfull, c * 64, q0 + s * T, h, b);
     }
@@ -144,7 +154,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     const int lrow = threadIdx.x & 127, row = q0 + sub * T + lrow;
     int2 span = make_int2(0, 0);
     if (sub < 2) {
-        const bool real = row < a.q_len;
+        const bool real = sub < C::SUBTILES && row < a.q_len;
         if (real) span = row_span(a, b, row, n);
         const bool some = span.y > span.x;
         const int lo = warp_min(some ? span.x : 0x7fffffff), hi = warp_max(some ? span.y : 0);
@@ -438,7 +448,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         meet[0] = l;
         both_here(ok);
         l += other[0];
-        const bool real = row < a.q_len;
+        const bool real = sub < C::SUBTILES && row < a.q_len;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint8_t* out = (uint8_t*)a.o.p + 2 * (b * a.o.sb + (int64_t)row * a.o.ss + h * a.o.sh);
         int8_t* low = a.o_low ? a.o_low + (((int64_t)b * a.q_len + row) * a.heads + h) * a.dim : nullptr;
@@ -539,7 +549,7 @@ int launch(const Prob& a, const Split& sp, cudaStream_t s) {
     int* status = nullptr;
     FD_TRY(status_word(&status));
     FD_TRY((allow_smem<forward_kernel<DP, F16, GEN>>(Cfg<DP>::SMEM)));
-    const int n_qt = (int)cdiv(a.q_len, 2 * T);
+    const int n_qt = (int)cdiv(a.q_len, Cfg<DP>::SUBTILES * T);
     const int64_t blocks = (int64_t)n_qt * a.heads * a.batch * sp.parts;
     FD_CHECK_ARG(blocks <= 0x7fffffff, "fd_attention: too many query tiles");
     forward_kernel<DP, F16, GEN><<<(unsigned)blocks, NTHREADS, Cfg<DP>::SMEM, s>>>(q, k, v, a, sp, n_qt, status);
@@ -579,7 +589,7 @@ int make_head_map(CUtensorMap* map, const View& v, int64_t rows, int heads, int 
 
 bool tc_applies(const Prob& a, int dtype, bool backward) {
     if (dtype != FD_DTYPE_F16 && dtype != FD_DTYPE_BF16) return false;
-    if (a.dim % 8 || a.dim > 128 || a.q_len == 0 || a.k_len == 0) return false;
+    if (a.dim % 8 || a.dim > (backward ? 128 : 256) || a.q_len == 0 || a.k_len == 0) return false;
     const int64_t qe[3] = {a.batch, a.q_len, a.heads}, ke[3] = {a.batch, a.k_len, a.kv_heads};
     if (!tma_view(a.q, qe) || !tma_view(a.k, ke) || !tma_view(a.v, ke) || !tma_view(a.o, qe)) return false;
     if (!backward) return true;
@@ -590,23 +600,24 @@ bool tc_applies(const Prob& a, int dtype, bool backward) {
 // about what a part's start, its fp32 rows and the join do (8 / 2 bf16 heads of 128, 512 causal rows: against 16384
 // keys 267 us whole, 59 us in 9 parts; against 4096 keys 79 and 35 us; two heads of 128 rows against 640 keys are as
 // fast whole, 20.5 us, as in two parts).
-static int split_parts(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window) {
-    const int64_t ctas = cdiv(q_len, 2 * T) * heads * batch;
+static int split_parts(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window, int64_t dim) {
+    const int64_t ctas = cdiv(q_len, (dim <= 128 ? 2 : 1) * T) * heads * batch;
     const int64_t keys = window > 0 ? std::min(k_len, window + 2 * T) : k_len;
     return (int)std::max<int64_t>(1, std::min<int64_t>(num_sms() / std::max<int64_t>(ctas, 1), cdiv(keys, T) / 4));
 }
 
 size_t tc_forward_bytes(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window, int64_t dim) {
-    const int64_t parts = split_parts(batch, heads, q_len, k_len, window);
+    const int64_t parts = split_parts(batch, heads, q_len, k_len, window, dim);
     return parts > 1 ? align256(sizeof(float) * parts * batch * q_len * heads * (dim + 1)) : 0;
 }
 
 int tc_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
     fwd::Split sp{};
-    sp.parts = split_parts(a.batch, a.heads, a.q_len, a.k_len, a.window);
+    sp.parts = split_parts(a.batch, a.heads, a.q_len, a.k_len, a.window, a.dim);
     sp.o = (float*)workspace;
     sp.lse2 = sp.o + (int64_t)sp.parts * a.batch * a.q_len * a.heads * a.dim;
-    return a.dim <= 64 ? fwd::by_type<64>(a, dtype, sp, s) : fwd::by_type<128>(a, dtype, sp, s);
+    if (a.dim <= 64) return fwd::by_type<64>(a, dtype, sp, s);
+    return a.dim <= 128 ? fwd::by_type<128>(a, dtype, sp, s) : fwd::by_type<256>(a, dtype, sp, s);
 }
 
 }  // namespace attn

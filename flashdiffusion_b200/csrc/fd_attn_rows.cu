@@ -735,7 +735,7 @@ int by_rows(const Prob& a, float* parts, cudaStream_t s) {
 
 }  // namespace rows
 
-bool rows_applies(const Prob& a) { return (int64_t)a.group * a.q_len <= MAX_ROWS; }
+bool rows_applies(const Prob& a) { return a.dim <= 128 && (int64_t)a.group * a.q_len <= MAX_ROWS; }
 
 size_t rows_bytes(int dim) {
     static_assert(rows::ctas_per_sm(4) * 4 >= rows::ctas_per_sm(1), "the widest kernel has the largest partials");

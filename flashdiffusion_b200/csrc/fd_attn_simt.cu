@@ -1,6 +1,6 @@
 // Softmax attention on the CUDA cores: every type, stride, head size up to 256
-// and length, in fp32.  The tensor-core kernels take 16-bit heads of up to 128
-// coordinates; what is left comes here.
+// and length, in fp32.  The tensor-core kernels take 16-bit heads of a multiple of
+// 8 coordinates, up to 256 forward and 128 backward; what is left comes here.
 //
 // A block of 256 threads holds a tile of rows of one side and walks over tiles of
 // the other, both as fp32 in shared memory.  Thread (ty, tx) owns M x M scores,

@@ -514,6 +514,49 @@ def test_split_axes_with_anything_in_masked_places(dtype):
     assert torch.equal(got[0, ~inside], clean["dv"][0, ~inside])
 
 
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("new,h,hk,d,cap,window", [(1, 8, 2, 256, None, None), (3, 4, 4, 136, 20.0, None),
+                                                   (1, 5, 1, 192, None, 90), (140, 2, 1, 256, None, None)])
+def test_wide_heads_against_a_cache(new, h, hk, d, cap, window, dtype):
+    from flashdiffusion_b200.attention import attend_cached
+    capacity = 2000
+    lengths = [1, 0, 127, 128, 129, 1000, capacity]
+    q, k, v, _ = _inputs(len(lengths), new, capacity, h, hk, d, dtype, seed=d)
+    n = torch.tensor(lengths, dtype=torch.int32)
+    for b, m in enumerate(lengths):
+        k[b, m:] = float("nan")
+        v[b, m:] = float("inf")
+    slopes = torch.linspace(0.5, 0.001, h, device="cuda")
+    lo, hi, pos = spans_of(new, capacity, len(lengths), causal=True, window=window, lengths=n)
+    o, lse = attend_cached(q, k, v, n.cuda(), cap=cap, window=window, slopes=slopes, return_lse=True)
+    ref = reference(q, k, v, lo, hi, pos, cap=cap or 0.0, slopes=slopes)
+    check("o", o, ref, FLOOR[dtype])
+    check("lse", lse, ref)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("d", [136, 256])
+def test_wide_heads_forward(d, dtype):
+    """Enough tiles not to be split; ends inside tiles, strided views, a visible infinity."""
+    b, sq, sk, h, hk = 3, 700, 390, 14, 2
+    q, k, v, _ = _inputs(b, sq, sk, h, hk, d, dtype, seed=65)
+    v[1, 300, 0, 3] = float("inf")
+    lo, hi, pos = spans_of(sq, sk, b, causal=True)
+    wide = torch.randn(b, sk, 2 * hk, d, device="cuda").to(dtype)
+    wide[:, :, hk:] = k
+    got = _run(q, wide[:, :, hk:], v, None, grad=False, causal=True)
+    vr = v.clone()
+    vr[1, 300, 0, 3] = 0
+    ref = reference(q, k, vr, lo, hi, pos)
+    check("lse", got["lse"], ref)
+    sees = (hi[1] > 300).cuda()
+    spoiled = got["o"][1, :, :7, 3]
+    assert (spoiled[sees] == float("inf")).all() and torch.isfinite(spoiled[~sees]).all()
+    o = got["o"].clone()
+    o[1, sees, :7, 3] = ref["o"][1, sees.cpu(), :7, 3].to(o)
+    check("o", o, ref, FLOOR[dtype])
+
+
 @pytest.mark.parametrize("dtype,d", [(BF, 64), (SF, 16)], ids=str)
 def test_very_many_heads(dtype, d):
     """More (sequence, head) pairs than a grid's second axis holds."""
