@@ -625,10 +625,9 @@ __device__ __forceinline__ bool compute_key(const Cta& c, const Bars& br, const 
             round32<F16>(x[g], p);
             ptx::tmem_st16(lanes + half * 64 + g * 16, p);
             if (GEN && sc.capped) {
-                if (masked) {   // a masked pair's bend may be a NaN
+                if (masked) {   // a masked pair's bend may be a NaN: the maximum takes the number
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        bend[e] = ptx::pack2(ptx::lo2(x[g][e]) == 0.f ? 0.f : ptx::lo2(bend[e]), ptx::hi2(x[g][e]) == 0.f ? 0.f : ptx::hi2(bend[e]));
+                    for (int e = 0; e < 16; ++e) bend[e] = ptx::pack2(fmaxf(ptx::lo2(bend[e]), 0.f), fmaxf(ptx::hi2(bend[e]), 0.f));
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
