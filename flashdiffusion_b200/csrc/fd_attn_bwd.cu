@@ -75,6 +75,7 @@ struct Shape {
     // masks are causal at heart (4 x 1531 rows with prefixes, 8 / 2 heads of 128, bias: 175 us with all counted, 137
     // so).
     double visible() const {
+        if (q_len < 1 || k_len < 1) return 1.0;
         if (spans) return 0.5;
         if (window > 0) return (window / T + 1.0) / (window / T + 2.0);
         return !causal ? 1.0 : q_len <= k_len ? 1.0 - 0.5 * q_len / k_len : 0.5 * k_len / q_len;
