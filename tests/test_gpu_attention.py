@@ -634,6 +634,42 @@ def test_two_streams_at_once(dtype):
         assert all(torch.equal(x, y) for g in got[i] for x, y in zip(g, want[i]))
 
 
+def test_two_threads_at_once():
+    """Two host threads, each with its own stream, type and head size, give the bits that each gives alone."""
+    import threading
+
+    from flashdiffusion_b200.attention import attend, attend_cached
+    sets = [_inputs(1, 300, 300, 4, 2, d, t, seed=d) for d, t in ((64, HF), (128, BF))]
+    n = torch.tensor([280], dtype=torch.int32, device="cuda")
+
+    def step(q, k, v, do):
+        a, b, c = (t.detach().requires_grad_(True) for t in (q, k, v))
+        o = attend(a, b, c, causal=True, cap=20.0)
+        return (o.detach(), attend_cached(q[:, -1:], k, v, n), *torch.autograd.grad(o, (a, b, c), do))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = step(*sets[i])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(x, y) for x, y in zip(got, want[i])):
+                        wrong.append(i)
+        except Exception as e:       # what a thread raises is lost otherwise
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, SF], ids=str)
 def test_two_captured_graphs_of_one_pool(dtype):
     """Two training steps captured into one memory pool and replayed in turn on changing inputs."""
