@@ -52,6 +52,25 @@ static View view(const void* p, const int64_t* s, int batch, int rows, int heads
     return {const_cast<void*>(p), batch > 1 ? s[0] : 0, rows > 1 ? s[1] : 0, heads > 1 ? s[2] : 0};
 }
 
+// The sizes and switches of a call.  The launches and the workspace query both read them from here, and so cut the
+// same work into the same parts.
+static Prob sizes_of(const fd_attention_args* r) {
+    Prob a{};
+    a.first = r->first;
+    a.end = r->end;
+    a.causal = r->causal != 0;
+    // a window that reaches every key is none; this also keeps pos - window inside 32 bits
+    a.window = r->window >= (int64_t)r->q_len + r->k_len ? 0 : r->window;
+    a.batch = r->batch;
+    a.q_len = r->q_len;
+    a.k_len = r->k_len;
+    a.heads = r->heads;
+    a.kv_heads = r->kv_heads;
+    a.dim = r->dim;
+    a.group = r->kv_heads > 0 ? r->heads / r->kv_heads : 0;
+    return a;
+}
+
 static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     FD_CHECK_ARG(r, "fd_attention: null arguments");
     FD_CHECK_ARG(r->dtype == FD_DTYPE_F32 || r->dtype == FD_DTYPE_F16 || r->dtype == FD_DTYPE_BF16,
@@ -68,7 +87,7 @@ static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     FD_CHECK_ARG(r->window >= 0, "fd_attention: window=%d", r->window);
     FD_CHECK_ARG(!r->first || (!r->causal && !r->window), "fd_attention: spans replace causal and window");
     FD_CHECK_ARG(r->window == 0 || r->causal, "fd_attention: a window needs causal");
-    Prob a{};
+    Prob a = sizes_of(r);
     a.q = view(r->q, r->q_stride, r->batch, r->q_len, r->heads);
     a.k = view(r->k, r->k_stride, r->batch, r->k_len, r->kv_heads);
     a.v = view(r->v, r->v_stride, r->batch, r->k_len, r->kv_heads);
@@ -79,23 +98,11 @@ static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     a.dv = view(r->dv, r->dv_stride, r->batch, r->k_len, r->kv_heads);
     a.lse = r->lse;
     a.o_low = r->o_low;
-    a.first = r->first;
-    a.end = r->end;
     a.span_stride = r->span_stride;
     a.lengths = r->lengths;
     a.slopes = r->slopes;
     a.scale = (float)r->scale;
     a.cap = (float)r->cap;
-    a.causal = r->causal != 0;
-    // a window that reaches every key is none; this also keeps pos - window inside 32 bits
-    a.window = r->window >= (int64_t)r->q_len + r->k_len ? 0 : r->window;
-    a.batch = r->batch;
-    a.q_len = r->q_len;
-    a.k_len = r->k_len;
-    a.heads = r->heads;
-    a.kv_heads = r->kv_heads;
-    a.dim = r->dim;
-    a.group = r->heads / r->kv_heads;
     *out = a;
     if (a.batch == 0) return FD_OK;
     FD_CHECK_ARG(a.q_len == 0 || (a.q.p && a.o.p), "fd_attention: null q or o");
@@ -107,8 +114,8 @@ static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
     return FD_OK;
 }
 
-static size_t delta_bytes(const fd_attention_args* r) {
-    return align256(sizeof(float) * (size_t)r->batch * r->heads * r->q_len);
+static size_t delta_bytes(const Prob& a) {
+    return align256(sizeof(float) * (size_t)a.batch * a.heads * a.q_len);
 }
 
 }  // namespace attn
@@ -120,12 +127,11 @@ extern "C" {
 
 size_t fd_attention_workspace_bytes(const fd_attention_args* r, int backward) {
     if (!r || r->batch < 0 || r->q_len < 0 || r->k_len < 0 || r->heads < 1) return 0;
-    const bool tc = r->dtype != FD_DTYPE_F32 && r->dim >= 1 && r->kv_heads >= 1;
-    if (backward) return std::max(attn::delta_bytes(r), tc && r->dim <= 128 ? attn::tc_backward_bytes(r) : 0);
+    const attn::Prob a = attn::sizes_of(r);
+    const bool tc = r->dtype != FD_DTYPE_F32 && a.dim >= 1 && a.kv_heads >= 1;
+    if (backward) return std::max(attn::delta_bytes(a), tc && a.dim <= 128 ? attn::tc_backward_bytes(a) : 0);
     if (!tc) return 0;
-    const bool few = r->dim <= 128 && (int64_t)(r->heads / r->kv_heads) * r->q_len <= attn::MAX_ROWS;
-    return few ? align256(attn::rows_bytes(r->dim))
-               : attn::tc_forward_bytes(r->batch, r->heads, r->q_len, r->k_len, r->window, r->dim);
+    return attn::rows_applies(a) ? align256(attn::rows_bytes(a.dim)) : attn::tc_forward_bytes(a);
 }
 
 int fd_attention_forward(const fd_attention_args* r, void* workspace, size_t workspace_bytes, void* stream) {

@@ -65,6 +65,9 @@ struct Work {
 struct Shape {
     int64_t batch, heads, kv_heads, q_len, k_len, dim, window;
     bool causal, spans;
+    explicit Shape(const Prob& a)
+        : batch(a.batch), heads(a.heads), kv_heads(a.kv_heads), q_len(a.q_len), k_len(a.k_len), dim(a.dim),
+          window(a.window), causal(a.causal != 0), spans(a.first != nullptr) {}
     int key_parts() const { return parts(tiles(q_len, k_len) * (heads / kv_heads)); }
     int query_parts() const { return parts(tiles(k_len, q_len)); }
     // tiles of one side that a tile of the other sees
@@ -1056,13 +1059,10 @@ int by_type(const Prob& a, int dtype, const Work& w, const Shape& z, cudaStream_
 
 }  // namespace bwd
 
-size_t tc_backward_bytes(const fd_attention_args* r) {
-    const bwd::Shape z{r->batch, r->heads, r->kv_heads, r->q_len, r->k_len, r->dim, r->window, r->causal != 0, r->first != nullptr};
-    return bwd::work_layout(nullptr, nullptr, z);
-}
+size_t tc_backward_bytes(const Prob& a) { return bwd::work_layout(nullptr, nullptr, bwd::Shape(a)); }
 
 int tc_backward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
-    const bwd::Shape z{a.batch, a.heads, a.kv_heads, a.q_len, a.k_len, a.dim, a.window, a.causal != 0, a.first != nullptr};
+    const bwd::Shape z(a);
     bwd::Work w;
     bwd::work_layout(&w, workspace, z);
     return a.dim <= 64 ? bwd::by_type<64>(a, dtype, w, z, s) : bwd::by_type<128>(a, dtype, w, z, s);

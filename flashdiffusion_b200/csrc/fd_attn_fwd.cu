@@ -600,20 +600,20 @@ bool tc_applies(const Prob& a, int dtype, bool backward) {
 // about what a part's start, its fp32 rows and the join do (8 / 2 bf16 heads of 128, 512 causal rows: against 16384
 // keys 267 us whole, 59 us in 9 parts; against 4096 keys 79 and 35 us; two heads of 128 rows against 640 keys are as
 // fast whole, 20.5 us, as in two parts).
-static int split_parts(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window, int64_t dim) {
-    const int64_t ctas = cdiv(q_len, (dim <= 128 ? 2 : 1) * T) * heads * batch;
-    const int64_t keys = window > 0 ? std::min(k_len, window + 2 * T) : k_len;
+static int split_parts(const Prob& a) {
+    const int64_t ctas = cdiv(a.q_len, (a.dim <= 128 ? 2 : 1) * T) * a.heads * a.batch;
+    const int64_t keys = a.window > 0 ? std::min<int64_t>(a.k_len, (int64_t)a.window + 2 * T) : a.k_len;
     return (int)std::max<int64_t>(1, std::min<int64_t>(num_sms() / std::max<int64_t>(ctas, 1), cdiv(keys, T) / 4));
 }
 
-size_t tc_forward_bytes(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window, int64_t dim) {
-    const int64_t parts = split_parts(batch, heads, q_len, k_len, window, dim);
-    return parts > 1 ? align256(sizeof(float) * parts * batch * q_len * heads * (dim + 1)) : 0;
+size_t tc_forward_bytes(const Prob& a) {
+    const int64_t parts = split_parts(a);
+    return parts > 1 ? align256(sizeof(float) * parts * a.batch * a.q_len * a.heads * (a.dim + 1)) : 0;
 }
 
 int tc_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s) {
     fwd::Split sp{};
-    sp.parts = split_parts(a.batch, a.heads, a.q_len, a.k_len, a.window, a.dim);
+    sp.parts = split_parts(a);
     sp.o = (float*)workspace;
     sp.lse2 = sp.o + (int64_t)sp.parts * a.batch * a.q_len * a.heads * a.dim;
     if (a.dim <= 64) return fwd::by_type<64>(a, dtype, sp, s);

@@ -324,7 +324,7 @@ __device__ __forceinline__ void store8(void* out, int8_t* low, const float* f) {
 
 // Launchers of the tensor-core kernels.
 bool tc_applies(const Prob& a, int dtype, bool backward);
-size_t tc_forward_bytes(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t window, int64_t dim);
+size_t tc_forward_bytes(const Prob& a);   // these two read the sizes and switches of a call only
 int tc_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
 // Few rows against many keys (fd_attn_rows.cu), where tc_applies: up to MAX_ROWS query rows per key head; above,
 // the 128-row tcgen05 tiles are full enough.
@@ -332,7 +332,7 @@ constexpr int MAX_ROWS = 64;
 bool rows_applies(const Prob& a);
 size_t rows_bytes(int dim);
 int rows_forward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
-size_t tc_backward_bytes(const fd_attention_args* r);
+size_t tc_backward_bytes(const Prob& a);
 int tc_backward(const Prob& a, int dtype, void* workspace, cudaStream_t s);
 
 }  // namespace attn

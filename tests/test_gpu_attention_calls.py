@@ -1,0 +1,76 @@
+"""Calls of attend and attend_cached that their documentation allows, against the same bits by another call or the
+definition in 64 bits (tests/attention_reference.py)."""
+import pytest
+import torch
+
+from tests.attention_reference import check, reference, spans_of
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, SF = torch.bfloat16, torch.float16, torch.float32
+# fp16 holds nothing finer than 2^-25 absolute: outputs that small, and the ds values they are summed from
+FLOOR = {BF: 0.0, HF: 2.0 ** -25, SF: 0.0}
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    """A bounded wait that gives up leaves its mark in the status word and its results unfinished."""
+    yield
+    from flashdiffusion_b200 import native
+    native.check_status()
+
+
+def _inputs(b, sq, sk, h, hk, d, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    mk = lambda *s: torch.randn(*s, device="cuda", generator=g).to(dtype)  # noqa: E731
+    return mk(b, sq, h, d), mk(b, sk, hk, d), mk(b, sk, hk, d), mk(b, sq, h, d)
+
+
+def _step(q, k, v, do, **kw):
+    from flashdiffusion_b200.attention import attend
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    o, lse = attend(q, k, v, return_lse=True, **kw)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
+    return {"o": o.detach(), "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+
+
+def _compare(out, ref, dtype):
+    for name in out:
+        check(name, out[name], ref, 0.0 if name == "lse" else FLOOR[dtype])
+
+
+@pytest.fixture
+def guarded(monkeypatch):
+    """Workspaces of exactly the size asked for, with bytes behind them that must not change."""
+    from flashdiffusion_b200 import attention, native
+
+    def call(fn, args, backward, q):
+        n = native.load().fd_attention_workspace_bytes(args, backward)
+        ws = torch.full((n + (32 << 20),), 0xA5, dtype=torch.uint8, device=q.device)
+        native.call(fn, q.device, args, ws.data_ptr(), n)
+        assert (ws[n:] == 0xA5).all()
+
+    monkeypatch.setattr(attention, "_call", call)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("b,s,h,hk,d,window", [(1, 1024, 32, 8, 128, 4096), (1, 2048, 16, 4, 128, 4096),
+                                               (1, 2048, 4, 1, 128, 4096), (1, 1900, 8, 4, 128, 2 ** 31 - 1),
+                                               (1, 3000, 4, 1, 64, 6000)])
+def test_a_window_that_reaches_every_key_is_no_window(guarded, b, s, h, hk, d, window, dtype):
+    """Sizes whose gradients are cut into parts with fp32 sums of their own in the workspace."""
+    q, k, v, do = _inputs(b, s, s, h, hk, d, dtype, seed=s)
+    want = _step(q, k, v, do, causal=True)
+    got = _step(q, k, v, do, causal=True, window=window)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,dtype,kw", [
+    (1, 300, 3001, 2, 1, 128, BF, dict(causal=True)), (1, 1500, 1500, 4, 1, 64, HF, dict(causal=True, window=700)),
+    (1, 2100, 140, 1, 1, 80, BF, dict()), (1, 3, 5000, 8, 2, 128, HF, dict()), (1, 200, 3000, 2, 1, 256, BF, dict()),
+    (2, 100, 130, 2, 1, 48, SF, dict(causal=True)), (1, 100, 2000, 2, 1, 20, BF, dict()), (3, 77, 77, 4, 4, 64, HF, dict()),
+], ids=str)
+def test_workspaces_are_not_left(guarded, b, sq, sk, h, hk, d, dtype, kw):
+    q, k, v, do = _inputs(b, sq, sk, h, hk, d, dtype, seed=sk)
+    lo, hi, pos = spans_of(sq, sk, b, causal=kw.get("causal", False), window=kw.get("window"))
+    _compare(_step(q, k, v, do, **kw), reference(q, k, v, lo, hi, pos, do=do), dtype)
