@@ -57,7 +57,7 @@ struct Work {
     float* lse2;         // -lse in base 2 (plus P_SHIFT_F16 for fp16); -inf for rows that see nothing and for the padding
     int2* spans;         // [batch][rows padded to 128]
     Bounds* bounds;      // [batch][query tiles]
-    unsigned* top;       // fp16: bits of the largest |dO row|^2 and |V row|^2
+    unsigned* top;       // fp16: bits of the largest |dO row|^2 and |V row|^2 that take part, [batch][key heads][2]
     float *dq, *dk, *dv; // fp32 sums of each part, [part][batch][row][head][dim], where there are parts
 };
 
@@ -107,7 +107,7 @@ inline size_t work_layout(Work* w, void* base, const Shape& z) {
     char* b = take(sizeof(float) * bh * n_qt * T);
     char* c = take(sizeof(int2) * batch * n_qt * T);
     char* d = take(sizeof(Bounds) * batch * n_qt);
-    char* e = take(2 * sizeof(unsigned));
+    char* e = take(2 * sizeof(unsigned) * batch * z.kv_heads);
     auto sums = [&](int parts, int64_t rows) { return parts > 1 ? sizeof(float) * parts * batch * rows * z.dim : 0; };
     char* f = take(sums(z.query_parts(), z.q_len * z.heads));
     char* g = take(sums(z.key_parts(), z.k_len * z.kv_heads));
@@ -116,10 +116,51 @@ inline size_t work_layout(Work* w, void* base, const Shape& z) {
     return at;
 }
 
+// Which of the keys k0 .. k0 + 127 some query row sees, as 128 bits.  All threads of a block of 256; the answer is the
+// same in all.  Causal rows and windows move on by one key a row, so their union is one run.  Of spans all are read,
+// those about the keys' own positions first: they show most keys of causal masks, and nothing is left to look for.
+__device__ __forceinline__ uint4 keys_seen(const Prob& a, int b, int n, int k0, uint32_t (&bits)[4]) {
+    auto run = [&](int w, int lo, int hi) {   // bits of word w within [lo, hi)
+        const int x = max(lo - k0 - 32 * w, 0), y = min(hi - k0 - 32 * w, 32);
+        return y > x ? ~0u >> (32 - (y - x)) << x : 0u;
+    };
+    if (!a.first) {
+        const int lo = row_span(a, b, 0, n).x, hi = row_span(a, b, a.q_len - 1, n).y;
+        return make_uint4(run(0, lo, hi), run(1, lo, hi), run(2, lo, hi), run(3, lo, hi));
+    }
+    if (threadIdx.x < 4) bits[threadIdx.x] = 0;
+    __syncthreads();
+    constexpr int CHUNK = 1024;
+    const int chunks = (int)cdiv(a.q_len, CHUNK), own = min(max(k0 - (n - a.q_len), 0), a.q_len - 1) / CHUNK;
+    for (int c = 0; c < chunks; ++c) {
+        const int at = (own + c) % chunks * CHUNK + (int)threadIdx.x;
+        uint32_t m[4] = {};
+#pragma unroll
+        for (int y = 0; y < CHUNK / 256; ++y) {
+            if (at + 256 * y >= a.q_len) continue;
+            const int2 sp = row_span(a, b, at + 256 * y, n);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m[w] |= run(w, sp.x, sp.y);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            m[w] = __reduce_or_sync(~0u, m[w]);
+            if ((threadIdx.x & 31) == 0 && m[w]) atomicOr(&bits[w], m[w]);
+        }
+        __syncthreads();
+        bool all = true;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) all = all && (~bits[w] & run(w, 0, n)) == 0;
+        if (__syncthreads_and(all)) break;
+    }
+    return make_uint4(bits[0], bits[1], bits[2], bits[3]);
+}
+
 // Block (t, h, b): delta and lse2 of 128 rows, 16 lanes a row (one 16-byte piece
 // each); head 0 also makes the tile's bounds.  fp16: the largest row norms of dO
-// and, in the blocks behind the query tiles, of V.  Bandwidth-bound: dO and o are
-// read once.
+// and, in the blocks behind the query tiles, of V, for each sequence and key head;
+// of V only the rows that some query sees, for the others may hold anything.
+// Bandwidth-bound: dO and o are read once.
 template <bool F16>
 __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob a, const __grid_constant__ Work w, int n_qt) {
     const int h = blockIdx.y, b = blockIdx.z, t = blockIdx.x;
@@ -128,10 +169,16 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
     asm volatile("griddepcontrol.launch_dependents;");   // the gradient kernel sets itself up and waits
     if (t >= n_qt) {
         if (h >= a.kv_heads) return;
-        for (int r = r0; r < T; r += 16) {
-            const int64_t j = (int64_t)(t - n_qt) * T + r;
+        __shared__ uint32_t bits[4];
+        const int k0 = (t - n_qt) * T;
+        const uint4 seen = keys_seen(a, b, keys_of(a, b), k0, bits);
+        const uint32_t word[4] = {seen.x, seen.y, seen.z, seen.w};
+#pragma unroll
+        for (int r8 = 0; r8 < T / 16; ++r8) {
+            const int r = r0 + 16 * r8;
+            const int64_t j = k0 + r;
             float s = 0.f;
-            if (j < a.k_len && piece * 8 < a.dim) {
+            if (word[r8 / 2] >> (r & 31) & 1 && piece * 8 < a.dim) {
                 const uint4 x = *(const uint4*)((const uint16_t*)a.v.p + b * a.v.sb + j * a.v.ss + h * a.v.sh + piece * 8);
                 const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -144,7 +191,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
             if (s < INFINITY) top = fmaxf(top, s);
         }
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&w.top[1], __float_as_uint(top));
+        if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&w.top[2 * (b * a.kv_heads + h) + 1], __float_as_uint(top));
         return;
     }
     __shared__ int sb[4];
@@ -216,7 +263,7 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
     }
     if (F16) {
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&w.top[0], __float_as_uint(top));
+        if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(&w.top[2 * (b * a.kv_heads + h / a.group)], __float_as_uint(top));
     }
 }
 
@@ -926,11 +973,12 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         const int half = warp >> 2;                 // columns 64 half .. of each score tile
         const int row = c.r0 + (threadIdx.x & 127); // this thread's key (key side) or query
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-        // fp16 keeps 2^-14 .. 65504: dS is scaled by a power of two that brings its bound 2 |dO| |V| to
-        // 2^14 .. 2^15, and the accumulator is scaled back at the end
+        // fp16 keeps 2^-14 .. 65504: dS is scaled by a power of two that brings its bound 2 |dO| |V|, over the rows of
+        // this sequence and key head that take part, to 2^14 .. 2^15, and the accumulator is scaled back at the end
         float up = 1.f, p_back = 1.f;
         if (F16) {
-            const float m2 = __uint_as_float(w.top[0]) * __uint_as_float(w.top[1]);
+            const unsigned* top = w.top + 2 * (c.b * a.kv_heads + (c.key_side ? c.h : c.h / a.group));
+            const float m2 = __uint_as_float(top[0]) * __uint_as_float(top[1]);
             if (m2 > 0.f && m2 < INFINITY) up = exp2f(14.f - ceilf(0.5f * log2f(m2)));
             up = fminf(fmaxf(up, 0x1p-60f), 0x1p60f);
             p_back = exp2f(-P_SHIFT_F16);
@@ -1024,7 +1072,7 @@ int launch(const Prob& a, const Work& w, const Shape& z, cudaStream_t s) {
     FD_CHECK_ARG(blocks <= 0x7fffffff && cdiv(a.q_len, T) + cdiv(a.k_len, T) <= 0x7fffffff, "fd_attention: too many tiles");
     args.first = (int)(args.keys_first ? keys : queries);
     const int v_blocks = F16 ? n_kt : 0;
-    if (F16) FD_CUDA_TRY(cudaMemsetAsync(w.top, 0, 2 * sizeof(unsigned), s));
+    if (F16) FD_CUDA_TRY(cudaMemsetAsync(w.top, 0, 2 * sizeof(unsigned) * a.batch * a.kv_heads, s));
     prep_kernel<F16><<<dim3(args.n_qt + v_blocks, a.heads, a.batch), 256, 0, s>>>(a, w, args.n_qt);
     FD_CUDA_TRY(cudaGetLastError());
     FD_TRY((allow_smem<gradient_kernel<DP, F16, GEN>>(Cfg<DP>::SMEM)));

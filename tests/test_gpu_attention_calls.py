@@ -74,3 +74,66 @@ def test_workspaces_are_not_left(guarded, b, sq, sk, h, hk, d, dtype, kw):
     q, k, v, do = _inputs(b, sq, sk, h, hk, d, dtype, seed=sk)
     lo, hi, pos = spans_of(sq, sk, b, causal=kw.get("causal", False), window=kw.get("window"))
     _compare(_step(q, k, v, do, **kw), reference(q, k, v, lo, hi, pos, do=do), dtype)
+
+
+def _spans(kind, sq, sk):
+    """Keyword arguments and the keys that no row sees (rows that see nothing are the caller's to find)."""
+    from flashdiffusion_b200.attention import Spans, document_spans
+    if kind == "documents":
+        spans = document_spans(torch.tensor([0, 100, sk - 190], dtype=torch.int32, device="cuda"), sq)
+    elif kind == "holes":        # rows in no order that see keys 3 .. 9, 40 .. 59 and 260 .. 399
+        i = torch.arange(sq)
+        first = torch.where(i % 3 == 0, 3, torch.where(i % 3 == 1, 40, 260)).int()
+        end = torch.where(i % 3 == 0, 10, torch.where(i % 3 == 1, 60, 400)).int()
+        end[5::7] = 0
+        spans = Spans(first.cuda(), end.cuda())
+    else:                        # the last rows of a window: keys before it are never seen
+        return dict(causal=True, window=50), torch.arange(sk) < sk - sq - 49, torch.zeros(sq, dtype=torch.bool)
+    first, end = spans.first[0].cpu(), spans.end[0].cpu()
+    j = torch.arange(sk)
+    return dict(spans=spans), ~((j >= first[:, None]) & (j < end[:, None])).any(0), end <= first
+
+
+@pytest.mark.parametrize("bad", [6e4, -6e4], ids=str)
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (HF, 128), (SF, 48)], ids=str)
+@pytest.mark.parametrize("kind,sq,sk", [("documents", 400, 400), ("holes", 2300, 500), ("window", 130, 700)])
+def test_masked_places_hold_large_numbers(kind, sq, sk, dtype, d, bad):
+    """Finite and large where NaN and infinities are looked for elsewhere: the same bits, gradients too."""
+    q, k, v, do = _inputs(1, sq, sk, 4, 2, d, dtype, seed=71)
+    kw, unseen, empty = _spans(kind, sq, sk)
+    assert unseen.any()
+    want = _step(q, k, v, do, **kw)
+    q2, k2, v2, do2 = (t.clone() for t in (q, k, v, do))
+    for t in (k2, v2):
+        t[:, unseen] = bad
+    for t in (q2, do2):
+        t[:, empty] = bad
+    got = _step(q2, k2, v2, do2, **kw)
+    for n in got:
+        assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+def test_sequences_and_key_heads_do_not_touch_each_other(dtype):
+    """A sequence's and a key head's results are the same bits whatever the others hold."""
+    b, s, h, hk, d = 2, 500, 4, 2, 64
+    q, k, v, do = _inputs(b, s, s, h, hk, d, dtype, seed=73)
+    want = _step(q, k, v, do, causal=True)
+    v2, do2 = v.clone(), do.clone()
+    v2[1, :, 1] *= 1000
+    do2[1, :, 2:] *= 16
+    got = _step(q, k, v2, do2, causal=True)
+    for n in got:
+        x, y = (t[n].transpose(1, 2) if n != "lse" else t[n] for t in (got, want))       # (batch, head, row ..)
+        one = 1 if n in ("dk", "dv") else 2                                                # heads of key head 0
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1, :one], y[1, :one]), n
+    lo, hi, pos = spans_of(s, s, b, causal=True)
+    ref = reference(q, k, v2, lo, hi, pos, do=do2)
+    if dtype is HF:
+        # |dS| reaches 16 sqrt(64) 1000 sqrt(64) here, so some exact gradients leave fp16: its largest number is 65504,
+        # and from half a step (16) above it on, less the bound, every value in reach rounds to an infinity
+        for n in ("dq", "dk", "dv"):
+            over = ref[n].abs() - ref[n + "_tol"] * 1.001 >= 65504 + 16
+            assert (got[n].cpu().double()[over] == ref[n][over].sign() * float("inf")).all()
+            ref[n][over] = got[n].cpu().double()[over]
+    _compare(got, ref, dtype)
