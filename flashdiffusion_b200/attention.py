@@ -21,7 +21,8 @@ Everything runs on the current stream and may be captured into a graph.  Where a
 captured step takes gradients of leaves (``backward`` into ``.grad``), run its
 warm-up on a side stream, or drop every output of earlier eager steps first: a
 leaf whose gradient node was made on the default stream, and is kept alive by
-such an output, pulls that stream into the capture, which torch cannot do.
+such an output, pulls that stream into the capture, which torch cannot do.  Forward-mode tangents (``torch.func.jvp``, dual tensors)
+are refused.
 """
 
 from __future__ import annotations
@@ -209,6 +210,7 @@ class _Attend(torch.autograd.Function):
     def backward(ctx, do, *_):
         if torch.is_grad_enabled():
             raise RuntimeError("attend has no second derivative: call backward without create_graph")
+        native.refuse_duals("the gradient of attend", do)
         q, k, v, o, kept, lse = ctx.saved_tensors[:6]
         do = _loadable(do)
         dq, dk, dv = _like(q), _like(k), _like(v)
@@ -240,6 +242,7 @@ def _check(q, k, v, slopes, scale, cap, names):
         raise ValueError(f"scale must be finite (got {scale})")
     if cap and not 1e-3 <= cap < math.inf:
         raise ValueError(f"cap must be None or at least 1e-3 (got {cap})")
+    native.refuse_duals("attention", q, k, v, slopes)
     native.require_device(q.device)
     return scale, cap
 

@@ -14,6 +14,7 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libfd_sm100.so")
@@ -163,6 +164,15 @@ def require_device(device=None) -> torch.device:
         cap = torch.cuda.get_device_capability(idx)
         raise RuntimeError(f"device {idx} has compute capability {cap}; libfd_sm100 needs 10.x (B200)")
     return _devices.setdefault(idx, torch.device("cuda", idx))
+
+
+def refuse_duals(what: str, *tensors) -> None:
+    """Raise where a tensor carries a forward-mode tangent: a kernel reads the primal alone, and the tangent of the
+    result would be gone without an error.  None stands for an argument that was not given."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: take reverse mode, or detach its inputs")
 
 
 def call(fn, device: torch.device, *args) -> None:

@@ -408,6 +408,7 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, *grads):
         if torch.is_grad_enabled():
             raise RuntimeError("apply_rotary has no second derivative: call backward without create_graph")
+        native.refuse_duals("the gradient of apply_rotary", *grads)
         positions, freqs = ctx.saved_tensors
         layout, magnitude, inverse = ctx.how
         return (None,) * 5 + tuple(_rotate_heads(grads, positions, freqs, layout, magnitude, not inverse, False))
@@ -424,7 +425,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: t
 
     layout "half" pairs coordinate p with p + R/2, "interleaved" 2p with 2p + 1 (as ROPE does).  ``magnitude``
     scales the rotated coordinates, ``inverse`` turns the other way.  ``inplace`` overwrites q and k (no
-    gradients; q and k must not overlap).  Returns the rotated q, or (q, k).
+    gradients; q and k must not overlap).  Forward-mode tangents are refused.  Returns the rotated q,
+    or (q, k).
     """
     xs = (q,) if k is None else (q, k)
     for name, x in zip("qk", xs):
@@ -453,6 +455,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: t
         raise ValueError("q, positions and freqs must be on one device")
     if positions.requires_grad or freqs.requires_grad:
         raise ValueError("apply_rotary has no gradient for positions and freqs: detach them")
+    native.refuse_duals("apply_rotary", q, k, positions, freqs)
     native.require_device(device)
     grad = torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad)
     if inplace and grad:
