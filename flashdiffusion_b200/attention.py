@@ -21,8 +21,8 @@ Everything runs on the current stream and may be captured into a graph.  Where a
 captured step takes gradients of leaves (``backward`` into ``.grad``), run its
 warm-up on a side stream, or drop every output of earlier eager steps first: a
 leaf whose gradient node was made on the default stream, and is kept alive by
-such an output, pulls that stream into the capture, which torch cannot do.  Forward-mode tangents (``torch.func.jvp``, dual tensors)
-are refused.
+such an output, pulls that stream into the capture, which torch cannot do.  Forward-mode tangents (``torch.func.jvp``, dual tensors) and tracing
+(``torch.jit.trace``, ``make_fx``) are refused.
 """
 
 from __future__ import annotations

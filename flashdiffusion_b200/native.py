@@ -175,8 +175,17 @@ def refuse_duals(what: str, *tensors) -> None:
                 raise RuntimeError(f"{what} has no forward-mode derivative: take reverse mode, or detach its inputs")
 
 
+_TRACERS = tuple(getattr(torch._C._TorchDispatchModeKey, k) for k in ("PROXY", "FAKE", "FUNCTIONAL"))
+
+
+def _tracing() -> bool:
+    return torch.jit.is_tracing() or any(torch._C._get_dispatch_mode(k) is not None for k in _TRACERS)
+
+
 def call(fn, device: torch.device, *args) -> None:
     """fn(*args, current stream of the device) with that device current; raises on an error code."""
+    if _tracing():     # a record of this call would hold the outputs' allocation and nothing that fills them
+        raise RuntimeError("calls of libfd_sm100 cannot be traced: capture them into a CUDA graph instead")
     if torch._C._cuda_getDevice() == device.index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:

@@ -425,7 +425,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, positions: t
 
     layout "half" pairs coordinate p with p + R/2, "interleaved" 2p with 2p + 1 (as ROPE does).  ``magnitude``
     scales the rotated coordinates, ``inverse`` turns the other way.  ``inplace`` overwrites q and k (no
-    gradients; q and k must not overlap).  Forward-mode tangents are refused.  Returns the rotated q,
+    gradients; q and k must not overlap).  Forward-mode tangents and tracing are refused.  Returns the rotated q,
     or (q, k).
     """
     xs = (q,) if k is None else (q, k)

@@ -1,7 +1,8 @@
-"""Derivatives that a call of the kernels would drop: refused, not lost (no GPU: the library is stubbed)."""
+"""Derivatives and records that a call of the kernels would drop: refused, not lost (no GPU: the library is stubbed)."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from flashdiffusion_b200 import attention, native, rope
 
@@ -58,3 +59,20 @@ def test_tangents_of_an_incoming_gradient_are_refused():
             g = fwd.make_dual(torch.ones_like(o), torch.ones_like(o))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(o, leaf, g)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("name", CALLS)
+def test_tracing_is_refused(name):
+    x, f = CALLS[name]
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(f, x.clone(), check_trace=False)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(f)(x.clone())
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_tracing_of_spans_is_refused():
+    for f in (lambda x: attention.document_spans(x, 8).end, lambda x: attention.prefix_spans(x, 8).end):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, torch.tensor([0, 8], dtype=torch.int32), check_trace=False)
