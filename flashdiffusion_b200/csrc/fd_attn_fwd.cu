@@ -51,8 +51,8 @@ struct Cfg {
     static constexpr uint32_t Q_BYTES = SUBTILES * TILE;
     static constexpr int SLOTS = DP == 64 ? 8 : DP == 128 ? 5 : 2;
     static constexpr uint32_t BAR_OFF = Q_BYTES + SLOTS * TILE;
-    // qfull, full[SLOTS], empty[SLOTS], sfull[2], pfull[2], ofull[2], toguard, guarded
-    static constexpr int NBARS = 1 + 2 * SLOTS + 6 + 2;
+    // qfull, full[SLOTS], empty[SLOTS], sfull[2], pfull[2], ofull[2], toguard, guarded, rest
+    static constexpr int NBARS = 1 + 2 * SLOTS + 6 + 3;
     static constexpr uint32_t MISC_OFF = BAR_OFF + NBARS * 8;
     // maxima and, at the end, sums of a row's two threads: [2 subtiles][2 halves][128]
     static constexpr uint32_t MEET_OFF = (MISC_OFF + 64 + 15) / 16 * 16;
@@ -99,6 +99,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
     uint64_t* ofull = pfull + 2;
     uint64_t* toguard = ofull + 2;
     uint64_t* guarded = toguard + 1;
+    uint64_t* rest = guarded + 1;
     Misc& ms = *(Misc*)(base + C::MISC_OFF);
     volatile int* abort = &ms.abort;
 
@@ -128,6 +129,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         }
         ptx::mbar_init(toguard, 1);
         ptx::mbar_init(guarded, 1);
+        ptx::mbar_init(rest, 1);
         ms.abort = 0;
         ms.poison = 0;
         ptx::fence_mbar_init();
@@ -273,6 +275,10 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
                 }
                 mma_commit(lead, &empty[slot_of(iv)]);
                 if (j + 1 < t1) mma_commit(lead, &empty[slot_of(ik)]);
+            }
+            if (!ok) {   // gave up: products in flight still read this block's memory and write its columns
+                mma_commit(lead, rest);
+                wait_landed(rest, 0);
             }
         }
     } else if (warp == GUARD_WARP) {
