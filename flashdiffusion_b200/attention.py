@@ -23,6 +23,11 @@ warm-up on a side stream, or drop every output of earlier eager steps first: a
 leaf whose gradient node was made on the default stream, and is kept alive by
 such an output, pulls that stream into the capture, which torch cannot do.  Forward-mode tangents (``torch.func.jvp``, dual tensors) and tracing
 (``torch.jit.trace``, ``make_fx``) are refused.
+
+The kernels' waits are bounded.  One that gives up (after two seconds, which nothing but a fault of the device or of
+these kernels should bring about) raises no error by itself, since a call does not wait for the GPU: it leaves NaN in
+the rows that were not finished and a mark that ``flashdiffusion_b200.native.check_status(device)`` turns into an
+``FDError``.  A program that wants to know calls that where it waits for results anyway, once a step say.
 """
 
 from __future__ import annotations

@@ -987,7 +987,9 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
                                    : compute_query<DP, F16, GEN>(c, br, lanes, half, row, up * p_back, abort, status);
         const bool have = c.items > 0 && ok && ptx::wait_bounded(br.accfull, 0, abort, status, WAIT_NS);
         ptx::tc_fence_after();
-        const float back = a.scale / up;
+        // gave up: NaN, not numbers that could pass for the sums (store_cols has zeros in their place)
+        const float given = c.items > 0 && !have ? __int_as_float(0x7fffffff) : 1.f;
+        const float back = given * a.scale / up;
         // this row's sums of this part, if there are parts
         auto sums = [&](float* to, int rows, int heads) {
             return parts > 1 ? to + ((((int64_t)part * a.batch + c.b) * rows + row) * heads + c.h) * a.dim : nullptr;
@@ -999,7 +1001,7 @@ gradient_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__
         } else if (half == 0) {
             uint8_t* out = (uint8_t*)a.dv.p + 2 * (c.b * a.dv.sb + (int64_t)row * a.dv.ss + c.h * a.dv.sh);
             float* to = sums(w.dv, a.k_len, a.kv_heads);
-            store_cols<DP, F16>(lanes + 256, p_back, out, to, 0, a.dim, row < a.k_len, have);
+            store_cols<DP, F16>(lanes + 256, given * p_back, out, to, 0, a.dim, row < a.k_len, have);
             if (have && row < a.k_len && *(volatile int*)&ms.poison) put_back<F16>(c, out, to, row);
         } else {
             uint8_t* out = (uint8_t*)a.dk.p + 2 * (c.b * a.dk.sb + (int64_t)row * a.dk.ss + c.h * a.dk.sh);

@@ -454,6 +454,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         meet[0] = l;
         both_here(ok);
         l += other[0];
+        if (!ok) l = __int_as_float(0x7fffffff);   // gave up: NaN, not numbers that could pass for the rows
         const bool real = sub < C::SUBTILES && row < a.q_len;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint8_t* out = (uint8_t*)a.o.p + 2 * (b * a.o.sb + (int64_t)row * a.o.ss + h * a.o.sh);
@@ -466,6 +467,9 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             if (it > 0 && ok) {
                 ptx::tmem_ld16(o_addr + g, o);
                 ptx::tmem_wait_ld16(o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = 0;
             }
             float(&f)[16] = reinterpret_cast<float(&)[16]>(o);
 #pragma unroll

@@ -137,3 +137,16 @@ def test_sequences_and_key_heads_do_not_touch_each_other(dtype):
             assert (got[n].cpu().double()[over] == ref[n][over].sign() * float("inf")).all()
             ref[n][over] = got[n].cpu().double()[over]
     _compare(got, ref, dtype)
+
+
+def test_a_wait_that_gave_up_is_reported():
+    """As the module says: the mark stays through later calls, and check_status raises for it once."""
+    from flashdiffusion_b200 import attention, native
+    q, k, v, do = _inputs(1, 200, 200, 2, 1, 64, BF)
+    native.check(native.load().fd_selftest_wait_timeout(10_000_000, native._stream(q.device)))
+    _step(q, k, v, do)
+    with pytest.raises(native.FDError) as e:
+        native.check_status(q.device)
+    assert e.value.code == native.FD_ERR_TIMEOUT
+    native.check_status(q.device)
+    assert "check_status" in attention.__doc__
