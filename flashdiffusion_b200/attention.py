@@ -290,7 +290,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     cap      scores become cap tanh(score / cap)
     slopes   (H,) float32: slope times the distance |position - j| is subtracted from the scores
     Returns the output (as q), or (output, lse): lse (B, H, Sq) float32 is the natural log of the sum of
-    exp(scores), -inf for rows that see nothing; it carries no gradient.
+    exp(scores), -inf for rows that see nothing; it carries no gradient.  A row that sees keys, but none above a score of
+    -infinity, is NaN.
     """
     _tensors(("q", "k", "v"), (q, k, v))
     scale, cap = _check(q, k, v, slopes, scale, cap, ("q", "k", "v"))

@@ -61,6 +61,12 @@ __device__ __forceinline__ int2 row_span(const Prob& a, int b, int i, int n) {
     return make_int2(min(lo, hi), hi);
 }
 
+// Sum of weights `l` of a row that sees keys `span`: a row whose visible scores are all -infinity has no softmax, and
+// says so, where a row that sees nothing is zeros.
+__device__ __forceinline__ float sum_or_nan(float l, int2 span) {
+    return l == 0.f && span.y > span.x ? __int_as_float(0x7fffffff) : l;
+}
+
 // Launchers (fd_attn_simt.cu).
 int simt_forward(const Prob& a, int dtype, cudaStream_t s);
 int simt_backward(const Prob& a, int dtype, float* delta, cudaStream_t s);   // delta: batch * heads * q_len floats

@@ -454,8 +454,10 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         meet[0] = l;
         both_here(ok);
         l += other[0];
-        if (!ok) l = __int_as_float(0x7fffffff);   // gave up: NaN, not numbers that could pass for the rows
         const bool real = sub < C::SUBTILES && row < a.q_len;
+        if (m == -INFINITY) l = 0.f;               // exponentials on the FMA pipe end at 2^-125, above zero
+        if (sp.parts == 1 && real) l = sum_or_nan(l, span);
+        if (!ok) l = __int_as_float(0x7fffffff);   // gave up: NaN, not numbers that could pass for the rows
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint8_t* out = (uint8_t*)a.o.p + 2 * (b * a.o.sb + (int64_t)row * a.o.ss + h * a.o.sh);
         int8_t* low = a.o_low ? a.o_low + (((int64_t)b * a.q_len + row) * a.heads + h) * a.dim : nullptr;
@@ -540,10 +542,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, f[e], acc[e]);
     }
+    const int64_t t = r / a.heads, b = t / a.q_len, row = t - b * a.q_len;
+    if (sum == 0.f) sum = sum_or_nan(sum, row_span(a, (int)b, (int)row, keys_of(a, (int)b)));
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] *= inv;
-    const int64_t t = r / a.heads, b = t / a.q_len, row = t - b * a.q_len;
     const int h = (int)(r - t * a.heads);
     store8<F16>((uint16_t*)a.o.p + b * a.o.sb + row * a.o.ss + h * a.o.sh + d, a.o_low ? a.o_low + r * a.dim + d : nullptr, acc);
     if (d == 0 && a.lse)

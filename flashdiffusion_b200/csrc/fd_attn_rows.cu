@@ -221,6 +221,7 @@ template <bool F16>
 __device__ __forceinline__ void store_row(const Prob& a, const Plan& p, int b, int hk, int gr, int d,
                                           const float (&acc)[8], float m, float l) {
     const int i = p.query(gr), h = hk * a.group + gr - i * a.group;
+    if (l == 0.f) l = sum_or_nan(l, row_span(a, b, i, keys_of(a, b)));
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (d < a.dim) {
         float f[8];

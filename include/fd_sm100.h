@@ -322,7 +322,8 @@ int fd_rotary(const fd_rotary_args* args, void* stream);
  * to [0, k_len]).  The span of row i is first[b, i] .. end[b, i] when both
  * arrays are given (clamped to [0, n)); otherwise end_i = pos_i + 1 when causal
  * != 0, else n, and first_i = pos_i - window + 1 when window > 0 (causal only),
- * else 0.  A row with an empty span gives zeros and lse = -inf and no gradient.
+ * else 0.  A row with an empty span gives zeros and lse = -inf and no gradient;
+ * one that sees keys but none above a score of -infinity gives NaN.
  * Keys outside a row's span never reach it, whatever their memory holds (NaN
  * and infinities included).
  * ------------------------------------------------------------------------- */

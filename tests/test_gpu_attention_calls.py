@@ -150,3 +150,56 @@ def test_a_wait_that_gave_up_is_reported():
     assert e.value.code == native.FD_ERR_TIMEOUT
     native.check_status(q.device)
     assert "check_status" in attention.__doc__
+
+
+# forward kernels: whole and cut key axes of both tile heights, few rows, fp32 and odd heads by tiles and by rows
+SIZES = [(1, 300, 700, 2, 1, 64, BF), (1, 300, 700, 2, 1, 128, HF), (4, 700, 300, 40, 4, 64, BF), (1, 200, 2000, 2, 1, 256, BF),
+         (1, 140, 3000, 1, 1, 128, BF), (1, 3, 700, 4, 2, 128, HF), (2, 8, 5000, 4, 2, 64, BF), (1, 300, 700, 2, 1, 48, SF),
+         (1, 300, 700, 2, 1, 20, BF), (1, 2, 700, 2, 1, 40, SF)]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,dtype", SIZES, ids=str)
+def test_a_row_of_minus_infinities_has_no_softmax(b, sq, sk, h, hk, d, dtype, causal):
+    """An infinite coordinate of q against keys of the other sign: NaN whatever the mask, and the other rows as ever."""
+    q, k, v, do = _inputs(b, sq, sk, h, hk, d, dtype, seed=81)
+    k[..., 0] = -1
+    kw = dict(causal=causal, cap=None)
+    want = _step(q, k, v, do, **kw)
+    at = sq // 2
+    if causal and sk < sq:
+        at = max(at, sq - sk)                     # a row that sees something
+    q[:, at, :, 0] = float("inf")
+    got = _step(q, k, v, do, **kw)
+    other = torch.arange(sq, device="cuda") != at
+    assert got["o"][:, at].isnan().all() and got["lse"][:, :, at].isnan().all() and got["dq"][:, at].isnan().all()
+    assert torch.equal(got["o"][:, other], want["o"][:, other]) and torch.equal(got["dq"][:, other], want["dq"][:, other])
+    assert torch.equal(got["lse"][:, :, other], want["lse"][:, :, other])
+
+
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,dtype", SIZES, ids=str)
+def test_keys_at_minus_infinity_weigh_nothing(b, sq, sk, h, hk, d, dtype):
+    """The first keys of all rows at score -infinity (whole tiles of them): as if they were masked."""
+    from flashdiffusion_b200.attention import attend
+    q, k, v, _ = _inputs(b, sq, sk, h, hk, d, dtype, seed=83)
+    q[..., 0], away = 1, 2 * sk // 3
+    k[:, :away, :, 0] = float("-inf")
+    o, lse = attend(q, k, v, return_lse=True)
+    first = torch.full((1, sq), away)
+    lo, hi, pos = spans_of(sq, sk, b, first=first, end=torch.full((1, sq), sk))
+    ref = reference(q, k, v, lo, hi, pos)
+    check("o", o, ref, FLOOR[dtype])
+    check("lse", lse, ref)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (BF, 256), (SF, 32)], ids=str)
+def test_a_cached_row_of_minus_infinities_has_no_softmax(dtype, d):
+    from flashdiffusion_b200.attention import attend_cached
+    lengths = torch.tensor([0, 1, 130, 900], dtype=torch.int32, device="cuda")
+    q, k, v, _ = _inputs(4, 2, 900, 4, 2, d, dtype, seed=85)
+    k[..., 0] = -1
+    q[:, 1, :, 0] = float("inf")
+    o, lse = attend_cached(q, k, v, lengths, return_lse=True)
+    assert (o[0] == 0).all() and (lse[0] == float("-inf")).all()
+    assert o[1:, 1].isnan().all() and lse[1:, :, 1].isnan().all()
+    assert (o[1, 0] == 0).all() and o[2:, 0].isfinite().all() and lse[2:, :, 0].isfinite().all()
