@@ -21,9 +21,11 @@
 // free (Q is loaded the same way), and so is the order of output coordinates in
 // V^T P^T; the pairs of keys that a V^T fragment wants are put together by byte
 // permutes, and P^T is turned from accumulator to operand by movmatrix.  P is
-// split in two 16-bit parts, so that it adds no rounding of its own.  m is raised
-// only when a score exceeds it by more than 8, so the usual block needs no
-// exchange between lanes.
+// split in two 16-bit parts, good to 2^-17 (bf16) and 2^-22 (fp16) of a weight, so
+// that it adds next to no rounding of its own.  fp16 ends at 2^-24: P is held times
+// 2^7 there, and weights down to 2^-31 of the largest keep a bit.  m is raised only
+// when a score exceeds it by more than 8 (P then stays below 2^8, fp16 2^15), so
+// the usual block needs no exchange between lanes.
 #include <algorithm>
 
 #include "fd_attn_tc.cuh"
@@ -39,6 +41,9 @@ constexpr int SETUP = 3;
 // three blocks, 44 so), else two.
 __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 __host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 2 : 3; }
+
+// log2 of what P, and with it l and O, are held times.
+template <bool F16> constexpr float P_SHIFT = F16 ? 7.f : 0.f;
 
 struct Range {
     int lo, hi;   // keys seen by any row of the sequence, lo on a multiple of 16
@@ -230,7 +235,7 @@ __device__ __forceinline__ void store_row(const Prob& a, const Plan& p, int b, i
         store8<F16>((uint16_t*)a.o.p + b * a.o.sb + (int64_t)i * a.o.ss + h * a.o.sh + d,
                     a.o_low ? a.o_low + (((int64_t)b * a.q_len + i) * a.heads + h) * a.dim + d : nullptr, f);
     }
-    if (d == 0 && a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    if (d == 0 && a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = l == 0.f ? -INFINITY : (m + (log2f(l) - P_SHIFT<F16>)) * LN2;
 }
 
 template <int DP, int NT>
@@ -404,7 +409,8 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                             s[y][k][z] = fmaf(-2.f * cap2, ptx::rcp_mufu(1.f + e), cap2);
                         }
             }
-            // s becomes score - m (score itself while m is not yet a number)
+            // s becomes score - m + SH (score + SH while m is not yet a number)
+            constexpr float SH = P_SHIFT<F16>;
             const float mul = cap2 > 0.f ? 1.f : c;
             float top[NT][2];
             bool raise = false;
@@ -412,7 +418,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
             for (int y = 0; y < NT; ++y)
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    const float nb = m[y][z] == -INFINITY ? 0.f : -m[y][z];
+                    const float nb = m[y][z] == -INFINITY ? SH : SH - m[y][z];
                     const float sl = slope2[y][z], far = at[y][z] - step, from = fmaf(-sl, far, nb);
 #pragma unroll
                     for (int k = 0; k < KT; ++k)
@@ -436,7 +442,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                     top[y][z] = fmaxf(s[y][0][z], s[y][0][2 + z]);
 #pragma unroll
                     for (int k = 1; k < KT; ++k) top[y][z] = fmaxf(top[y][z], fmaxf(s[y][k][z], s[y][k][2 + z]));
-                    raise = raise || top[y][z] > (m[y][z] == -INFINITY ? -INFINITY : 8.f);
+                    raise = raise || top[y][z] > (m[y][z] == -INFINITY ? -INFINITY : 8.f + SH);
                 }
             if (__any_sync(~0u, raise)) {
 #pragma unroll
@@ -448,6 +454,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 8));
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 16));
                         const bool fresh = m[y][z] == -INFINITY;
+                        tp -= SH;                                 // by how much m rises, or its first value
                         if (!fresh) tp = fmaxf(tp, 0.f);
                         if (tp == -INFINITY) continue;            // still nothing seen
                         const float fix = fresh ? 0.f : ptx::ex2_mufu(-tp);

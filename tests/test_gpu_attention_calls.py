@@ -203,3 +203,28 @@ def test_a_cached_row_of_minus_infinities_has_no_softmax(dtype, d):
     assert (o[0] == 0).all() and (lse[0] == float("-inf")).all()
     assert o[1:, 1].isnan().all() and lse[1:, :, 1].isnan().all()
     assert (o[1, 0] == 0).all() and o[2:, 0].isfinite().all() and lse[2:, :, 0].isfinite().all()
+
+
+@pytest.mark.parametrize("new,h,hk,d", [(1, 8, 4, 128), (1, 4, 4, 64), (3, 8, 4, 64), (4, 16, 4, 128)])
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("above", [15.0, 17.0])
+def test_small_weights_of_a_cache_are_kept(above, dtype, new, h, hk, d):
+    """The newest tokens' keys `above` nats over all others, with values of zero: the output is the small weights' alone.
+    2^-24 of the largest weight is below fp16's own range, and here the many small ones are all there is.  So many
+    sequences that one warp goes on from the newest keys to a quarter of the others."""
+    from flashdiffusion_b200.attention import attend_cached
+    b, keys = 160, 600
+    q, k, v, _ = _inputs(b, new, keys, h, hk, d, dtype, seed=87)
+    q[..., 0], k[..., 0] = 4, 0
+    q[..., 1:] /= 16
+    k[:, -new:, :, 0] = above * d ** 0.5 / 4
+    v[:, -new:] = 0
+    v = v.abs()
+    n = torch.full((b,), keys, dtype=torch.int32, device="cuda")
+    lo, hi, pos = spans_of(new, keys, b, causal=True, lengths=n.cpu())
+    ref = reference(q, k, v, lo, hi, pos)
+    o, lse = attend_cached(q, k, v, n, return_lse=True)
+    # beside the definition's bounds: fp16 holds a weight to 2^-25 at 2^7 times the largest, and the sum of weights is at
+    # least the largest, so each value may come with 2^-32 too much or too little
+    check("o", o, ref, 2.0 ** -32 * float(v.double().sum(1).max()) + FLOOR[dtype])
+    check("lse", lse, ref)
