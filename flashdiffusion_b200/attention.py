@@ -162,6 +162,9 @@ def _arguments(q, k, v, o, lse, low, how, gradients=_NO_GRADIENTS) -> bytes:
 
 
 def _call(fn, args, backward, q):
+    if torch._C._cuda_getDevice() != q.device.index:      # sizes depend on the number of SMs of the current device
+        with torch.cuda.device(q.device):
+            return _call(fn, args, backward, q)
     # the caching allocator's own buffer for each call: streams and captured graphs never share it
     nbytes = native.load().fd_attention_workspace_bytes(args, backward)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
