@@ -123,9 +123,13 @@ __device__ __forceinline__ bool inside32(const uint64_t (&s)[16], float limit) {
     for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(ptx::lo2(s[i])), fabsf(ptx::hi2(s[i]))));
     return __all_sync(~0u, top <= limit);
 }
-// x = cap2 tanh(c x)
-__device__ __forceinline__ void cap32(uint64_t (&x)[16], const Score& sc) {
-    if (inside32(x, sc.limit)) {
+// x = cap2 tanh(c x).  `hide(x)` takes masked places out (zeros) and says whether there can be any: what lies in them
+// must not choose the form for the others, whose last bits differ between the two.
+template <class Hide>
+__device__ __forceinline__ void cap32(uint64_t (&x)[16], const Score& sc, Hide hide) {
+    bool inside = inside32(x, sc.limit);
+    if (!inside && hide(x)) inside = inside32(x, sc.limit);
+    if (inside) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = ptx::mul2(sc.ratio(x[i]), x[i]);
     } else {

@@ -228,3 +228,37 @@ def test_small_weights_of_a_cache_are_kept(above, dtype, new, h, hk, d):
     # least the largest, so each value may come with 2^-32 too much or too little
     check("o", o, ref, 2.0 ** -32 * float(v.double().sum(1).max()) + FLOOR[dtype])
     check("lse", lse, ref)
+
+
+@pytest.mark.parametrize("bad", [6e4, float("inf"), float("nan")], ids=str)
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (SF, 48)], ids=str)
+@pytest.mark.parametrize("kind,sq,sk", [("documents", 400, 400), ("holes", 2300, 500), ("window", 130, 700)])
+def test_masked_places_hold_anything_under_a_wide_cap(kind, sq, sk, dtype, d, bad):
+    """All visible scores well inside their cap, masked ones beyond it: the same bits."""
+    q, k, v, do = _inputs(1, sq, sk, 4, 2, d, dtype, seed=91)
+    kw, unseen, empty = _spans(kind, sq, sk)
+    kw["cap"] = 50.0
+    want = _step(q, k, v, do, **kw)
+    q2, k2, v2, do2 = (t.clone() for t in (q, k, v, do))
+    for t in (k2, v2):
+        t[:, unseen] = bad
+    for t in (q2, do2):
+        t[:, empty] = bad
+    got = _step(q2, k2, v2, do2, **kw)
+    for n in got:
+        assert torch.equal(got[n], want[n]), n
+
+
+@pytest.mark.parametrize("dtype,d,new", [(BF, 128, 1), (HF, 64, 3), (BF, 256, 1), (SF, 64, 2)], ids=str)
+def test_a_cache_holds_anything_behind_a_row_under_a_wide_cap(dtype, d, new):
+    """Several new tokens: the keys of later ones are hidden from the earlier, whatever they hold, and the end of the
+    cache from all."""
+    from flashdiffusion_b200.attention import attend_cached
+    q, k, v, _ = _inputs(2, new, 300, 4, 2, d, dtype, seed=93)
+    n = torch.tensor([290, 17], dtype=torch.int32, device="cuda")
+    want = attend_cached(q, k, v, n, cap=50.0)
+    k2, v2 = k.clone(), v.clone()
+    for b, m in ((0, 290), (1, 17)):
+        k2[b, m - new + 1:] = v2[b, m - new + 1:] = 6e4
+    got = attend_cached(q, k2, v2, n, cap=50.0)
+    assert torch.equal(got[:, 0], want[:, 0])
