@@ -572,13 +572,12 @@ __device__ __forceinline__ void watch(const Cta& c, const Bars& br, uint8_t* bas
     }
 }
 
-// Raw products of one row, 32 columns, to weights: x = 2^(score + add); with a cap, bend = 1 - tanh^2 (`hide` as cap32
-// has it).
-template <bool GEN, class Hide>
+// Raw products of one row, 32 columns, to weights: x = 2^(score + add); with a cap, bend = 1 - tanh^2.
+template <bool GEN>
 __device__ __forceinline__ void weights32(uint64_t (&x)[16], const uint64_t (&add)[16], const Score& sc, float slope2,
-                                          float dist, float by, int side, uint64_t (&bend)[GEN ? 16 : 1], Hide hide) {
+                                          float dist, float by, int side, uint64_t (&bend)[GEN ? 16 : 1]) {
     if (GEN && sc.capped) {
-        cap32(x, sc, hide);
+        cap32(x, sc);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             bend[e] = ptx::fma2(ptx::mul2(x[e], sc.shrink), x[e], ptx::both2(1.f));
@@ -663,23 +662,19 @@ __device__ __forceinline__ bool compute_key(const Cta& c, const Bars& br, const 
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             uint64_t bend[GEN ? 16 : 1];
-            // zeros where this key is not seen
-            auto hide = [&](uint64_t (&y)[16]) {
-                if (!masked) return false;
+            weights32<GEN>(x[g], add[g], sc, slope2, (float)(shift + q0 + g * 32 - row), 1.f, side, bend);
+            if (masked) {
                 if (!a.first) {
                     // the queries that see this key are a run: i >= row - shift, and i < that + window
                     const int lo = a.causal ? row - shift : row < c.n ? INT_MIN / 2 : INT_MAX / 2;
                     const int64_t hi = row >= c.n ? lo : a.window ? (int64_t)row - shift + a.window : a.q_len;
                     const int l0 = max(lo, 0) - (q0 + g * 32), l1 = (int)min(hi, (int64_t)a.q_len) - (q0 + g * 32);
-                    if (!__all_sync(~0u, l0 <= 0 && l1 >= 32)) mask32(y, l0, (uint32_t)max(l1 - l0, 0), 0.f);
+                    if (!__all_sync(~0u, l0 <= 0 && l1 >= 32)) mask32(x[g], l0, (uint32_t)max(l1 - l0, 0), 0.f);
                 } else {
                     const uint32_t bits = seen32(see[g], row - lane, lane);
-                    if (!__all_sync(~0u, bits == ~0u)) keep32(y, bits);
+                    if (!__all_sync(~0u, bits == ~0u)) keep32(x[g], bits);
                 }
-                return true;
-            };
-            weights32<GEN>(x[g], add[g], sc, slope2, (float)(shift + q0 + g * 32 - row), 1.f, side, bend, hide);
-            hide(x[g]);
+            }
             uint32_t p[16];
             round32<F16>(x[g], p);
             ptx::tmem_st16(lanes + half * 64 + g * 16, p);
@@ -775,18 +770,16 @@ __device__ __forceinline__ bool compute_query(const Cta& c, const Bars& br, uint
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             uint64_t bend[GEN ? 16 : 1];
-            const int lo = span.x - k0 - g * 32;
-            auto hide = [&](uint64_t (&y)[16]) {
-                if (masked && !__all_sync(~0u, lo <= 0 && (int64_t)lo + (span.y - span.x) >= 32))
-                    mask32(y, lo, (uint32_t)(span.y - span.x), 0.f);
-                return masked;
-            };
-            weights32<GEN>(x[g], add, sc, slope2, (float)(shift + row - k0 - g * 32), -1.f, side, bend, hide);
+            weights32<GEN>(x[g], add, sc, slope2, (float)(shift + row - k0 - g * 32), -1.f, side, bend);
             if (GEN && sc.capped) {   // before the mask: a masked pair's bend may be a NaN
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[g][e] = ptx::mul2(x[g][e], bend[e]);
             }
-            hide(x[g]);
+            if (masked) {
+                const int lo = span.x - k0 - g * 32;
+                if (!__all_sync(~0u, lo <= 0 && (int64_t)lo + (span.y - span.x) >= 32))
+                    mask32(x[g], lo, (uint32_t)(span.y - span.x), 0.f);
+            }
         }
         const uint32_t dp = lanes + 128 + buf * 128 + half * 64;
         if (!ptx::wait_bounded(&br.dpfull[buf], (i >> 1) & 1, abort, status, WAIT_NS)) return false;

@@ -372,10 +372,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
 #pragma unroll
                     for (int g = 0; g < 2; ++g) {
                         if (sc.capped) {
-                            cap32(x[g], sc, [&](uint64_t (&y)[16]) {
-                                if (masked) mask32(y, lo - g * 32, (uint32_t)len, 0.f);
-                                return masked;
-                            });
+                            cap32(x[g], sc);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 16; ++i) x[g][i] = ptx::mul2(x[g][i], sc.c);

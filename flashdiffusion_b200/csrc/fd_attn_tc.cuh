@@ -85,12 +85,12 @@ __device__ __forceinline__ void product_sum(uint32_t lead, uint32_t d, uint32_t 
 //   x = cap2 tanh(c s) + add            (c = scale / cap, cap2 = cap log2(e))
 // minus slope2 |distance| (slope2 = slope log2(e)).
 //
-// The tanh has two forms.  |c s| <= 0.45 for the whole warp (scores well inside
-// their cap, the usual case): an odd degree-7 polynomial in the raw product, with
-// c and cap2 in its coefficients, on the FMA pipe in packed pairs (absolute error
-// of the tanh 9e-8; weighted least squares on Chebyshev nodes).  Otherwise
-// 1 - 2 / (1 + e^2u) with two MUFU operations, absolute error 2e-7: with the
-// softmax's own that makes three MUFU operations a pair, and MUFU the bound.
+// The tanh has two forms.  |c s| <= 0.45 (scores well inside their cap, the usual
+// case): an odd degree-7 polynomial in the raw product, with c and cap2 in its
+// coefficients, on the FMA pipe in packed pairs (absolute error of the tanh 9e-8;
+// weighted least squares on Chebyshev nodes).  Otherwise 1 - 2 / (1 + e^2u) with
+// two MUFU operations, absolute error 2e-7: with the softmax's own that makes
+// three MUFU operations a pair, and MUFU the bound.
 struct Score {
     uint64_t c, cap2;            // both halves the same
     uint64_t b0, b1, b2, b3;     // cap2 tanh(c s) = s (b0 + b1 s^2 + b2 s^4 + b3 s^6)
@@ -123,13 +123,10 @@ __device__ __forceinline__ bool inside32(const uint64_t (&s)[16], float limit) {
     for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(fabsf(ptx::lo2(s[i])), fabsf(ptx::hi2(s[i]))));
     return __all_sync(~0u, top <= limit);
 }
-// x = cap2 tanh(c x).  `hide(x)` takes masked places out (zeros) and says whether there can be any: what lies in them
-// must not choose the form for the others, whose last bits differ between the two.
-template <class Hide>
-__device__ __forceinline__ void cap32(uint64_t (&x)[16], const Score& sc, Hide hide) {
-    bool inside = inside32(x, sc.limit);
-    if (!inside && hide(x)) inside = inside32(x, sc.limit);
-    if (inside) {
+// x = cap2 tanh(c x).  Each score is a function of its own product alone, and so what lies in masked places, or in
+// another row, changes no bit of it: the vote only leaves out the form that no score of the warp takes.
+__device__ __forceinline__ void cap32(uint64_t (&x)[16], const Score& sc) {
+    if (inside32(x, sc.limit)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = ptx::mul2(sc.ratio(x[i]), x[i]);
     } else {
@@ -137,8 +134,11 @@ __device__ __forceinline__ void cap32(uint64_t (&x)[16], const Score& sc, Hide h
         const float c = ptx::lo2(sc.c) * (2.f * LOG2E), top = ptx::lo2(sc.cap2);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float e0 = ptx::ex2_mufu(ptx::lo2(x[i]) * c), e1 = ptx::ex2_mufu(ptx::hi2(x[i]) * c);
-            x[i] = ptx::pack2(fmaf(-2.f * top, ptx::rcp_mufu(1.f + e0), top), fmaf(-2.f * top, ptx::rcp_mufu(1.f + e1), top));
+            const float s0 = ptx::lo2(x[i]), s1 = ptx::hi2(x[i]);
+            const uint64_t near = ptx::mul2(sc.ratio(x[i]), x[i]);
+            const float e0 = ptx::ex2_mufu(s0 * c), e1 = ptx::ex2_mufu(s1 * c);
+            const float far0 = fmaf(-2.f * top, ptx::rcp_mufu(1.f + e0), top), far1 = fmaf(-2.f * top, ptx::rcp_mufu(1.f + e1), top);
+            x[i] = ptx::pack2(fabsf(s0) <= sc.limit ? ptx::lo2(near) : far0, fabsf(s1) <= sc.limit ? ptx::hi2(near) : far1);
         }
     }
 }
