@@ -245,7 +245,8 @@ struct Smem {
     static constexpr uint32_t HALF = KEYS * DP * 2;               // K or V of a block, 4 KB
     static constexpr uint32_t RING = WARPS * STAGES * 2 * HALF;
     static constexpr int PIECES = DP / 16 + 1;                    // 16-byte pieces of one lane's sums: O, and m and l
-    static constexpr uint32_t BYTES = RING + 2 * PIECES * 32 * 16;
+    static constexpr uint32_t CAP_OFF = RING + 2 * PIECES * 32 * 16;   // the tanh's coefficients
+    static constexpr uint32_t BYTES = CAP_OFF + 16;
     // 228 KB to an SM, of which each CTA takes 1 KB for itself
     static_assert(CTAS * (BYTES + 1024) <= 228 * 1024, "shared memory budget");
 };
@@ -269,6 +270,15 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
     w.u = u0;
     w.u1 = cut.start(blockIdx.x + 1);
     const float c = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
+    float limit;
+    {
+        const Score sc(a);
+        limit = sc.limit;
+        // in shared memory: registers are short, and only a cap wants them.  All warps write the same.
+        if (lane == 0)
+            *(float4*)(smem + S::CAP_OFF) = make_float4(ptx::lo2(sc.b0), ptx::lo2(sc.b1), ptx::lo2(sc.b2), ptx::lo2(sc.b3));
+        __syncwarp();
+    }
     const uint32_t ring = ptx::smem_u32(smem) + warp * STAGES * 2 * S::HALF;
 
     // ---- the copies run ahead: lane (lr, ch) copies piece ch of rows lr, lr + RP, ... of each block
@@ -399,14 +409,30 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
             const bool edge = k0 < flo || k0 + KEYS > fhi || hole;
             const float step = (float)(k0 - kfirst);
             if (cap2 > 0.f) {
+                // the two forms of the tanh, as cap32 has them: each score from its own product alone
+                float big = 0.f;
+#pragma unroll
+                for (int y = 0; y < NT; ++y)
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) big = fmaxf(big, fabsf(s[y][k][z]));
+                const bool inside = __all_sync(~0u, big <= limit);
+                const uint4 bw = lds16(ptx::smem_u32(smem) + S::CAP_OFF);
+                const float b0 = __uint_as_float(bw.x), b1 = __uint_as_float(bw.y), b2 = __uint_as_float(bw.z), b3 = __uint_as_float(bw.w);
 #pragma unroll
                 for (int y = 0; y < NT; ++y)
 #pragma unroll
                     for (int k = 0; k < KT; ++k)
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const float e = ptx::ex2_mufu(s[y][k][z] * (c * 2.f * LOG2E));
-                            s[y][k][z] = fmaf(-2.f * cap2, ptx::rcp_mufu(1.f + e), cap2);
+                            const float v = s[y][k][z], w2 = v * v, near = fmaf(fmaf(fmaf(b3, w2, b2), w2, b1), w2, b0) * v;
+                            if (inside) {
+                                s[y][k][z] = near;
+                                continue;
+                            }
+                            const float e = ptx::ex2_mufu(v * (c * 2.f * LOG2E));
+                            s[y][k][z] = fabsf(v) <= limit ? near : fmaf(-2.f * cap2, ptx::rcp_mufu(1.f + e), cap2);
                         }
             }
             // s becomes score - m + SH (score + SH while m is not yet a number)

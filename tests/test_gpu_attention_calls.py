@@ -262,3 +262,16 @@ def test_a_cache_holds_anything_behind_a_row_under_a_wide_cap(dtype, d, new):
         k2[b, m - new + 1:] = v2[b, m - new + 1:] = 6e4
     got = attend_cached(q, k2, v2, n, cap=50.0)
     assert torch.equal(got[:, 0], want[:, 0])
+
+
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e12])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,dtype", SIZES, ids=str)
+def test_a_very_wide_cap_changes_nothing(b, sq, sk, h, hk, d, dtype, cap):
+    """Scores of a few units: cap tanh(s / cap) is s to within s (s / cap)^2 / 3, some 1e-6 at the smallest cap here."""
+    from flashdiffusion_b200.attention import attend
+    q, k, v, _ = _inputs(b, sq, sk, h, hk, d, dtype, seed=95)
+    lo, hi, pos = spans_of(sq, sk, b, causal=True)
+    o, lse = attend(q, k, v, causal=True, cap=cap, return_lse=True)
+    ref = reference(q, k, v, lo, hi, pos)
+    check("o", o, ref, FLOOR[dtype])
+    check("lse", lse, ref)
