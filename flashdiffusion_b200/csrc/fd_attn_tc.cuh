@@ -107,8 +107,11 @@ struct Score {
         b2 = ptx::both2(0.13208261f * f * f * f * f * f * top);
         b3 = ptx::both2(-0.04522878f * f * f * f * f * f * f * f * top);
         shrink = ptx::both2(capped ? -1.f / (top * top) : 0.f);
-        // steep enough for a coefficient to overflow: the polynomial is never taken
-        limit = !(fabsf(ptx::lo2(b3)) < INFINITY) ? -1.f : f != 0.f ? 0.45f / fabsf(f) : INFINITY;
+        // Steep enough for a coefficient to overflow: the polynomial is never taken.  So flat that b3, b2 or b1 leaves
+        // the normal numbers (caps are 1e-3 and more): it is taken as far as what is left of it is good to 1e-8.
+        // s^2 must not overflow either.
+        const float flat = fabsf(f), upto = flat >= 2e-5f ? 0.45f : flat >= 2e-7f ? 0.1f : flat >= 1e-11f ? 0.037f : 0.003f;
+        limit = !(fabsf(ptx::lo2(b3)) < INFINITY) ? -1.f : flat > 0.f ? fminf(upto / flat, 1e18f) : 1e18f;
     }
     // the factor of s in the polynomial
     __device__ __forceinline__ uint64_t ratio(uint64_t s) const {

@@ -275,3 +275,18 @@ def test_a_very_wide_cap_changes_nothing(b, sq, sk, h, hk, d, dtype, cap):
     ref = reference(q, k, v, lo, hi, pos)
     check("o", o, ref, FLOOR[dtype])
     check("lse", lse, ref)
+
+
+@pytest.mark.parametrize("cap", [20.0, 1e4, 1e6, 1e9])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,dtype", SIZES, ids=str)
+def test_wide_caps_over_their_whole_range(b, sq, sk, h, hk, d, dtype, cap):
+    """Scores up to 0.44 of the cap, large heads and a small scale: the coefficients of a series of the tanh in the raw
+    products leave fp32's normal numbers one by one."""
+    from flashdiffusion_b200.attention import attend
+    q, k, v, _ = _inputs(b, sq, sk, h, hk, d, dtype, seed=97)
+    q, k = q * 1000, k * 1000
+    lo, hi, pos = spans_of(sq, sk, b)
+    top = max(float((q[:, :, i].double() @ k[:, :, i * hk // h].double().transpose(1, 2)).abs().max()) for i in range(h))
+    scale = 0.44 * cap / top
+    lse = attend(q, k, v, cap=cap, scale=scale, return_lse=True)[1]
+    check("lse", lse, reference(q, k, v, lo, hi, pos, cap=cap, scale=scale))
