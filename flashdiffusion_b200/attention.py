@@ -32,8 +32,6 @@ the rows that were not finished and a mark that ``flashdiffusion_b200.native.che
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import native
@@ -246,10 +244,10 @@ def _check(q, k, v, slopes, scale, cap, names):
             raise ValueError("there is no gradient for slopes: detach them")
     scale = qs[-1] ** -0.5 if scale is None else float(scale)
     cap = 0.0 if cap is None else float(cap)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite (got {scale})")
-    if cap and not 1e-3 <= cap < math.inf:
-        raise ValueError(f"cap must be None or at least 1e-3 (got {cap})")
+    if not abs(scale) <= 1e30:
+        raise ValueError(f"scale must be finite and at most 1e30 (got {scale})")
+    if cap and not 1e-3 <= cap <= 1e18:
+        raise ValueError(f"cap must be None or 1e-3 to 1e18 (got {cap})")
     native.refuse_duals("attention", q, k, v, slopes)
     native.require_device(q.device)
     return scale, cap
@@ -290,7 +288,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float | 
     scale    of the products, D^-1/2 by default
     causal   keys up to the row's own position; ``window``: at most that many of them
     spans    a ``Spans`` in the place of causal and window
-    cap      scores become cap tanh(score / cap)
+    cap      scores become cap tanh(score / cap); 1e-3 to 1e18
     slopes   (H,) float32: slope times the distance |position - j| is subtracted from the scores
     Returns the output (as q), or (output, lse): lse (B, H, Sq) float32 is the natural log of the sum of
     exp(scores), -inf for rows that see nothing; it carries no gradient.  A row that sees keys, but none above a score of

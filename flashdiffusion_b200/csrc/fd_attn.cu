@@ -1,6 +1,7 @@
 // Entry points of softmax attention over key spans (declared in
 // include/fd_sm100.h): argument checks and the choice of kernels.
 #include <algorithm>
+#include <cmath>
 
 #include "fd_attn_tc.cuh"
 
@@ -82,7 +83,9 @@ static int to_prob(const fd_attention_args* r, bool backward, Prob* out) {
                  "fd_attention: heads=%d must be a multiple of kv_heads=%d", r->heads, r->kv_heads);
     FD_CHECK_ARG(r->batch <= 65535 && r->heads <= 65535, "fd_attention: batch=%d or heads=%d above 65535", r->batch, r->heads);
     FD_CHECK_ARG(((uintptr_t)r->o_low & 7) == 0, "fd_attention: o_low must be 8-byte aligned");
-    FD_CHECK_ARG(r->scale == r->scale && r->cap >= 0.0, "fd_attention: scale and cap must be numbers, cap >= 0");
+    // beyond these the constants of a score (scale / cap and the like) leave fp32
+    FD_CHECK_ARG(std::abs(r->scale) <= 1e30, "fd_attention: scale=%g must be a number of at most 1e30", r->scale);
+    FD_CHECK_ARG(r->cap == 0.0 || (r->cap >= 1e-3 && r->cap <= 1e18), "fd_attention: cap=%g must be 0 or 1e-3 to 1e18", r->cap);
     FD_CHECK_ARG((r->first == nullptr) == (r->end == nullptr), "fd_attention: first and end come together");
     FD_CHECK_ARG(r->window >= 0, "fd_attention: window=%d", r->window);
     FD_CHECK_ARG(!r->first || (!r->causal && !r->window), "fd_attention: spans replace causal and window");

@@ -314,7 +314,7 @@ int fd_rotary(const fd_rotary_args* args, void* stream);
  * the newest tokens against a cache.
  *
  *     s_ij = scale q_i.k_j                        (cap = 0)
- *          = cap tanh(scale q_i.k_j / cap)        (cap > 0)
+ *          = cap tanh(scale q_i.k_j / cap)        (1e-3 <= cap <= 1e18)
  *     s_ij -= slopes[h] |pos_i - j|               (slopes != NULL)
  *     o_i  = sum_j softmax_j(s_ij) v_j            over first_i <= j < end_i
  *
