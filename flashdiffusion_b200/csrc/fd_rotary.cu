@@ -56,7 +56,7 @@ struct alignas(sizeof(T) * N) Vec {
 
 __device__ __forceinline__ int64_t batch_of(const Args& a, int64_t t) {
     if (a.tokens == a.total) return 0;
-    return (uint64_t)t >> 32 ? t / a.tokens : (uint32_t)t / (uint32_t)a.tokens;
+    return (uint64_t)(t | a.tokens) >> 32 ? t / a.tokens : (uint32_t)t / (uint32_t)a.tokens;
 }
 
 __device__ __forceinline__ double position(const Args& a, int64_t t) {
