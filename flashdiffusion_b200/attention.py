@@ -192,10 +192,10 @@ class _Attend(torch.autograd.Function):
     def forward(ctx, q, k, v, how, return_lse):
         q, k, v = _loadable(q), _loadable(k), _loadable(v)
         b, sq, h, d = q.shape
-        # one buffer for what the gradients want besides o: lse (unless it is an output), and for 16-bit heads on the
-        # tensor cores eight more bits of o
+        # one buffer for what the gradients want besides o: lse (unless it is an output), and for 16-bit heads whose
+        # forward pass is on the tensor cores eight more bits of o
         rows = b * sq * h
-        low = rows * d if q.dtype is not torch.float32 and d % 8 == 0 and d <= 128 else 0
+        low = rows * d if q.dtype is not torch.float32 and d % 8 == 0 else 0
         ctx.low_at = (0 if return_lse else (rows + 1) // 2 * 8) if low else None
         kept = torch.empty((0 if return_lse else (rows + 1) // 2 * 8) + low, dtype=torch.uint8, device=q.device)
         o, lse = _like(q), _lse_like(q) if return_lse else None

@@ -162,6 +162,7 @@ int fd_attention_backward(const fd_attention_args* r, void* workspace, size_t wo
     FD_CHECK_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0),
                  "fd_attention_backward: workspace must be 256-byte aligned");
     if (attn::tc_applies(a, r->dtype, true)) return attn::tc_backward(a, r->dtype, workspace, (cudaStream_t)stream);
+    if (!attn::tc_applies(a, r->dtype, false)) a.o_low = nullptr;   // the forward pass was not the one that writes it
     return attn::simt_backward(a, r->dtype, (float*)workspace, (cudaStream_t)stream);
 }
 

@@ -67,6 +67,14 @@ __device__ __forceinline__ float sum_or_nan(float l, int2 span) {
     return l == 0.f && span.y > span.x ? __int_as_float(0x7fffffff) : l;
 }
 
+// A rounded output with the eight bits kept below it, in units of 2^8 (bf16) or 2^5 (fp16) last places of fp32.
+// delta = d_o . o summed from rounded outputs would be the largest error of dq and dk after their own rounding and
+// that of dS.
+template <bool F16>
+__device__ __forceinline__ float with_low(float back, int low) {
+    return __int_as_float(__float_as_int(back) + low * (F16 ? 32 : 256));
+}
+
 // Launchers (fd_attn_simt.cu).
 int simt_forward(const Prob& a, int dtype, cudaStream_t s);
 int simt_backward(const Prob& a, int dtype, float* delta, cudaStream_t s);   // delta: batch * heads * q_len floats

@@ -20,6 +20,8 @@
 // pair whether it is seen.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "fd_attn.cuh"
 #include "fd_tc_common.cuh"
 
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(THREADS) few_kernel(const __grid_constant__ Pr
     cluster.sync();   // nobody leaves while its shared memory is read
 }
 
-// delta[b, h, i] = dO . o, a warp a row
+// delta[b, h, i] = dO . o, with the low bits of o where the forward pass kept them; a warp a row
 template <class T>
 __global__ void __launch_bounds__(THREADS) delta_kernel(const __grid_constant__ Prob a, float* __restrict__ delta) {
     const int lane = threadIdx.x & 31;
@@ -402,8 +404,13 @@ __global__ void __launch_bounds__(THREADS) delta_kernel(const __grid_constant__ 
     const int64_t bh = x / a.q_len;
     const int i = (int)(x - bh * a.q_len), b = (int)(bh / a.heads), h = (int)(bh - (int64_t)b * a.heads);
     const T *g = row<T>(a.d_o, b, i, h), *o = row<T>(a.o, b, i, h);
+    const int8_t* low = a.o_low ? a.o_low + (((int64_t)b * a.q_len + i) * a.heads + h) * a.dim : nullptr;
     float d = 0.f;
-    for (int c = lane; c < a.dim; c += 32) d = fmaf(up<T>(g[c]), up<T>(o[c]), d);
+    for (int c = lane; c < a.dim; c += 32) {
+        float f = up<T>(o[c]);
+        if (sizeof(T) == 2 && low) f = with_low<std::is_same<T, __half>::value>(f, low[c]);
+        d = fmaf(up<T>(g[c]), f, d);
+    }
     d = warp_sum(d);
     if (lane == 0) delta[x] = d;
 }

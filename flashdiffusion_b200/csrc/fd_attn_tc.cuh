@@ -292,18 +292,12 @@ __device__ __forceinline__ bool clear_bad(uint8_t* tile, int bytes, int lane) {
 __device__ __forceinline__ int warp_min(int x) { return __reduce_min_sync(~0u, x); }
 __device__ __forceinline__ int warp_max(int x) { return __reduce_max_sync(~0u, x); }
 
-// The eight bits below a rounded output, in units of 2^8 (bf16) or 2^5 (fp16) last places of fp32: `bits` is the
-// unrounded value, `back` the rounded one.  delta = d_o . o summed from rounded outputs would be the largest error of
-// dq and dk after their own rounding and that of dS.
+// The eight bits below a rounded output (with_low reads them): `f` is the unrounded value, `back` the rounded one.
 template <bool F16>
 __device__ __forceinline__ int low_bits(float f, float back) {
     constexpr int SH = F16 ? 5 : 8;
     if (!(fabsf(back) < INFINITY)) return 0;
     return min(max((__float_as_int(f) - __float_as_int(back) + (1 << (SH - 1))) >> SH, -128), 127);
-}
-template <bool F16>
-__device__ __forceinline__ float with_low(float back, int low) {
-    return __int_as_float(__float_as_int(back) + low * (F16 ? 32 : 256));
 }
 template <bool F16>
 __device__ __forceinline__ float2 pair_of(uint32_t w) {

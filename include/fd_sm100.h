@@ -336,8 +336,8 @@ typedef struct fd_attention_args {
     float* lse;                /* (batch, heads, q_len) contiguous, natural log; may be NULL (forward) */
     int8_t* o_low;             /* (batch, q_len, heads, dim) contiguous and 8-byte aligned, or NULL: eight more
                                   bits of o (16-bit types), written by forward where it runs on the tensor cores and
-                                  read by backward there, so that d_o . o is not summed from rounded outputs; give
-                                  both calls the same pointer */
+                                  read by backward for the same q, k, v and o, so that d_o . o is not summed from
+                                  rounded outputs; give both calls the same pointer */
     const int32_t *first, *end; /* (batch, q_len) spans, or both NULL */
     int64_t span_stride;       /* elements between batches (0 = the same spans for all) */
     const int32_t* lengths;    /* (batch) keys in use, or NULL */

@@ -290,3 +290,56 @@ def test_wide_caps_over_their_whole_range(b, sq, sk, h, hk, d, dtype, cap):
     scale = 0.44 * cap / top
     lse = attend(q, k, v, cap=cap, scale=scale, return_lse=True)[1]
     check("lse", lse, reference(q, k, v, lo, hi, pos, cap=cap, scale=scale))
+
+
+@pytest.mark.parametrize("d", [64, 136, 256])
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("rows", [1, 130])
+def test_rows_that_cancel(rows, dtype, d):
+    """Queries that look at two keys whose values differ little: dS = P (dP - delta) is the small difference of large
+    numbers."""
+    from flashdiffusion_b200.attention import attend
+    g = torch.Generator("cuda").manual_seed(57)
+    q, k = (torch.randn(1, n, 1, d, device="cuda", generator=g).to(dtype) for n in (rows, 2))
+    u = torch.finfo(dtype).eps / 2
+    v = torch.ones(1, 2, 1, d, device="cuda", dtype=dtype)
+    v[0, 1] += 4 * u
+    do = torch.ones(1, rows, 1, d, device="cuda", dtype=dtype)
+    lo, hi, pos = spans_of(rows, 2, 1)
+    ref = reference(q, k, v, lo, hi, pos, do=do)
+    dq, = torch.autograd.grad(attend(q.requires_grad_(True), k, v), q, do)
+    # p (1 - p) <= 1/4, dP - delta <= 4 u d.  delta is off by d 2 (2^-8 u of the kept bits and 2^-20 of fp32 steps), P by
+    # 2^-15, and dS is rounded once.  Where the weights of P V are rounded to 16 bits (all but few rows of narrow heads),
+    # o = sum_j p_j (1 + e_j) v_j with |e_j| <= u and v_j <= 1 + 4 u, so that delta is off by up to d u (1 + 4 u) more, and
+    # P times that is at most 1 / 2 for the smaller weight and the whole for the larger
+    p = 0.25
+    ds_tol = d ** -0.5 * (2 * p * d * 2 * (2.0 ** -8 * u + 2.0 ** -20) + p * 4 * u * d * (2.0 ** -15 + u))
+    if rows > 1 or d > 128:
+        ds_tol += d ** -0.5 * d * u * (1 + 4 * u)
+    room = u * ref["dq"].abs() + ds_tol * k.double().cpu().abs().sum(1, keepdim=True)
+    assert ((dq.double().cpu() - ref["dq"]).abs() <= room + FLOOR[dtype]).all()
+
+
+@pytest.mark.parametrize("d", [64, 136, 256])
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+@pytest.mark.parametrize("rows", [1, 130])
+def test_the_low_bits_of_the_output_serve_the_gradients(rows, dtype, d):
+    """Two equal weights, which are exact, and values 1 and 1 + 2 u: o = 1 + u lies between two numbers of its type, and
+    dS = -+ P u d scale.  From the rounded output, 1, it would be 0 and twice that."""
+    from flashdiffusion_b200.attention import attend
+    g = torch.Generator("cuda").manual_seed(59)
+    u = torch.finfo(dtype).eps / 2
+    q = torch.zeros(1, rows, 1, d, device="cuda", dtype=dtype, requires_grad=True)
+    k = torch.randn(1, 2, 1, d, device="cuda", generator=g).to(dtype)
+    v = torch.ones(1, 2, 1, d, device="cuda", dtype=dtype)
+    v[0, 1] += 2 * u
+    do = torch.ones(1, rows, 1, d, device="cuda", dtype=dtype)
+    dq, = torch.autograd.grad(attend(q, k, v), q, do)
+    k64 = k.double()[0, :, 0]
+    ds = 0.5 * u * d ** 0.5
+    want = ds * (k64[1] - k64[0])
+    # delta = d (1 + u) is kept exactly and summed in fp32 (d 2^-24 of it at most); P is off by 2^-15 and rounded once, so
+    # is dS, and the output
+    ds_tol = ds * (2.0 ** -15 + 2 * u) + 0.5 * d ** -0.5 * d * d * 2.0 ** -24
+    room = u * want.abs() + ds_tol * k64.abs().sum(0)
+    assert ((dq.double()[0, :, 0] - want).abs() <= room + FLOOR[dtype]).all()
