@@ -12,9 +12,9 @@ constexpr uint64_t WAIT_NS = 2000000000ull;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
-// Tensor-core kernels take 16-bit heads of a multiple of 8 coordinates up to
-// 128 whose rows start on 16-byte boundaries (TMA's rule); the rest runs on the
-// CUDA cores.
+// Tensor-core kernels take 16-bit heads of a multiple of 8 coordinates, up to 256
+// forward and 128 in the gradients, whose rows start on 16-byte boundaries (TMA's
+// rule); the rest runs on the CUDA cores.
 inline bool tma_view(const View& v, const int64_t (&extent)[3]) {
     if ((uintptr_t)v.p & 15) return false;
     const int64_t st[3] = {v.sb, v.ss, v.sh};
