@@ -117,8 +117,8 @@ inline size_t work_layout(Work* w, void* base, const Shape& z) {
 }
 
 // Which of the keys k0 .. k0 + 127 some query row sees, as 128 bits.  All threads of a block of 256; the answer is the
-// same in all.  Causal rows and windows move on by one key a row, so their union is one run.  Of spans all are read,
-// those about the keys' own positions first: they show most keys of causal masks, and nothing is left to look for.
+// same in all.  Causal rows and windows move on by one key a row, so their union is one run.  Of spans those about the
+// keys' own positions are read first: they show the keys of most masks, and nothing is left to look for in the others.
 __device__ __forceinline__ uint4 keys_seen(const Prob& a, int b, int n, int k0, uint32_t (&bits)[4]) {
     auto run = [&](int w, int lo, int hi) {   // bits of word w within [lo, hi)
         const int x = max(lo - k0 - 32 * w, 0), y = min(hi - k0 - 32 * w, 32);
@@ -130,29 +130,30 @@ __device__ __forceinline__ uint4 keys_seen(const Prob& a, int b, int n, int k0, 
     }
     if (threadIdx.x < 4) bits[threadIdx.x] = 0;
     __syncthreads();
-    constexpr int CHUNK = 1024;
-    const int chunks = (int)cdiv(a.q_len, CHUNK), own = min(max(k0 - (n - a.q_len), 0), a.q_len - 1) / CHUNK;
-    for (int c = 0; c < chunks; ++c) {
-        const int at = (own + c) % chunks * CHUNK + (int)threadIdx.x;
+    auto rows = [&](int lo, int hi) {
         uint32_t m[4] = {};
+        constexpr int AHEAD = 8;   // spans in flight
+        for (int i0 = lo + (int)threadIdx.x; i0 < hi; i0 += AHEAD * 256) {
+            int2 sp[AHEAD];
 #pragma unroll
-        for (int y = 0; y < CHUNK / 256; ++y) {
-            if (at + 256 * y >= a.q_len) continue;
-            const int2 sp = row_span(a, b, at + 256 * y, n);
+            for (int y = 0; y < AHEAD; ++y) sp[y] = i0 + 256 * y < hi ? row_span(a, b, i0 + 256 * y, n) : make_int2(0, 0);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) m[w] |= run(w, sp.x, sp.y);
+            for (int y = 0; y < AHEAD; ++y)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) m[w] |= run(w, sp[y].x, sp[y].y);
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            m[w] = __reduce_or_sync(~0u, m[w]);
-            if ((threadIdx.x & 31) == 0 && m[w]) atomicOr(&bits[w], m[w]);
-        }
+        for (int w = 0; w < 4; ++w)
+            if (m[w]) atomicOr(&bits[w], m[w]);
         __syncthreads();
-        bool all = true;
+    };
+    // the row that stands at the tile's first key is lo + 64
+    const int lo = min(max(k0 - (n - a.q_len) - 64, 0), a.q_len), hi = min(lo + 256, a.q_len);
+    rows(lo, hi);
+    bool all = true;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) all = all && (~bits[w] & run(w, 0, n)) == 0;
-        if (__syncthreads_and(all)) break;
-    }
+    for (int w = 0; w < 4; ++w) all = all && (~bits[w] & run(w, 0, n)) == 0;
+    if (!__syncthreads_and(all)) rows(0, a.q_len);
     return make_uint4(bits[0], bits[1], bits[2], bits[3]);
 }
 
