@@ -61,11 +61,12 @@ __device__ __forceinline__ int2 row_span(const Prob& a, int b, int i, int n) {
     return make_int2(min(lo, hi), hi);
 }
 
-// Sum of weights `l` of a row that sees keys `span`: a row whose visible scores are all -infinity has no softmax, and
-// says so, where a row that sees nothing is zeros.
-__device__ __forceinline__ float sum_or_nan(float l, int2 span) {
-    return l == 0.f && span.y > span.x ? __int_as_float(0x7fffffff) : l;
-}
+// A row that sees keys but none above a score of -infinity has no softmax and is NaN; a row that sees nothing is zeros.
+// Kernels that join parts of a row tell the two by the maximum of an unfinished row: LOWEST, or -infinity for a row
+// that sees nothing.  Both have a sum of zero.
+constexpr float LOWEST = -3.402823466e38f;
+__device__ __forceinline__ float not_a_number() { return __int_as_float(0x7fffffff); }
+__device__ __forceinline__ float sum_or_nan(float l, bool sees) { return l == 0.f && sees ? not_a_number() : l; }
 
 // A rounded output with the eight bits kept below it, in units of 2^8 (bf16) or 2^5 (fp16) last places of fp32.
 // delta = d_o . o summed from rounded outputs would be the largest error of dq and dk after their own rounding and

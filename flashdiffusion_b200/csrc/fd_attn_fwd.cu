@@ -456,8 +456,9 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
         l += other[0];
         const bool real = sub < C::SUBTILES && row < a.q_len;
         if (m == -INFINITY) l = 0.f;               // exponentials on the FMA pipe end at 2^-125, above zero
-        if (sp.parts == 1 && real) l = sum_or_nan(l, span);
-        if (!ok) l = __int_as_float(0x7fffffff);   // gave up: NaN, not numbers that could pass for the rows
+        const bool sees = real && span.y > span.x;
+        if (sp.parts == 1) l = sum_or_nan(l, sees);
+        if (!ok) l = not_a_number();               // gave up: NaN, not numbers that could pass for the rows
         const float inv = l == 0.f ? 0.f : 1.f / l;
         uint8_t* out = (uint8_t*)a.o.p + 2 * (b * a.o.sb + (int64_t)row * a.o.ss + h * a.o.sh);
         int8_t* low = a.o_low ? a.o_low + (((int64_t)b * a.q_len + row) * a.heads + h) * a.dim : nullptr;
@@ -507,7 +508,7 @@ forward_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ 
             }
         }
         if (half == 0 && real) {
-            const float lse2 = l == 0.f ? -INFINITY : m * c + (log2f(l) - P_SHIFT);
+            const float lse2 = l == 0.f ? (sees ? LOWEST : -INFINITY) : m * c + (log2f(l) - P_SHIFT);
             if (sp.parts > 1) sp.lse2[(((int64_t)part * a.batch + b) * a.q_len + row) * a.heads + h] = lse2;
             else if (a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + row] = lse2 * LN2;
         }
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
     float m = -INFINITY;
     for (int p = 0; p < sp.parts; ++p) m = fmaxf(m, sp.lse2[p * rows + r]);
     const float base = m == -INFINITY ? 0.f : m;
-    float sum = 0.f, acc[8] = {};
+    float sum = m == LOWEST ? not_a_number() : 0.f, acc[8] = {};
 #pragma unroll 4
     for (int p = 0; p < sp.parts; ++p) {
         const float w = exp2f(sp.lse2[p * rows + r] - base);
@@ -543,7 +544,6 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Prob 
         for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, f[e], acc[e]);
     }
     const int64_t t = r / a.heads, b = t / a.q_len, row = t - b * a.q_len;
-    if (sum == 0.f) sum = sum_or_nan(sum, row_span(a, (int)b, (int)row, keys_of(a, (int)b)));
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] *= inv;

@@ -42,7 +42,7 @@ constexpr int SETUP = 3;
 __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 __host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 2 : 3; }
 
-// log2 of what P, and with it l and O, are held times.
+// How far m is set below a row's maximum: log2 of what P, and with it l and O, are held times.
 template <bool F16> constexpr float P_SHIFT = F16 ? 7.f : 0.f;
 
 struct Range {
@@ -226,7 +226,7 @@ template <bool F16>
 __device__ __forceinline__ void store_row(const Prob& a, const Plan& p, int b, int hk, int gr, int d,
                                           const float (&acc)[8], float m, float l) {
     const int i = p.query(gr), h = hk * a.group + gr - i * a.group;
-    if (l == 0.f) l = sum_or_nan(l, row_span(a, b, i, keys_of(a, b)));
+    l = sum_or_nan(l, m == LOWEST);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (d < a.dim) {
         float f[8];
@@ -235,7 +235,7 @@ __device__ __forceinline__ void store_row(const Prob& a, const Plan& p, int b, i
         store8<F16>((uint16_t*)a.o.p + b * a.o.sb + (int64_t)i * a.o.ss + h * a.o.sh + d,
                     a.o_low ? a.o_low + (((int64_t)b * a.q_len + i) * a.heads + h) * a.dim + d : nullptr, f);
     }
-    if (d == 0 && a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = l == 0.f ? -INFINITY : (m + (log2f(l) - P_SHIFT<F16>)) * LN2;
+    if (d == 0 && a.lse) a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
 template <int DP, int NT>
@@ -245,8 +245,8 @@ struct Smem {
     static constexpr uint32_t HALF = KEYS * DP * 2;               // K or V of a block, 4 KB
     static constexpr uint32_t RING = WARPS * STAGES * 2 * HALF;
     static constexpr int PIECES = DP / 16 + 1;                    // 16-byte pieces of one lane's sums: O, and m and l
-    static constexpr uint32_t CAP_OFF = RING + 2 * PIECES * 32 * 16;   // the tanh's coefficients
-    static constexpr uint32_t BYTES = CAP_OFF + 16;
+    static constexpr uint32_t CAP_OFF = RING + 2 * PIECES * 32 * 16;   // the tanh's coefficients and their limit
+    static constexpr uint32_t BYTES = CAP_OFF + 32;
     // 228 KB to an SM, of which each CTA takes 1 KB for itself
     static_assert(CTAS * (BYTES + 1024) <= 228 * 1024, "shared memory budget");
 };
@@ -270,13 +270,14 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
     w.u = u0;
     w.u1 = cut.start(blockIdx.x + 1);
     const float c = a.cap > 0.f ? a.scale / a.cap : a.scale * LOG2E, cap2 = a.cap * LOG2E;
-    float limit;
-    {
-        const Score sc(a);
-        limit = sc.limit;
-        // in shared memory: registers are short, and only a cap wants them.  All warps write the same.
-        if (lane == 0)
-            *(float4*)(smem + S::CAP_OFF) = make_float4(ptx::lo2(sc.b0), ptx::lo2(sc.b1), ptx::lo2(sc.b2), ptx::lo2(sc.b3));
+    if (cap2 > 0.f) {
+        // in shared memory, for registers are short and only a cap wants them.  All warps write the same.
+        if (lane == 0) {
+            const Score sc(a);
+            float* to = (float*)(smem + S::CAP_OFF);
+            *(float4*)to = make_float4(ptx::lo2(sc.b0), ptx::lo2(sc.b1), ptx::lo2(sc.b2), ptx::lo2(sc.b3));
+            to[4] = sc.limit;
+        }
         __syncwarp();
     }
     const uint32_t ring = ptx::smem_u32(smem) + warp * STAGES * 2 * S::HALF;
@@ -362,8 +363,12 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                 l[y][z] = 0.f;
                 if (real) {
                     const int2 sp = row_span(a, b, i, n);
-                    if (sp.y > sp.x) flo = max(flo, sp.x);
-                    else hole = true;
+                    if (sp.y > sp.x) {
+                        flo = max(flo, sp.x);
+                        m[y][z] = LOWEST;
+                    } else {
+                        hole = true;
+                    }
                     fhi = min(fhi, sp.y);
                 }
             }
@@ -417,8 +422,9 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                     for (int k = 0; k < KT; ++k)
 #pragma unroll
                         for (int z = 0; z < 4; ++z) big = fmaxf(big, fabsf(s[y][k][z]));
-                const bool inside = __all_sync(~0u, big <= limit);
                 const uint4 bw = lds16(ptx::smem_u32(smem) + S::CAP_OFF);
+                const float limit = *(volatile float*)(smem + S::CAP_OFF + 16);
+                const bool inside = __all_sync(~0u, big <= limit);
                 const float b0 = __uint_as_float(bw.x), b1 = __uint_as_float(bw.y), b2 = __uint_as_float(bw.z), b3 = __uint_as_float(bw.w);
 #pragma unroll
                 for (int y = 0; y < NT; ++y)
@@ -435,7 +441,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                             s[y][k][z] = fabsf(v) <= limit ? near : fmaf(-2.f * cap2, ptx::rcp_mufu(1.f + e), cap2);
                         }
             }
-            // s becomes score - m + SH (score + SH while m is not yet a number)
+            // s becomes score - m (score itself while m is not yet a number)
             constexpr float SH = P_SHIFT<F16>;
             const float mul = cap2 > 0.f ? 1.f : c;
             float top[NT][2];
@@ -444,7 +450,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
             for (int y = 0; y < NT; ++y)
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    const float nb = m[y][z] == -INFINITY ? SH : SH - m[y][z];
+                    const float nb = m[y][z] <= LOWEST ? 0.f : -m[y][z];
                     const float sl = slope2[y][z], far = at[y][z] - step, from = fmaf(-sl, far, nb);
 #pragma unroll
                     for (int k = 0; k < KT; ++k)
@@ -468,7 +474,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                     top[y][z] = fmaxf(s[y][0][z], s[y][0][2 + z]);
 #pragma unroll
                     for (int k = 1; k < KT; ++k) top[y][z] = fmaxf(top[y][z], fmaxf(s[y][k][z], s[y][k][2 + z]));
-                    raise = raise || top[y][z] > (m[y][z] == -INFINITY ? -INFINITY : 8.f + SH);
+                    raise = raise || top[y][z] > (m[y][z] <= LOWEST ? -INFINITY : 8.f + SH);
                 }
             if (__any_sync(~0u, raise)) {
 #pragma unroll
@@ -479,7 +485,7 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 4));
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 8));
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 16));
-                        const bool fresh = m[y][z] == -INFINITY;
+                        const bool fresh = m[y][z] <= LOWEST;
                         tp -= SH;                                 // by how much m rises, or its first value
                         if (!fresh) tp = fmaxf(tp, 0.f);
                         if (tp == -INFINITY) continue;            // still nothing seen

@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 128 ? 2 : 1) forward_kernel(con
         const int q = q0 + ty * M + i;
         float sum = warp_sum(l[i], 8);
         if (q >= a.q_len) continue;
-        sum = sum_or_nan(sum, make_int2(rows.first[ty * M + i], rows.end[ty * M + i]));
+        sum = sum_or_nan(sum, rows.end[ty * M + i] > rows.first[ty * M + i]);
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         T* o = row<T>(a.o, b, q, h);
 #pragma unroll
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(THREADS) few_kernel(const __grid_constant__ Pr
                 o = fmaf(f, oo[x * 256 + threadIdx.x], o);
             }
         }
-        sum = sum_or_nan(sum, sp);
+        sum = sum_or_nan(sum, sp.y > sp.x);
         if ((int)threadIdx.x < a.dim) row<T>(a.o, b, i, h)[threadIdx.x] = down<T>(sum == 0.f ? 0.f : o / sum);
         if (a.lse && threadIdx.x == 0)
             a.lse[((int64_t)b * a.heads + h) * a.q_len + i] = sum == 0.f ? -INFINITY : m + logf(sum);
