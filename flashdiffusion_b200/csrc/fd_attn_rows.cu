@@ -486,9 +486,9 @@ rows_kernel(const __grid_constant__ Prob a, const __grid_constant__ Plan p, floa
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 8));
                         tp = fmaxf(tp, __shfl_xor_sync(~0u, tp, 16));
                         const bool fresh = m[y][z] <= LOWEST;
+                        // nothing seen yet, or no need: what another row of the warp sees moves no bit of this one
+                        if (!(tp > (fresh ? -INFINITY : 8.f + SH))) continue;
                         tp -= SH;                                 // by how much m rises, or its first value
-                        if (!fresh) tp = fmaxf(tp, 0.f);
-                        if (tp == -INFINITY) continue;            // still nothing seen
                         const float fix = fresh ? 0.f : ptx::ex2_mufu(-tp);
                         m[y][z] = fresh ? tp : m[y][z] + tp;
                         l[y][z] *= fix;

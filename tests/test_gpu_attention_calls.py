@@ -343,3 +343,61 @@ def test_the_low_bits_of_the_output_serve_the_gradients(rows, dtype, d):
     ds_tol = ds * (2.0 ** -15 + 2 * u) + 0.5 * d ** -0.5 * d * d * 2.0 ** -24
     room = u * want.abs() + ds_tol * k64.abs().sum(0)
     assert ((dq.double()[0, :, 0] - want).abs() <= room + FLOOR[dtype]).all()
+
+
+@pytest.mark.parametrize("cap", [None, 50.0])
+@pytest.mark.parametrize("dtype,d,new,h,hk", [(BF, 128, 4, 8, 2), (HF, 64, 3, 4, 1), (BF, 64, 8, 4, 1), (HF, 128, 2, 2, 2),
+                                              (BF, 256, 3, 4, 2), (SF, 64, 3, 4, 2)], ids=str)
+def test_keys_of_later_tokens_do_not_touch_earlier_ones(dtype, d, new, h, hk, cap):
+    """Several new tokens: a key that only the last of them see may be large, and moves no bit of the others."""
+    from flashdiffusion_b200.attention import attend_cached
+    b, capacity = 40, 400
+    q, k, v, _ = _inputs(b, new, capacity, h, hk, d, dtype, seed=99)
+    n = torch.linspace(new, capacity, b, device="cuda").int()
+    want = attend_cached(q, k, v, n, cap=cap)
+    at = n.long()[:, None] - 1                                     # the last token's key
+    k2 = k.scatter(1, at[:, :, None, None].expand(b, 1, hk, d), k.gather(1, at[:, :, None, None].expand(b, 1, hk, d)) * 24)
+    got = attend_cached(q, k2, v, n, cap=cap)
+    assert not torch.equal(got[:, -1], want[:, -1])
+    assert torch.equal(got[:, :-1], want[:, :-1])
+
+
+@pytest.mark.parametrize("cap", [None, 50.0])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,dtype", SIZES, ids=str)
+def test_later_keys_do_not_touch_earlier_rows(b, sq, sk, h, hk, d, dtype, cap):
+    q, k, v, do = _inputs(b, sq, sk, h, hk, d, dtype, seed=101)
+    want = _step(q, k, v, do, causal=True, cap=cap)
+    row = sq - 1 if sq < 40 else sq // 3                           # the first row that sees the keys below
+    k2, v2 = k.clone(), v.clone()
+    for t in (k2, v2):
+        t[:, max(sk - sq + row, 0):] *= 24
+    got = _step(q, k2, v2, do, causal=True, cap=cap)
+    assert torch.equal(got["o"][:, :row], want["o"][:, :row])
+    assert torch.equal(got["lse"][:, :, :row], want["lse"][:, :, :row])
+    x, y = got["dq"][:, :row], want["dq"][:, :row]
+    if dtype is not HF or d > 128:
+        assert torch.equal(x, y)
+        return
+    # fp16 gradients hold dS at a power of two that brings 2 |dO| |V|, of all rows of a sequence that take part, to 2^14 or
+    # more: below fp16's normal numbers it is off by at most half of 2^-24 there, in either run, and dq with it
+    v2 = v2.double().flatten(0, 2).norm(dim=1).max()
+    ds = 2.0 ** -24 * 2 * float(do.double().flatten(0, 2).norm(dim=1).max() * v2) / 2.0 ** 14
+    room = d ** -0.5 * ds * k.double().abs().sum(1, keepdim=True).repeat_interleave(h // hk, 2)
+    assert ((x.double() - y.double()).abs() <= room + 2 * 2.0 ** -11 * y.double().abs() + FLOOR[HF]).all()
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, HF), (128, HF), (40, SF)], ids=str)
+def test_keys_of_other_rows_do_not_touch_a_row(d, dtype):
+    """Few rows with spans of their own: keys that half of them see may be large, and move no bit of the others.  So many
+    sequences that a warp goes from keys that all rows see to these."""
+    from flashdiffusion_b200.attention import Spans, attend
+    b, sq, sk, h, hk = 400, 4, 256, 8, 2
+    q, k, v, _ = _inputs(b, sq, sk, h, hk, d, dtype, seed=103)
+    first = torch.tensor([72, 64, 72, 64], dtype=torch.int32, device="cuda")
+    spans = Spans(first, torch.full_like(first, 230))
+    want = attend(q, k, v, spans=spans)
+    k2, v2 = k.clone(), v.clone()
+    for t in (k2, v2):
+        t[:, 66:72] *= 24
+    got = attend(q, k2, v2, spans=spans)
+    assert torch.equal(got[:, 0::2], want[:, 0::2]) and not torch.equal(got[:, 1::2], want[:, 1::2])
