@@ -24,6 +24,12 @@ leaf whose gradient node was made on the default stream, and is kept alive by
 such an output, pulls that stream into the capture, which torch cannot do.  Forward-mode tangents (``torch.func.jvp``, dual tensors) and tracing
 (``torch.jit.trace``, ``make_fx``) are refused.
 
+16-bit heads are summed by the tensor core in fp32, from weights of 16 bits (``attend_cached`` splits them in two), and
+its adder rounds toward zero: beside its rounding an output can come out low by 6e-9 of its weighted sum of |v| for each
+key, 1e-4 at 16384 keys of values of one sign, and a gradient for each row that it sums likewise.  Gradients of fp16
+heads hold dS at one power of two for a sequence and key head, so that very large values or output gradients there cost
+the smallest dS bits.
+
 The kernels' waits are bounded.  One that gives up (after two seconds, which nothing but a fault of the device or of
 these kernels should bring about) raises no error by itself, since a call does not wait for the GPU: it leaves NaN in
 the rows that were not finished and a mark that ``flashdiffusion_b200.native.check_status(device)`` turns into an

@@ -401,3 +401,25 @@ def test_keys_of_other_rows_do_not_touch_a_row(d, dtype):
         t[:, 66:72] *= 24
     got = attend(q, k2, v2, spans=spans)
     assert torch.equal(got[:, 0::2], want[:, 0::2]) and not torch.equal(got[:, 1::2], want[:, 1::2])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=str)
+def test_very_long_rows_in_one_part(dtype):
+    """131072 keys a row, and so many query tiles that the key axis is not cut: what the accumulator loses by adding up
+    values of one sign, rounding toward zero, stays inside its bound."""
+    from flashdiffusion_b200.attention import attend
+    sq, sk, h, d = 512, 131072, 40, 64
+    g = torch.Generator(device="cuda").manual_seed(105)
+    q, k, v = (torch.randn(1, n, x, d, device="cuda", generator=g).to(dtype) for n, x in ((sq, h), (sk, 1), (sk, 1)))
+    v = v.abs()
+    o = attend(q, k, v)
+    u, w = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    for head in (0, h - 1):
+        s = q[0, :, head].double() @ k[0, :, 0].double().T * d ** -0.5
+        size = float((q[0, :, head].double().abs() @ k[0, :, 0].double().abs().T).max()) * d ** -0.5
+        want = torch.softmax(s, -1) @ v[0, :, 0].double()
+        es = 2 * (d + 8) * w * size + 8 * w * (float(s.abs().max()) + 1)
+        # the weights' and the output's rounding; scores and exponentials; one last place for each step of 16 keys; the
+        # sum of weights, tile by tile
+        rel = 2 * u + 2 * es + 8e-6 + sk / 16 * 2.0 ** -23 + 2 * (sk / 128 + 64) * w
+        assert ((o[0, :, head].double() - want).abs() <= rel * want).all()
