@@ -145,8 +145,10 @@ __device__ __forceinline__ uint4 keys_seen(const Prob& a, int b, int n, int k0, 
                 for (int w = 0; w < 4; ++w) m[w] |= run(w, sp[y].x, sp[y].y);
         }
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-            if (m[w]) atomicOr(&bits[w], m[w]);
+        for (int w = 0; w < 4; ++w) {
+            m[w] = __reduce_or_sync(~0u, m[w]);
+            if ((threadIdx.x & 31) == 0 && m[w]) atomicOr(&bits[w], m[w]);
+        }
         __syncthreads();
     };
     // the row that stands at the tile's first key is lo + 64
@@ -166,7 +168,8 @@ __device__ __forceinline__ uint4 keys_seen(const Prob& a, int b, int n, int k0, 
 // Bandwidth-bound: dO and o are read once.
 template <bool F16>
 __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob a, const __grid_constant__ Work w, int n_qt) {
-    const int h = blockIdx.y, b = blockIdx.z, t = blockIdx.x;
+    // V's blocks first: theirs is the longer chain where spans have to be read
+    const int h = blockIdx.y, b = blockIdx.z, t = (int)(gridDim.x - 1 - blockIdx.x);
     const int piece = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     float top = 0.f;
     asm volatile("griddepcontrol.launch_dependents;");   // the gradient kernel sets itself up and waits
@@ -174,16 +177,21 @@ __global__ void __launch_bounds__(256) prep_kernel(const __grid_constant__ Prob 
         if (h >= a.kv_heads) return;
         __shared__ uint32_t bits[4];
         const int k0 = (t - n_qt) * T;
+        uint4 x[T / 16];         // on their way while the spans are looked at
+#pragma unroll
+        for (int r8 = 0; r8 < T / 16; ++r8) {
+            const int64_t j = k0 + r0 + 16 * r8;
+            x[r8] = make_uint4(0, 0, 0, 0);
+            if (j < a.k_len && piece * 8 < a.dim)
+                x[r8] = *(const uint4*)((const uint16_t*)a.v.p + b * a.v.sb + j * a.v.ss + h * a.v.sh + piece * 8);
+        }
         const uint4 seen = keys_seen(a, b, keys_of(a, b), k0, bits);
         const uint32_t word[4] = {seen.x, seen.y, seen.z, seen.w};
 #pragma unroll
         for (int r8 = 0; r8 < T / 16; ++r8) {
-            const int r = r0 + 16 * r8;
-            const int64_t j = k0 + r;
             float s = 0.f;
-            if (word[r8 / 2] >> (r & 31) & 1 && piece * 8 < a.dim) {
-                const uint4 x = *(const uint4*)((const uint16_t*)a.v.p + b * a.v.sb + j * a.v.ss + h * a.v.sh + piece * 8);
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+            if (word[r8 / 2] >> ((r0 + 16 * r8) & 31) & 1) {
+                const uint32_t xs[4] = {x[r8].x, x[r8].y, x[r8].z, x[r8].w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 f = pair_of<F16>(xs[i]);
