@@ -13,10 +13,11 @@
 // too few for that (few key heads, few query rows), a CTA's tiles are shared
 // between several, whose fp32 sums sum_kernel adds up in their order.
 //
-// Measured, bf16: 2 x 4096 rows of 16 / 4 heads of 128 727 us, 945 TFLOP/s of the
-// five products, causal 433 us, 793, with a cap 716 us; the tensor pipe is busy 63 %
-// of the time, S and dP being bound by the shared memory they read both operands
-// from (128 bytes a clock).  A CTA's start and end take about 8 us.
+// Measured, bf16: 2 x 4096 rows of 16 / 4 heads of 128 688 us, 999 TFLOP/s of the
+// five products, causal 401 us, 857, with a cap 647 us (881 where most blocks of
+// scores reach beyond 0.45 of it); the tensor pipe is busy 66 % of the time, S and
+// dP being bound by the shared memory they read both operands from (128 bytes a
+// clock).  A CTA's start and end take about 8 us.
 //
 // CTA: two compute warpgroups that share the 128 rows of the accumulators (64
 // columns of each score tile apiece), and a warpgroup with a TMA producer, an

@@ -24,8 +24,9 @@
 // Measured, bf16: 2 x 4096 rows of 16 / 4 heads of 128 298 us, 922 TFLOP/s, causal
 // 164 us, 840; 16384 causal rows of 8 / 2 heads 504 us, 1091, with a cap and a
 // window of 4096 (fp16) 351 us, 685; 8192 causal rows of 8 / 4 heads of 256 328 us,
-// 839.  Bound by the shared memory that feeds S and P V (tensor pipe 36 % at 2 x
-// 4096 causal rows) and by the exponentials' issue slots (44 %), which take turns.
+// 839.  No pipe is full (2 x 4096 causal rows: tensor 41 %, issue slots 46 %, MUFU
+// 32 %): a subtile's next scores wait for its own P V and that for its
+// exponentials, and two subtiles hide only a part of the chain.
 #include <algorithm>
 
 #include "fd_attn_tc.cuh"

@@ -325,7 +325,9 @@ int fd_rotary(const fd_rotary_args* args, void* stream);
  * else 0.  A row with an empty span gives zeros and lse = -inf and no gradient;
  * one that sees keys but none above a score of -infinity gives NaN.
  * Keys outside a row's span never reach it, whatever their memory holds (NaN
- * and infinities included).
+ * and infinities included).  fp16 gradients hold dS at one power of two for a
+ * batch entry and key head, from the rows of d_o and v there that take part.
+ * Rows that a wait left unfinished when it gave up are NaN.
  * ------------------------------------------------------------------------- */
 
 typedef struct fd_attention_args {
